@@ -531,6 +531,109 @@ MPO_API int mpo_allreduce_sum_f32_p2p(const float* value, float scale, float* ou
                                       uint32_t seq, int64_t timeout_ns, int32_t* status,
                                       void* stream);
 
+/* ------------------------------------------------------------------ attention of serialised clouds
+ * No counterpart in the reference: the layer that Pointcept's later networks
+ * put on top of the neighbour operations (mps_pointops/pointcept.py): points
+ * ordered along a space-filling curve attend to their neighbours along it.
+ * Element types of q, k, v, out and their gradients. */
+#define MPO_F32 0
+#define MPO_F16 1
+#define MPO_BF16 2
+
+/* Norms of queries and keys for each head, then the rotation by position.
+ *   q (rows, heads, dim) and k (rows, kv_heads, dim) of `dtype`, innermost
+ *   axis dense, other strides in elements; out_q / out_k dense.
+ *   y = w * x / sqrt(mean(x^2) + eps), then pair t of the first 2 * pairs
+ *   elements turns by theta_t = sum_a position[row, a] * freqs[a, t]:
+ *   (u, v) -> (u cos - v sin, u sin + v cos).  Pairs are (t, pairs + t), or
+ *   (2t, 2t + 1) when interleaved.  dim is a multiple of 8 up to 256, pairs a
+ *   multiple of 4 with 2 * pairs <= dim (0: no rotation).
+ *   position (rows, axes <= 3) dense, int32 or (position_float) float32; freqs
+ *   (axes, pairs) float32; q_weight / k_weight (dim) float32, nullable (ones).
+ * Theta is formed in double and reduced before the sine; the rest is float32,
+ * rounded once to the output's type. */
+typedef struct {
+    const void *q, *k;
+    int64_t q_row, q_head, k_row, k_head; /* strides, elements */
+    const void *grad_q, *grad_k;          /* backward: dense */
+    void *out_q, *out_k;                  /* forward: results; backward: input gradients; dense */
+    const float *q_weight, *k_weight;
+    float *grad_q_weight, *grad_k_weight; /* backward: (dim), nullable */
+    const void* position;
+    const float* freqs;
+    void* workspace; /* backward */
+    size_t workspace_bytes;
+    int64_t rows;
+    int32_t heads, kv_heads, dim, pairs, axes, position_float, interleaved, dtype;
+    float eps;
+    int32_t reserved;
+} mpo_rotate;
+MPO_API int mpo_norm_rotate(const mpo_rotate* args, void* stream);
+MPO_API size_t mpo_norm_rotate_workspace_bytes(const mpo_rotate* args);
+MPO_API int mpo_norm_rotate_backward(const mpo_rotate* args, void* stream);
+
+/* Tiles of a ragged batch, computed on the host: ends and other_ends (segs)
+ * are inclusive cumulative row counts (Pointcept offsets) of the owning side
+ * and of the other side.  Each cloud's rows on the owning side are cut into
+ * tiles of 128 rows; a tile is eight int32 words {row, rows, first, other, lq,
+ * lk, base, cloud}, `first` being the position i + Lk - Lq of its first row
+ * (keys == 0: queries own) or its index in the cloud (keys != 0).  Returns the
+ * tile count, writing at most `capacity` of them to `tiles` (nullable: count
+ * only), or -1 with mpo_last_error set when an offset decreases, is negative
+ * or does not fit 30 bits. */
+MPO_API int64_t mpo_attention_plan(const int64_t* ends, const int64_t* other_ends, int64_t segs,
+                                   int keys, int32_t* tiles, int64_t capacity);
+
+/* Attention with a sliding window, first rows that stay visible (sinks) and a
+ * learned relative position bias by buckets, over a ragged batch.
+ *   q (q_rows, heads, dim), k and v (k_rows, kv_heads, dim) of `dtype`, heads a
+ *   multiple of kv_heads, dim a multiple of 8 up to 128; innermost axis dense,
+ *   16-byte aligned rows, strides in elements.  Key j of a cloud is visible to
+ *   its query row i, at position p = i + Lk - Lq, when (j < sinks or
+ *   p - left <= j <= p + right) and (not causal or j <= p); left or right < 0:
+ *   no limit on that side.
+ *   Scores: scale * q.k + sum_a table[a, bucket_a, head] with bucket_a =
+ *   clamp(kpos[j, a] - qpos[i, a], -reach, reach) + reach, through `map`
+ *   (2 reach + 1 int32 on the device, clamped to [0, buckets)) when given, else
+ *   buckets = 2 reach + 1.
+ *   table (axes, buckets, heads), axes * buckets <= 256; qpos / kpos dense
+ *   int32 (rows, axes), magnitudes below 2^30.  table NULL: no bias.
+ *   out (q_rows, heads, dim) dense; lse (heads, q_rows) float32, nullable in
+ *   the forward: natural logarithm of the softmax denominators.  A row that
+ *   sees no key gets zeros and -inf.  out_f32 (nullable): the result before
+ *   its rounding, which the backward needs for the table's gradient.
+ * Backward: grad_out dense like out; out, lse and (table gradient) out_f32 as
+ * the forward gave them; delta (heads, q_rows) float32 scratch; grad_q,
+ * grad_k, grad_v dense, overwritten; grad_table (axes, buckets, heads)
+ * float32, nullable.  Sums run in a fixed order (bit-reproducible).
+ * q_tiles / k_tiles: device copies of mpo_attention_plan's tiles; max_rows the
+ * largest Lq and max_keys the largest Lk.  The device reads rows only through
+ * the tiles, which must describe these tensors. */
+typedef struct {
+    const void *q, *k, *v;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head; /* strides, elements */
+    void* out;
+    float *out_f32, *lse;
+    const void* grad_out;
+    float* delta;
+    void *grad_q, *grad_k, *grad_v;
+    const void* table;
+    float* grad_table;
+    const int32_t *qpos, *kpos;
+    const int32_t* map;
+    const int32_t *q_tiles, *k_tiles;
+    int64_t q_tile_count, k_tile_count, q_rows, k_rows;
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t heads, kv_heads, dim, dtype, table_dtype, axes, buckets, reach;
+    int32_t left, right, sinks, causal, max_rows, max_keys;
+    float scale;
+    int32_t backward; /* workspace query: 0 forward, 1 backward */
+} mpo_attention;
+MPO_API size_t mpo_window_attention_workspace_bytes(const mpo_attention* args);
+MPO_API int mpo_window_attention(const mpo_attention* args, void* stream);
+MPO_API int mpo_window_attention_backward(const mpo_attention* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

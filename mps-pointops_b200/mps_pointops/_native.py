@@ -32,6 +32,37 @@ _f32 = ctypes.c_float
 _i32 = ctypes.c_int32
 _sz = ctypes.c_size_t
 
+
+
+def _fields(*groups):
+    return [(name, kind) for kind, names in groups for name in names.split()]
+
+
+class RotateArgs(ctypes.Structure):
+    """mpo_rotate of include/mpo_b200.h."""
+
+    _fields_ = _fields(
+        (_vp, "q k"), (_i64, "q_row q_head k_row k_head"),
+        (_vp, "grad_q grad_k out_q out_k q_weight k_weight grad_q_weight grad_k_weight position "
+              "freqs workspace"),
+        (_sz, "workspace_bytes"), (_i64, "rows"),
+        (_i32, "heads kv_heads dim pairs axes position_float interleaved dtype"), (_f32, "eps"),
+        (_i32, "reserved"))
+
+
+class AttentionArgs(ctypes.Structure):
+    """mpo_attention of include/mpo_b200.h."""
+
+    _fields_ = _fields(
+        (_vp, "q k v"), (_i64, "q_row q_head k_row k_head v_row v_head"),
+        (_vp, "out out_f32 lse grad_out delta grad_q grad_k grad_v table grad_table qpos kpos map "
+              "q_tiles k_tiles"),
+        (_i64, "q_tile_count k_tile_count q_rows k_rows"), (_vp, "workspace"),
+        (_sz, "workspace_bytes"),
+        (_i32, "heads kv_heads dim dtype table_dtype axes buckets reach left right sinks causal "
+               "max_rows max_keys"), (_f32, "scale"), (_i32, "backward"))
+
+
 # name -> (restype, argtypes); mirrors include/mpo_b200.h one to one.
 SIGNATURES = {
     "mpo_abi_version": (ctypes.c_int32, []),
@@ -101,6 +132,13 @@ SIGNATURES = {
     "mpo_flat_fps_workspace_bytes": (_sz, [_i64, _i64]),
     "mpo_flat_fps": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _sz,
                             _vp]),
+    "mpo_norm_rotate": (_int, [_vp, _vp]),
+    "mpo_norm_rotate_workspace_bytes": (_sz, [_vp]),
+    "mpo_norm_rotate_backward": (_int, [_vp, _vp]),
+    "mpo_attention_plan": (_i64, [_vp, _vp, _i64, _int, _vp, _i64]),
+    "mpo_window_attention_workspace_bytes": (_sz, [_vp]),
+    "mpo_window_attention": (_int, [_vp, _vp]),
+    "mpo_window_attention_backward": (_int, [_vp, _vp]),
     "mpo_p2p_slots_bytes": (_sz, []),
     "mpo_p2p_slots_create": (_int, [_vp, _vp]),
     "mpo_p2p_slots_open": (_int, [_vp, _vp]),

@@ -1,0 +1,508 @@
+"""Attention of serialised point clouds on B200.
+
+The layer that transformers over serialised clouds put on top of the point
+operations of this package: points are ordered along a space-filling curve,
+the clouds of a batch lie one after another in flat rows (Pointcept offsets:
+inclusive cumulative ends, mps_pointops/pointcept.py:46-56 of
+gamzerA/mps-pointops, which has no such layer itself), and a point attends to
+its neighbours along the order of its own cloud.
+
+* ``norm_rotate``: norms of queries and keys for each head and the rotation by
+  position, in one pass over both.
+* ``window_attention``: softmax attention inside each cloud with a sliding
+  window, a few first rows that stay visible to all (sinks), shared key heads
+  and a learned relative position bias by buckets.  One call serves training
+  (every input but the positions has a gradient), inference over whole clouds
+  and single new rows over cached keys.
+* ``Segments``: the layout of a ragged batch, made once for a batch and used by
+  all of its layers (making it reads the offsets on the host).
+* ``log_buckets``: the bucket map of logarithmic distances.
+
+float32, float16 and bfloat16; scores, softmax, sums and norms are held in
+float32, weights and score gradients of 16-bit inputs are rounded to the input
+type as operands of the tensor cores.  All results are bit-reproducible.
+CUDA tensors only; other tensors raise ``RuntimeError`` after validation.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import _native as N
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_MAX_ENTRIES = 256
+_MAX_REACH = 1024
+
+
+def _ends(value: Tensor, name: str) -> list[int]:
+    if not isinstance(value, Tensor) or value.ndim != 1 or value.dtype not in (torch.int32,
+                                                                                 torch.int64):
+        raise ValueError(f"{name} must be a one-dimensional int32/int64 tensor")
+    return value.tolist()
+
+
+class Segments:
+    """The clouds of a ragged batch.
+
+    ``offset`` holds the inclusive cumulative ends of each cloud's query rows
+    (``[4, 9]`` = rows 0-3 and 4-8), ``key_offset`` those of its key rows when
+    keys are others than the queries' own rows (cached keys, a chunk of new
+    rows).  Query row i of a cloud of Lq query and Lk key rows stands at
+    position ``i + Lk - Lq`` of its keys.  Offsets are read on the host once,
+    here (a synchronisation); the object may be used by any number of calls,
+    on any stream of its device.
+    """
+
+    def __init__(self, offset: Tensor, key_offset: Tensor | None = None):
+        ends = _ends(offset, "offset")
+        key_ends = ends if key_offset is None else _ends(key_offset, "key_offset")
+        if len(ends) != len(key_ends):
+            raise ValueError("offset and key_offset must have the same batch count")
+        if key_offset is not None and key_offset.device != offset.device:
+            raise ValueError("offset and key_offset must be on the same device")
+        self.device = offset.device
+        self.clouds = len(ends)
+        self.rows = ends[-1] if ends else 0
+        self.keys = key_ends[-1] if key_ends else 0
+        self.query_tiles = self._plan(ends, key_ends, 0)
+        self.key_tiles = self._plan(key_ends, ends, 1)
+        self.max_rows = max((b - a for a, b in zip((0, *ends), ends)), default=0)
+        self.max_keys = max((b - a for a, b in zip((0, *key_ends), key_ends)), default=0)
+        self._stream = None
+        if self.device.type == "cuda":
+            # Blocking copies: the tiles are on the device when this returns.
+            self.query_tiles = self.query_tiles.to(self.device)
+            self.key_tiles = self.key_tiles.to(self.device)
+            self._stream = torch.cuda.current_stream(self.device).cuda_stream
+
+    @staticmethod
+    def _plan(own: list[int], other: list[int], keys: int) -> Tensor:
+        n = len(own)
+        a, b = (ctypes.c_int64 * n)(*own), (ctypes.c_int64 * n)(*other)
+        count = N.lib().mpo_attention_plan(a, b, n, keys, None, 0)
+        if count < 0:
+            raise ValueError(N.last_error())
+        tiles = torch.empty((count, 8), dtype=torch.int32)
+        N.lib().mpo_attention_plan(a, b, n, keys, N.ptr(tiles), count)
+        return tiles
+
+    def _use(self) -> None:
+        """Keep the tiles' memory until the work queued now on this stream is done."""
+        stream = torch.cuda.current_stream(self.device)
+        if stream.cuda_stream != self._stream:
+            self.query_tiles.record_stream(stream)
+            self.key_tiles.record_stream(stream)
+
+
+def log_buckets(buckets: int, max_distance: int, bidirectional: bool = True,
+                device: torch.device | str | None = None) -> Tensor:
+    """Bucket of each difference key - query in [-max_distance, max_distance]:
+    an int32 map for ``window_attention(buckets=...)``.
+
+    Of the buckets of one direction the first half holds one distance each, the
+    second half spans logarithmically what is left up to ``max_distance``; all
+    beyond shares the last.  ``bidirectional``: keys ahead of the query have the
+    upper half of the buckets; otherwise they share bucket 0."""
+    if buckets < (4 if bidirectional else 2):
+        raise ValueError("too few buckets")
+    if not 0 < max_distance <= _MAX_REACH:
+        raise ValueError(f"max_distance must be in [1, {_MAX_REACH}]")
+    per_side = buckets // 2 if bidirectional else buckets
+    exact = per_side // 2
+    if max_distance <= exact:
+        raise ValueError("max_distance must exceed half of a direction's buckets")
+    out = []
+    for d in range(-max_distance, max_distance + 1):
+        base = per_side if bidirectional and d > 0 else 0
+        n = abs(d) if bidirectional else max(-d, 0)
+        if n >= exact:
+            step = math.log(n / exact) / math.log(max_distance / exact) * (per_side - exact)
+            n = min(per_side - 1, exact + int(step))
+        out.append(base + n)
+    return torch.tensor(out, dtype=torch.int32, device=device)
+
+
+# ----------------------------------------------------------------------------- checks
+
+def _heads(value: Tensor, name: str, dim: int | None = None) -> None:
+    if not isinstance(value, Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if value.ndim != 3:
+        raise ValueError(f"{name} must have shape (N, heads, D), got {tuple(value.shape)}")
+    if value.dtype not in _DTYPES:
+        raise TypeError(f"{name} must be float32, float16 or bfloat16")
+    if dim is not None and value.shape[2] != dim:
+        raise ValueError(f"{name} must have head size {dim}, got {value.shape[2]}")
+
+
+def _same(value: Tensor, like: Tensor, name: str) -> None:
+    if value.dtype != like.dtype:
+        raise TypeError(f"{name} must be {like.dtype} like q")
+    if value.device != like.device:
+        raise ValueError(f"{name} must be on {like.device}")
+
+
+def _rows(x: Tensor, elements: int) -> Tensor:
+    """``x`` itself where its innermost axis is dense and each row starts on a
+    multiple of ``elements`` elements, else a dense copy."""
+    if (x.stride(2) == 1 and x.stride(0) % elements == 0 and x.stride(1) % elements == 0
+            and x.data_ptr() % (elements * x.element_size()) == 0) or x.numel() == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _dense(x: Tensor | None) -> Tensor | None:
+    """A dense copy of ``x`` unless it is dense and starts on 16 bytes."""
+    if x is None:
+        return None
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
+def _address(x: Tensor | None):
+    return None if x is None else x.data_ptr()
+
+
+# ----------------------------------------------------------------------------- norm and rotation
+
+class _NormRotate(torch.autograd.Function):
+    @staticmethod
+    def _args(q, k, wq, wk, position, freqs, eps, interleaved) -> N.RotateArgs:
+        return N.RotateArgs(
+            q=q.data_ptr(), k=k.data_ptr(), q_row=q.stride(0), q_head=q.stride(1),
+            k_row=k.stride(0), k_head=k.stride(1), q_weight=_address(wq), k_weight=_address(wk),
+            position=_address(position), freqs=_address(freqs), rows=q.shape[0], heads=q.shape[1],
+            kv_heads=k.shape[1], dim=q.shape[2], pairs=0 if freqs is None else freqs.shape[1],
+            axes=0 if freqs is None else freqs.shape[0],
+            position_float=int(position is not None and position.dtype == torch.float32),
+            interleaved=int(interleaved), dtype=_DTYPES[q.dtype], eps=eps)
+
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, position, freqs, eps, interleaved):
+        q, k = _rows(q, 4), _rows(k, 4)
+        out_q = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out_k = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        args = _NormRotate._args(q, k, wq, wk, position, freqs, eps, interleaved)
+        args.out_q, args.out_k = out_q.data_ptr(), out_k.data_ptr()
+        with N.on_device(q.device):
+            N.check(N.lib().mpo_norm_rotate(ctypes.byref(args), N.stream(q.device)), "norm_rotate")
+        ctx.save_for_backward(q, k, wq, wk, position, freqs)
+        ctx.options = (eps, interleaved)
+        return out_q, out_k
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_q, grad_k):
+        q, k, wq, wk, position, freqs = ctx.saved_tensors
+        args = _NormRotate._args(q, k, wq, wk, position, freqs, *ctx.options)
+        grad_q, grad_k = _dense(grad_q), _dense(grad_k)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
+        dwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None
+        args.grad_q, args.grad_k = grad_q.data_ptr(), grad_k.data_ptr()
+        args.out_q, args.out_k = dq.data_ptr(), dk.data_ptr()
+        args.grad_q_weight, args.grad_k_weight = _address(dwq), _address(dwk)
+        with N.on_device(q.device):
+            nbytes = int(N.lib().mpo_norm_rotate_workspace_bytes(ctypes.byref(args)))
+            ws = N.workspace(nbytes, q.device)
+            args.workspace, args.workspace_bytes = _address(ws), nbytes
+            N.check(N.lib().mpo_norm_rotate_backward(ctypes.byref(args), N.stream(q.device)),
+                    "norm_rotate backward")
+        return dq, dk, dwq, dwk, None, None, None, None
+
+
+def norm_rotate(q: Tensor, k: Tensor, position: Tensor | None, freqs: Tensor | None, *,
+                q_weight: Tensor | None = None, k_weight: Tensor | None = None,
+                eps: float = 1e-6, interleaved: bool = False) -> tuple[Tensor, Tensor]:
+    """Root-mean-square norm of each head of q (N, H, D) and k (N, K, D), times
+    ``q_weight`` / ``k_weight`` (D,), then the rotation by position.
+
+    Pair t of the first 2P elements of a head, (t, P + t) or with
+    ``interleaved`` (2t, 2t + 1), turns by ``sum_a position[n, a] * freqs[a, t]``;
+    elements beyond 2P are left as they are.  ``position`` is (N, A) or (N,),
+    integers or float32, A up to 3 (grid coordinates, say, or a row index);
+    ``freqs`` is (A, P) float32, P a multiple of 4.  Both None: no rotation.
+    D is a multiple of 8 up to 256.  q and k may be strided views (of a packed
+    projection); results are dense.  Gradients reach q, k and the weights, not
+    the positions or frequencies.
+    """
+    _heads(q, "q")
+    _heads(k, "k", q.shape[2])
+    _same(k, q, "k")
+    n, dim = q.shape[0], q.shape[2]
+    if k.shape[0] != n:
+        raise ValueError("q and k must have the same row count")
+    if dim % 8 or not 8 <= dim <= 256:
+        raise ValueError("the head size must be a multiple of 8 up to 256")
+    if q.shape[1] < 1 or k.shape[1] < 1:
+        raise ValueError("q and k must have at least one head")
+    if (position is None) != (freqs is None):
+        raise ValueError("position and freqs must be given together")
+    if not (math.isfinite(eps) and eps >= 0):
+        raise ValueError("eps must be finite and not negative")
+    if freqs is not None:
+        if not isinstance(freqs, Tensor) or freqs.ndim != 2 or freqs.dtype != torch.float32:
+            raise ValueError("freqs must be a float32 tensor of shape (A, P)")
+        axes, pairs = freqs.shape
+        if not 1 <= axes <= 3:
+            raise ValueError("freqs must have 1 to 3 axes")
+        if pairs % 4 or 2 * pairs > dim:
+            raise ValueError("freqs must have a multiple of 4 pairs, at most half of the head size")
+        if not isinstance(position, Tensor) or position.dtype not in (torch.int32, torch.int64,
+                                                                      torch.float32):
+            raise ValueError("position must be an int32, int64 or float32 tensor")
+        if position.ndim == 1:
+            position = position.unsqueeze(1)
+        if tuple(position.shape) != (n, axes):
+            raise ValueError(f"position must have shape ({n}, {axes})")
+        if position.device != q.device or freqs.device != q.device:
+            raise ValueError(f"position and freqs must be on {q.device}")
+    weights = []
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            if not isinstance(w, Tensor) or tuple(w.shape) != (dim,) or w.dtype not in _DTYPES:
+                raise ValueError(f"{name} must be a floating-point tensor of shape ({dim},)")
+            if w.device != q.device:
+                raise ValueError(f"{name} must be on {q.device}")
+            w = _dense(w.float())
+        weights.append(w)
+    N.require_cuda(q, "attention.norm_rotate")
+    if freqs is not None:
+        position = position.detach()
+        if position.dtype == torch.int64:
+            position = position.to(torch.int32)
+        position, freqs = position.contiguous(), _dense(freqs.detach())
+        if freqs.shape[1] == 0:
+            position = freqs = None
+    return _NormRotate.apply(q, k, *weights, position, freqs, float(eps), bool(interleaved))
+
+
+# ----------------------------------------------------------------------------- attention
+
+class _Options:
+    """What a call of ``window_attention`` fixes besides its tensors."""
+
+    __slots__ = ("segments", "left", "right", "sinks", "causal", "scale", "qpos", "kpos", "map",
+                 "reach", "train", "want_lse", "precise")
+
+
+def _attention_args(q, k, v, table, o: _Options) -> N.AttentionArgs:
+    seg = o.segments
+    args = N.AttentionArgs(
+        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_row=q.stride(0), q_head=q.stride(1),
+        k_row=k.stride(0), k_head=k.stride(1), v_row=v.stride(0), v_head=v.stride(1),
+        q_tiles=seg.query_tiles.data_ptr(), k_tiles=seg.key_tiles.data_ptr(),
+        q_tile_count=seg.query_tiles.shape[0], k_tile_count=seg.key_tiles.shape[0],
+        q_rows=q.shape[0], k_rows=k.shape[0], heads=q.shape[1], kv_heads=k.shape[1],
+        dim=q.shape[2], dtype=_DTYPES[q.dtype], left=o.left, right=o.right, sinks=o.sinks,
+        causal=o.causal, max_rows=seg.max_rows, max_keys=seg.max_keys, scale=o.scale)
+    if table is not None:
+        args.table, args.table_dtype = table.data_ptr(), _DTYPES[table.dtype]
+        args.axes, args.buckets, args.reach = table.shape[0], table.shape[1], o.reach
+        args.qpos, args.kpos, args.map = o.qpos.data_ptr(), o.kpos.data_ptr(), _address(o.map)
+    return args
+
+
+def _with_workspace(args: N.AttentionArgs, device: torch.device, backward: bool) -> Tensor | None:
+    args.backward = int(backward)
+    nbytes = int(N.lib().mpo_window_attention_workspace_bytes(ctypes.byref(args)))
+    ws = N.workspace(nbytes, device)
+    args.workspace, args.workspace_bytes = _address(ws), nbytes
+    return ws
+
+
+def _forward(q, k, v, table, o: _Options):
+    device = q.device
+    out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    lse = precise = None
+    if o.train or o.want_lse:
+        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=device)
+    if o.precise and q.dtype != torch.float32:
+        precise = torch.empty(q.shape, dtype=torch.float32, device=device)
+    args = _attention_args(q, k, v, table, o)
+    args.out, args.lse, args.out_f32 = out.data_ptr(), _address(lse), _address(precise)
+    with N.on_device(device):
+        ws = _with_workspace(args, device, False)
+        o.segments._use()
+        N.check(N.lib().mpo_window_attention(ctypes.byref(args), N.stream(device)),
+                "window_attention")
+    del ws
+    return out, lse, precise
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, o: _Options):
+        vec = 16 // q.element_size()
+        q, k, v = _rows(q, vec), _rows(k, vec), _rows(v, vec)
+        out, lse, precise = _forward(q, k, v, table, o)
+        ctx.save_for_backward(q, k, v, table, out, lse, precise)
+        ctx.options = o
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, _):
+        q, k, v, table, out, lse, precise = ctx.saved_tensors
+        o = ctx.options
+        device = q.device
+        grad = _dense(grad)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=device)
+        dv = torch.empty(v.shape, dtype=v.dtype, device=device)
+        delta = torch.empty_like(lse)
+        dtable = None
+        if table is not None and ctx.needs_input_grad[3]:
+            dtable = torch.empty(table.shape, dtype=torch.float32, device=device)
+        args = _attention_args(q, k, v, table, o)
+        args.out, args.lse, args.out_f32 = out.data_ptr(), lse.data_ptr(), _address(precise)
+        args.grad_out, args.delta = grad.data_ptr(), delta.data_ptr()
+        args.grad_q, args.grad_k, args.grad_v = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        args.grad_table = _address(dtable)
+        with N.on_device(device):
+            ws = _with_workspace(args, device, True)
+            o.segments._use()
+            N.check(N.lib().mpo_window_attention_backward(ctypes.byref(args), N.stream(device)),
+                    "window_attention backward")
+        del ws
+        if dtable is not None:
+            dtable = dtable.to(table.dtype)
+        return dq, dk, dv, dtable, None
+
+
+def _limit(value, name: str) -> int:
+    if isinstance(value, bool) or not isinstance(value, int):
+        raise ValueError(f"{name} must be an integer")
+    return -1 if value < 0 else min(value, 1 << 30)
+
+
+def _positions(value: Tensor | None, rows: int, axes: int, like: Tensor, name: str) -> Tensor:
+    if not isinstance(value, Tensor) or value.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be an int32 or int64 tensor")
+    if value.ndim == 1:
+        value = value.unsqueeze(1)
+    if tuple(value.shape) != (rows, axes):
+        raise ValueError(f"{name} must have shape ({rows}, {axes}), got {tuple(value.shape)}")
+    if value.device != like.device:
+        raise ValueError(f"{name} must be on {like.device}")
+    return value
+
+
+def window_attention(q: Tensor, k: Tensor, v: Tensor, segments: Segments | Tensor, *,
+                     window: tuple[int, int] = (-1, -1), sinks: int = 0, causal: bool = False,
+                     scale: float | None = None, bias_table: Tensor | None = None,
+                     position: Tensor | None = None, key_position: Tensor | None = None,
+                     buckets: Tensor | None = None,
+                     return_lse: bool = False) -> Tensor | tuple[Tensor, Tensor]:
+    """Attention of q (N, H, D) over k and v (M, K, D) inside each cloud.
+
+    ``segments``: a ``Segments``, or the offset of a self-attention batch.  H is
+    a multiple of K (each K head serves H / K query heads); D is a multiple of
+    8 up to 128.  q, k and v may be strided views of a packed projection.
+
+    Key j of a cloud is visible to its query at position p when
+    ``j < sinks or p - left <= j <= p + right`` (``window = (left, right)``,
+    negative: no limit on that side) and, if ``causal``, ``j <= p``.  A query that
+    sees no key gets zeros.  Scores are ``scale * q.k`` (default 1 / sqrt(D)) plus
+    the bias ``sum_a bias_table[a, bucket_a, h]``: ``position`` (N, A) and
+    ``key_position`` (M, A; default ``position``) are integers below 2^30 in
+    magnitude, ``bias_table`` (A, buckets, H) is learned, and the bucket of an axis
+    is the difference key - query clamped to [-R, R], plus R, where
+    ``buckets = 2 R + 1``; or, with the map ``buckets`` (2 R + 1,), what the map
+    names there (``log_buckets``; names are clamped to the table).  A * buckets
+    is at most 256.
+
+    ``return_lse``: also the logarithm of each row's softmax denominator, (H, N)
+    float32, -inf for a row that sees no key (no gradient through it).
+    Gradients reach q, k, v and bias_table.
+    """
+    _heads(q, "q")
+    _heads(k, "k", q.shape[2])
+    _heads(v, "v", q.shape[2])
+    _same(k, q, "k")
+    _same(v, q, "v")
+    if k.shape != v.shape:
+        raise ValueError("k and v must have the same shape")
+    if q.shape[2] % 8 or not 8 <= q.shape[2] <= 128:
+        raise ValueError("the head size must be a multiple of 8 up to 128")
+    if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
+        raise ValueError("q must have a multiple of k's heads")
+    o = _Options()
+    if not isinstance(window, (tuple, list)) or len(window) != 2:
+        raise ValueError("window must be (left, right)")
+    o.left, o.right = _limit(window[0], "window"), _limit(window[1], "window")
+    if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
+        raise ValueError("sinks must be a nonnegative integer")
+    o.sinks, o.causal = min(sinks, 1 << 30), int(bool(causal))
+    o.scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    if not math.isfinite(o.scale):
+        raise ValueError("scale must be finite")
+    if not isinstance(segments, Segments):
+        segments = Segments(segments)
+    if segments.rows != q.shape[0]:
+        raise ValueError(f"segments must end at q's row count ({q.shape[0]})")
+    if segments.keys != k.shape[0]:
+        raise ValueError(f"segments must end at k's row count ({k.shape[0]})")
+    if segments.device != q.device:
+        raise ValueError(f"segments must be on {q.device}")
+    o.segments = segments
+    o.qpos = o.kpos = o.map = None
+    o.reach = 0
+    if bias_table is None:
+        if position is not None or key_position is not None or buckets is not None:
+            raise ValueError("position, key_position and buckets need a bias_table")
+    else:
+        if not isinstance(bias_table, Tensor) or bias_table.ndim != 3 or \
+                bias_table.dtype not in _DTYPES:
+            raise ValueError("bias_table must be a floating-point tensor of shape (A, buckets, H)")
+        axes, entries, heads = bias_table.shape
+        if heads != q.shape[1] or not 1 <= axes <= 3 or entries < 1:
+            raise ValueError(f"bias_table must have shape (A, buckets, {q.shape[1]}) with A in 1..3")
+        if axes * entries > _MAX_ENTRIES:
+            raise ValueError(f"bias_table must have at most {_MAX_ENTRIES} axes * buckets")
+        if bias_table.device != q.device:
+            raise ValueError(f"bias_table must be on {q.device}")
+        if buckets is not None:
+            if not isinstance(buckets, Tensor) or buckets.ndim != 1 or buckets.dtype != torch.int32:
+                raise ValueError("buckets must be a one-dimensional int32 tensor")
+            if buckets.device != q.device:
+                raise ValueError(f"buckets must be on {q.device}")
+        span = entries if buckets is None else buckets.shape[0]
+        if span % 2 == 0 or span > 2 * _MAX_REACH + 1:
+            raise ValueError("an axis must span 2 R + 1 differences, R at most 1024")
+        o.reach = span // 2
+        o.qpos = _positions(position, q.shape[0], axes, q, "position")
+        if key_position is None:
+            if q.shape[0] != k.shape[0]:
+                raise ValueError("key_position is needed where keys are not the queries' rows")
+            o.kpos = o.qpos
+        else:
+            o.kpos = _positions(key_position, k.shape[0], axes, q, "key_position")
+    N.require_cuda(q, "attention.window_attention")
+    if bias_table is not None:
+        same = o.kpos is o.qpos
+        o.qpos = o.qpos.to(torch.int32).contiguous()
+        o.kpos = o.qpos if same else o.kpos.to(torch.int32).contiguous()
+        o.map = None if buckets is None else buckets.contiguous()
+        bias_table = bias_table.contiguous()
+    grad = torch.is_grad_enabled()
+    o.precise = grad and bias_table is not None and bias_table.requires_grad
+    o.train = grad and (q.requires_grad or k.requires_grad or v.requires_grad or o.precise)
+    o.want_lse = bool(return_lse)
+    if o.train:
+        out, lse = _WindowAttention.apply(q, k, v, bias_table, o)
+    else:
+        vec = 16 // q.element_size()
+        out, lse, _ = _forward(_rows(q, vec), _rows(k, vec), _rows(v, vec), bias_table, o)
+    return (out, lse) if return_lse else out
+
+
+__all__ = ["Segments", "log_buckets", "norm_rotate", "window_attention"]

@@ -1,0 +1,223 @@
+"""Attention of serialised clouds: what runs without a GPU.  Refusals, the tiles
+of a ragged batch, the bucket maps and the checks at the C entries."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from mps_pointops import _native as N
+from mps_pointops import attention
+
+
+def qkv(n=10, m=10, H=4, K=2, D=32, dtype=torch.float32):
+    return (torch.zeros(n, H, D, dtype=dtype), torch.zeros(m, K, D, dtype=dtype),
+            torch.zeros(m, K, D, dtype=dtype))
+
+
+OFF = torch.tensor([4, 10])
+
+
+def call(*tensors, seg=OFF, **kw):
+    return attention.window_attention(*tensors, seg, **kw)
+
+
+def test_cpu_tensors_fail_loudly():
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        call(*qkv())
+    q, k, _ = qkv()
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        attention.norm_rotate(q, k, None, None)
+
+
+def test_attention_refusals():
+    q, k, v = qkv()
+    with pytest.raises(TypeError, match="torch.Tensor"):
+        call([1], k, v)
+    with pytest.raises(ValueError, match="shape"):
+        call(q[0], k, v)
+    with pytest.raises(TypeError, match="float32, float16"):
+        call(q.double(), k, v)
+    with pytest.raises(TypeError, match="like q"):
+        call(q, k.half(), v)
+    with pytest.raises(ValueError, match="head size 32"):
+        call(q, k[..., :16], v)
+    with pytest.raises(ValueError, match="same shape"):
+        call(q, k, v[:, :1])
+    with pytest.raises(ValueError, match="multiple of 8"):
+        call(*(x[..., :12] for x in (q, k, v)))
+    with pytest.raises(ValueError, match="multiple of 8"):
+        call(*qkv(D=136))
+    with pytest.raises(ValueError, match="multiple of k's heads"):
+        call(*qkv(H=3, K=2))
+    with pytest.raises(ValueError, match=r"\(left, right\)"):
+        call(q, k, v, window=5)
+    with pytest.raises(ValueError, match="integer"):
+        call(q, k, v, window=(1.5, 2))
+    with pytest.raises(ValueError, match="sinks"):
+        call(q, k, v, sinks=-1)
+    with pytest.raises(ValueError, match="scale"):
+        call(q, k, v, scale=float("nan"))
+    with pytest.raises(ValueError, match="q's row count"):
+        call(q, k, v, seg=torch.tensor([4, 9]))
+    with pytest.raises(ValueError, match="k's row count"):
+        call(q, k, v, seg=attention.Segments(OFF, torch.tensor([4, 12])))
+
+
+def test_segment_refusals():
+    for bad in (torch.tensor([[1]]), torch.tensor([1.0]), [1, 2]):
+        with pytest.raises(ValueError, match="one-dimensional"):
+            attention.Segments(bad)
+    with pytest.raises(ValueError, match="nondecreasing"):
+        attention.Segments(torch.tensor([5, 3]))
+    with pytest.raises(ValueError, match="nondecreasing"):
+        attention.Segments(torch.tensor([-1, 3]))
+    with pytest.raises(ValueError, match="batch count"):
+        attention.Segments(OFF, torch.tensor([10]))
+    with pytest.raises(ValueError, match="2\\^30"):
+        attention.Segments(torch.tensor([1 << 30]))
+
+
+def test_bias_refusals():
+    q, k, v = qkv()
+    pos = torch.zeros(10, 3, dtype=torch.int32)
+    table = torch.zeros(3, 9, 4)
+    with pytest.raises(ValueError, match="need a bias_table"):
+        call(q, k, v, position=pos)
+    with pytest.raises(ValueError, match="position must be an int32"):
+        call(q, k, v, bias_table=table)
+    with pytest.raises(ValueError, match="position must be an int32"):
+        call(q, k, v, bias_table=table, position=pos.float())
+    with pytest.raises(ValueError, match=r"shape \(10, 3\)"):
+        call(q, k, v, bias_table=table, position=pos[:, :2])
+    with pytest.raises(ValueError, match=r"\(A, buckets, 4\)"):
+        call(q, k, v, bias_table=table[..., :3], position=pos)
+    with pytest.raises(ValueError, match="at most 256"):
+        call(q, k, v, bias_table=torch.zeros(3, 87, 4), position=pos)
+    with pytest.raises(ValueError, match="2 R \\+ 1"):
+        call(q, k, v, bias_table=torch.zeros(3, 8, 4), position=pos)
+    with pytest.raises(ValueError, match="2 R \\+ 1"):
+        call(q, k, v, bias_table=table, position=pos, buckets=torch.zeros(10, dtype=torch.int32))
+    with pytest.raises(ValueError, match="int32"):
+        call(q, k, v, bias_table=table, position=pos, buckets=torch.zeros(11))
+    q2, k2, v2 = qkv(m=12)
+    with pytest.raises(ValueError, match="key_position is needed"):
+        call(q2, k2, v2, seg=attention.Segments(OFF, torch.tensor([6, 12])), bias_table=table,
+             position=pos)
+
+
+def test_norm_rotate_refusals():
+    q, k, _ = qkv()
+    pos, freqs = torch.zeros(10, 1, dtype=torch.int32), torch.zeros(1, 16)
+
+    def refused(match, *args, error=ValueError, **kw):
+        with pytest.raises(error, match=match):
+            attention.norm_rotate(*args, **kw)
+
+    refused("together", q, k, pos, None)
+    refused("row count", q, k[:9], None, None)
+    refused("like q", q, k.half(), None, None, error=TypeError)
+    refused("multiple of 8", q[..., :12], k[..., :12], None, None)
+    refused("float32 tensor", q, k, pos, freqs.double())
+    refused("multiple of 4", q, k, pos, torch.zeros(1, 6))
+    refused("at most half", q, k, pos, torch.zeros(1, 20))
+    refused("1 to 3 axes", q, k, torch.zeros(10, 4, dtype=torch.int32), torch.zeros(4, 16))
+    refused("shape", q, k, pos[:4], freqs)
+    refused("position must be", q, k, pos.double(), freqs)
+    refused("q_weight", q, k, None, None, q_weight=torch.ones(31))
+    refused("k_weight", q, k, None, None, k_weight=torch.ones(32, dtype=torch.int32))
+    refused("eps", q, k, None, None, eps=-1.0)
+
+
+def plan(ends, other, keys):
+    return attention.Segments._plan(ends, other, keys).tolist()
+
+
+def test_tiles_cover_each_row_once():
+    ends, key_ends = [0, 1, 130, 130, 386], [5, 5, 300, 301, 400]
+    tiles = plan(ends, key_ends, 0)
+    covered = []
+    for row, rows, first, other, lq, lk, base, cloud in tiles:
+        assert 1 <= rows <= 128
+        start = 0 if cloud == 0 else ends[cloud - 1]
+        kstart = 0 if cloud == 0 else key_ends[cloud - 1]
+        assert base == start and other == kstart
+        assert lq == ends[cloud] - start and lk == key_ends[cloud] - kstart
+        assert first == row - start + lk - lq
+        covered += range(row, row + rows)
+    assert covered == list(range(386))
+    covered = []
+    for row, rows, first, other, lq, lk, base, cloud in plan(key_ends, ends, 1):
+        assert first == row - base
+        covered += range(row, row + rows)
+    assert covered == list(range(400))
+    assert plan([], [], 0) == []
+
+
+def test_segments_on_cpu():
+    seg = attention.Segments(torch.tensor([3, 3, 200]), torch.tensor([3, 8, 500]))
+    assert (seg.clouds, seg.rows, seg.keys, seg.max_rows, seg.max_keys) == (3, 200, 500, 197, 492)
+    empty = attention.Segments(torch.zeros(0, dtype=torch.int64))
+    assert (empty.clouds, empty.rows, empty.max_rows) == (0, 0, 0)
+
+
+def test_log_buckets():
+    m = attention.log_buckets(8, 16, bidirectional=False)
+    assert m.dtype == torch.int32 and m.numel() == 33
+    at = lambda d: int(m[d + 16])  # noqa: E731
+    assert [at(d) for d in (5, 0, -1, -2, -3)] == [0, 0, 1, 2, 3]
+    # 4 + floor(4 log(n / 4) / log(4)): 4..5 -> 4, 6..7 -> 5, 8..11 -> 6, 12.. -> 7
+    assert [at(-n) for n in (4, 5, 6, 7, 8, 11, 12, 15, 16)] == [4, 4, 5, 5, 6, 6, 7, 7, 7]
+    b = attention.log_buckets(8, 16)
+    assert int(b[16]) == 0 and int(b[15]) == 1 and int(b[17]) == 5
+    assert b.max() == 7 and b.min() == 0
+    for bad in ((2, 16, True), (8, 0, True), (8, 2, True), (8, 5000, True)):
+        with pytest.raises(ValueError):
+            attention.log_buckets(*bad)
+
+
+def test_c_entries_validate_before_device_work():
+    lib = N.lib()
+    a = N.AttentionArgs(heads=4, kv_heads=3, dim=32, scale=1.0)
+    assert lib.mpo_window_attention(ctypes.byref(a), None) == 1
+    assert "multiple of kv_heads" in N.last_error()
+    a = N.AttentionArgs(heads=4, kv_heads=2, dim=20, scale=1.0)
+    assert lib.mpo_window_attention(ctypes.byref(a), None) == 1 and "multiple of 8" in N.last_error()
+    a = N.AttentionArgs(heads=4, kv_heads=2, dim=32, scale=1.0, table=16, axes=3, buckets=100)
+    assert lib.mpo_window_attention(ctypes.byref(a), None) == 1 and "256" in N.last_error()
+    a = N.AttentionArgs(heads=4, kv_heads=2, dim=32, scale=1.0, q_tile_count=1)
+    assert lib.mpo_window_attention(ctypes.byref(a), None) == 1 and "null" in N.last_error()
+    assert lib.mpo_window_attention(None, None) == 1
+    assert lib.mpo_window_attention_backward(None, None) == 1
+    a = N.AttentionArgs(heads=4, kv_heads=2, dim=32, scale=1.0)
+    assert lib.mpo_window_attention(ctypes.byref(a), None) == 0  # nothing to do
+    r = N.RotateArgs(heads=2, kv_heads=2, dim=32, pairs=6, axes=1)
+    assert lib.mpo_norm_rotate(ctypes.byref(r), None) == 1 and "pairs" in N.last_error()
+    r = N.RotateArgs(heads=2, kv_heads=2, dim=32, rows=3)
+    assert lib.mpo_norm_rotate(ctypes.byref(r), None) == 1 and "null" in N.last_error()
+    assert lib.mpo_norm_rotate(None, None) == 1
+
+
+def test_argument_blocks_match_the_header(tmp_path):
+    """Sizes and the last members' offsets of the structures, by the C compiler."""
+    import shutil
+    import subprocess
+
+    from conftest import ROOT
+
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include "mpo_b200.h"\nint main(void){printf("%zu %zu %zu '
+                   '%zu %zu\\n", sizeof(mpo_rotate), offsetof(mpo_rotate, eps), '
+                   'sizeof(mpo_attention), offsetof(mpo_attention, workspace), '
+                   'offsetof(mpo_attention, scale));return 0;}\n')
+    subprocess.run([cc, "-I", str(ROOT / "include"), str(src), "-o", str(tmp_path / "sizes")],
+                   check=True)
+    out = subprocess.run([str(tmp_path / "sizes")], check=True, capture_output=True, text=True)
+    want = [ctypes.sizeof(N.RotateArgs), N.RotateArgs.eps.offset, ctypes.sizeof(N.AttentionArgs),
+            N.AttentionArgs.workspace.offset, N.AttentionArgs.scale.offset]
+    assert [int(x) for x in out.stdout.split()] == want

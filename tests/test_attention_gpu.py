@@ -1,0 +1,464 @@
+"""Attention of serialised clouds on the GPU against its definition in 64 bits
+(bounds: attention_cases.py), at the sizes, masks and layouts where it can go
+wrong."""
+
+from __future__ import annotations
+
+import math
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+
+sys.path.insert(0, str(Path(__file__).resolve().parent))
+
+import attention_cases as C
+from mps_pointops import attention
+from mps_pointops import _native as N
+
+pytestmark = pytest.mark.gpu
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+def ends(lens, device):
+    return torch.tensor(lens, dtype=torch.int64).cumsum(0).to(device)
+
+
+def rand(g, *shape, dtype=FP, scale=1.0):
+    return (torch.randn(*shape, generator=g) * scale).to(dtype)
+
+
+def run(device, dtype, H, K, D, lens, key_lens=None, *, left=-1, right=-1, sinks=0, causal=False,
+        bias=None, reach=7, train=True, scale=None, seed=0, table_dtype=FP, packed=False, edit=None):
+    """Runs one case and checks everything it returns; returns the results."""
+    g = torch.Generator().manual_seed(seed)
+    key_lens = list(lens) if key_lens is None else key_lens
+    nq, nk = sum(lens), sum(key_lens)
+    if packed:
+        rows = rand(g, nq, H + 2 * K, D, dtype=dtype).to(device)
+        q, k, v = rows.split([H, K, K], dim=1)
+    else:
+        q, k, v = (rand(g, *s, dtype=dtype).to(device) for s in ((nq, H, D), (nk, K, D), (nk, K, D)))
+    kw, ref = {}, {}
+    table = None
+    if bias:
+        axes = 3 if bias == "grid" else 1
+        mapping = None
+        if bias == "grid":
+            kpos = torch.randint(-3 * reach, 3 * reach, (nk, 3), generator=g, dtype=torch.int32)
+            entries = 2 * reach + 1
+        else:
+            kpos = torch.cat([torch.arange(n, dtype=torch.int32) for n in key_lens] or
+                             [torch.zeros(0, dtype=torch.int32)])
+            entries, mapping = 16, attention.log_buckets(16, reach, not causal)
+        if key_lens == list(lens):
+            qpos = kpos
+        else:
+            qpos = torch.randint(-5, 60, (nq, axes), generator=g, dtype=torch.int32)
+            kpos = kpos.reshape(nk, axes)
+        table = rand(g, axes, entries, H, scale=0.7, dtype=table_dtype).to(device)
+        kw = dict(position=qpos.to(device), key_position=kpos.to(device),
+                  buckets=None if mapping is None else mapping.to(device))
+        ref = dict(table=table, qpos=qpos, kpos=kpos, mapping=mapping)
+    grad = rand(g, nq, H, D, dtype=dtype).to(device) if train else None
+    if edit:
+        edit(q, k, v, grad, table)
+    seg = attention.Segments(ends(lens, device), ends(key_lens, device))
+    opts = dict(window=(left, right), sinks=sinks, causal=causal, scale=scale)
+    want = C.attention(q, k, v, lens, key_lens, left=left, right=right, sinks=sinks, causal=causal,
+                       scale=scale, grad=grad, **ref)
+    leaves = [x.detach().requires_grad_(train) for x in (q, k, v)]
+    if bias:
+        leaves.append(table.detach().requires_grad_(train))
+        kw["bias_table"] = leaves[3]
+    out, lse = attention.window_attention(*leaves[:3], seg, **opts, **kw, return_lse=True)
+    got = {"out": out, "lse": lse}
+    assert out.dtype == dtype and out.is_contiguous()
+    if train:
+        grads = torch.autograd.grad(out, leaves, grad)
+        got.update(zip(("dq", "dk", "dv", "dtable"), grads))
+    for name in got:
+        w = want[name]
+        if name == "dtable" and table_dtype != FP:
+            w = (w[0], w[1] + C.UNIT[table_dtype] * w[0].abs())
+        # Results below a type's smallest normal number round to its grid.
+        C.check(got[name], w, name, floor=2.0 ** -24 if dtype == HF and name != "lse" else 1e-30)
+    return got
+
+
+LENS = [1, 0, 63, 64, 65, 129, 200]
+
+
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+@pytest.mark.parametrize("D", [8, 16, 24, 32, 64, 80, 128])
+def test_head_sizes(cuda_device, dtype, D):
+    run(cuda_device, dtype, 2, 2, D, LENS, left=40, right=30, sinks=3)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("bias", ["grid", "log"])
+def test_bias(cuda_device, dtype, D, bias):
+    run(cuda_device, dtype, 3, 3, D, LENS, left=70, right=69, sinks=2, bias=bias,
+        reach=7 if bias == "grid" else 50)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("left,right,sinks,causal", [
+    (-1, -1, 0, False), (-1, -1, 0, True), (0, 0, 0, False), (0, 0, 1, True), (5, -1, 0, False),
+    (-1, 7, 2, False), (100, 3, 200, True), (17, 0, 65, True), (1, 2, 1000, False), (300, 300, 0, False)])
+def test_windows(cuda_device, dtype, left, right, sinks, causal):
+    run(cuda_device, dtype, 2, 1, 32, [257, 31, 130], left=left, right=right, sinks=sinks,
+        causal=causal)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+@pytest.mark.parametrize("lens,key_lens", [
+    ([1, 1, 1], [1, 300, 77]), ([5, 2, 8], [64, 2, 500]), ([40, 0, 9], [700, 12, 0]),
+    ([130, 64], [129, 1]), ([300], [50]), ([0, 0], [5, 9]), ([3], [2])])
+@pytest.mark.parametrize("causal", [False, True])
+def test_new_rows_over_other_keys(cuda_device, dtype, lens, key_lens, causal):
+    """Chunks and single rows over longer keys; more queries than keys (rows
+    that see nothing), clouds without keys or queries."""
+    run(cuda_device, dtype, 4, 2, 64, lens, key_lens, causal=causal, left=-1, right=-1)
+    run(cuda_device, dtype, 4, 2, 64, lens, key_lens, causal=causal, left=20, right=4, sinks=2,
+        bias="log", reach=60, seed=1)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("H,K", [(1, 1), (6, 2), (8, 1), (12, 12), (32, 8)])
+def test_shared_heads(cuda_device, dtype, H, K):
+    run(cuda_device, dtype, H, K, 32, [150, 70], left=64, right=63, sinks=1, bias="grid")
+
+
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+@pytest.mark.parametrize("H,K,D", [(8, 8, 64), (32, 8, 128), (5, 5, 24), (10, 1, 80), (16, 1, 16)])
+@pytest.mark.parametrize("new", [1, 3])
+def test_single_rows(cuda_device, dtype, H, K, D, new):
+    keys = [700, 1, 64, 65, 333, 2000]
+    lens = [min(new, n) for n in keys]
+    run(cuda_device, dtype, H, K, D, lens, keys, causal=True, right=0, train=False)
+    run(cuda_device, dtype, H, K, D, lens, keys, causal=True, right=0, left=100, sinks=70,
+        bias="log", reach=128, train=False)
+
+
+def test_empty_batch(cuda_device):
+    got = run(cuda_device, BF, 2, 2, 32, [])
+    assert got["out"].shape == (0, 2, 32)
+    run(cuda_device, BF, 2, 2, 32, [0, 0], bias="grid")
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_packed_and_unaligned_views(cuda_device, dtype):
+    run(cuda_device, dtype, 4, 2, 64, [200, 77], left=50, right=50, packed=True)
+    # Rows that start off 16-byte boundaries, a stride over the elements, a transposed layout.
+    g = torch.Generator().manual_seed(3)
+    lens = [90, 41]
+    base = rand(g, 131, 2, 40, dtype=dtype).to(cuda_device)
+    odd = base[:, :, 3:35]
+    even = rand(g, 131, 2, 64, dtype=dtype).to(cuda_device)[:, :, ::2]
+    swapped = rand(g, 2, 131, 32, dtype=dtype).to(cuda_device).transpose(0, 1)
+    seg = attention.Segments(ends(lens, cuda_device))
+    leaves = [x.detach().requires_grad_() for x in (odd, even, swapped)]
+    out = attention.window_attention(*leaves, seg, window=(20, 20))
+    grad = rand(g, 2, 131, 32, dtype=dtype).to(cuda_device).transpose(0, 1)
+    grads = torch.autograd.grad(out, leaves, grad)
+    want = C.attention(odd, even, swapped, lens, lens, left=20, right=20, grad=grad)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+        C.check(got, want[name], name)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+def test_table_types_and_negative_scale(cuda_device, dtype):
+    run(cuda_device, dtype, 2, 2, 32, [100], bias="grid", table_dtype=BF, scale=-0.3)
+    run(cuda_device, dtype, 2, 2, 32, [100], bias="grid", table_dtype=HF, scale=0.0)
+
+
+def test_large_scores(cuda_device):
+    """Scores of some hundreds: the running maximum carries the sums."""
+    def edit(q, k, v, grad, table):
+        q.mul_(12)
+        k.mul_(4)
+    run(cuda_device, BF, 2, 2, 64, [400], left=200, right=200, edit=edit, train=False)
+    run(cuda_device, FP, 2, 2, 64, [400], left=200, right=200, edit=edit, train=False)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_far_apart_positions(cuda_device, dtype):
+    """Coordinates near the limits of their range clamp, they do not wrap."""
+    g = torch.Generator().manual_seed(5)
+    n = 100
+    big = (1 << 30) - 1
+    pos = torch.tensor([-big, big, 0, 5, -big + 3], dtype=torch.int32)[
+        torch.randint(0, 5, (n, 2), generator=g)]
+    q, k, v = (rand(g, n, 1, 32, dtype=dtype).to(cuda_device) for _ in range(3))
+    table = rand(g, 2, 11, 1).to(cuda_device)
+    out = attention.window_attention(q, k, v, ends([n], cuda_device), bias_table=table,
+                                     position=pos.to(cuda_device))
+    want = C.attention(q, k, v, [n], [n], table=table, qpos=pos, kpos=pos)
+    C.check(out, want["out"], "out")
+
+
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_values_that_a_row_may_not_see(cuda_device, dtype, value):
+    """NaN and infinities in keys, values and gradients of rows outside a
+    query's window, or of other clouds, leave the query's results alone."""
+    lens, D = [100, 150], 32
+    g = torch.Generator().manual_seed(7)
+    q, k, v, grad = (rand(g, 250, 2, D, dtype=dtype).to(cuda_device) for _ in range(4))
+    seg = attention.Segments(ends(lens, cuda_device))
+    opts = dict(window=(10, 10))
+
+    def results(k, v, grad):
+        leaves = [x.detach().clone().requires_grad_() for x in (q, k, v)]
+        out = attention.window_attention(*leaves, seg, **opts)
+        return (out.detach(), *torch.autograd.grad(out, leaves, grad))
+
+    clean = results(k, v, grad)
+    bad_k, bad_v, bad_g = k.clone(), v.clone(), grad.clone()
+    bad_v[60, 0, 5] = value          # seen by queries 50..70 of cloud 0, head 0
+    bad_k[120, 1, 0] = math.nan      # row 20 of cloud 1: seen by its rows 10..30
+    bad_g[200, 0, 3] = value         # row 100 of cloud 1
+    got = results(bad_k, bad_v, bad_g)
+    keep_q = torch.ones(250, 2, dtype=torch.bool)
+    keep_q[50:71, 0] = False
+    keep_q[110:131, 1] = False
+    keep_g = keep_q.clone()
+    keep_g[200, 0] = False
+    keep_kv = torch.ones(250, 2, dtype=torch.bool)
+    keep_kv[40:81, 0] = False        # keys seen by a query that saw the bad value
+    keep_kv[100:141, 1] = False
+    keep_kv[190:211, 0] = False
+    # The touched tiles go row by row through 32-bit sums, so they differ from the tile's
+    # results by what both may be off: twice the bound of 64-bit results.
+    want = C.attention(q, k, v, lens, lens, left=10, right=10, grad=grad)
+    for name, a, b, keep in (("out", clean[0], got[0], keep_q), ("dq", clean[1], got[1], keep_g),
+                             ("dk", clean[2], got[2], keep_kv), ("dv", clean[3], got[3], keep_kv)):
+        a, b = a.cpu().double()[keep], b.cpu().double()[keep]
+        bound = want[name][1][keep]
+        assert torch.isfinite(b).all(), name
+        assert ((a - b).abs() <= 2.04 * bound + 2.0 ** -24).all(), name
+    # What may be seen is seen: element 5 of these queries, and no other element.
+    assert not torch.isfinite(got[0][50:71, 0, 5]).any()
+    other = [d for d in range(D) if d != 5]
+    assert torch.isfinite(got[0][50:71, 0][:, other]).all()
+    assert torch.isnan(got[0][110:131, 1]).all()
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_table_of_minus_infinity(cuda_device, dtype):
+    """A bucket of -inf hides its keys; of the type's lowest number, all but."""
+    g = torch.Generator().manual_seed(9)
+    n = 80
+    q, k, v = (rand(g, n, 1, 16, dtype=dtype).to(cuda_device) for _ in range(3))
+    pos = torch.arange(n, dtype=torch.int32)
+    for low in (-math.inf, torch.finfo(torch.float32).min):
+        table = torch.zeros(1, 7, 1)
+        table[0, 0] = low                # keys three or more behind
+        table[0, 6] = low                # keys three or more ahead
+        table = table.to(cuda_device)
+        out = attention.window_attention(q, k, v, ends([n], cuda_device), bias_table=table,
+                                         position=pos.to(cuda_device))
+        want = C.attention(q, k, v, [n], [n], left=2, right=2)
+        C.check(out, want["out"], "out")
+    table = torch.full((1, 7, 1), -math.inf, device=cuda_device)
+    out, lse = attention.window_attention(q, k, v, ends([n], cuda_device), bias_table=table,
+                                          position=pos.to(cuda_device), return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+def test_results_repeat(cuda_device, dtype):
+    def once():
+        return run(cuda_device, dtype, 4, 2, 64, [500, 1, 260], left=100, right=90, sinks=5,
+                   bias="grid")
+    a, b = once(), once()
+    for name in a:
+        assert torch.equal(a[name], b[name]), name
+
+
+def test_other_stream(cuda_device):
+    """A layout made on one stream used on another, with work queued before it."""
+    g = torch.Generator().manual_seed(11)
+    q, k, v = (rand(g, 300, 2, 64, dtype=BF).to(cuda_device) for _ in range(3))
+    want = C.attention(q, k, v, [300], [300], left=30, right=30)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        seg = attention.Segments(ends([300], cuda_device))
+    third = torch.cuda.Stream()
+    with torch.cuda.stream(third):
+        torch.cuda._sleep(1_000_000)
+        q2, k2, v2 = q * 1, k * 1, v * 1
+        out = attention.window_attention(q2, k2, v2, seg, window=(30, 30))
+        del seg
+    third.synchronize()
+    C.check(out, want["out"], "out")
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_many_queries_see_the_sinks(cuda_device, dtype):
+    """The sinks' gradients gather every query of a long cloud."""
+    run(cuda_device, dtype, 2, 1, 16, [5000, 300], left=8, right=8, sinks=130)
+
+
+@pytest.mark.parametrize("bias", [None, "grid"])
+def test_gradients_against_differences(cuda_device, bias):
+    """Along a random direction, (L(x + h d) - L(x - h d)) / 2h in 64-bit sums of float32
+    results.  L's rounding error is below 2^-22 sum |g o|, divided by 2h; the third
+    derivative's share is h^2 times a quantity of the size of the gradient's."""
+    device, lens = cuda_device, [70, 33]
+    g = torch.Generator().manual_seed(13)
+    n, H, K, D = 103, 4, 2, 16
+    leaves = [rand(g, n, H, D), rand(g, n, K, D), rand(g, n, K, D)]
+    kw = dict(window=(20, 10), sinks=2)
+    if bias:
+        leaves.append(rand(g, 3, 9, H, scale=0.5))
+        kw["position"] = torch.randint(0, 12, (n, 3), generator=g, dtype=torch.int32).to(device)
+    leaves = [x.to(device) for x in leaves]
+    grad = rand(g, n, H, D).to(device)
+    seg = attention.Segments(ends(lens, device))
+
+    def call(xs):
+        extra = {"bias_table": xs[3]} if bias else {}
+        return attention.window_attention(*xs[:3], seg, **kw, **extra)
+
+    xs = [x.clone().requires_grad_() for x in leaves]
+    got = torch.autograd.grad(call(xs), xs, grad)
+    h = 2.0 ** -7
+    for i, x in enumerate(leaves):
+        d = rand(g, *x.shape).to(device)
+        d = d / d.norm()
+
+        def loss(sign):
+            ys = list(leaves)
+            ys[i] = x + sign * h * d
+            o = call(ys).double()
+            return (o * grad.double()).sum().item(), (o * grad.double()).abs().sum().item()
+
+        (up, mag), (down, _) = loss(1), loss(-1)
+        numeric = (up - down) / (2 * h)
+        analytic = (got[i].double() * d.double()).sum().item()
+        size = got[i].double().norm().item()
+        assert abs(numeric - analytic) <= 2.0 ** -20 * mag / (2 * h) + 2 * h * h * size, i
+
+
+# ----------------------------------------------------------------------------- norms and rotation
+
+def rotate_reference(x, w, position, freqs, eps, interleaved, grad):
+    """(y, dx, dw, magnitudes) in 64 bits."""
+    x = x.detach().cpu().double().requires_grad_()
+    w = torch.ones(x.shape[2], dtype=torch.float64) if w is None else w.detach().cpu().double()
+    w = w.clone().requires_grad_()
+    r = (x.square().mean(-1, keepdim=True) + eps).rsqrt()
+    y = x * r * w
+    if freqs is not None:
+        P = freqs.shape[1]
+        theta = (position.cpu().double() @ freqs.cpu().double())[:, None]
+        c, s = theta.cos(), theta.sin()
+        if interleaved:
+            a, b = y[..., 0:2 * P:2], y[..., 1:2 * P:2]
+            y = torch.cat([torch.stack([a * c - b * s, a * s + b * c], -1).flatten(-2),
+                           y[..., 2 * P:]], -1)
+        else:
+            a, b = y[..., :P], y[..., P:2 * P]
+            y = torch.cat([a * c - b * s, a * s + b * c, y[..., 2 * P:]], -1)
+    dx, dw = torch.autograd.grad(y, (x, w), grad.cpu().double())
+    return y.detach(), dx, dw
+
+
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+@pytest.mark.parametrize("n,H,K,D,P,A,interleaved", [
+    (1, 1, 1, 8, 4, 1, False), (1, 32, 8, 128, 64, 1, False), (63, 4, 4, 64, 24, 3, False),
+    (257, 6, 2, 48, 12, 1, True), (100, 3, 1, 24, 12, 2, True), (65, 2, 2, 256, 128, 3, False),
+    (3001, 8, 8, 64, 32, 3, False), (50, 5, 5, 80, 0, 0, False), (40, 2, 1, 16, 4, 2, False)])
+def test_norm_rotate(cuda_device, dtype, n, H, K, D, P, A, interleaved):
+    """Values to a few roundings of float32 and one of the type; weight
+    gradients to n H 2^-24 of the sum of magnitudes."""
+    g = torch.Generator().manual_seed(n + D)
+    packed = rand(g, n, H + K, D, dtype=dtype, scale=2.0).to(cuda_device)
+    q, k = packed[:, :H], packed[:, H:]
+    wq, wk = (1 + 0.3 * rand(g, D)).to(cuda_device), (1 + 0.3 * rand(g, D)).to(cuda_device)
+    pos = freqs = None
+    if P:
+        pos = torch.randint(-100000, 100000, (n, A), generator=g, dtype=torch.int32).to(cuda_device)
+        freqs = torch.rand(A, P, generator=g).to(cuda_device)
+    gq, gk = rand(g, n, H, D, dtype=dtype).to(cuda_device), rand(g, n, K, D, dtype=dtype).to(cuda_device)
+    leaves = [x.detach().requires_grad_() for x in (q, k, wq, wk)]
+    yq, yk = attention.norm_rotate(leaves[0], leaves[1], pos, freqs, q_weight=leaves[2],
+                                   k_weight=leaves[3], interleaved=interleaved)
+    grads = torch.autograd.grad((yq, yk), leaves, (gq, gk))
+    u = C.UNIT[dtype]
+    for x, w, gr, y, dx, dw in ((q, wq, gq, yq, grads[0], grads[2]), (k, wk, gk, yk, grads[1], grads[3])):
+        ry, rdx, rdw = rotate_reference(x, w, pos, freqs, 1e-6, interleaved, gr)
+        size = ry.abs().amax(-1, keepdim=True)
+        floor = 2.0 ** -24 if dtype == HF else 0.0
+        assert ((y.cpu().double() - ry).abs() <= 1.02 * u * ry.abs() + 2.0 ** -20 * size + floor).all()
+        dsize = rdx.abs().amax(-1, keepdim=True) + \
+            gr.cpu().double().abs().amax(-1, keepdim=True) * \
+            x.cpu().double().square().mean(-1, keepdim=True).add(1e-6).rsqrt() * 2
+        assert ((dx.cpu().double() - rdx).abs() <= 1.02 * u * rdx.abs() + 2.0 ** -18 * dsize + floor).all()
+        mag = (gr.cpu().double().abs().amax(-1) * 4).sum() * (2.0 ** -20 + 2.0 ** -24 * 64)
+        assert ((dw.cpu().double() - rdw).abs() <= mag).all()
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_norm_rotate_without_weights_and_odd_views(cuda_device, dtype):
+    g = torch.Generator().manual_seed(2)
+    q = rand(g, 30, 3, 40, dtype=dtype).to(cuda_device)[:, :, 1:33]
+    k = rand(g, 1, 30, 32, dtype=dtype).to(cuda_device).transpose(0, 1)
+    pos = torch.randn(30, generator=g).to(cuda_device)
+    freqs = torch.rand(1, 8, generator=g).to(cuda_device)
+    yq, yk = attention.norm_rotate(q, k, pos, freqs)
+    for x, y in ((q, yq), (k, yk)):
+        ry, _, _ = rotate_reference(x, None, pos[:, None], freqs, 1e-6, False, torch.zeros_like(x))
+        assert ((y.cpu().double() - ry).abs() <= 1.02 * C.UNIT[dtype] * ry.abs() + 2.0 ** -20 * 4).all()
+    a, _ = attention.norm_rotate(q, k, None, None)
+    ra, _, _ = rotate_reference(q, None, None, None, 1e-6, False, torch.zeros_like(q))
+    assert ((a.cpu().double() - ra).abs() <= 1.02 * C.UNIT[dtype] * ra.abs() + 2.0 ** -20 * 4).all()
+
+
+def test_norm_rotate_zero_rows_and_zero_vectors(cuda_device):
+    z = torch.zeros(0, 2, 32, device=cuda_device, requires_grad=True)
+    w = torch.ones(32, device=cuda_device, requires_grad=True)
+    yq, yk = attention.norm_rotate(z, z, None, None, q_weight=w)
+    assert yq.shape == (0, 2, 32)
+    gz, gw = torch.autograd.grad((yq, yk), (z, w), (torch.zeros_like(yq), torch.zeros_like(yk)))
+    assert (gw == 0).all()
+    x = torch.zeros(5, 2, 32, device=cuda_device, requires_grad=True)
+    y, _ = attention.norm_rotate(x, x, None, None)
+    (gx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert (y == 0).all() and torch.isfinite(gx).all()
+
+
+def test_norm_rotate_gradient_against_differences(cuda_device):
+    """As above: rounding 2^-22 sum |g y| / 2h, curvature h^2."""
+    g = torch.Generator().manual_seed(4)
+    leaves = [rand(g, 40, 3, 16), rand(g, 40, 1, 16), 1 + 0.2 * rand(g, 16), 1 + 0.2 * rand(g, 16)]
+    leaves = [x.to(cuda_device) for x in leaves]
+    pos = torch.randint(0, 50, (40, 3), generator=g, dtype=torch.int32).to(cuda_device)
+    freqs = torch.rand(3, 8, generator=g).to(cuda_device)
+    gq, gk = rand(g, 40, 3, 16).to(cuda_device), rand(g, 40, 1, 16).to(cuda_device)
+
+    def call(xs):
+        return attention.norm_rotate(xs[0], xs[1], pos, freqs, q_weight=xs[2], k_weight=xs[3])
+
+    xs = [x.clone().requires_grad_() for x in leaves]
+    got = torch.autograd.grad(call(xs), xs, (gq, gk))
+    h = 2.0 ** -7
+    for i, x in enumerate(leaves):
+        d = rand(g, *x.shape).to(cuda_device)
+        d = d / d.norm()
+        sums = []
+        for sign in (1, -1):
+            ys = list(leaves)
+            ys[i] = x + sign * h * d
+            a, b = call(ys)
+            parts = torch.cat([(a.double() * gq).flatten(), (b.double() * gk).flatten()])
+            sums.append((parts.sum().item(), parts.abs().sum().item()))
+        numeric = (sums[0][0] - sums[1][0]) / (2 * h)
+        analytic = (got[i].double() * d).sum().item()
+        bound = 2.0 ** -20 * sums[0][1] / (2 * h) + 4 * h * h * got[i].double().norm().item()
+        assert abs(numeric - analytic) <= bound, i
