@@ -607,8 +607,11 @@ MPO_API int64_t mpo_attention_plan(const int64_t* ends, const int64_t* other_end
  * grad_k, grad_v dense, overwritten; grad_table (axes, buckets, heads)
  * float32, nullable.  Sums run in a fixed order (bit-reproducible).
  * q_tiles / k_tiles: device copies of mpo_attention_plan's tiles; max_rows the
- * largest Lq and max_keys the largest Lk.  The device reads rows only through
- * the tiles, which must describe these tensors. */
+ * largest Lq, max_keys the largest Lk, clouds the count of clouds; q_rows + k_rows below 2^30.  The
+ * device reads rows only through the tiles, which must describe these tensors.
+ * status (nullable, an int32 that the device can write, pinned host memory for
+ * one): becomes 1 if a bounded wait inside a kernel ran out, in which case the
+ * results are not to be used. */
 typedef struct {
     const void *q, *k, *v;
     int64_t q_row, q_head, k_row, k_head, v_row, v_head; /* strides, elements */
@@ -622,11 +625,12 @@ typedef struct {
     const int32_t *qpos, *kpos;
     const int32_t* map;
     const int32_t *q_tiles, *k_tiles;
+    int32_t* status;
     int64_t q_tile_count, k_tile_count, q_rows, k_rows;
     void* workspace;
     size_t workspace_bytes;
     int32_t heads, kv_heads, dim, dtype, table_dtype, axes, buckets, reach;
-    int32_t left, right, sinks, causal, max_rows, max_keys;
+    int32_t left, right, sinks, causal, max_rows, max_keys, clouds;
     float scale;
     int32_t backward; /* workspace query: 0 forward, 1 backward */
 } mpo_attention;

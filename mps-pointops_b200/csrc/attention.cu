@@ -28,7 +28,8 @@ attn_table_reduce_kernel(const float* __restrict__ partial, int64_t blocks, int 
     }
 }
 
-int partial_blocks_per_tile(const mpo_attention&) { return 2; }
+// Blocks of the query kernel for one planned tile: the 32-bit kernel takes 64 rows.
+int partial_blocks_per_tile(const mpo_attention& a) { return a.dtype == MPO_F32 ? 2 : 1; }
 
 size_t table_partial_bytes(const mpo_attention& a) {
     if (!a.grad_table) return 0;
@@ -45,8 +46,8 @@ int check_attention(const mpo_attention* a, bool backward, const char* what) {
     auto bad = [&](const char* m) { return fail(kInvalidArgument, std::string(what) + ": " + m); };
     if (!a) return bad("null arguments");
     if (a->dtype < MPO_F32 || a->dtype > MPO_BF16) return bad("unknown dtype");
-    if (a->q_rows < 0 || a->k_rows < 0 || a->q_rows >= kFar || a->k_rows >= kFar)
-        return bad("row counts must be in [0, 2^30)");
+    if (a->q_rows < 0 || a->k_rows < 0 || a->q_rows + a->k_rows >= kFar)
+        return bad("rows of queries and keys must be below 2^30 together");
     if (a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads)
         return bad("heads must be a multiple of kv_heads");
     if (a->heads > 65535) return bad("too many heads");
@@ -56,6 +57,7 @@ int check_attention(const mpo_attention* a, bool backward, const char* what) {
     if (a->q_tile_count < 0 || a->k_tile_count < 0 || a->q_tile_count >= kFar ||
         a->k_tile_count >= kFar)
         return bad("bad tile counts");
+    if (a->max_rows < 0 || a->max_keys < 0 || a->clouds < 0) return bad("bad cloud sizes");
     if (!std::isfinite(a->scale)) return bad("scale must be finite");
     if (a->table) {
         if (a->table_dtype < MPO_F32 || a->table_dtype > MPO_BF16) return bad("unknown table dtype");
@@ -96,16 +98,20 @@ AttnArgs derive(const mpo_attention& a) {
     AttnArgs A;
     A.a = a;
     if (!a.table) A.a.axes = A.a.buckets = 0;
-    A.left = a.left < 0 || a.left > kFar ? kFar : a.left;
-    A.right = a.causal ? 0 : (a.right < 0 || a.right > kFar ? kFar : a.right);
+    A.left = a.left < 0 || a.left > kUnlimited ? kUnlimited : a.left;
+    A.right = a.right < 0 || a.right > kUnlimited ? kUnlimited : a.right;
+    if (a.causal) A.right = 0;
+    A.a.sinks = (int)min64(a.sinks, a.max_keys);
     A.group = a.heads / a.kv_heads;
     A.scale_log2 = a.scale * kLog2e;
     return A;
 }
 
-size_t workspace_bytes(const mpo_attention& a, bool backward) {
-    if (backward) return table_partial_bytes(a);
-    return 0;
+// Backward workspace: what the kernels share out (sinks), then the table's partials.
+size_t backward_bytes(const AttnArgs& A) { return A.a.dtype == MPO_F32 ? 0 : attn_tc_backward_bytes(A); }
+
+size_t workspace_bytes(const AttnArgs& A, bool backward) {
+    return backward ? backward_bytes(A) + table_partial_bytes(A.a) : 0;
 }
 
 }  // namespace
@@ -148,15 +154,17 @@ int64_t mpo_attention_plan(const int64_t* ends, const int64_t* other_ends, int64
 
 size_t mpo_window_attention_workspace_bytes(const mpo_attention* args) {
     using namespace mpo;
-    if (!args) return 0;
-    return workspace_bytes(*args, args->backward != 0);
+    if (check_attention(args, false, __func__) != kOk) return 0;
+    return workspace_bytes(derive(*args), args->backward != 0);
 }
 
 int mpo_window_attention(const mpo_attention* args, void* stream) {
     using namespace mpo;
     const int st = check_attention(args, false, __func__);
     if (st != kOk || args->q_tile_count == 0) return st;
-    return attn_simt_forward(derive(*args), (cudaStream_t)stream);
+    const AttnArgs A = derive(*args);
+    cudaStream_t s = (cudaStream_t)stream;
+    return A.a.dtype == MPO_F32 ? attn_simt_forward(A, s) : attn_tc_forward(A, s);
 }
 
 int mpo_window_attention_backward(const mpo_attention* args, void* stream) {
@@ -165,15 +173,15 @@ int mpo_window_attention_backward(const mpo_attention* args, void* stream) {
     if (st != kOk) return st;
     MPO_REQUIRE_WORKSPACE(args->workspace);
     cudaStream_t s = (cudaStream_t)stream;
-    const size_t need = workspace_bytes(*args, true);
+    const AttnArgs A = derive(*args);
+    const size_t need = workspace_bytes(A, true);
     if (need && (!args->workspace || args->workspace_bytes < need))
         return fail(kWorkspaceTooSmall, std::string(__func__) + ": workspace too small");
-    const AttnArgs A = derive(*args);
-    st = attn_simt_backward(A, s);
+    st = A.a.dtype == MPO_F32 ? attn_simt_backward(A, s) : attn_tc_backward(A, s);
     if (st != kOk || !A.a.grad_table) return st;
     const int entries = A.a.axes * A.a.buckets;
     attn_table_reduce_kernel<<<dim3((unsigned)ceil_div(entries, 32), (unsigned)A.a.heads), 256, 0, s>>>(
-        static_cast<const float*>(A.a.workspace),
+        reinterpret_cast<const float*>(static_cast<const unsigned char*>(A.a.workspace) + backward_bytes(A)),
         A.a.q_tile_count * partial_blocks_per_tile(A.a), A.a.heads, entries, A.a.grad_table);
     return check_launch("attn_table_reduce_kernel");
 }

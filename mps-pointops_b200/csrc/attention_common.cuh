@@ -44,17 +44,19 @@ static_assert(sizeof(AttnTile) == 32, "eight 32-bit words per tile");
 // The argument block of the C ABI with what the kernels derive from it.
 struct AttnArgs {
     mpo_attention a;
-    int left, right;  // saturated to a large distance when unlimited; right 0 when causal
+    int left, right;  // kUnlimited where there is none; right 0 when causal
     int group;        // query heads per key head
     float scale_log2; // scale * log2(e)
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+// Rows of queries and keys stay below kFar together, so a position plus or
+// minus the distance that stands for "no limit" reaches every key and fits 32 bits.
 constexpr int kFar = 1 << 30;
+constexpr int kUnlimited = kFar - 2;
 
 __device__ __forceinline__ bool attn_visible(const AttnArgs& A, int p, int j) {
-    // p + right and p - left stay in 32 bits: |p| < 2^30 and the distances are at most 2^30.
     return ((j < A.a.sinks) | ((j >= p - A.left) & (j <= p + A.right))) & (!A.a.causal | (j <= p));
 }
 
@@ -200,6 +202,10 @@ __device__ __forceinline__ float table_entry(const mpo_attention& a, int e, int 
 }
 
 // ---------------------------------------------------------------- launchers
+// attention_tc_fwd.cu, attention_tc_bwd.cu: 16-bit types on the tensor cores.
+int attn_tc_forward(const AttnArgs& A, cudaStream_t s);
+size_t attn_tc_backward_bytes(const AttnArgs& A);
+int attn_tc_backward(const AttnArgs& A, cudaStream_t s);
 // attention_simt.cu: 32-bit arithmetic throughout.
 int attn_simt_forward(const AttnArgs& A, cudaStream_t s);
 int attn_simt_backward(const AttnArgs& A, cudaStream_t s);

@@ -1,4 +1,4 @@
-// Attention of serialised clouds in 32-bit arithmetic (definitions:
+// Attention of serialised clouds for float32 (definitions:
 // attention_common.cuh): tiles of 64 x 64 pairs with fused multiply-adds.
 //
 // 128 threads; thread (ty, tx) = (tid / 16, tid % 16) holds rows 8 ty .. 8 ty + 7
@@ -203,7 +203,7 @@ struct Half {
 
 // ---------------------------------------------------------------- forward
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attn_simt_fwd_kernel(const AttnArgs A) {
+__global__ void __launch_bounds__(kThreads) attn_simt_fwd_kernel(const __grid_constant__ AttnArgs A) {
     extern __shared__ __align__(16) unsigned char smem[];
     const SimtSmem S(smem, DP, 3);
     constexpr int W = DP / 16;
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_fwd_kernel(const AttnArgs 
 
 // ---------------------------------------------------------------- backward: queries
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attn_simt_grad_q_kernel(const AttnArgs A, float* partial) {
+__global__ void __launch_bounds__(kThreads) attn_simt_grad_q_kernel(const __grid_constant__ AttnArgs A, float* partial) {
     extern __shared__ __align__(16) unsigned char smem[];
     const SimtSmem S(smem, DP, 4);
     constexpr int W = DP / 16;
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_q_kernel(const AttnAr
 
 // ---------------------------------------------------------------- backward: keys and values
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const AttnArgs A) {
+__global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __grid_constant__ AttnArgs A) {
     extern __shared__ __align__(16) unsigned char smem[];
     const SimtSmem S(smem, DP, 4);
     constexpr int W = DP / 16;
@@ -539,22 +539,16 @@ int run_bwd(const AttnArgs& A, cudaStream_t s) {
     }
     return st;
 }
-template <typename T>
 int by_dim(const AttnArgs& A, bool backward, cudaStream_t s) {
-    if (A.a.dim <= 16) return backward ? run_bwd<T, 16>(A, s) : run_fwd<T, 16>(A, s);
-    if (A.a.dim <= 32) return backward ? run_bwd<T, 32>(A, s) : run_fwd<T, 32>(A, s);
-    if (A.a.dim <= 64) return backward ? run_bwd<T, 64>(A, s) : run_fwd<T, 64>(A, s);
-    return backward ? run_bwd<T, 128>(A, s) : run_fwd<T, 128>(A, s);
-}
-int by_type(const AttnArgs& A, bool backward, cudaStream_t s) {
-    if (A.a.dtype == MPO_F32) return by_dim<float>(A, backward, s);
-    if (A.a.dtype == MPO_F16) return by_dim<__half>(A, backward, s);
-    return by_dim<__nv_bfloat16>(A, backward, s);
+    if (A.a.dim <= 16) return backward ? run_bwd<float, 16>(A, s) : run_fwd<float, 16>(A, s);
+    if (A.a.dim <= 32) return backward ? run_bwd<float, 32>(A, s) : run_fwd<float, 32>(A, s);
+    if (A.a.dim <= 64) return backward ? run_bwd<float, 64>(A, s) : run_fwd<float, 64>(A, s);
+    return backward ? run_bwd<float, 128>(A, s) : run_fwd<float, 128>(A, s);
 }
 
 }  // namespace
 
-int attn_simt_forward(const AttnArgs& A, cudaStream_t s) { return by_type(A, false, s); }
-int attn_simt_backward(const AttnArgs& A, cudaStream_t s) { return by_type(A, true, s); }
+int attn_simt_forward(const AttnArgs& A, cudaStream_t s) { return by_dim(A, false, s); }
+int attn_simt_backward(const AttnArgs& A, cudaStream_t s) { return by_dim(A, true, s); }
 
 }  // namespace mpo

@@ -1,0 +1,275 @@
+// Tensor-core (tcgen05) pieces of the attention kernels for 16-bit types.
+//
+// Operand tiles are rows of DP elements (the head size rounded up to 16, 32,
+// 64 or 128, zero-filled) in shared memory with the swizzle of their row
+// length: 32, 64 or 128 bytes; DP = 128 is two halves of 64 elements.  One
+// tile serves both ways: as a K-major operand (rows = M or N, elements = K)
+// for scores, and as an MN-major B operand (rows = K, elements = N) for the
+// products with the weights.  Rows are copied with 16-byte cp.async whose
+// source size is 0 past a cloud's end, so no value of another cloud enters a
+// product; a tensor-map copy could only bound the whole tensor.
+#pragma once
+
+#include <string>
+
+#include "attention_common.cuh"
+
+namespace mpo {
+namespace {
+
+constexpr int kTcThreads = 128;  // one thread per row (TMEM lane)
+constexpr int kTcCols = 64;      // columns of a score tile
+constexpr unsigned long long kTcWaitNs = 2000000000ull;
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+    return (uint32_t)__cvta_generic_to_shared(p);
+}
+
+// ---------------------------------------------------------------- barriers
+__device__ __forceinline__ void mbar_init(uint32_t bar) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Wait of at most kTcWaitNs.  A thread whose wait ran out reports it, waits no
+// more and goes on through the same control flow (barriers of the block stay
+// matched, memory accesses do not depend on the data that failed to come).
+struct Waiter {
+    uint32_t bar;
+    uint32_t phase = 0;
+    int32_t* status;
+    bool dead = false;
+    __device__ __forceinline__ Waiter(uint32_t b, int32_t* st) : bar(b), status(st) {}
+    __device__ __forceinline__ void wait() {
+        if (!dead && !mbar_try(bar, phase)) {
+            const unsigned long long t0 = globaltimer_ns();
+            while (!mbar_try(bar, phase))
+                if (globaltimer_ns() - t0 > kTcWaitNs) {
+                    dead = true;
+                    if (status) *status = 1;
+                    break;
+                }
+        }
+        phase ^= 1;
+        __syncwarp();  // the TMEM accesses that follow are warp-wide
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    }
+};
+
+// ---------------------------------------------------------------- TMEM
+__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot),
+                 "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t taddr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// Ties registers that a load fills to the wait before their first use.
+template <int N>
+__device__ __forceinline__ void tmem_use(float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
+}
+__device__ __forceinline__ void tmem_wait_st() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_before() {
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+// 16 consecutive 32-bit columns of this thread's lane; wait before use.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+        : "memory");
+}
+
+// ---------------------------------------------------------------- operands
+template <int DP>
+struct TcTile {
+    static constexpr int kRowBytes = DP * 2 < 128 ? DP * 2 : 128;
+    static constexpr int kHalves = DP * 2 / kRowBytes;
+    static constexpr int kChunks = DP / 8;                    // 16-byte chunks of a row
+    static constexpr int kHalfChunks = kRowBytes / 16;
+    // Layout code of the matrix descriptor: 2 = 128-byte, 4 = 64-byte, 6 = 32-byte swizzle.
+    static constexpr uint64_t kSwizzle = kRowBytes == 128 ? 2 : kRowBytes == 64 ? 4 : 6;
+    static constexpr uint32_t bytes(int rows) { return rows * DP * 2; }
+    // Byte offset of chunk c of row r in a tile of `rows` rows.
+    static __device__ __forceinline__ uint32_t at(int rows, int r, int c) {
+        const int half = c / kHalfChunks, cc = c % kHalfChunks;
+        const int turn = kRowBytes == 128 ? (r & 7) : kRowBytes == 64 ? ((r >> 1) & 3) : ((r >> 2) & 1);
+        return half * rows * kRowBytes + r * kRowBytes + ((cc ^ turn) << 4);
+    }
+    static __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo) {
+        return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
+               ((uint64_t)(8 * kRowBytes >> 4) << 32) | (1ull << 46) | (kSwizzle << 61);
+    }
+    // K-major operand, elements 16 k .. 16 k + 15 of every row.
+    static __device__ __forceinline__ uint64_t k_major(uint32_t tile, int rows, int k) {
+        const int half = k / (kRowBytes / 32), kk = k % (kRowBytes / 32);
+        return desc(tile + half * rows * kRowBytes + kk * 32, 16);
+    }
+    // MN-major operand, rows 16 k .. 16 k + 15, all DP elements.
+    static __device__ __forceinline__ uint64_t mn_major(uint32_t tile, int rows, int k) {
+        return desc(tile + k * 16 * kRowBytes, rows * kRowBytes);
+    }
+};
+
+// Rows [r0, r0 + n) of one head into a tile of ROWS rows, zeros past n and dim.
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void tc_load(uint32_t tile, const void* base, int64_t r0, int n, int h,
+                                        int64_t row_stride, int64_t head_stride, int dim) {
+    using L = TcTile<DP>;
+    const T* src = attn_row<T>(base, r0, h, row_stride, head_stride);
+    constexpr int kPer = ROWS * L::kChunks / kTcThreads;
+    const int c = threadIdx.x % L::kChunks;
+    constexpr int kStep = kTcThreads / L::kChunks;
+    int r = threadIdx.x / L::kChunks;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i, r += kStep) {
+        const bool live = r < n && c * 8 < dim;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tile + L::at(ROWS, r, c)),
+                     "l"(live ? src + r * row_stride + c * 8 : src), "r"(live ? 16 : 0)
+                     : "memory");
+    }
+}
+__device__ __forceinline__ void tc_load_done() {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// kind::f16 (both operands the same 16-bit type), float accumulators, M = 128.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t tc_idesc(int n, bool b_mn) {
+    return (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10)) |
+           (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(0u)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(0u)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+        : "memory");
+}
+// D (128 x NB) = A (128 rows of tile a) . B (NB rows of tile b)^T over DP elements.
+template <typename T, int DP, int NB>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b) {
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k)
+        mma_ss(d, TcTile<DP>::k_major(a, 128, k), TcTile<DP>::k_major(b, NB, k),
+               tc_idesc<T>(NB, false), k > 0);
+}
+// D (128 x DP) += weights (128 x NB, 16-bit pairs in TMEM from column a) . B (NB rows of tile b).
+template <typename T, int DP, int NB>
+__device__ __forceinline__ void mma_weighted(uint32_t d, uint32_t a, uint32_t b, bool acc) {
+#pragma unroll
+    for (int k = 0; k < NB / 16; ++k)
+        mma_ts(d, a + 8 * k, TcTile<DP>::mn_major(b, NB, k), tc_idesc<T>(DP, true), acc || k > 0);
+}
+
+// ---------------------------------------------------------------- masks
+// Bits [lo, hi) of 64.
+__device__ __forceinline__ uint64_t bit_range(int lo, int hi) {
+    lo = max(lo, 0);
+    hi = min(hi, 64);
+    return hi > lo ? (~0ull >> (64 - hi)) & (~0ull << lo) : 0ull;
+}
+// Columns of the key tile [k0, k0 + n) that a query at p sees.
+__device__ __forceinline__ uint64_t seen_keys(const AttnArgs& A, int p, int k0, int n) {
+    uint64_t m = bit_range(p - A.left - k0, p + A.right + 1 - k0) | bit_range(0, A.a.sinks - k0);
+    if (A.a.causal) m &= bit_range(0, p + 1 - k0);
+    return m & bit_range(0, n);
+}
+// Columns of the query tile at positions [p0, p0 + n) that see key j.
+__device__ __forceinline__ uint64_t seeing_queries(const AttnArgs& A, int j, int p0, int n) {
+    uint64_t m = j < A.a.sinks ? ~0ull : bit_range(j - A.right - p0, j + A.left + 1 - p0);
+    if (A.a.causal) m &= bit_range(j - p0, 64);
+    return m & bit_range(0, n);
+}
+
+// ---------------------------------------------------------------- bias
+// The table of a head in shared memory, times log2(e), one copy per lane:
+// entry e of lane l at word 32 e + l.  A lane reads its own bank, so a read
+// costs one wavefront whatever the buckets (one shared copy: about three, for
+// neighbouring points that differ).
+__device__ __forceinline__ void tc_load_table(const AttnArgs& A, float* table, int h) {
+    for (int e = threadIdx.x; e < A.a.axes * A.a.buckets * 32; e += kTcThreads)
+        table[e] = table_entry(A.a, e >> 5, h) * kLog2e;
+}
+// Word offset 32 e of the bucket of one axis (without the lane).
+template <bool MAPPED>
+__device__ __forceinline__ int bucket_word(const AttnArgs& A, int diff) {
+    int c = max(min(diff, A.a.reach), -A.a.reach) + A.a.reach;
+    if (MAPPED) c = min(max(__ldg(A.a.map + c), 0), A.a.buckets - 1);
+    return c << 5;
+}
+// Positions of rows [r0, r0 + n) by axis: dst[axis * 64 + row].
+__device__ __forceinline__ void tc_load_pos(int* dst, const int32_t* pos, int64_t r0, int n, int axes) {
+    if (threadIdx.x < kTcCols)
+        for (int a = 0; a < axes; ++a)
+            dst[a * kTcCols + threadIdx.x] =
+                threadIdx.x < n ? pos[(r0 + threadIdx.x) * axes + a] : 0;
+}
+
+template <typename K>
+int tc_prepare(K kernel, size_t bytes, const char* what) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) !=
+        cudaSuccess)
+        return fail(kCudaError, std::string(what) + ": cannot reserve shared memory");
+    return kOk;
+}
+
+}  // namespace
+}  // namespace mpo

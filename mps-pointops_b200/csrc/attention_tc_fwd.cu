@@ -1,0 +1,289 @@
+// Forward attention of serialised clouds for 16-bit types on the tensor cores
+// (definitions: attention_common.cuh; operands: attention_tc.cuh).
+//
+// A block owns 128 query rows of one head, one thread per row.  It streams the
+// visible key tiles (64 keys) through two shared-memory stages.  Per tile the
+// tensor core forms S = Q K^T into TMEM; a thread reads its row of scores,
+// carries the running maximum and sum of the softmax, writes its weights back
+// over S as 16-bit pairs, and the tensor core adds P V to the rows in TMEM,
+// followed in the same issue by the next tile's S.  The rows in TMEM are
+// rescaled only when a row's maximum grew by more than 2^8 since its last
+// rescale: weights then reach 256, which costs a 16-bit float no precision.
+#include <string>
+
+#include "attention_exact.cuh"
+#include "attention_tc.cuh"
+
+namespace mpo {
+namespace {
+
+// PARTS: 16-bit parts of a weight.  1: its rounding (relative 2^-9 or 2^-12 on
+// average) stays below that of the stored result.  3: exact to float32, for the
+// D = o . do that the table's gradient subtracts from every pair: rounded
+// weights would leave about 2e-3 of that gradient wrong, which is kept in float32.
+template <int DP, int PARTS>
+struct FwdShape {
+    static constexpr int kS = 0, kO = kTcCols;  // TMEM columns
+    static constexpr int kP2 = kO + DP;         // third part (the first two lie over S)
+    static constexpr int kUsed = PARTS == 3 ? kP2 + 32 : kO + DP;
+    static constexpr int kCols = kUsed <= 128 ? 128 : 256;
+    static constexpr int kBlocks = 512 / kCols;
+    static constexpr uint32_t kQ = 0, kK = TcTile<DP>::bytes(128), kStage = TcTile<DP>::bytes(64),
+                              kV = kK + 2 * kStage, kPos = kV + 2 * kStage,
+                              kBar = kPos + 2 * 3 * kTcCols * 4, kTable = kBar + 16;
+    static size_t bytes(int entries) {
+        // At least what keeps more blocks than TMEM serves off an SM (they would wait for it).
+        const size_t need = kTable + (size_t)entries * 128 + 1024;
+        const size_t least = 233472 / (kBlocks + 1);
+        return need > least ? need : least;
+    }
+};
+
+template <typename T, int DP, int BIAS, int PARTS>
+__global__ void __launch_bounds__(kTcThreads, (FwdShape<DP, PARTS>::kBlocks))
+attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
+    using Shape = FwdShape<DP, PARTS>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t sb = smem_u32(smem);
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int h = blockIdx.y, hk = h / A.group;
+    const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.q_tiles)[blockIdx.x];
+    const int p = t.first + tid;
+    int* kpos = reinterpret_cast<int*>(smem + Shape::kPos);
+    float* table = reinterpret_cast<float*>(smem + Shape::kTable);
+    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kBar + 8);
+
+    if (tid < 32) tmem_alloc(smem_u32(slot), Shape::kCols);
+    if (tid == 0) mbar_init(sb + Shape::kBar);
+    const KeySpan span = key_span(A, t.first, t.first + t.rows - 1, t.lk, kTcCols);
+    const int tiles = span.count();
+    auto load_tile = [&](int i) {
+        const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
+        const int64_t row = (int64_t)t.other + k0;
+        const uint32_t stage = (i & 1) * Shape::kStage;
+        tc_load<T, DP, kTcCols>(sb + Shape::kK + stage, A.a.k, row, n, hk, A.a.k_row, A.a.k_head, A.a.dim);
+        tc_load<T, DP, kTcCols>(sb + Shape::kV + stage, A.a.v, row, n, hk, A.a.v_row, A.a.v_head, A.a.dim);
+        if (BIAS) tc_load_pos(kpos + (i & 1) * 3 * kTcCols, A.a.kpos, row, n, A.a.axes);
+    };
+    tc_load<T, DP, 128>(sb + Shape::kQ, A.a.q, t.row, t.rows, h, A.a.q_row, A.a.q_head, A.a.dim);
+    if (tiles > 0) load_tile(0);
+    int qpos[3] = {0, 0, 0};
+    if (BIAS) {
+        tc_load_table(A, table, h);
+        if (tid < t.rows)
+            for (int a = 0; a < A.a.axes; ++a)
+                qpos[a] = A.a.qpos[((int64_t)t.row + tid) * A.a.axes + a];
+    }
+    tc_load_done();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *slot;
+    const uint32_t mine = tmem + ((uint32_t)(tid & ~31) << 16);  // this warp's lanes
+    Waiter done(sb + Shape::kBar, A.a.status);
+    if (tid == 0 && tiles > 0) {
+        mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kQ, sb + Shape::kK);
+        mma_commit(sb + Shape::kBar);
+    }
+
+    // Running maximum in units of s2 = S * mul + bias (log2), as of the last rescale.
+    float top = -INFINITY, sum = 0.f;
+    const float mul = BIAS ? 1.f : (A.scale_log2 > 0.f ? A.scale_log2 : 1.f);
+    for (int i = 0; i < tiles; ++i) {
+        done.wait();
+        if (i + 1 < tiles) load_tile(i + 1);
+        float s[kTcCols];
+#pragma unroll
+        for (int c = 0; c < kTcCols; c += 16) tmem_ld16(mine + Shape::kS + c, s + c);
+        tmem_wait_ld();
+        tmem_use(s);
+        const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
+        if (BIAS) {
+            const int* kp = kpos + (i & 1) * 3 * kTcCols;
+#pragma unroll
+            for (int c = 0; c < kTcCols; ++c) s[c] *= A.scale_log2;
+            for (int a = 0; a < A.a.axes; ++a) {
+                const float* tab = table + (a * A.a.buckets * 32 + lane);
+                const int q = qpos[a];
+#pragma unroll
+                for (int c = 0; c < kTcCols; c += 4) {
+                    const int4 k4 = *reinterpret_cast<const int4*>(kp + a * kTcCols + c);
+                    s[c] += tab[bucket_word<BIAS == 2>(A, k4.x - q)];
+                    s[c + 1] += tab[bucket_word<BIAS == 2>(A, k4.y - q)];
+                    s[c + 2] += tab[bucket_word<BIAS == 2>(A, k4.z - q)];
+                    s[c + 3] += tab[bucket_word<BIAS == 2>(A, k4.w - q)];
+                }
+            }
+        } else if (!(A.scale_log2 > 0.f)) {
+#pragma unroll
+            for (int c = 0; c < kTcCols; ++c) s[c] *= A.scale_log2;
+        }
+        if (n < kTcCols || !all_visible(A, t.first, t.first + t.rows - 1, k0, k0 + kTcCols - 1)) {
+            const uint64_t seen = seen_keys(A, p, k0, n);
+            const uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+                s[c] = (lo >> c) & 1u ? s[c] : -INFINITY;
+                s[c + 32] = (hi >> c) & 1u ? s[c + 32] : -INFINITY;
+            }
+        }
+        float m[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int c = 4; c < kTcCols; c += 4) {
+            m[0] = fmaxf(m[0], s[c]);
+            m[1] = fmaxf(m[1], s[c + 1]);
+            m[2] = fmaxf(m[2], s[c + 2]);
+            m[3] = fmaxf(m[3], s[c + 3]);
+        }
+        const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+        // (most - top) is NaN only when both are the same infinity: no growth.
+        const bool grow = (most - top) * mul > 8.f;
+        if (__any_sync(FULL_MASK, grow)) {
+            float f = 1.f;
+            if (grow) {
+                f = exp2_sfu((top - most) * mul);
+                top = most;
+                sum *= f;
+            }
+            if (i > 0) {
+#pragma unroll
+                for (int c = 0; c < DP; c += 16) {
+                    float o[16];
+                    tmem_ld16(mine + Shape::kO + c, o);
+                    tmem_wait_ld();
+                    tmem_use(o);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[e] *= f;
+                    tmem_st16(mine + Shape::kO + c, reinterpret_cast<const uint32_t*>(o));
+                }
+            }
+        }
+        const float ref = top == -INFINITY ? 0.f : -top * mul;
+        f32x2 part[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+        const f32x2 mul2v = pack2(mul, mul), ref2 = pack2(ref, ref);
+#pragma unroll
+        for (int c = 0; c < kTcCols; c += 16) {
+            uint32_t w[3][8];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                float a, b;
+                unpack2(fma2(pack2(s[c + e], s[c + e + 1]), mul2v, ref2), a, b);
+                a = exp2_sfu(a);
+                b = exp2_sfu(b);
+                part[(e >> 1) & 1] = add2(part[(e >> 1) & 1], pack2(a, b));
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) {
+                    w[q][e / 2] = Elem<T>::two(a, b);
+                    if (q + 1 < PARTS) {
+                        float r[2];
+                        Elem<T>::two(w[q][e / 2], r);
+                        a -= r[0];
+                        b -= r[1];
+                    }
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q)
+                tmem_st8(mine + (q == 2 ? Shape::kP2 : Shape::kS + 32 * q) + c / 2, w[q]);
+        }
+        {
+            float a, b;
+            unpack2(add2(part[0], part[1]), a, b);
+            sum += a + b;
+        }
+        tmem_wait_st();
+        tc_load_done();
+        tc_fence_before();
+        __syncthreads();
+        if (tid == 0) {
+            tc_fence_after();
+            const uint32_t stage = (i & 1) * Shape::kStage;
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q)
+                mma_weighted<T, DP, kTcCols>(tmem + Shape::kO,
+                                             tmem + (q == 2 ? Shape::kP2 : Shape::kS + 32 * q),
+                                             sb + Shape::kV + stage, i > 0 || q > 0);
+            // Issued after P V and executed in order after it: S may overwrite the weights.
+            if (i + 1 < tiles)
+                mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kQ,
+                                           sb + Shape::kK + (Shape::kStage - stage));
+            mma_commit(sb + Shape::kBar);
+        }
+    }
+    if (tiles > 0) done.wait();
+    bool nan = false;
+    const bool live = tid < t.rows;
+    const int64_t at = (((int64_t)t.row + tid) * A.a.heads + h) * A.a.dim;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int c = 0; c < DP; c += 16) {
+        float o[16];
+        if (tiles > 0) {
+            tmem_ld16(mine + Shape::kO + c, o);
+            tmem_wait_ld();
+            tmem_use(o);
+        }
+        if (!live) continue;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            o[e] = sum == 0.f ? (isnan(o[e]) && tiles > 0 ? o[e] : 0.f) : o[e] * inv;
+            nan |= isnan(o[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e += 8) {
+            if (c + e >= A.a.dim) continue;
+            *reinterpret_cast<uint4*>(static_cast<T*>(A.a.out) + at + c + e) = Elem<T>::pack(o + e);
+            if (A.a.out_f32) {
+                float4* dst = reinterpret_cast<float4*>(A.a.out_f32 + at + c + e);
+                dst[0] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                dst[1] = make_float4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]);
+            }
+        }
+    }
+    if (live && A.a.lse)
+        A.a.lse[(int64_t)h * A.a.q_rows + t.row + tid] =
+            sum == 0.f ? -INFINITY : fmaf(top * mul, kLn2, logf(sum));
+    __syncwarp();
+    for (unsigned bad = __ballot_sync(FULL_MASK, nan); bad; bad &= bad - 1) {
+        const int r = (tid & ~31) + __ffs(bad) - 1;
+        exact_forward_row<T>(A, (int64_t)t.row + r, t.first + r, t.other, t.lk, h);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (tid < 32) {
+        tc_fence_after();
+        tmem_free(tmem, Shape::kCols);
+    }
+}
+
+template <typename T, int DP, int BIAS, int PARTS>
+int run(const AttnArgs& A, cudaStream_t s) {
+    const size_t bytes = FwdShape<DP, PARTS>::bytes(BIAS ? A.a.axes * A.a.buckets : 0);
+    const int st = tc_prepare(attn_tc_fwd_kernel<T, DP, BIAS, PARTS>, bytes, "attn_tc_fwd_kernel");
+    if (st != kOk) return st;
+    const dim3 grid((unsigned)A.a.q_tile_count, (unsigned)A.a.heads);
+    attn_tc_fwd_kernel<T, DP, BIAS, PARTS><<<grid, kTcThreads, bytes, s>>>(A);
+    return check_launch("attn_tc_fwd_kernel");
+}
+template <typename T, int DP>
+int by_bias(const AttnArgs& A, cudaStream_t s) {
+    if (!A.a.table) return run<T, DP, 0, 1>(A, s);
+    if (A.a.map) return A.a.out_f32 ? run<T, DP, 2, 3>(A, s) : run<T, DP, 2, 1>(A, s);
+    return A.a.out_f32 ? run<T, DP, 1, 3>(A, s) : run<T, DP, 1, 1>(A, s);
+}
+template <typename T>
+int by_dim(const AttnArgs& A, cudaStream_t s) {
+    if (A.a.dim <= 16) return by_bias<T, 16>(A, s);
+    if (A.a.dim <= 32) return by_bias<T, 32>(A, s);
+    if (A.a.dim <= 64) return by_bias<T, 64>(A, s);
+    return by_bias<T, 128>(A, s);
+}
+
+}  // namespace
+
+int attn_tc_forward(const AttnArgs& A, cudaStream_t s) {
+    return A.a.dtype == MPO_F16 ? by_dim<__half>(A, s) : by_dim<__nv_bfloat16>(A, s);
+}
+
+}  // namespace mpo

@@ -286,6 +286,23 @@ def norm_rotate(q: Tensor, k: Tensor, position: Tensor | None, freqs: Tensor | N
 
 # ----------------------------------------------------------------------------- attention
 
+_statuses: dict[int, Tensor] = {}
+
+
+def _status(device: torch.device) -> Tensor:
+    """The word that a kernel on ``device`` sets when a bounded wait runs out, in
+    pinned host memory: read here without waiting for the GPU."""
+    key = device.index if device.index is not None else torch.cuda.current_device()
+    word = _statuses.get(key)
+    if word is None:
+        word = _statuses[key] = torch.zeros(1, dtype=torch.int32).pin_memory()
+    elif word[0] != 0:
+        word.zero_()
+        raise RuntimeError("mps_pointops: a wait inside an earlier window_attention kernel ran out; "
+                           "its results are not valid")
+    return word
+
+
 class _Options:
     """What a call of ``window_attention`` fixes besides its tensors."""
 
@@ -302,7 +319,7 @@ def _attention_args(q, k, v, table, o: _Options) -> N.AttentionArgs:
         q_tile_count=seg.query_tiles.shape[0], k_tile_count=seg.key_tiles.shape[0],
         q_rows=q.shape[0], k_rows=k.shape[0], heads=q.shape[1], kv_heads=k.shape[1],
         dim=q.shape[2], dtype=_DTYPES[q.dtype], left=o.left, right=o.right, sinks=o.sinks,
-        causal=o.causal, max_rows=seg.max_rows, max_keys=seg.max_keys, scale=o.scale)
+        status=_status(q.device).data_ptr(), causal=o.causal, max_rows=seg.max_rows, max_keys=seg.max_keys, clouds=seg.clouds, scale=o.scale)
     if table is not None:
         args.table, args.table_dtype = table.data_ptr(), _DTYPES[table.dtype]
         args.axes, args.buckets, args.reach = table.shape[0], table.shape[1], o.reach
