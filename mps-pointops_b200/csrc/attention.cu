@@ -111,7 +111,8 @@ AttnArgs derive(const mpo_attention& a) {
 size_t backward_bytes(const AttnArgs& A) { return A.a.dtype == MPO_F32 ? 0 : attn_tc_backward_bytes(A); }
 
 size_t workspace_bytes(const AttnArgs& A, bool backward) {
-    return backward ? backward_bytes(A) + table_partial_bytes(A.a) : 0;
+    if (backward) return backward_bytes(A) + table_partial_bytes(A.a);
+    return A.a.q_tile_count && attn_rows_eligible(A) ? attn_rows_workspace(A) : 0;
 }
 
 }  // namespace
@@ -164,6 +165,13 @@ int mpo_window_attention(const mpo_attention* args, void* stream) {
     if (st != kOk || args->q_tile_count == 0) return st;
     const AttnArgs A = derive(*args);
     cudaStream_t s = (cudaStream_t)stream;
+    if (attn_rows_eligible(A)) {
+        MPO_REQUIRE_WORKSPACE(args->workspace);
+        const size_t need = attn_rows_workspace(A);
+        if (need && (!args->workspace || args->workspace_bytes < need))
+            return fail(kWorkspaceTooSmall, std::string(__func__) + ": workspace too small");
+        return attn_rows_forward(A, s);
+    }
     return A.a.dtype == MPO_F32 ? attn_simt_forward(A, s) : attn_tc_forward(A, s);
 }
 

@@ -206,6 +206,10 @@ __device__ __forceinline__ float table_entry(const mpo_attention& a, int e, int 
 int attn_tc_forward(const AttnArgs& A, cudaStream_t s);
 size_t attn_tc_backward_bytes(const AttnArgs& A);
 int attn_tc_backward(const AttnArgs& A, cudaStream_t s);
+// attention_rows.cu: few query rows per cloud.
+bool attn_rows_eligible(const AttnArgs& A);
+size_t attn_rows_workspace(const AttnArgs& A);
+int attn_rows_forward(const AttnArgs& A, cudaStream_t s);
 // attention_simt.cu: 32-bit arithmetic throughout.
 int attn_simt_forward(const AttnArgs& A, cudaStream_t s);
 int attn_simt_backward(const AttnArgs& A, cudaStream_t s);

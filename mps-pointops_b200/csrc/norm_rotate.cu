@@ -10,9 +10,9 @@
 // Bound by HBM: the forward reads and writes q and k once, the backward reads
 // x and its gradient and writes dx.  A warp owns one row (or, when rows are
 // few, a share of one row's heads), so the angles of a row are formed once for
-// all of its heads; `lanes` = dim / 8 rounded up to a power of two serve one
-// head, each holding the two halves of four pairs as two vectors of four, so
-// the rotation needs no exchange and the sums one butterfly.  Angles: position
+// all of its heads, one pair per lane; `lanes` = dim / 8 rounded up to a power
+// of two serve one head, each holding the two halves of four pairs as two
+// vectors of four, so the rotation needs no exchange and the sums one butterfly.  Angles: position
 // x frequency / pi is summed in double and reduced to one turn there (positions
 // of 10^5 would cost a float sum 2 decimal digits), then sincospif.
 #include <string>
@@ -24,6 +24,7 @@ namespace {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotWarps = kRotThreads / 32;
+constexpr int kFwdBlocksPerSm = 3, kBwdBlocksPerSm = 2;  // resident, by registers
 
 template <typename T>
 struct Four;  // four consecutive elements as one vector
@@ -61,133 +62,221 @@ struct Four<__nv_bfloat16> {
     }
 };
 
-// How a lane's eight elements sit in a head, and its angles.
+// How a lane's eight elements sit in a head.
 struct Lane {
     int lo, hi;    // first element of each vector of four
     bool live;     // chunk inside the head
     bool turns;    // elements that rotate
-    float c[4], s[4];
     __device__ __forceinline__ Lane(const mpo_rotate& a, int chunk) {
         live = chunk * 8 < a.dim;
         turns = live && chunk * 4 < a.pairs;
         lo = (turns && !a.interleaved) ? chunk * 4 : chunk * 8;
         hi = (turns && !a.interleaved) ? a.pairs + chunk * 4 : chunk * 8 + 4;
     }
-    // Cosine and sine of the lane's four pairs at `row`.
-    __device__ __forceinline__ void angles(const mpo_rotate& a, int chunk, int64_t row) {
-        if (!turns) return;
-        double t[4] = {0., 0., 0., 0.};
-        for (int ax = 0; ax < a.axes; ++ax) {
-            const int64_t at = row * a.axes + ax;
-            const double p = a.position_float ? (double)static_cast<const float*>(a.position)[at]
-                                              : (double)static_cast<const int32_t*>(a.position)[at];
-            const float4 f = *reinterpret_cast<const float4*>(a.freqs + (int64_t)ax * a.pairs + chunk * 4);
-            t[0] = fma(p, (double)f.x, t[0]);
-            t[1] = fma(p, (double)f.y, t[1]);
-            t[2] = fma(p, (double)f.z, t[2]);
-            t[3] = fma(p, (double)f.w, t[3]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const double half_turns = t[i] * 0.31830988618379067154;  // / pi
-            const double whole = 2.0 * rint(half_turns * 0.5);
-            sincospif((float)(half_turns - whole), &s[i], &c[i]);
-        }
-    }
-    // Turn the lane's pairs by theta (sign 1) or -theta (sign -1).
-    __device__ __forceinline__ void turn(float (&x)[8], bool interleaved, float sign) const {
-        if (!turns) return;
-        if (interleaved) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) rotate(x[2 * i], x[2 * i + 1], c[i], sign * s[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) rotate(x[i], x[4 + i], c[i], sign * s[i]);
-        }
-    }
-    static __device__ __forceinline__ void rotate(float& u, float& v, float c, float s) {
-        const float a = fmaf(u, c, -__fmul_rn(v, s)), b = fmaf(u, s, __fmul_rn(v, c));
-        u = a;
-        v = b;
-    }
 };
 
+// Eight elements as packed pairs.  Where they rotate, v[0], v[1] hold the first
+// halves of the lane's four pairs and v[2], v[3] the second halves.
+struct Eight {
+    f32x2 v[4];
+};
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, const Lane& L, float (&x)[8]) {
-    using F = Four<T>;
-    F::get(*reinterpret_cast<const typename F::V*>(p + L.lo), x);
-    F::get(*reinterpret_cast<const typename F::V*>(p + L.hi), x + 4);
+struct Raw {  // eight elements as loaded
+    typename Four<T>::V lo, hi;
+};
+template <typename T>
+__device__ __forceinline__ Raw<T> load_raw(const T* p, const Lane& L) {
+    Raw<T> r;
+    r.lo = *reinterpret_cast<const typename Four<T>::V*>(p + L.lo);
+    r.hi = *reinterpret_cast<const typename Four<T>::V*>(p + L.hi);
+    return r;
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const Lane& L, const float (&x)[8]) {
-    using F = Four<T>;
-    *reinterpret_cast<typename F::V*>(p + L.lo) = F::put(x);
-    *reinterpret_cast<typename F::V*>(p + L.hi) = F::put(x + 4);
-}
-__device__ __forceinline__ void load_weight(const float* w, const Lane& L, float (&x)[8]) {
+__device__ __forceinline__ Eight unpack(const Raw<T>& r, bool interleaved) {
+    float x[8];
+    Four<T>::get(r.lo, x);
+    Four<T>::get(r.hi, x + 4);
+    Eight e;
+    if (interleaved) {
+        e.v[0] = pack2(x[0], x[2]);
+        e.v[1] = pack2(x[4], x[6]);
+        e.v[2] = pack2(x[1], x[3]);
+        e.v[3] = pack2(x[5], x[7]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 1.f;
-    if (w && L.live) load8<float>(w, L, x);
+        for (int i = 0; i < 4; ++i) e.v[i] = pack2(x[2 * i], x[2 * i + 1]);
+    }
+    return e;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const Lane& L, const Eight& e, bool interleaved) {
+    float x[8];
+    if (interleaved) {
+        unpack2(e.v[0], x[0], x[2]);
+        unpack2(e.v[1], x[4], x[6]);
+        unpack2(e.v[2], x[1], x[3]);
+        unpack2(e.v[3], x[5], x[7]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) unpack2(e.v[i], x[2 * i], x[2 * i + 1]);
+    }
+    *reinterpret_cast<typename Four<T>::V*>(p + L.lo) = Four<T>::put(x);
+    *reinterpret_cast<typename Four<T>::V*>(p + L.hi) = Four<T>::put(x + 4);
+}
+// Weights of q and k in shared memory, by chunk in the order of an Eight (ones
+// where none is given).
+__device__ __forceinline__ void stage_weights(const mpo_rotate& a, float (&w)[2][32][8], int lanes) {
+    for (int t = threadIdx.x; t < 2 * lanes; t += kRotThreads) {
+        const int which = t / lanes, chunk = t - which * lanes;
+        const Lane L(a, chunk);
+        const float* src = which ? a.k_weight : a.q_weight;
+        float x[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+        if (src && L.live) {
+            Four<float>::get(*reinterpret_cast<const float4*>(src + L.lo), x);
+            Four<float>::get(*reinterpret_cast<const float4*>(src + L.hi), x + 4);
+        }
+        const bool il = a.interleaved && L.turns;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[which][chunk][il ? (i & 1) * 4 + (i >> 1) : i] = x[i];
+    }
+}
+__device__ __forceinline__ Eight read_weight(const float* w) {
+    const float4 lo = reinterpret_cast<const float4*>(w)[0], hi = reinterpret_cast<const float4*>(w)[1];
+    Eight e;
+    e.v[0] = pack2(lo.x, lo.y);
+    e.v[1] = pack2(lo.z, lo.w);
+    e.v[2] = pack2(hi.x, hi.y);
+    e.v[3] = pack2(hi.z, hi.w);
+    return e;
+}
+__device__ __forceinline__ float pair_sum(f32x2 a, f32x2 b) {
+    float x, y;
+    unpack2(add2(a, b), x, y);
+    return x + y;
+}
+__device__ __forceinline__ float dot8(const Eight& a, const Eight& b) {
+    const f32x2 p = fma2(a.v[2], b.v[2], mul2(a.v[0], b.v[0]));
+    const f32x2 q = fma2(a.v[3], b.v[3], mul2(a.v[1], b.v[1]));
+    return pair_sum(p, q);
 }
 __device__ __forceinline__ float lanes_sum(float v, int lanes) {
     for (int o = lanes >> 1; o; o >>= 1) v += __shfl_xor_sync(FULL_MASK, v, o);
     return v;
 }
+__device__ __forceinline__ f32x2 neg2(f32x2 a) { return a ^ 0x8000000080000000ull; }
+
+// Cosines and sines of the lane's four pairs.
+struct Turn {
+    f32x2 c[2], s[2];
+    // (u, v) -> (u c - v s, u s + v c); back: by -theta.
+    __device__ __forceinline__ void apply(Eight& e, bool back) const {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const f32x2 sn = back ? neg2(s[i]) : s[i];
+            const f32x2 u = e.v[i], v = e.v[2 + i];
+            e.v[i] = fma2(u, c[i], neg2(mul2(v, sn)));
+            e.v[2 + i] = fma2(u, sn, mul2(v, c[i]));
+        }
+    }
+};
+// The angles of a row: each lane forms those of pairs lane, lane + 32, .., and
+// the warp shares them through `cs` (cosines, then sines, kMaxPairs each).
+constexpr int kMaxPairs = 128;
+__device__ __forceinline__ void row_angles(const mpo_rotate& a, int64_t row, float* cs) {
+    double pos[kAttnMaxAxes];
+#pragma unroll
+    for (int ax = 0; ax < kAttnMaxAxes; ++ax)
+        if (ax < a.axes) {
+            const int64_t at = row * a.axes + ax;
+            pos[ax] = a.position_float ? (double)static_cast<const float*>(a.position)[at]
+                                       : (double)static_cast<const int32_t*>(a.position)[at];
+        }
+    __syncwarp();  // the previous row's angles have been read
+    for (int t = threadIdx.x & 31; t < a.pairs; t += 32) {
+        double theta = 0.;
+#pragma unroll
+        for (int ax = 0; ax < kAttnMaxAxes; ++ax)
+            if (ax < a.axes) theta = fma(pos[ax], (double)a.freqs[ax * a.pairs + t], theta);
+        const double half_turns = theta * 0.31830988618379067154;  // / pi
+        const double whole = 2.0 * rint(half_turns * 0.5);
+        sincospif((float)(half_turns - whole), cs + kMaxPairs + t, cs + t);
+    }
+    __syncwarp();
+}
+__device__ __forceinline__ Turn read_turn(const float* cs, int chunk) {
+    const float4 c = *reinterpret_cast<const float4*>(cs + 4 * chunk);
+    const float4 s = *reinterpret_cast<const float4*>(cs + kMaxPairs + 4 * chunk);
+    Turn t;
+    t.c[0] = pack2(c.x, c.y);
+    t.c[1] = pack2(c.z, c.w);
+    t.s[0] = pack2(s.x, s.y);
+    t.s[1] = pack2(s.z, s.w);
+    return t;
+}
 
 // Units of work: (row, share of the row's q and k heads); a warp takes units
-// in grid strides.  A share's heads are consecutive, `step` = 32 / lanes of
-// them at a time, U rounds of loads in flight.
+// in grid strides.  A round serves 32 / lanes heads; U rounds of loads are in
+// flight, as loaded (packed), and the first of them go out before the row's
+// angles are formed.
 template <typename T, int U>
-__global__ void __launch_bounds__(kRotThreads)
+__global__ void __launch_bounds__(kRotThreads, kFwdBlocksPerSm)
 norm_rotate_kernel(const mpo_rotate a, int lanes, int shares) {
+    __shared__ __align__(16) float angles[kRotWarps][2 * kMaxPairs];
+    __shared__ __align__(16) float weights[2][32][8];
+    float* cs = angles[threadIdx.x >> 5];
     const int lane = threadIdx.x & 31, chunk = lane & (lanes - 1), sub = lane / lanes;
     const int step = 32 / lanes, total = a.heads + a.kv_heads;
     const int rounds = (total + step - 1) / step;
-    Lane L(a, chunk);
-    float wq[8], wk[8];
-    load_weight(a.q_weight, L, wq);
-    load_weight(a.k_weight, L, wk);
+    const Lane L(a, chunk);
+    const bool il = a.interleaved && L.turns;
+    stage_weights(a, weights, lanes);
+    __syncthreads();
     const float inv = 1.f / (float)a.dim;
     const int64_t units = a.rows * shares;
     for (int64_t u = (int64_t)blockIdx.x * kRotWarps + (threadIdx.x >> 5); u < units;
          u += (int64_t)gridDim.x * kRotWarps) {
-        const int64_t row = u / shares;
-        const int share = (int)(u - row * shares);
-        const int r0 = (int)((int64_t)rounds * share / shares);
-        const int r1 = (int)((int64_t)rounds * (share + 1) / shares);
-        float x[U][8];
-        auto fetch = [&](int r, float (&v)[8]) {
+        const int64_t row = shares == 1 ? u : u / shares;
+        int r0 = 0, r1 = rounds;
+        if (shares > 1) {
+            const int share = (int)(u - row * shares);
+            r0 = rounds * share / shares;
+            r1 = rounds * (share + 1) / shares;
+        }
+        const T* q = static_cast<const T*>(a.q) + row * a.q_row;
+        const T* k = static_cast<const T*>(a.k) + row * a.k_row;
+        T* oq = static_cast<T*>(a.out_q) + row * a.heads * a.dim;
+        T* ok = static_cast<T*>(a.out_k) + row * a.kv_heads * a.dim;
+        Raw<T> raw[U] = {};
+        auto fetch = [&](int r) {
             const int h = r * step + sub;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.f;
             if (L.live && r < r1 && h < total)
-                load8<T>(h < a.heads ? attn_row<T>(a.q, row, h, a.q_row, a.q_head)
-                                     : attn_row<T>(a.k, row, h - a.heads, a.k_row, a.k_head),
-                         L, v);
+                return load_raw<T>(h < a.heads ? q + h * a.q_head : k + (h - a.heads) * a.k_head, L);
+            return Raw<T>{};
         };
 #pragma unroll
-        for (int i = 0; i < U; ++i) fetch(r0 + i, x[i]);
-        L.angles(a, chunk, row);  // while the first loads are in flight
+        for (int i = 0; i < U; ++i) raw[i] = fetch(r0 + i);
+        Turn turn;
+        if (a.pairs) {
+            row_angles(a, row, cs);
+            if (L.turns) turn = read_turn(cs, chunk);
+        }
         for (int r = r0; r < r1; r += U) {
 #pragma unroll
             for (int i = 0; i < U; ++i) {
                 if (r + i < r1) {  // uniform over the warp
                     const int h = (r + i) * step + sub;
-                    float ss = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) ss = fmaf(x[i][e], x[i][e], ss);
-                    ss = lanes_sum(ss, lanes);
-                    const float rs = rsqrtf(fmaf(ss, inv, a.eps));
                     const bool is_q = h < a.heads;
+                    Eight x = unpack<T>(raw[i], il);
+                    raw[i] = fetch(r + i + U);
+                    const float ss = lanes_sum(dot8(x, x), lanes);
+                    const float rs = rsqrtf(fmaf(ss, inv, a.eps));
+                    const f32x2 rs2 = pack2(rs, rs);
+                    const Eight w = read_weight(weights[is_q ? 0 : 1][chunk]);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[i][e] = x[i][e] * rs * (is_q ? wq[e] : wk[e]);
-                    L.turn(x[i], a.interleaved, 1.f);
+                    for (int e = 0; e < 4; ++e) x.v[e] = mul2(mul2(x.v[e], rs2), w.v[e]);
+                    if (L.turns) turn.apply(x, false);
                     if (L.live && h < total)
-                        store8<T>(is_q ? attn_row<T>(a.out_q, row, h, (int64_t)a.heads * a.dim, a.dim)
-                                       : attn_row<T>(a.out_k, row, h - a.heads,
-                                                     (int64_t)a.kv_heads * a.dim, a.dim),
-                                  L, x[i]);
-                    fetch(r + i + U, x[i]);
+                        store8<T>(is_q ? oq + h * a.dim : ok + (h - a.heads) * a.dim, L, x, il);
                 }
             }
         }
@@ -197,86 +286,111 @@ norm_rotate_kernel(const mpo_rotate a, int lanes, int shares) {
 // Backward.  A lane keeps the weight gradients of its eight elements over all
 // of its units; the block's warps and head slots join in shared memory in a
 // fixed order and each block writes one partial (2, dim) row.
-template <typename T>
-__global__ void __launch_bounds__(kRotThreads)
+template <typename T, int U>
+__global__ void __launch_bounds__(kRotThreads, kBwdBlocksPerSm)
 norm_rotate_bwd_kernel(const mpo_rotate a, int lanes, int shares, float* __restrict__ partial) {
+    __shared__ __align__(16) union {
+        float angles[kRotWarps][2 * kMaxPairs];
+        float sums[kRotWarps][32][17];
+    } sh;
+    __shared__ __align__(16) float weights[2][32][8];
+    float* cs = sh.angles[threadIdx.x >> 5];
     const int lane = threadIdx.x & 31, chunk = lane & (lanes - 1), sub = lane / lanes;
     const int step = 32 / lanes, total = a.heads + a.kv_heads;
     const int rounds = (total + step - 1) / step;
-    Lane L(a, chunk);
-    float wq[8], wk[8], gq[8], gk[8];
-    load_weight(a.q_weight, L, wq);
-    load_weight(a.k_weight, L, wk);
+    const Lane L(a, chunk);
+    const bool il = a.interleaved && L.turns;
+    stage_weights(a, weights, lanes);
+    __syncthreads();
+    Eight gq, gk;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) gq[e] = gk[e] = 0.f;
+    for (int e = 0; e < 4; ++e) gq.v[e] = gk.v[e] = pack2(0.f, 0.f);
     const float inv = 1.f / (float)a.dim;
     const int64_t units = a.rows * shares;
-    const int64_t q_dense = (int64_t)a.heads * a.dim, k_dense = (int64_t)a.kv_heads * a.dim;
     for (int64_t u = (int64_t)blockIdx.x * kRotWarps + (threadIdx.x >> 5); u < units;
          u += (int64_t)gridDim.x * kRotWarps) {
-        const int64_t row = u / shares;
-        const int share = (int)(u - row * shares);
-        const int r0 = (int)((int64_t)rounds * share / shares);
-        const int r1 = (int)((int64_t)rounds * (share + 1) / shares);
-        float x[8], g[8];
-        auto fetch = [&](int r) {
+        const int64_t row = shares == 1 ? u : u / shares;
+        int r0 = 0, r1 = rounds;
+        if (shares > 1) {
+            const int share = (int)(u - row * shares);
+            r0 = rounds * share / shares;
+            r1 = rounds * (share + 1) / shares;
+        }
+        const T* q = static_cast<const T*>(a.q) + row * a.q_row;
+        const T* k = static_cast<const T*>(a.k) + row * a.k_row;
+        const int64_t dq = row * a.heads * a.dim, dk = row * a.kv_heads * a.dim;
+        const T* gyq = static_cast<const T*>(a.grad_q) + dq;
+        const T* gyk = static_cast<const T*>(a.grad_k) + dk;
+        Raw<T> rx[U] = {}, rg[U] = {};
+        auto fetch = [&](int r, Raw<T>& x, Raw<T>& g) {
             const int h = r * step + sub;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = g[i] = 0.f;
+            x = Raw<T>{};
+            g = Raw<T>{};
             if (L.live && r < r1 && h < total) {
-                if (h < a.heads) {
-                    load8<T>(attn_row<T>(a.q, row, h, a.q_row, a.q_head), L, x);
-                    load8<T>(attn_row<T>(a.grad_q, row, h, q_dense, a.dim), L, g);
-                } else {
-                    load8<T>(attn_row<T>(a.k, row, h - a.heads, a.k_row, a.k_head), L, x);
-                    load8<T>(attn_row<T>(a.grad_k, row, h - a.heads, k_dense, a.dim), L, g);
-                }
+                const bool is_q = h < a.heads;
+                const int hk = h - a.heads;
+                x = load_raw<T>(is_q ? q + h * a.q_head : k + hk * a.k_head, L);
+                g = load_raw<T>(is_q ? gyq + h * a.dim : gyk + hk * a.dim, L);
             }
         };
-        fetch(r0);
-        L.angles(a, chunk, row);
-        for (int r = r0; r < r1; ++r) {
-            const int h = r * step + sub;
-            const bool is_q = h < a.heads;
-            float y[8], b[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                y[e] = x[e];
-                b[e] = g[e];
-            }
-            fetch(r + 1);
-            L.turn(b, a.interleaved, -1.f);
-            float ss = 0.f, hx = 0.f;
+        for (int i = 0; i < U; ++i) fetch(r0 + i, rx[i], rg[i]);
+        Turn turn;
+        if (a.pairs) {
+            row_angles(a, row, cs);
+            if (L.turns) turn = read_turn(cs, chunk);
+        }
+        for (int r = r0; r < r1; r += U) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                ss = fmaf(y[e], y[e], ss);
-                hx = fmaf(__fmul_rn(b[e], is_q ? wq[e] : wk[e]), y[e], hx);
-            }
-            ss = lanes_sum(ss, lanes);
-            hx = lanes_sum(hx, lanes);
-            const float rs = rsqrtf(fmaf(ss, inv, a.eps));
-            const float back = hx * inv * rs * rs * rs;
+            for (int i = 0; i < U; ++i) {
+                if (r + i < r1) {
+                    const int h = (r + i) * step + sub;
+                    const bool is_q = h < a.heads;
+                    Eight y = unpack<T>(rx[i], il), b = unpack<T>(rg[i], il), hw;
+                    fetch(r + i + U, rx[i], rg[i]);
+                    if (L.turns) turn.apply(b, true);
+                    const Eight w = read_weight(weights[is_q ? 0 : 1][chunk]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float dw = __fmul_rn(b[e], __fmul_rn(y[e], rs));
-                if (h < total) {
-                    if (is_q) gq[e] += dw;
-                    else gk[e] += dw;
+                    for (int e = 0; e < 4; ++e) hw.v[e] = mul2(b.v[e], w.v[e]);
+                    const float ss = lanes_sum(dot8(y, y), lanes);
+                    const float hx = lanes_sum(dot8(hw, y), lanes);
+                    const float rs = rsqrtf(fmaf(ss, inv, a.eps));
+                    const float back = -(hx * inv * rs * rs * rs);
+                    const f32x2 rs2 = pack2(rs, rs), back2 = pack2(back, back);
+                    if (h < total) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const f32x2 xr = mul2(y.v[e], rs2);
+                            if (is_q) gq.v[e] = fma2(b.v[e], xr, gq.v[e]);
+                            else gk.v[e] = fma2(b.v[e], xr, gk.v[e]);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y.v[e] = fma2(y.v[e], back2, mul2(rs2, hw.v[e]));
+                    if (L.live && h < total)
+                        store8<T>(is_q ? static_cast<T*>(a.out_q) + dq + h * a.dim
+                                       : static_cast<T*>(a.out_k) + dk + (h - a.heads) * a.dim,
+                                  L, y, il);
                 }
-                y[e] = fmaf(-y[e], back, __fmul_rn(rs, __fmul_rn(b[e], is_q ? wq[e] : wk[e])));
             }
-            if (L.live && h < total)
-                store8<T>(is_q ? attn_row<T>(a.out_q, row, h, q_dense, a.dim)
-                               : attn_row<T>(a.out_k, row, h - a.heads, k_dense, a.dim),
-                          L, y);
         }
     }
     if (!partial) return;
-    __shared__ float sums[kRotWarps][32][17];
+    __syncthreads();
+    // Sums slot e < 8: q, else k; within a weight: lo's four elements, then hi's.
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        sums[threadIdx.x >> 5][lane][e] = gq[e];
-        sums[threadIdx.x >> 5][lane][8 + e] = gk[e];
+    for (int which = 0; which < 2; ++which) {
+        const Eight& g = which ? gk : gq;
+        float* dst = &sh.sums[threadIdx.x >> 5][lane][8 * which];
+        if (il) {
+            unpack2(g.v[0], dst[0], dst[2]);
+            unpack2(g.v[1], dst[4], dst[6]);
+            unpack2(g.v[2], dst[1], dst[3]);
+            unpack2(g.v[3], dst[5], dst[7]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) unpack2(g.v[e], dst[2 * e], dst[2 * e + 1]);
+        }
     }
     __syncthreads();
     // Element e of chunk c: over the warps, then the head slots.
@@ -285,27 +399,29 @@ norm_rotate_bwd_kernel(const mpo_rotate a, int lanes, int shares, float* __restr
         if (c * 8 >= a.dim) continue;
         float v = 0.f;
         for (int w = 0; w < kRotWarps; ++w)
-            for (int sl = 0; sl < step; ++sl) v += sums[w][sl * lanes + c][e];
+            for (int sl = 0; sl < step; ++sl) v += sh.sums[w][sl * lanes + c][e];
         const Lane at(a, c);
         const int el = (e & 7) < 4 ? at.lo + (e & 3) : at.hi + (e & 3);
         partial[((int64_t)blockIdx.x * 2 + (e >> 3)) * a.dim + el] = v;
     }
 }
 
-// grad_weight[d] = sum of the blocks' partials in block order (8 strided runs,
-// then their sum).
-__global__ void __launch_bounds__(256)
+// grad_weight[d] = sum of the blocks' partials: 32 strided runs in block order,
+// then theirs.
+__global__ void __launch_bounds__(1024)
 norm_weight_reduce_kernel(const float* __restrict__ partial, int blocks, int dim,
                           float* __restrict__ gq, float* __restrict__ gk) {
-    __shared__ float run[8][33];
+    __shared__ float run[32][33];
     const int col = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
     float v = 0.f;
-    if (col < 2 * dim)
-        for (int b = part; b < blocks; b += 8) v += partial[(int64_t)b * 2 * dim + col];
+    if (col < 2 * dim) {
+#pragma unroll 4
+        for (int b = part; b < blocks; b += 32) v += partial[(int64_t)b * 2 * dim + col];
+    }
     run[part][threadIdx.x & 31] = v;
     __syncthreads();
     if (part == 0 && col < 2 * dim) {
-        for (int i = 1; i < 8; ++i) v += run[i][threadIdx.x & 31];
+        for (int i = 1; i < 32; ++i) v += run[i][threadIdx.x & 31];
         float* out = col < dim ? gq : gk;
         if (out) out[col < dim ? col : col - dim] = v;
     }
@@ -320,8 +436,8 @@ struct RotateGrid {
     int lanes, shares;
     unsigned blocks;
 };
-// At most 8 blocks of 8 warps per SM (its 64 warps); rows are shared out over
-// several warps when there are fewer rows than half of those warps.
+// As many blocks as are resident at once; a row's heads are shared out over
+// several warps when there are fewer rows than half of the resident warps.
 RotateGrid rotate_grid(const mpo_rotate& a, int per_sm) {
     RotateGrid g;
     g.lanes = rotate_lanes(a.dim);
@@ -332,8 +448,6 @@ RotateGrid rotate_grid(const mpo_rotate& a, int per_sm) {
                                         (int64_t)sm_count() * per_sm));
     return g;
 }
-constexpr int kBwdBlocksPerSm = 4;
-
 bool vec_ok(const void* p, int64_t row, int64_t head, int dtype) {
     const uintptr_t bytes = dtype == MPO_F32 ? 16 : 8;
     return aligned_to(p, bytes) && row % 4 == 0 && head % 4 == 0;
@@ -369,19 +483,21 @@ int check_rotate(const mpo_rotate* a, bool backward, const char* what) {
 
 template <typename T>
 int run_rotate(const mpo_rotate& a, cudaStream_t s) {
-    const RotateGrid g = rotate_grid(a, 8);
-    norm_rotate_kernel<T, 2><<<g.blocks, kRotThreads, 0, s>>>(a, g.lanes, g.shares);
+    constexpr int kDepth = sizeof(T) == 2 ? 4 : 2;
+    const RotateGrid g = rotate_grid(a, kFwdBlocksPerSm);
+    norm_rotate_kernel<T, kDepth><<<g.blocks, kRotThreads, 0, s>>>(a, g.lanes, g.shares);
     return check_launch("norm_rotate_kernel");
 }
 template <typename T>
 int run_rotate_bwd(const mpo_rotate& a, cudaStream_t s) {
+    constexpr int kDepth = sizeof(T) == 2 ? 4 : 2;
     const RotateGrid g = rotate_grid(a, kBwdBlocksPerSm);
     const bool weights = a.grad_q_weight || a.grad_k_weight;
     float* partial = weights ? static_cast<float*>(a.workspace) : nullptr;
-    norm_rotate_bwd_kernel<T><<<g.blocks, kRotThreads, 0, s>>>(a, g.lanes, g.shares, partial);
+    norm_rotate_bwd_kernel<T, kDepth><<<g.blocks, kRotThreads, 0, s>>>(a, g.lanes, g.shares, partial);
     int st = check_launch("norm_rotate_bwd_kernel");
     if (st != kOk || !weights) return st;
-    norm_weight_reduce_kernel<<<(unsigned)ceil_div(2 * a.dim, 32), 256, 0, s>>>(
+    norm_weight_reduce_kernel<<<(unsigned)ceil_div(2 * a.dim, 32), 1024, 0, s>>>(
         partial, (int)g.blocks, a.dim, a.grad_q_weight, a.grad_k_weight);
     return check_launch("norm_weight_reduce_kernel");
 }

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -36,6 +37,20 @@ _sz = ctypes.c_size_t
 
 def _fields(*groups):
     return [(name, kind) for kind, names in groups for name in names.split()]
+
+
+def packer(block: type[ctypes.Structure]):
+    """A function that packs values, in field order, into the bytes of ``block``:
+    one call instead of one attribute store per field (None is a null pointer)."""
+    codes = {_vp: "P", _i64: "q", _sz: "N", _i32: "i", _f32: "f"}
+    layout = struct.Struct("".join(codes[kind] for _, kind in block._fields_))
+    assert layout.size == ctypes.sizeof(block) or ctypes.sizeof(block) - layout.size < 8
+    pad = b"\0" * (ctypes.sizeof(block) - layout.size)
+
+    def pack(*values) -> bytes:
+        return layout.pack(*values) + pad
+
+    return pack
 
 
 class RotateArgs(ctypes.Structure):

@@ -92,12 +92,13 @@ class Segments:
         N.lib().mpo_attention_plan(a, b, n, keys, N.ptr(tiles), count)
         return tiles
 
-    def _use(self) -> None:
-        """Keep the tiles' memory until the work queued now on this stream is done."""
-        stream = torch.cuda.current_stream(self.device)
-        if stream.cuda_stream != self._stream:
-            self.query_tiles.record_stream(stream)
-            self.key_tiles.record_stream(stream)
+    def _use(self, stream: int) -> None:
+        """Keep the tiles' memory until the work queued now on this stream, the
+        current one, is done."""
+        if stream != self._stream:
+            current = torch.cuda.current_stream(self.device)
+            self.query_tiles.record_stream(current)
+            self.key_tiles.record_stream(current)
 
 
 def log_buckets(buckets: int, max_distance: int, bidirectional: bool = True,
@@ -165,56 +166,70 @@ def _dense(x: Tensor | None) -> Tensor | None:
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
-def _address(x: Tensor | None):
-    return None if x is None else x.data_ptr()
+def _address(x: Tensor | None) -> int:
+    return 0 if x is None else x.data_ptr()
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 # ----------------------------------------------------------------------------- norm and rotation
 
-class _NormRotate(torch.autograd.Function):
-    @staticmethod
-    def _args(q, k, wq, wk, position, freqs, eps, interleaved) -> N.RotateArgs:
-        return N.RotateArgs(
-            q=q.data_ptr(), k=k.data_ptr(), q_row=q.stride(0), q_head=q.stride(1),
-            k_row=k.stride(0), k_head=k.stride(1), q_weight=_address(wq), k_weight=_address(wk),
-            position=_address(position), freqs=_address(freqs), rows=q.shape[0], heads=q.shape[1],
-            kv_heads=k.shape[1], dim=q.shape[2], pairs=0 if freqs is None else freqs.shape[1],
-            axes=0 if freqs is None else freqs.shape[0],
-            position_float=int(position is not None and position.dtype == torch.float32),
-            interleaved=int(interleaved), dtype=_DTYPES[q.dtype], eps=eps)
+_pack_rotate = N.packer(N.RotateArgs)
 
+
+def _rotate_call(backward: bool, q, k, wq, wk, position, freqs, eps, interleaved, out_q, out_k,
+                 grad_q=None, grad_k=None, grad_wq=None, grad_wk=None) -> None:
+    device = q.device
+
+    def pack(ws, nbytes):
+        return _pack_rotate(
+            q.data_ptr(), k.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+            _address(grad_q), _address(grad_k), out_q.data_ptr(), out_k.data_ptr(), _address(wq),
+            _address(wk), _address(grad_wq), _address(grad_wk), _address(position),
+            _address(freqs), _address(ws), nbytes, q.shape[0], q.shape[1], k.shape[1], q.shape[2],
+            0 if freqs is None else freqs.shape[1], 0 if freqs is None else freqs.shape[0],
+            int(position is not None and position.dtype == torch.float32), int(interleaved),
+            _DTYPES[q.dtype], eps, 0)
+
+    with N.on_device(device):
+        lib = N.lib()
+        if not backward:
+            N.check(lib.mpo_norm_rotate(pack(None, 0), _stream(device)), "norm_rotate")
+            return
+        nbytes = int(lib.mpo_norm_rotate_workspace_bytes(pack(None, 0)))
+        ws = N.workspace(nbytes, device)
+        N.check(lib.mpo_norm_rotate_backward(pack(ws, nbytes), _stream(device)),
+                "norm_rotate backward")
+
+
+def _rotate_forward(q, k, *rest):
+    out_q = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out_k = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    _rotate_call(False, q, k, *rest, out_q, out_k)
+    return out_q, out_k
+
+
+class _NormRotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, position, freqs, eps, interleaved):
         q, k = _rows(q, 4), _rows(k, 4)
-        out_q = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        out_k = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        args = _NormRotate._args(q, k, wq, wk, position, freqs, eps, interleaved)
-        args.out_q, args.out_k = out_q.data_ptr(), out_k.data_ptr()
-        with N.on_device(q.device):
-            N.check(N.lib().mpo_norm_rotate(ctypes.byref(args), N.stream(q.device)), "norm_rotate")
         ctx.save_for_backward(q, k, wq, wk, position, freqs)
         ctx.options = (eps, interleaved)
-        return out_q, out_k
+        return _rotate_forward(q, k, wq, wk, position, freqs, eps, interleaved)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_q, grad_k):
         q, k, wq, wk, position, freqs = ctx.saved_tensors
-        args = _NormRotate._args(q, k, wq, wk, position, freqs, *ctx.options)
         grad_q, grad_k = _dense(grad_q), _dense(grad_k)
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
         dwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
         dwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None
-        args.grad_q, args.grad_k = grad_q.data_ptr(), grad_k.data_ptr()
-        args.out_q, args.out_k = dq.data_ptr(), dk.data_ptr()
-        args.grad_q_weight, args.grad_k_weight = _address(dwq), _address(dwk)
-        with N.on_device(q.device):
-            nbytes = int(N.lib().mpo_norm_rotate_workspace_bytes(ctypes.byref(args)))
-            ws = N.workspace(nbytes, q.device)
-            args.workspace, args.workspace_bytes = _address(ws), nbytes
-            N.check(N.lib().mpo_norm_rotate_backward(ctypes.byref(args), N.stream(q.device)),
-                    "norm_rotate backward")
+        _rotate_call(True, q, k, wq, wk, position, freqs, *ctx.options, dq, dk, grad_q, grad_k,
+                     dwq, dwk)
         return dq, dk, dwq, dwk, None, None, None, None
 
 
@@ -281,26 +296,30 @@ def norm_rotate(q: Tensor, k: Tensor, position: Tensor | None, freqs: Tensor | N
         position, freqs = position.contiguous(), _dense(freqs.detach())
         if freqs.shape[1] == 0:
             position = freqs = None
-    return _NormRotate.apply(q, k, *weights, position, freqs, float(eps), bool(interleaved))
+    args = (*weights, position, freqs, float(eps), bool(interleaved))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or any(
+            w is not None and w.requires_grad for w in weights)):
+        return _NormRotate.apply(q, k, *args)
+    return _rotate_forward(_rows(q, 4), _rows(k, 4), *args)
 
 
 # ----------------------------------------------------------------------------- attention
 
-_statuses: dict[int, Tensor] = {}
+_statuses: dict[int, tuple[Tensor, ctypes.c_int32]] = {}
 
 
-def _status(device: torch.device) -> Tensor:
-    """The word that a kernel on ``device`` sets when a bounded wait runs out, in
-    pinned host memory: read here without waiting for the GPU."""
-    key = device.index if device.index is not None else torch.cuda.current_device()
-    word = _statuses.get(key)
-    if word is None:
-        word = _statuses[key] = torch.zeros(1, dtype=torch.int32).pin_memory()
-    elif word[0] != 0:
-        word.zero_()
+def _status(device: torch.device) -> int:
+    """Address of the word that a kernel on ``device`` sets when a bounded wait runs
+    out; it lies in pinned host memory and is read here without waiting for the GPU."""
+    entry = _statuses.get(device.index)
+    if entry is None:
+        word = torch.zeros(1, dtype=torch.int32).pin_memory()
+        entry = _statuses[device.index] = (word, ctypes.c_int32.from_address(word.data_ptr()))
+    elif entry[1].value:
+        entry[1].value = 0
         raise RuntimeError("mps_pointops: a wait inside an earlier window_attention kernel ran out; "
                            "its results are not valid")
-    return word
+    return entry[0].data_ptr()
 
 
 class _Options:
@@ -310,29 +329,39 @@ class _Options:
                  "reach", "train", "want_lse", "precise")
 
 
-def _attention_args(q, k, v, table, o: _Options) -> N.AttentionArgs:
-    seg = o.segments
-    args = N.AttentionArgs(
-        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_row=q.stride(0), q_head=q.stride(1),
-        k_row=k.stride(0), k_head=k.stride(1), v_row=v.stride(0), v_head=v.stride(1),
-        q_tiles=seg.query_tiles.data_ptr(), k_tiles=seg.key_tiles.data_ptr(),
-        q_tile_count=seg.query_tiles.shape[0], k_tile_count=seg.key_tiles.shape[0],
-        q_rows=q.shape[0], k_rows=k.shape[0], heads=q.shape[1], kv_heads=k.shape[1],
-        dim=q.shape[2], dtype=_DTYPES[q.dtype], left=o.left, right=o.right, sinks=o.sinks,
-        status=_status(q.device).data_ptr(), causal=o.causal, max_rows=seg.max_rows, max_keys=seg.max_keys, clouds=seg.clouds, scale=o.scale)
-    if table is not None:
-        args.table, args.table_dtype = table.data_ptr(), _DTYPES[table.dtype]
-        args.axes, args.buckets, args.reach = table.shape[0], table.shape[1], o.reach
-        args.qpos, args.kpos, args.map = o.qpos.data_ptr(), o.kpos.data_ptr(), _address(o.map)
-    return args
+_pack_attention = N.packer(N.AttentionArgs)
 
 
-def _with_workspace(args: N.AttentionArgs, device: torch.device, backward: bool) -> Tensor | None:
-    args.backward = int(backward)
-    nbytes = int(N.lib().mpo_window_attention_workspace_bytes(ctypes.byref(args)))
-    ws = N.workspace(nbytes, device)
-    args.workspace, args.workspace_bytes = _address(ws), nbytes
-    return ws
+def _attention_call(backward: bool, o: _Options, q, k, v, table, out, lse, precise, grad=None,
+                    delta=None, dq=None, dk=None, dv=None, dtable=None) -> None:
+    seg, device = o.segments, q.device
+    bias = (0,) * 4 if table is None else (_DTYPES[table.dtype], table.shape[0], table.shape[1],
+                                           o.reach)
+
+    def pack(ws, nbytes):
+        return _pack_attention(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0),
+            k.stride(1), v.stride(0), v.stride(1), out.data_ptr(), _address(precise),
+            _address(lse), _address(grad), _address(delta), _address(dq), _address(dk),
+            _address(dv), _address(table), _address(dtable), _address(o.qpos), _address(o.kpos),
+            _address(o.map), seg.query_tiles.data_ptr(), seg.key_tiles.data_ptr(),
+            _status(device), seg.query_tiles.shape[0], seg.key_tiles.shape[0], q.shape[0],
+            k.shape[0], _address(ws), nbytes, q.shape[1], k.shape[1], q.shape[2],
+            _DTYPES[q.dtype], *bias, o.left, o.right, o.sinks, o.causal, seg.max_rows,
+            seg.max_keys, seg.clouds, o.scale, int(backward))
+
+    with N.on_device(device):
+        lib = N.lib()
+        args = pack(None, 0)
+        nbytes = int(lib.mpo_window_attention_workspace_bytes(args))
+        ws = None
+        if nbytes:
+            ws = N.workspace(nbytes, device)
+            args = pack(ws, nbytes)
+        stream = _stream(device)
+        seg._use(stream)
+        call = lib.mpo_window_attention_backward if backward else lib.mpo_window_attention
+        N.check(call(args, stream), "window_attention backward" if backward else "window_attention")
 
 
 def _forward(q, k, v, table, o: _Options):
@@ -343,14 +372,7 @@ def _forward(q, k, v, table, o: _Options):
         lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=device)
     if o.precise and q.dtype != torch.float32:
         precise = torch.empty(q.shape, dtype=torch.float32, device=device)
-    args = _attention_args(q, k, v, table, o)
-    args.out, args.lse, args.out_f32 = out.data_ptr(), _address(lse), _address(precise)
-    with N.on_device(device):
-        ws = _with_workspace(args, device, False)
-        o.segments._use()
-        N.check(N.lib().mpo_window_attention(ctypes.byref(args), N.stream(device)),
-                "window_attention")
-    del ws
+    _attention_call(False, o, q, k, v, table, out, lse, precise)
     return out, lse, precise
 
 
@@ -379,17 +401,7 @@ class _WindowAttention(torch.autograd.Function):
         dtable = None
         if table is not None and ctx.needs_input_grad[3]:
             dtable = torch.empty(table.shape, dtype=torch.float32, device=device)
-        args = _attention_args(q, k, v, table, o)
-        args.out, args.lse, args.out_f32 = out.data_ptr(), lse.data_ptr(), _address(precise)
-        args.grad_out, args.delta = grad.data_ptr(), delta.data_ptr()
-        args.grad_q, args.grad_k, args.grad_v = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        args.grad_table = _address(dtable)
-        with N.on_device(device):
-            ws = _with_workspace(args, device, True)
-            o.segments._use()
-            N.check(N.lib().mpo_window_attention_backward(ctypes.byref(args), N.stream(device)),
-                    "window_attention backward")
-        del ws
+        _attention_call(True, o, q, k, v, table, out, lse, precise, grad, delta, dq, dk, dv, dtable)
         if dtable is not None:
             dtable = dtable.to(table.dtype)
         return dq, dk, dv, dtable, None
