@@ -600,10 +600,8 @@ MPO_API int64_t mpo_attention_plan(const int64_t* ends, const int64_t* other_end
  *   int32 (rows, axes), magnitudes below 2^30.  table NULL: no bias.
  *   out (q_rows, heads, dim) dense; lse (heads, q_rows) float32, nullable in
  *   the forward: natural logarithm of the softmax denominators.  A row that
- *   sees no key gets zeros and -inf.  out_f32 (nullable): the result before
- *   its rounding, which the backward needs for the table's gradient.
- * Backward: grad_out dense like out; out, lse and (table gradient) out_f32 as
- * the forward gave them; delta (heads, q_rows) float32 scratch; grad_q,
+ *   sees no key gets zeros and -inf.
+ * Backward: grad_out dense like out; out and lse as the forward gave them; delta (heads, q_rows) float32 scratch; grad_q,
  * grad_k, grad_v dense, overwritten; grad_table (axes, buckets, heads)
  * float32, nullable.  Sums run in a fixed order (bit-reproducible).
  * q_tiles / k_tiles: device copies of mpo_attention_plan's tiles; max_rows the
@@ -616,7 +614,7 @@ typedef struct {
     const void *q, *k, *v;
     int64_t q_row, q_head, k_row, k_head, v_row, v_head; /* strides, elements */
     void* out;
-    float *out_f32, *lse;
+    float* lse;
     const void* grad_out;
     float* delta;
     void *grad_q, *grad_k, *grad_v;

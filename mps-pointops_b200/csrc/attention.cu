@@ -88,8 +88,6 @@ int check_attention(const mpo_attention* a, bool backward, const char* what) {
         if (!aligned_to(a->grad_out, 16) || !aligned_to(a->grad_q, 16) ||
             !aligned_to(a->grad_k, 16) || !aligned_to(a->grad_v, 16))
             return bad("rows must start on 16-byte boundaries");
-        if (a->grad_table && a->q_tile_count > 0 && !a->out_f32 && a->dtype != MPO_F32)
-            return bad("the table's gradient needs out_f32");
     }
     return kOk;
 }

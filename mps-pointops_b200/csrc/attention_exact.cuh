@@ -32,16 +32,16 @@ __device__ __forceinline__ float lane_dot(const float (&a)[4], const float (&b)[
     for (int i = 0; i < 4; ++i) s = fmaf(a[i], b[i], s);
     return warp_sum(s);
 }
-// Bias of (query row, key row), global, in units of log2.
+// Bucket and bias (units of log2) of (query row, key row), global.
+__device__ __forceinline__ int pair_bucket(const AttnArgs& A, int64_t q, int64_t k, int ax) {
+    const int b = bias_bucket(A.a.kpos[k * A.a.axes + ax], A.a.qpos[q * A.a.axes + ax], A.a.reach, nullptr);
+    return A.a.map ? min(max(A.a.map[b], 0), A.a.buckets - 1) : b;
+}
 __device__ __forceinline__ float pair_bias(const AttnArgs& A, int64_t q, int64_t k, int h) {
     if (!A.a.table) return 0.f;
     float s = 0.f;
-    for (int ax = 0; ax < A.a.axes; ++ax) {
-        int b = bias_bucket(A.a.kpos[k * A.a.axes + ax], A.a.qpos[q * A.a.axes + ax], A.a.reach,
-                            nullptr);
-        if (A.a.map) b = min(max(A.a.map[b], 0), A.a.buckets - 1);
-        s += table_entry(A.a, ax * A.a.buckets + b, h) * kLog2e;
-    }
+    for (int ax = 0; ax < A.a.axes; ++ax)
+        s += table_entry(A.a, ax * A.a.buckets + pair_bucket(A, q, k, ax), h) * kLog2e;
     return s;
 }
 // Key ranges of one query at p: [0, s1) and [lo, hi) with s1 <= lo.
@@ -59,7 +59,7 @@ __device__ __forceinline__ void row_keys(const AttnArgs& A, int p, int lk, int& 
     }
 }
 
-// out row (and out_f32 row) of query row q (global) at position p, head h.
+// out and lse of query row q (global) at position p, head h.
 template <typename T>
 __device__ __noinline__ void exact_forward_row(const AttnArgs& A, int64_t q, int p, int64_t k0,
                                                int lk, int h) {
@@ -90,8 +90,9 @@ __device__ __noinline__ void exact_forward_row(const AttnArgs& A, int64_t q, int
         if (d >= A.a.dim) continue;
         const float o = l == 0.f ? 0.f : acc[i] * r;
         static_cast<T*>(A.a.out)[at + d] = Elem<T>::from(o);
-        if (A.a.out_f32) A.a.out_f32[at + d] = o;
     }
+    if (A.a.lse && lane == 0)
+        A.a.lse[(int64_t)h * A.a.q_rows + q] = l == 0.f ? -INFINITY : fmaf(m, kLn2, logf(l));
 }
 
 __device__ __forceinline__ float load_lse2(const AttnArgs& A, int64_t q, int h) {
@@ -99,10 +100,34 @@ __device__ __forceinline__ float load_lse2(const AttnArgs& A, int64_t q, int h) 
     return l == -INFINITY ? INFINITY : l * kLog2e;
 }
 
-// grad_q row.
+// D of query row q as sum P dP.
+template <typename T>
+__device__ __noinline__ float exact_delta_row(const AttnArgs& A, int64_t q, int p, int64_t k0, int lk,
+                                              int h) {
+    float x[4], g[4], y[4], sum = 0.f;
+    lane_row(attn_row<T>(A.a.q, q, h, A.a.q_row, A.a.q_head), A.a.dim, x);
+    lane_row(static_cast<const T*>(A.a.grad_out) + (q * A.a.heads + h) * A.a.dim, A.a.dim, g);
+    const float lse2 = load_lse2(A, q, h);
+    const int hk = h / A.group;
+    int s1, lo, hi;
+    row_keys(A, p, lk, s1, lo, hi);
+    for (int j = 0; j < hi; ++j) {
+        if (j == s1) j = lo;
+        if (j >= hi) break;
+        lane_row(attn_row<T>(A.a.v, k0 + j, hk, A.a.v_row, A.a.v_head), A.a.dim, y);
+        const float dp = lane_dot(g, y);
+        lane_row(attn_row<T>(A.a.k, k0 + j, hk, A.a.k_row, A.a.k_head), A.a.dim, y);
+        const float s = fmaf(lane_dot(x, y), A.scale_log2, pair_bias(A, q, k0 + j, h));
+        sum = fmaf(exp2_sfu(s - lse2), dp, sum);
+    }
+    return sum;
+}
+
+// grad_q row; `cells` (nullable): this warp's table cells ([entry][32]), to which
+// lane 0 adds the row's score gradients.
 template <typename T>
 __device__ __noinline__ void exact_grad_q_row(const AttnArgs& A, int64_t q, int p, int64_t k0,
-                                              int lk, int h) {
+                                              int lk, int h, float* cells = nullptr) {
     const int lane = threadIdx.x & 31, hk = h / A.group;
     float x[4], g[4], y[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
     lane_row(attn_row<T>(A.a.q, q, h, A.a.q_row, A.a.q_head), A.a.dim, x);
@@ -119,6 +144,9 @@ __device__ __noinline__ void exact_grad_q_row(const AttnArgs& A, int64_t q, int 
         lane_row(attn_row<T>(A.a.k, k0 + j, hk, A.a.k_row, A.a.k_head), A.a.dim, y);
         const float s = fmaf(lane_dot(x, y), A.scale_log2, pair_bias(A, q, k0 + j, h));
         const float ds = exp2_sfu(s - lse2) * (dp - delta);
+        if (cells && lane == 0)
+            for (int ax = 0; ax < A.a.axes; ++ax)
+                cells[(ax * A.a.buckets + pair_bucket(A, q, k0 + j, ax)) * 32] += ds;
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] = fmaf(ds, y[i], acc[i]);
     }

@@ -81,7 +81,6 @@ __device__ __forceinline__ void store_row(const AttnArgs& A, int64_t q, int h, i
     nan |= isnan(v);
     const int64_t at = (q * A.a.heads + h) * A.a.dim + d;
     static_cast<T*>(A.a.out)[at] = Elem<T>::from(v);
-    if (A.a.out_f32) A.a.out_f32[at] = v;
 }
 __device__ __forceinline__ void store_lse(const AttnArgs& A, int64_t q, int h, float m, float l) {
     if (A.a.lse) A.a.lse[(int64_t)h * A.a.q_rows + q] = l == 0.f ? -INFINITY : fmaf(m, kLn2, logf(l));
@@ -500,7 +499,7 @@ int run(const AttnArgs& A, cudaStream_t s) {
 // key is read by one unit (by group / 16 where more heads share it), where a
 // tile kernel would fill 1/8 of its rows or less.
 bool attn_rows_eligible(const AttnArgs& A) {
-    return !A.a.out_f32 && (int64_t)A.a.max_rows * min64(A.group, 16) <= 16;
+    return (int64_t)A.a.max_rows * min64(A.group, 16) <= 16;
 }
 size_t attn_rows_workspace(const AttnArgs& A) {
     const RowsPlan P = rows_plan(A);

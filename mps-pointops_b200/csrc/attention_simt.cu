@@ -270,7 +270,6 @@ __global__ void __launch_bounds__(kThreads) attn_simt_fwd_kernel(const __grid_co
                 nan |= isnan(v);
                 if (tx * W + e < A.a.dim) {
                     static_cast<T*>(A.a.out)[at + e] = Elem<T>::from(v);
-                    if (A.a.out_f32) A.a.out_f32[at + e] = v;
                 }
             }
             if (A.a.lse && tx == 0)
@@ -320,8 +319,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_q_kernel(const __grid
         if (r < H.rows) {
             const int64_t at = ((H.row + r) * A.a.heads + h) * A.a.dim;
             for (int d = threadIdx.x & 1; d < A.a.dim; d += 2) {
-                const float ov = A.a.out_f32 ? A.a.out_f32[at + d]
-                                             : Elem<T>::to(static_cast<const T*>(A.a.out)[at + d]);
+                const float ov = Elem<T>::to(static_cast<const T*>(A.a.out)[at + d]);
                 sum = fmaf(ov, S.rows[1][r * Pitch<DP>::v + d], sum);
             }
         }

@@ -220,6 +220,11 @@ __device__ __forceinline__ void mma_weighted(uint32_t d, uint32_t a, uint32_t b,
 }
 
 // ---------------------------------------------------------------- masks
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 // Bits [lo, hi) of 64.
 __device__ __forceinline__ uint64_t bit_range(int lo, int hi) {
     lo = max(lo, 0);
@@ -241,26 +246,86 @@ __device__ __forceinline__ uint64_t seeing_queries(const AttnArgs& A, int j, int
 
 // ---------------------------------------------------------------- bias
 // The table of a head in shared memory, times log2(e), one copy per lane:
-// entry e of lane l at word 32 e + l.  A lane reads its own bank, so a read
+// entry e of lane l at byte 128 e + 4 l.  A lane reads its own bank, so a read
 // costs one wavefront whatever the buckets (one shared copy: about three, for
 // neighbouring points that differ).
+//
+// Positions are staged relative to the tile's first row and times 128, so that
+// column + row, clamped to the axis' entries, is the address: two instructions
+// per pair and axis.  Columns beyond +-2^22 of the first row are clamped there;
+// a row beyond +-2^21 of it (`far`) could then be wrong, is left out of the tile
+// and formed pair by pair (attention_exact.cuh).
+constexpr int kNear = 1 << 21;
 __device__ __forceinline__ void tc_load_table(const AttnArgs& A, float* table, int h) {
     for (int e = threadIdx.x; e < A.a.axes * A.a.buckets * 32; e += kTcThreads)
         table[e] = table_entry(A.a, e >> 5, h) * kLog2e;
 }
-// Word offset 32 e of the bucket of one axis (without the lane).
-template <bool MAPPED>
-__device__ __forceinline__ int bucket_word(const AttnArgs& A, int diff) {
-    int c = max(min(diff, A.a.reach), -A.a.reach) + A.a.reach;
-    if (MAPPED) c = min(max(__ldg(A.a.map + c), 0), A.a.buckets - 1);
-    return c << 5;
+struct BiasRow {
+    int add[kAttnMaxAxes], lo[kAttnMaxAxes], hi[kAttnMaxAxes];
+    int ref[kAttnMaxAxes];
+    bool far = false;
+    // sign 1: rows are queries, columns keys (key - query = column - row); -1: the reverse.
+    __device__ __forceinline__ void init(const AttnArgs& A, const int32_t* pos, int64_t first, int row,
+                                         bool live, uint32_t table, int sign) {
+#pragma unroll
+        for (int a = 0; a < kAttnMaxAxes; ++a) {
+            add[a] = lo[a] = hi[a] = ref[a] = 0;
+            if (a >= A.a.axes) continue;
+            ref[a] = pos[first * A.a.axes + a];
+            const int d = live ? pos[(first + row) * A.a.axes + a] - ref[a] : 0;
+            if (d > kNear || d < -kNear) far = true;
+            lo[a] = (int)table + a * A.a.buckets * 128 + (threadIdx.x & 31) * 4;
+            hi[a] = lo[a] + 256 * A.a.reach;
+            add[a] = lo[a] + 128 * A.a.reach - (far ? 0 : sign * d * 128);
+        }
+    }
+    // Staged value of a column.
+    static __device__ __forceinline__ int column(int pos, int ref, int sign) {
+        return sign * max(min(pos - ref, 2 * kNear), -2 * kNear) * 128;
+    }
+    template <bool MAPPED>
+    __device__ __forceinline__ int address(const AttnArgs& A, int a, int col) const {
+        int at = max(__viaddmin_s32(col, add[a], hi[a]), lo[a]);
+        if (MAPPED) at = lo[a] + 128 * min(max(__ldg(A.a.map + ((at - lo[a]) >> 7)), 0), A.a.buckets - 1);
+        return at;
+    }
+};
+// Columns [r0, r0 + n) by axis: dst[axis * 64 + column].
+__device__ __forceinline__ void tc_load_columns(int* dst, const int32_t* pos, int64_t r0, int n, int axes,
+                                                const BiasRow& row, int sign) {
+    if (threadIdx.x < kTcCols) {
+#pragma unroll
+        for (int a = 0; a < kAttnMaxAxes; ++a)
+            if (a < axes)
+                dst[a * kTcCols + threadIdx.x] =
+                    threadIdx.x < n
+                        ? BiasRow::column(pos[(r0 + threadIdx.x) * axes + a], row.ref[a], sign)
+                        : 0;
+    }
 }
-// Positions of rows [r0, r0 + n) by axis: dst[axis * 64 + row].
-__device__ __forceinline__ void tc_load_pos(int* dst, const int32_t* pos, int64_t r0, int n, int axes) {
-    if (threadIdx.x < kTcCols)
-        for (int a = 0; a < axes; ++a)
-            dst[a * kTcCols + threadIdx.x] =
-                threadIdx.x < n ? pos[(r0 + threadIdx.x) * axes + a] : 0;
+// The table does not change while columns are read: free to move.
+__device__ __forceinline__ float lds_table(int addr) {
+    float v;
+    asm("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
+}
+// Bias of 16 columns as pairs; cols: the staged columns of axis 0 at column c.
+template <bool MAPPED>
+__device__ __forceinline__ void bias16(const AttnArgs& A, const BiasRow& row, const int* cols, f32x2 (&t)[8]) {
+#pragma unroll
+    for (int a = 0; a < kAttnMaxAxes; ++a)
+        if (a < A.a.axes) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int4 c4 = *reinterpret_cast<const int4*>(cols + a * kTcCols + e);
+                const f32x2 x = pack2(lds_table(row.address<MAPPED>(A, a, c4.x)),
+                                      lds_table(row.address<MAPPED>(A, a, c4.y)));
+                const f32x2 y = pack2(lds_table(row.address<MAPPED>(A, a, c4.z)),
+                                      lds_table(row.address<MAPPED>(A, a, c4.w)));
+                t[e / 2] = a ? add2(t[e / 2], x) : x;
+                t[e / 2 + 1] = a ? add2(t[e / 2 + 1], y) : y;
+            }
+        }
 }
 
 template <typename K>

@@ -25,77 +25,87 @@ namespace {
 constexpr size_t kTcPairBytes = 233472 / 3;
 
 // ---------------------------------------------------------------- queries
+// What the query kernel forms.  kGradQ: dq, with D = o . do from the stored
+// result.  For the table's gradient, which is kept in float32, D has to be the
+// sum over the pairs of the very weights and dP that it is subtracted from:
+// stored and tensor-core results are off by 2e-3 and (sums rounded towards zero)
+// 3e-6 of it, always the same way for all pairs of a row.  kDelta forms D = sum
+// P dP in float32 first; kGradQTable then forms dq and the table's gradient.
+enum QueryMode { kGradQ = 0, kDelta = 1, kGradQTable = 2 };
+
 // With the table's gradient and DP = 128, the lanes' cells (up to 128 KB) leave
 // room for one stage of keys and values and one copy of the table.
-template <int DP, bool GRAD_TABLE>
+template <int DP, int MODE>
 struct GradQShape {
-    static constexpr bool kTight = GRAD_TABLE && DP == 128;
+    static constexpr bool kCells = MODE == kGradQTable, kTight = kCells && DP == 128;
     static constexpr int kStages = kTight ? 1 : 2;
-    static constexpr int kS = 0, kDP = kTcCols, kDQ = 2 * kTcCols, kCols = 256;
+    static constexpr int kS = 0, kDP = kTcCols, kDQ = 2 * kTcCols, kCols = MODE == kDelta ? 128 : 256;
     static constexpr uint32_t kQ = 0, kG = TcTile<DP>::bytes(128), kStage = TcTile<DP>::bytes(64),
                               kK = 2 * kG, kV = kK + kStages * kStage, kPos = kV + kStages * kStage,
                               kBar = kPos + kStages * 3 * kTcCols * 4, kTable = kBar + 16;
-    static constexpr int kBlocks = DP == 128 || GRAD_TABLE ? 1 : 2;
+    static constexpr int kBlocks = kCells || DP == 128 ? 1 : MODE == kDelta && DP < 64 ? 3 : 2;
     static __host__ __device__ constexpr int table_words(int entries) {
         return kTight ? (entries + 3) / 4 * 4 : entries * 32;
     }
     static size_t bytes(int entries) {
         const size_t need = kTable + (size_t)table_words(entries) * 4 +
-                            (GRAD_TABLE ? (size_t)entries * 512 : 0) + 1024;
-        return need > kTcPairBytes ? need : kTcPairBytes;
+                            (kCells ? (size_t)entries * 512 : 0) + 1024;
+        const size_t least = 233472 / (512 / kCols + 1);  // no more blocks than TMEM serves
+        return need > least ? need : least;
     }
 };
 
 // Table gradient: every lane of every warp keeps its own cell of each entry
 // ([warp][entry][lane], its own bank: a plain read, add and write, no atomics).
-template <typename T, int DP, int BIAS, bool GRAD_TABLE>
-__global__ void __launch_bounds__(kTcThreads, (GradQShape<DP, GRAD_TABLE>::kBlocks))
-attn_tc_grad_q_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ partial) {
-    using Shape = GradQShape<DP, GRAD_TABLE>;
+template <typename T, int DP, int BIAS, int MODE>
+__global__ void __launch_bounds__(kTcThreads, (GradQShape<DP, MODE>::kBlocks))
+attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ partial) {
+    using Shape = GradQShape<DP, MODE>;
     constexpr int kStages = Shape::kStages;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sb = smem_u32(smem);
-    const int tid = threadIdx.x, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int h = blockIdx.y, hk = h / A.group;
     const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.q_tiles)[blockIdx.x];
     const int p = t.first + tid, entries = A.a.axes * A.a.buckets;
     int* kpos = reinterpret_cast<int*>(smem + Shape::kPos);
     float* table = reinterpret_cast<float*>(smem + Shape::kTable);
-    float* hist = table + Shape::table_words(entries) + (tid >> 5) * entries * 32 + lane;  // this lane's cells
+    float* cells = table + Shape::table_words(entries) + warp * entries * 32;  // this warp's
     uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kBar + 8);
 
     if (tid < 32) tmem_alloc(smem_u32(slot), Shape::kCols);
     if (tid == 0) mbar_init(sb + Shape::kBar);
     const KeySpan span = key_span(A, t.first, t.first + t.rows - 1, t.lk, kTcCols);
     const int tiles = span.count();
+    const bool live = tid < t.rows;
+    // Addresses are those of the cells where there are cells, else of the table.
+    BiasRow bias;
+    if (BIAS) bias.init(A, A.a.qpos, t.row, tid, live, Shape::kCells ? smem_u32(cells) : sb + Shape::kTable, 1);
+    const int to_table = (int)(sb + Shape::kTable - smem_u32(cells));
     auto load_tile = [&](int i) {
         const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
         const int64_t row = (int64_t)t.other + k0;
         const uint32_t stage = (i % kStages) * Shape::kStage;
         tc_load<T, DP, kTcCols>(sb + Shape::kK + stage, A.a.k, row, n, hk, A.a.k_row, A.a.k_head, A.a.dim);
         tc_load<T, DP, kTcCols>(sb + Shape::kV + stage, A.a.v, row, n, hk, A.a.v_row, A.a.v_head, A.a.dim);
-        if (BIAS) tc_load_pos(kpos + (i % kStages) * 3 * kTcCols, A.a.kpos, row, n, A.a.axes);
+        if (BIAS) tc_load_columns(kpos + (i % kStages) * 3 * kTcCols, A.a.kpos, row, n, A.a.axes, bias, 1);
     };
     tc_load<T, DP, 128>(sb + Shape::kQ, A.a.q, t.row, t.rows, h, A.a.q_row, A.a.q_head, A.a.dim);
     tc_load<T, DP, 128>(sb + Shape::kG, A.a.grad_out, t.row, t.rows, h,
                         (int64_t)A.a.heads * A.a.dim, A.a.dim, A.a.dim);
     if (tiles > 0) load_tile(0);
-    const bool live = tid < t.rows;
     const int64_t at = (((int64_t)t.row + tid) * A.a.heads + h) * A.a.dim;
-    int qpos[3] = {0, 0, 0};
+    float* delta_at = A.a.delta + (int64_t)h * A.a.q_rows + t.row + tid;
     if (BIAS) {
         if (Shape::kTight) {
             for (int e = tid; e < entries; e += kTcThreads) table[e] = table_entry(A.a, e, h) * kLog2e;
         } else {
             tc_load_table(A, table, h);
         }
-        if (live)
-            for (int a = 0; a < A.a.axes; ++a)
-                qpos[a] = A.a.qpos[((int64_t)t.row + tid) * A.a.axes + a];
     }
-    if (GRAD_TABLE)
-        for (int e = 0; e < entries; ++e) hist[e * 32] = 0.f;
+    if (Shape::kCells)
+        for (int e = lane; e < entries * 32; e += 32) cells[e] = 0.f;
     const float lse2 = live ? load_lse2(A, t.row + tid, h) : INFINITY;
     tc_load_done();
     tc_fence_before();
@@ -109,23 +119,20 @@ attn_tc_grad_q_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ pa
         mma_scores<T, DP, kTcCols>(tmem + Shape::kDP, sb + Shape::kG, sb + Shape::kV);
         mma_commit(sb + Shape::kBar);
     }
-    float delta = 0.f;  // D = o . do
-    if (live) {
+    float delta = 0.f;  // D; kDelta: its sum so far
+    if (MODE == kGradQTable) {
+        if (live) delta = *delta_at;
+    } else if (MODE == kGradQ && live) {
         for (int c = 0; c * 8 < A.a.dim; ++c) {
             float g[8], o[8];
             Elem<T>::unpack(*reinterpret_cast<const uint4*>(smem + Shape::kG + TcTile<DP>::at(128, tid, c)), g);
-            if (A.a.out_f32) {
-                const float4* src = reinterpret_cast<const float4*>(A.a.out_f32 + at + c * 8);
-                Elem<float>::unpack(reinterpret_cast<const uint4*>(src)[0], o);
-                Elem<float>::unpack(reinterpret_cast<const uint4*>(src)[1], o + 4);
-            } else {
-                Elem<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(A.a.out) + at + c * 8), o);
-            }
+            Elem<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(A.a.out) + at + c * 8), o);
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = fmaf(g[e], o[e], delta);
         }
-        A.a.delta[(int64_t)h * A.a.q_rows + t.row + tid] = delta;
+        *delta_at = delta;
     }
+    const f32x2 scale2 = pack2(A.scale_log2, A.scale_log2), lse22 = pack2(-lse2, -lse2);
 
     for (int i = 0; i < tiles; ++i) {
         done.wait();
@@ -133,8 +140,10 @@ attn_tc_grad_q_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ pa
         const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
         const bool whole = n == kTcCols && t.rows == 128 &&
                            all_visible(A, t.first, t.first + 127, k0, k0 + kTcCols - 1);
-        const uint64_t seen = whole ? ~0ull : live ? seen_keys(A, p, k0, n) : 0ull;
-        const int* kp = kpos + (i % kStages) * 3 * kTcCols;
+        uint64_t seen = whole ? ~0ull : live ? seen_keys(A, p, k0, n) : 0ull;
+        if (BIAS && bias.far) seen = 0ull;
+        const bool all = __all_sync(FULL_MASK, seen == ~0ull);
+        const int* cols = kpos + (i % kStages) * 3 * kTcCols;
 #pragma unroll
         for (int c = 0; c < kTcCols; c += 16) {
             float s[16], dp[16];
@@ -143,44 +152,78 @@ attn_tc_grad_q_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ pa
             tmem_wait_ld();
             tmem_use(s);
             tmem_use(dp);
-            int words[3][16];
+            int cell[kAttnMaxAxes][16];
+            f32x2 b[8];
+            if (Shape::kCells) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = fmaf(s[e], A.scale_log2, -lse2);
-            if (BIAS) {
-#pragma unroll
-                for (int a = 0; a < 3; ++a)
+                for (int a = 0; a < kAttnMaxAxes; ++a)
                     if (a < A.a.axes) {
-                        const float* tab = Shape::kTight ? table + a * A.a.buckets
-                                                         : table + (a * A.a.buckets * 32 + lane);
 #pragma unroll
                         for (int e = 0; e < 16; e += 4) {
-                            const int4 k4 = *reinterpret_cast<const int4*>(kp + a * kTcCols + c + e);
-                            words[a][e] = bucket_word<BIAS == 2>(A, k4.x - qpos[a]);
-                            words[a][e + 1] = bucket_word<BIAS == 2>(A, k4.y - qpos[a]);
-                            words[a][e + 2] = bucket_word<BIAS == 2>(A, k4.z - qpos[a]);
-                            words[a][e + 3] = bucket_word<BIAS == 2>(A, k4.w - qpos[a]);
+                            const int4 c4 = *reinterpret_cast<const int4*>(cols + a * kTcCols + c + e);
+                            cell[a][e] = bias.address<BIAS == 2>(A, a, c4.x);
+                            cell[a][e + 1] = bias.address<BIAS == 2>(A, a, c4.y);
+                            cell[a][e + 2] = bias.address<BIAS == 2>(A, a, c4.z);
+                            cell[a][e + 3] = bias.address<BIAS == 2>(A, a, c4.w);
                         }
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) s[e] += tab[Shape::kTight ? words[a][e] >> 5 : words[a][e]];
+                        for (int e = 0; e < 16; e += 2) {
+                            const int x = Shape::kTight ? (int)(sb + Shape::kTable) + 4 * a * A.a.buckets +
+                                                              ((cell[a][e] - bias.lo[a]) >> 5)
+                                                        : cell[a][e] + to_table;
+                            const int y = Shape::kTight ? (int)(sb + Shape::kTable) + 4 * a * A.a.buckets +
+                                                              ((cell[a][e + 1] - bias.lo[a]) >> 5)
+                                                        : cell[a][e + 1] + to_table;
+                            const f32x2 v = pack2(lds_table(x), lds_table(y));
+                            b[e / 2] = a ? add2(b[e / 2], v) : v;
+                        }
                     }
+            } else if (BIAS) {
+                bias16<BIAS == 2>(A, bias, cols + c, b);
             }
             const uint32_t bits = (uint32_t)(seen >> c);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float ds = exp2_sfu(s[e]) * (dp[e] - delta);
-                s[e] = whole || ((bits >> e) & 1u) ? ds : 0.f;
+            for (int e = 0; e < 16; e += 2) {
+                f32x2 x = fma2(pack2(s[e], s[e + 1]), scale2, lse22);
+                if (BIAS) x = add2(x, b[e / 2]);
+                float u, v;
+                unpack2(x, u, v);
+                u = exp2_sfu(u);
+                v = exp2_sfu(v);
+                if (MODE == kDelta) {
+                    s[e] = u * dp[e];
+                    s[e + 1] = v * dp[e + 1];
+                } else {
+                    s[e] = u * (dp[e] - delta);
+                    s[e + 1] = v * (dp[e + 1] - delta);
+                }
             }
-            if (GRAD_TABLE) {
+            if (!all) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = (bits >> e) & 1u ? s[e] : 0.f;
+            }
+            if (MODE == kDelta) {
+                f32x2 sum = pack2(s[0], s[1]);
+#pragma unroll
+                for (int e = 2; e < 16; e += 2) sum = add2(sum, pack2(s[e], s[e + 1]));
+                float u, v;
+                unpack2(sum, u, v);
+                delta += u + v;
+                continue;
+            }
+            if (Shape::kCells) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     // Cells of different axes are different: read the three, then write them.
-                    float v[3];
+                    float v[kAttnMaxAxes];
 #pragma unroll
-                    for (int a = 0; a < 3; ++a)
-                        if (a < A.a.axes) v[a] = hist[a * A.a.buckets * 32 + words[a][e]];
+                    for (int a = 0; a < kAttnMaxAxes; ++a)
+                        if (a < A.a.axes)
+                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[a]) : "r"(cell[a][e]));
 #pragma unroll
-                    for (int a = 0; a < 3; ++a)
-                        if (a < A.a.axes) hist[a * A.a.buckets * 32 + words[a][e]] = v[a] + s[e];
+                    for (int a = 0; a < kAttnMaxAxes; ++a)
+                        if (a < A.a.axes)
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(cell[a][e]), "f"(v[a] + s[e]));
                 }
             }
             uint32_t w[8];
@@ -195,7 +238,8 @@ attn_tc_grad_q_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ pa
         if (tid == 0) {
             tc_fence_after();
             const uint32_t stage = (i % kStages) * Shape::kStage, next = Shape::kStage - stage;
-            mma_weighted<T, DP, kTcCols>(tmem + Shape::kDQ, tmem + Shape::kS, sb + Shape::kK + stage, i > 0);
+            if (MODE != kDelta)
+                mma_weighted<T, DP, kTcCols>(tmem + Shape::kDQ, tmem + Shape::kS, sb + Shape::kK + stage, i > 0);
             if (kStages == 2 && i + 1 < tiles) {
                 mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kQ, sb + Shape::kK + next);
                 mma_scores<T, DP, kTcCols>(tmem + Shape::kDP, sb + Shape::kG, sb + Shape::kV + next);
@@ -217,32 +261,45 @@ attn_tc_grad_q_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ pa
         }
     }
     if (tiles > 0) done.wait();
-    bool nan = false;
-#pragma unroll
-    for (int c = 0; c < DP; c += 16) {
-        float o[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[e] = 0.f;
-        if (tiles > 0) {
-            tmem_ld16(mine + Shape::kDQ + c, o);
-            tmem_wait_ld();
-            tmem_use(o);
+    const bool far = BIAS && live && bias.far;
+    if (MODE == kDelta) {
+        if (live) *delta_at = delta;
+        __syncwarp();
+        for (unsigned bad = __ballot_sync(FULL_MASK, far); bad; bad &= bad - 1) {
+            const int r = (tid & ~31) + __ffs(bad) - 1;
+            const float d = exact_delta_row<T>(A, (int64_t)t.row + r, t.first + r, t.other, t.lk, h);
+            if (r == tid) *delta_at = d;
         }
-        if (!live) continue;
+    } else {
+        bool nan = far;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            o[e] *= A.a.scale;
-            nan |= isnan(o[e]);
+        for (int c = 0; c < DP; c += 16) {
+            float o[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = 0.f;
+            if (tiles > 0) {
+                tmem_ld16(mine + Shape::kDQ + c, o);
+                tmem_wait_ld();
+                tmem_use(o);
+            }
+            if (!live) continue;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                o[e] *= A.a.scale;
+                nan |= isnan(o[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; e += 8)
+                if (c + e < A.a.dim)
+                    *reinterpret_cast<uint4*>(static_cast<T*>(A.a.grad_q) + at + c + e) = Elem<T>::pack(o + e);
         }
-#pragma unroll
-        for (int e = 0; e < 16; e += 8)
-            if (c + e < A.a.dim)
-                *reinterpret_cast<uint4*>(static_cast<T*>(A.a.grad_q) + at + c + e) = Elem<T>::pack(o + e);
-    }
-    __syncwarp();
-    for (unsigned bad = __ballot_sync(FULL_MASK, nan); bad; bad &= bad - 1) {
-        const int r = (tid & ~31) + __ffs(bad) - 1;
-        exact_grad_q_row<T>(A, (int64_t)t.row + r, t.first + r, t.other, t.lk, h);
+        __syncwarp();
+        const unsigned apart = __ballot_sync(FULL_MASK, far);
+        for (unsigned bad = __ballot_sync(FULL_MASK, nan); bad; bad &= bad - 1) {
+            const int r = __ffs(bad) - 1;
+            exact_grad_q_row<T>(A, (int64_t)t.row + (tid & ~31) + r, t.first + (tid & ~31) + r, t.other, t.lk,
+                                h, Shape::kCells && ((apart >> r) & 1u) ? cells : nullptr);
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -250,12 +307,12 @@ attn_tc_grad_q_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ pa
         tc_fence_after();
         tmem_free(tmem, Shape::kCols);
     }
-    if (GRAD_TABLE)
+    if (Shape::kCells)
         for (int e = tid; e < entries; e += kTcThreads) {
             float v = 0.f;
-            const float* cells = table + Shape::table_words(entries);
+            const float* all = table + Shape::table_words(entries);
             for (int w = 0; w < 4; ++w)
-                for (int l = 0; l < 32; ++l) v += cells[(w * entries + e) * 32 + ((l + e) & 31)];
+                for (int l = 0; l < 32; ++l) v += all[(w * entries + e) * 32 + ((l + e) & 31)];
             partial[((int64_t)blockIdx.x * A.a.heads + h) * entries + e] = v;
         }
 }
@@ -294,7 +351,8 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
     const int hk = blockIdx.y, h0 = hk * A.group;
     const int j = t.first + tid;
     int* qpos = reinterpret_cast<int*>(smem + Shape::kPos);
-    float* rows = reinterpret_cast<float*>(smem + Shape::kRow);  // [stage][lse2, D][64]
+    float* rows = reinterpret_cast<float*>(smem + Shape::kRow);  // [stage][-lse2, -D][64]
+    const f32x2 scale2 = pack2(A.scale_log2, A.scale_log2);
     float* table = reinterpret_cast<float*>(smem + Shape::kTable);
     uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kBar + 8);
 
@@ -308,6 +366,9 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
         per = (int)((int64_t)per * (blockIdx.z + 1) / shares) - first;
     }
     const int tiles = per * A.group;
+    const bool live = tid < t.rows;
+    BiasRow bias;
+    if (BIAS) bias.init(A, A.a.kpos, t.row, tid, live, sb + Shape::kTable, -1);
     auto query0 = [&](int i) { return lo + (first + i % per) * kTcCols; };
     auto load_tile = [&](int i) {
         const int i0 = query0(i), n = min(kTcCols, hi - i0), h = h0 + i / per;
@@ -318,24 +379,17 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
                                 (int64_t)A.a.heads * A.a.dim, A.a.dim, A.a.dim);
         float* dst = rows + (i & 1) * 2 * kTcCols;
         if (tid < kTcCols) {
-            dst[tid] = tid < n ? load_lse2(A, row + tid, h) : INFINITY;
+            dst[tid] = tid < n ? -load_lse2(A, row + tid, h) : -INFINITY;
         } else {
             const int r = tid - kTcCols;
-            dst[tid] = r < n ? A.a.delta[(int64_t)h * A.a.q_rows + row + r] : 0.f;
+            dst[tid] = r < n ? -A.a.delta[(int64_t)h * A.a.q_rows + row + r] : 0.f;
         }
-        if (BIAS) tc_load_pos(qpos + (i & 1) * 3 * kTcCols, A.a.qpos, row, n, A.a.axes);
+        if (BIAS) tc_load_columns(qpos + (i & 1) * 3 * kTcCols, A.a.qpos, row, n, A.a.axes, bias, -1);
     };
     tc_load<T, DP, 128>(sb + Shape::kK, A.a.k, t.row, t.rows, hk, A.a.k_row, A.a.k_head, A.a.dim);
     tc_load<T, DP, 128>(sb + Shape::kV, A.a.v, t.row, t.rows, hk, A.a.v_row, A.a.v_head, A.a.dim);
     if (tiles > 0) load_tile(0);
-    const bool live = tid < t.rows;
-    int kpos[3] = {0, 0, 0};
-    if (BIAS) {
-        tc_load_table(A, table, h0);
-        if (live)
-            for (int a = 0; a < A.a.axes; ++a)
-                kpos[a] = A.a.kpos[((int64_t)t.row + tid) * A.a.axes + a];
-    }
+    if (BIAS) tc_load_table(A, table, h0);
     tc_load_done();
     tc_fence_before();
     __syncthreads();
@@ -358,8 +412,10 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
         const int i0 = query0(i), n = min(kTcCols, hi - i0), p0 = i0 + t.lk - t.lq;
         const bool whole = n == kTcCols && t.rows == 128 &&
                            all_visible(A, p0, p0 + kTcCols - 1, t.first, t.first + 127);
-        const uint64_t seen = whole ? ~0ull : live ? seeing_queries(A, j, p0, n) : 0ull;
-        const int* qp = qpos + (i & 1) * 3 * kTcCols;
+        uint64_t seen = whole ? ~0ull : live ? seeing_queries(A, j, p0, n) : 0ull;
+        if (BIAS && bias.far) seen = 0ull;
+        const bool all = __all_sync(FULL_MASK, seen == ~0ull);
+        const int* cols = qpos + (i & 1) * 3 * kTcCols;
         const float* row = rows + (i & 1) * 2 * kTcCols;
 #pragma unroll
         for (int c = 0; c < kTcCols; c += 16) {
@@ -369,41 +425,39 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
             tmem_wait_ld();
             tmem_use(s);
             tmem_use(dp);
+            f32x2 b[8];
+            if (BIAS) bias16<BIAS == 2>(A, bias, cols + c, b);
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
-                const float4 l = *reinterpret_cast<const float4*>(row + c + e);
-                s[e] = fmaf(s[e], A.scale_log2, -l.x);
-                s[e + 1] = fmaf(s[e + 1], A.scale_log2, -l.y);
-                s[e + 2] = fmaf(s[e + 2], A.scale_log2, -l.z);
-                s[e + 3] = fmaf(s[e + 3], A.scale_log2, -l.w);
-                const float4 d = *reinterpret_cast<const float4*>(row + kTcCols + c + e);
-                dp[e] -= d.x;
-                dp[e + 1] -= d.y;
-                dp[e + 2] -= d.z;
-                dp[e + 3] -= d.w;
-            }
-            if (BIAS) {
-#pragma unroll
-                for (int a = 0; a < 3; ++a)
-                    if (a < A.a.axes) {
-                        const float* tab = table + (a * A.a.buckets * 32 + lane);
-#pragma unroll
-                        for (int e = 0; e < 16; e += 4) {
-                            const int4 q4 = *reinterpret_cast<const int4*>(qp + a * kTcCols + c + e);
-                            s[e] += tab[bucket_word<BIAS == 2>(A, kpos[a] - q4.x)];
-                            s[e + 1] += tab[bucket_word<BIAS == 2>(A, kpos[a] - q4.y)];
-                            s[e + 2] += tab[bucket_word<BIAS == 2>(A, kpos[a] - q4.z)];
-                            s[e + 3] += tab[bucket_word<BIAS == 2>(A, kpos[a] - q4.w)];
-                        }
-                    }
+                // Staged negated: -lse2 and -D.
+                f32x2 l0, l1, d0, d1;
+                lds_pairs<0>(smem_u32(row + c + e), l0, l1);
+                lds_pairs<0>(smem_u32(row + kTcCols + c + e), d0, d1);
+                f32x2 x = fma2(pack2(s[e], s[e + 1]), scale2, l0);
+                f32x2 y = fma2(pack2(s[e + 2], s[e + 3]), scale2, l1);
+                if (BIAS) {
+                    x = add2(x, b[e / 2]);
+                    y = add2(y, b[e / 2 + 1]);
+                }
+                unpack2(x, s[e], s[e + 1]);
+                unpack2(y, s[e + 2], s[e + 3]);
+                unpack2(add2(pack2(dp[e], dp[e + 1]), d0), dp[e], dp[e + 1]);
+                unpack2(add2(pack2(dp[e + 2], dp[e + 3]), d1), dp[e + 2], dp[e + 3]);
             }
             const uint32_t bits = (uint32_t)(seen >> c);
             uint32_t w[8], g[8];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const bool on = whole || ((bits >> e) & 1u);
-                s[e] = on ? exp2_sfu(s[e]) : 0.f;
-                dp[e] = on ? s[e] * dp[e] : 0.f;
+                s[e] = exp2_sfu(s[e]);
+                dp[e] *= s[e];
+            }
+            if (!all) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const bool on = (bits >> e) & 1u;
+                    s[e] = on ? s[e] : 0.f;
+                    dp[e] = on ? dp[e] : 0.f;
+                }
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -430,7 +484,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
         }
     }
     if (tiles > 0) done.wait();
-    bool nan = false;
+    bool nan = BIAS && live && bias.far;
     const int64_t at = (((int64_t)t.row + tid) * A.a.kv_heads + hk) * A.a.dim;
     const int sink_tiles = (A.a.sinks + kAttnTile - 1) / kAttnTile;
     float* sums = nullptr;
@@ -455,6 +509,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
             for (int e = 0; e < 16; ++e) {
                 if (!which) o[e] *= A.a.scale;
                 nan |= isnan(o[e]);
+                if (BIAS && bias.far) o[e] = __int_as_float(0x7fffffff);  // for the join: form it again
             }
 #pragma unroll
             for (int e = 0; e < 16; e += 8) {
@@ -526,14 +581,14 @@ size_t sink_bytes(const AttnArgs& A) {
     return (size_t)(tiles * A.a.kv_heads * shares * 2 * kAttnTile * A.a.dim) * sizeof(float);
 }
 
-template <typename T, int DP, int BIAS, bool GRAD_TABLE>
+template <typename T, int DP, int BIAS, int MODE>
 int run_q(const AttnArgs& A, float* partial, cudaStream_t s) {
-    const size_t bytes = GradQShape<DP, GRAD_TABLE>::bytes(BIAS ? A.a.axes * A.a.buckets : 0);
-    const int st = tc_prepare(attn_tc_grad_q_kernel<T, DP, BIAS, GRAD_TABLE>, bytes, "attn_tc_grad_q_kernel");
+    const size_t bytes = GradQShape<DP, MODE>::bytes(BIAS ? A.a.axes * A.a.buckets : 0);
+    const int st = tc_prepare(attn_tc_query_kernel<T, DP, BIAS, MODE>, bytes, "attn_tc_query_kernel");
     if (st != kOk) return st;
     const dim3 grid((unsigned)A.a.q_tile_count, (unsigned)A.a.heads);
-    attn_tc_grad_q_kernel<T, DP, BIAS, GRAD_TABLE><<<grid, kTcThreads, bytes, s>>>(A, partial);
-    return check_launch("attn_tc_grad_q_kernel");
+    attn_tc_query_kernel<T, DP, BIAS, MODE><<<grid, kTcThreads, bytes, s>>>(A, partial);
+    return check_launch("attn_tc_query_kernel");
 }
 template <typename T, int DP, int BIAS>
 int run_kv(const AttnArgs& A, float* partial, cudaStream_t s) {
@@ -556,9 +611,14 @@ int run(const AttnArgs& A, cudaStream_t s) {
     if (A.a.q_tile_count) {
         if constexpr (BIAS != 0) {
             float* partial = reinterpret_cast<float*>(static_cast<unsigned char*>(A.a.workspace) + sink_bytes(A));
-            st = A.a.grad_table ? run_q<T, DP, BIAS, true>(A, partial, s) : run_q<T, DP, BIAS, false>(A, nullptr, s);
+            if (A.a.grad_table) {
+                st = run_q<T, DP, BIAS, kDelta>(A, nullptr, s);
+                if (st == kOk) st = run_q<T, DP, BIAS, kGradQTable>(A, partial, s);
+            } else {
+                st = run_q<T, DP, BIAS, kGradQ>(A, nullptr, s);
+            }
         } else {
-            st = run_q<T, DP, BIAS, false>(A, nullptr, s);
+            st = run_q<T, DP, BIAS, kGradQ>(A, nullptr, s);
         }
     }
     if (st == kOk && A.a.k_tile_count) st = run_kv<T, DP, BIAS>(A, sums, s);

@@ -17,16 +17,10 @@
 namespace mpo {
 namespace {
 
-// PARTS: 16-bit parts of a weight.  1: its rounding (relative 2^-9 or 2^-12 on
-// average) stays below that of the stored result.  3: exact to float32, for the
-// D = o . do that the table's gradient subtracts from every pair: rounded
-// weights would leave about 2e-3 of that gradient wrong, which is kept in float32.
-template <int DP, int PARTS>
+template <int DP>
 struct FwdShape {
     static constexpr int kS = 0, kO = kTcCols;  // TMEM columns
-    static constexpr int kP2 = kO + DP;         // third part (the first two lie over S)
-    static constexpr int kUsed = PARTS == 3 ? kP2 + 32 : kO + DP;
-    static constexpr int kCols = kUsed <= 128 ? 128 : 256;
+    static constexpr int kCols = kO + DP <= 128 ? 128 : 256;
     static constexpr int kBlocks = 512 / kCols;
     static constexpr uint32_t kQ = 0, kK = TcTile<DP>::bytes(128), kStage = TcTile<DP>::bytes(64),
                               kV = kK + 2 * kStage, kPos = kV + 2 * kStage,
@@ -39,10 +33,10 @@ struct FwdShape {
     }
 };
 
-template <typename T, int DP, int BIAS, int PARTS>
-__global__ void __launch_bounds__(kTcThreads, (FwdShape<DP, PARTS>::kBlocks))
+template <typename T, int DP, int BIAS>
+__global__ void __launch_bounds__(kTcThreads, (BIAS && DP <= 64 ? 3 : FwdShape<DP>::kBlocks))
 attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
-    using Shape = FwdShape<DP, PARTS>;
+    using Shape = FwdShape<DP>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sb = smem_u32(smem);
@@ -58,23 +52,19 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
     if (tid == 0) mbar_init(sb + Shape::kBar);
     const KeySpan span = key_span(A, t.first, t.first + t.rows - 1, t.lk, kTcCols);
     const int tiles = span.count();
+    BiasRow bias;
+    if (BIAS) bias.init(A, A.a.qpos, t.row, tid, tid < t.rows, sb + Shape::kTable, 1);
     auto load_tile = [&](int i) {
         const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
         const int64_t row = (int64_t)t.other + k0;
         const uint32_t stage = (i & 1) * Shape::kStage;
         tc_load<T, DP, kTcCols>(sb + Shape::kK + stage, A.a.k, row, n, hk, A.a.k_row, A.a.k_head, A.a.dim);
         tc_load<T, DP, kTcCols>(sb + Shape::kV + stage, A.a.v, row, n, hk, A.a.v_row, A.a.v_head, A.a.dim);
-        if (BIAS) tc_load_pos(kpos + (i & 1) * 3 * kTcCols, A.a.kpos, row, n, A.a.axes);
+        if (BIAS) tc_load_columns(kpos + (i & 1) * 3 * kTcCols, A.a.kpos, row, n, A.a.axes, bias, 1);
     };
     tc_load<T, DP, 128>(sb + Shape::kQ, A.a.q, t.row, t.rows, h, A.a.q_row, A.a.q_head, A.a.dim);
     if (tiles > 0) load_tile(0);
-    int qpos[3] = {0, 0, 0};
-    if (BIAS) {
-        tc_load_table(A, table, h);
-        if (tid < t.rows)
-            for (int a = 0; a < A.a.axes; ++a)
-                qpos[a] = A.a.qpos[((int64_t)t.row + tid) * A.a.axes + a];
-    }
+    if (BIAS) tc_load_table(A, table, h);
     tc_load_done();
     tc_fence_before();
     __syncthreads();
@@ -100,20 +90,16 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
         tmem_use(s);
         const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
         if (BIAS) {
-            const int* kp = kpos + (i & 1) * 3 * kTcCols;
+            const int* cols = kpos + (i & 1) * 3 * kTcCols;
+            const f32x2 scale2 = pack2(A.scale_log2, A.scale_log2);
 #pragma unroll
-            for (int c = 0; c < kTcCols; ++c) s[c] *= A.scale_log2;
-            for (int a = 0; a < A.a.axes; ++a) {
-                const float* tab = table + (a * A.a.buckets * 32 + lane);
-                const int q = qpos[a];
+            for (int c = 0; c < kTcCols; c += 16) {
+                f32x2 b[8];
+                bias16<BIAS == 2>(A, bias, cols + c, b);
 #pragma unroll
-                for (int c = 0; c < kTcCols; c += 4) {
-                    const int4 k4 = *reinterpret_cast<const int4*>(kp + a * kTcCols + c);
-                    s[c] += tab[bucket_word<BIAS == 2>(A, k4.x - q)];
-                    s[c + 1] += tab[bucket_word<BIAS == 2>(A, k4.y - q)];
-                    s[c + 2] += tab[bucket_word<BIAS == 2>(A, k4.z - q)];
-                    s[c + 3] += tab[bucket_word<BIAS == 2>(A, k4.w - q)];
-                }
+                for (int e = 0; e < 8; ++e)
+                    unpack2(fma2(pack2(s[c + 2 * e], s[c + 2 * e + 1]), scale2, b[e]), s[c + 2 * e],
+                            s[c + 2 * e + 1]);
             }
         } else if (!(A.scale_log2 > 0.f)) {
 #pragma unroll
@@ -130,12 +116,11 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
         }
         float m[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int c = 4; c < kTcCols; c += 4) {
-            m[0] = fmaxf(m[0], s[c]);
-            m[1] = fmaxf(m[1], s[c + 1]);
-            m[2] = fmaxf(m[2], s[c + 2]);
-            m[3] = fmaxf(m[3], s[c + 3]);
-        }
+        for (int c = 4; c < 60; c += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m[e] = fmax3(m[e], s[c + e], s[c + 4 + e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], s[60 + e]);
         const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
         // (most - top) is NaN only when both are the same infinity: no growth.
         const bool grow = (most - top) * mul > 8.f;
@@ -164,7 +149,7 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
         const f32x2 mul2v = pack2(mul, mul), ref2 = pack2(ref, ref);
 #pragma unroll
         for (int c = 0; c < kTcCols; c += 16) {
-            uint32_t w[3][8];
+            uint32_t w[8];
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
                 float a, b;
@@ -172,20 +157,9 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
                 a = exp2_sfu(a);
                 b = exp2_sfu(b);
                 part[(e >> 1) & 1] = add2(part[(e >> 1) & 1], pack2(a, b));
-#pragma unroll
-                for (int q = 0; q < PARTS; ++q) {
-                    w[q][e / 2] = Elem<T>::two(a, b);
-                    if (q + 1 < PARTS) {
-                        float r[2];
-                        Elem<T>::two(w[q][e / 2], r);
-                        a -= r[0];
-                        b -= r[1];
-                    }
-                }
+                w[e / 2] = Elem<T>::two(a, b);
             }
-#pragma unroll
-            for (int q = 0; q < PARTS; ++q)
-                tmem_st8(mine + (q == 2 ? Shape::kP2 : Shape::kS + 32 * q) + c / 2, w[q]);
+            tmem_st8(mine + Shape::kS + c / 2, w);
         }
         {
             float a, b;
@@ -199,11 +173,7 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
         if (tid == 0) {
             tc_fence_after();
             const uint32_t stage = (i & 1) * Shape::kStage;
-#pragma unroll
-            for (int q = 0; q < PARTS; ++q)
-                mma_weighted<T, DP, kTcCols>(tmem + Shape::kO,
-                                             tmem + (q == 2 ? Shape::kP2 : Shape::kS + 32 * q),
-                                             sb + Shape::kV + stage, i > 0 || q > 0);
+            mma_weighted<T, DP, kTcCols>(tmem + Shape::kO, tmem + Shape::kS, sb + Shape::kV + stage, i > 0);
             // Issued after P V and executed in order after it: S may overwrite the weights.
             if (i + 1 < tiles)
                 mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kQ,
@@ -212,8 +182,8 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
         }
     }
     if (tiles > 0) done.wait();
-    bool nan = false;
     const bool live = tid < t.rows;
+    bool nan = BIAS && live && bias.far;
     const int64_t at = (((int64_t)t.row + tid) * A.a.heads + h) * A.a.dim;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
@@ -234,11 +204,6 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
         for (int e = 0; e < 16; e += 8) {
             if (c + e >= A.a.dim) continue;
             *reinterpret_cast<uint4*>(static_cast<T*>(A.a.out) + at + c + e) = Elem<T>::pack(o + e);
-            if (A.a.out_f32) {
-                float4* dst = reinterpret_cast<float4*>(A.a.out_f32 + at + c + e);
-                dst[0] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                dst[1] = make_float4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]);
-            }
         }
     }
     if (live && A.a.lse)
@@ -257,20 +222,19 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
     }
 }
 
-template <typename T, int DP, int BIAS, int PARTS>
+template <typename T, int DP, int BIAS>
 int run(const AttnArgs& A, cudaStream_t s) {
-    const size_t bytes = FwdShape<DP, PARTS>::bytes(BIAS ? A.a.axes * A.a.buckets : 0);
-    const int st = tc_prepare(attn_tc_fwd_kernel<T, DP, BIAS, PARTS>, bytes, "attn_tc_fwd_kernel");
+    const size_t bytes = FwdShape<DP>::bytes(BIAS ? A.a.axes * A.a.buckets : 0);
+    const int st = tc_prepare(attn_tc_fwd_kernel<T, DP, BIAS>, bytes, "attn_tc_fwd_kernel");
     if (st != kOk) return st;
     const dim3 grid((unsigned)A.a.q_tile_count, (unsigned)A.a.heads);
-    attn_tc_fwd_kernel<T, DP, BIAS, PARTS><<<grid, kTcThreads, bytes, s>>>(A);
+    attn_tc_fwd_kernel<T, DP, BIAS><<<grid, kTcThreads, bytes, s>>>(A);
     return check_launch("attn_tc_fwd_kernel");
 }
 template <typename T, int DP>
 int by_bias(const AttnArgs& A, cudaStream_t s) {
-    if (!A.a.table) return run<T, DP, 0, 1>(A, s);
-    if (A.a.map) return A.a.out_f32 ? run<T, DP, 2, 3>(A, s) : run<T, DP, 2, 1>(A, s);
-    return A.a.out_f32 ? run<T, DP, 1, 3>(A, s) : run<T, DP, 1, 1>(A, s);
+    if (!A.a.table) return run<T, DP, 0>(A, s);
+    return A.a.map ? run<T, DP, 2>(A, s) : run<T, DP, 1>(A, s);
 }
 template <typename T>
 int by_dim(const AttnArgs& A, cudaStream_t s) {

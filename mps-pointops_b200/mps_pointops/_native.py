@@ -70,7 +70,7 @@ class AttentionArgs(ctypes.Structure):
 
     _fields_ = _fields(
         (_vp, "q k v"), (_i64, "q_row q_head k_row k_head v_row v_head"),
-        (_vp, "out out_f32 lse grad_out delta grad_q grad_k grad_v table grad_table qpos kpos map "
+        (_vp, "out lse grad_out delta grad_q grad_k grad_v table grad_table qpos kpos map "
               "q_tiles k_tiles status"),
         (_i64, "q_tile_count k_tile_count q_rows k_rows"), (_vp, "workspace"),
         (_sz, "workspace_bytes"),

@@ -326,13 +326,13 @@ class _Options:
     """What a call of ``window_attention`` fixes besides its tensors."""
 
     __slots__ = ("segments", "left", "right", "sinks", "causal", "scale", "qpos", "kpos", "map",
-                 "reach", "train", "want_lse", "precise")
+                 "reach", "train", "want_lse")
 
 
 _pack_attention = N.packer(N.AttentionArgs)
 
 
-def _attention_call(backward: bool, o: _Options, q, k, v, table, out, lse, precise, grad=None,
+def _attention_call(backward: bool, o: _Options, q, k, v, table, out, lse, grad=None,
                     delta=None, dq=None, dk=None, dv=None, dtable=None) -> None:
     seg, device = o.segments, q.device
     bias = (0,) * 4 if table is None else (_DTYPES[table.dtype], table.shape[0], table.shape[1],
@@ -341,8 +341,8 @@ def _attention_call(backward: bool, o: _Options, q, k, v, table, out, lse, preci
     def pack(ws, nbytes):
         return _pack_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0),
-            k.stride(1), v.stride(0), v.stride(1), out.data_ptr(), _address(precise),
-            _address(lse), _address(grad), _address(delta), _address(dq), _address(dk),
+            k.stride(1), v.stride(0), v.stride(1), out.data_ptr(), _address(lse),
+            _address(grad), _address(delta), _address(dq), _address(dk),
             _address(dv), _address(table), _address(dtable), _address(o.qpos), _address(o.kpos),
             _address(o.map), seg.query_tiles.data_ptr(), seg.key_tiles.data_ptr(),
             _status(device), seg.query_tiles.shape[0], seg.key_tiles.shape[0], q.shape[0],
@@ -367,13 +367,11 @@ def _attention_call(backward: bool, o: _Options, q, k, v, table, out, lse, preci
 def _forward(q, k, v, table, o: _Options):
     device = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    lse = precise = None
+    lse = None
     if o.train or o.want_lse:
         lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=device)
-    if o.precise and q.dtype != torch.float32:
-        precise = torch.empty(q.shape, dtype=torch.float32, device=device)
-    _attention_call(False, o, q, k, v, table, out, lse, precise)
-    return out, lse, precise
+    _attention_call(False, o, q, k, v, table, out, lse)
+    return out, lse
 
 
 class _WindowAttention(torch.autograd.Function):
@@ -381,8 +379,8 @@ class _WindowAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, table, o: _Options):
         vec = 16 // q.element_size()
         q, k, v = _rows(q, vec), _rows(k, vec), _rows(v, vec)
-        out, lse, precise = _forward(q, k, v, table, o)
-        ctx.save_for_backward(q, k, v, table, out, lse, precise)
+        out, lse = _forward(q, k, v, table, o)
+        ctx.save_for_backward(q, k, v, table, out, lse)
         ctx.options = o
         ctx.mark_non_differentiable(lse)
         return out, lse
@@ -390,7 +388,7 @@ class _WindowAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, _):
-        q, k, v, table, out, lse, precise = ctx.saved_tensors
+        q, k, v, table, out, lse = ctx.saved_tensors
         o = ctx.options
         device = q.device
         grad = _dense(grad)
@@ -401,7 +399,7 @@ class _WindowAttention(torch.autograd.Function):
         dtable = None
         if table is not None and ctx.needs_input_grad[3]:
             dtable = torch.empty(table.shape, dtype=torch.float32, device=device)
-        _attention_call(True, o, q, k, v, table, out, lse, precise, grad, delta, dq, dk, dv, dtable)
+        _attention_call(True, o, q, k, v, table, out, lse, grad, delta, dq, dk, dv, dtable)
         if dtable is not None:
             dtable = dtable.to(table.dtype)
         return dq, dk, dv, dtable, None
@@ -523,14 +521,14 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, segments: Segments | Tenso
         o.map = None if buckets is None else buckets.contiguous()
         bias_table = bias_table.contiguous()
     grad = torch.is_grad_enabled()
-    o.precise = grad and bias_table is not None and bias_table.requires_grad
-    o.train = grad and (q.requires_grad or k.requires_grad or v.requires_grad or o.precise)
+    o.train = grad and (q.requires_grad or k.requires_grad or v.requires_grad or
+                        (bias_table is not None and bias_table.requires_grad))
     o.want_lse = bool(return_lse)
     if o.train:
         out, lse = _WindowAttention.apply(q, k, v, bias_table, o)
     else:
         vec = 16 // q.element_size()
-        out, lse, _ = _forward(_rows(q, vec), _rows(k, vec), _rows(v, vec), bias_table, o)
+        out, lse = _forward(_rows(q, vec), _rows(k, vec), _rows(v, vec), bias_table, o)
     return (out, lse) if return_lse else out
 
 
