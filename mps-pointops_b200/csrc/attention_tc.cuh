@@ -17,8 +17,8 @@
 namespace mpo {
 namespace {
 
-constexpr int kTcThreads = 128;  // one thread per row (TMEM lane)
-constexpr int kTcCols = 64;      // columns of a score tile
+constexpr int kTcRows = 128;  // rows of a tile: TMEM lanes, one thread (per column group) each
+constexpr int kTcCols = 64;   // columns of a score tile
 constexpr unsigned long long kTcWaitNs = 2000000000ull;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -154,17 +154,18 @@ struct TcTile {
 };
 
 // Rows [r0, r0 + n) of one head into a tile of ROWS rows, zeros past n and dim.
-template <typename T, int DP, int ROWS>
+template <typename T, int DP, int ROWS, int THREADS>
 __device__ __forceinline__ void tc_load(uint32_t tile, const void* base, int64_t r0, int n, int h,
                                         int64_t row_stride, int64_t head_stride, int dim) {
     using L = TcTile<DP>;
     const T* src = attn_row<T>(base, r0, h, row_stride, head_stride);
-    constexpr int kPer = ROWS * L::kChunks / kTcThreads;
+    constexpr int kStep = THREADS / L::kChunks;
+    constexpr int kPer = (ROWS + kStep - 1) / kStep;
     const int c = threadIdx.x % L::kChunks;
-    constexpr int kStep = kTcThreads / L::kChunks;
     int r = threadIdx.x / L::kChunks;
 #pragma unroll
     for (int i = 0; i < kPer; ++i, r += kStep) {
+        if (ROWS % kStep && r >= ROWS) break;
         const bool live = r < n && c * 8 < dim;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tile + L::at(ROWS, r, c)),
                      "l"(live ? src + r * row_stride + c * 8 : src), "r"(live ? 16 : 0)
@@ -211,12 +212,15 @@ __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b) {
         mma_ss(d, TcTile<DP>::k_major(a, 128, k), TcTile<DP>::k_major(b, NB, k),
                tc_idesc<T>(NB, false), k > 0);
 }
-// D (128 x DP) += weights (128 x NB, 16-bit pairs in TMEM from column a) . B (NB rows of tile b).
+// D (128 x DP) += weights (128 x NB) . B (NB rows of tile b).  The weights are 16-bit
+// pairs in TMEM: those of columns 16 k .. lie in the first 8 of the 16 columns
+// from a + 16 k, over the scores that they come from, so a thread overwrites
+// nothing but what it has read itself.
 template <typename T, int DP, int NB>
 __device__ __forceinline__ void mma_weighted(uint32_t d, uint32_t a, uint32_t b, bool acc) {
 #pragma unroll
     for (int k = 0; k < NB / 16; ++k)
-        mma_ts(d, a + 8 * k, TcTile<DP>::mn_major(b, NB, k), tc_idesc<T>(DP, true), acc || k > 0);
+        mma_ts(d, a + 16 * k, TcTile<DP>::mn_major(b, NB, k), tc_idesc<T>(DP, true), acc || k > 0);
 }
 
 // ---------------------------------------------------------------- masks
@@ -257,7 +261,7 @@ __device__ __forceinline__ uint64_t seeing_queries(const AttnArgs& A, int j, int
 // and formed pair by pair (attention_exact.cuh).
 constexpr int kNear = 1 << 21;
 __device__ __forceinline__ void tc_load_table(const AttnArgs& A, float* table, int h) {
-    for (int e = threadIdx.x; e < A.a.axes * A.a.buckets * 32; e += kTcThreads)
+    for (int e = threadIdx.x; e < A.a.axes * A.a.buckets * 32; e += blockDim.x)
         table[e] = table_entry(A.a, e >> 5, h) * kLog2e;
 }
 struct BiasRow {

@@ -21,9 +21,6 @@
 namespace mpo {
 namespace {
 
-// Shared memory that keeps a third block, which TMEM could not serve, off an SM.
-constexpr size_t kTcPairBytes = 233472 / 3;
-
 // ---------------------------------------------------------------- queries
 // What the query kernel forms.  kGradQ: dq, with D = o . do from the stored
 // result.  For the table's gradient, which is kept in float32, D has to be the
@@ -33,106 +30,132 @@ constexpr size_t kTcPairBytes = 233472 / 3;
 // P dP in float32 first; kGradQTable then forms dq and the table's gradient.
 enum QueryMode { kGradQ = 0, kDelta = 1, kGradQTable = 2 };
 
-// With the table's gradient and DP = 128, the lanes' cells (up to 128 KB) leave
-// room for one stage of keys and values and one copy of the table.
+// Threads: NG groups of 128; thread `row` of each group shares the row and takes
+// 64 / NG columns of every tile, so that 16 warps are on an SM (one thread per
+// row left 4 to 8, and most of the time went to fixed latencies).
+//
+// Table gradient: a thread may only add to cells that no other adds to, so lane
+// l of quarter w (rows 32 w ..) has its own cell of each entry ([w][entry][l],
+// its own bank: a plain read, add and write, no atomics), and group a keeps
+// those of axis a: the groups leave their score gradients in TMEM as float32
+// (two buffers), and after the tile's barrier group a adds all 64 columns of
+// them to its axis while the tensor core forms the next tile's S and dP.  With
+// DP = 128 the cells (up to 128 KB) leave room for one stage of keys and values
+// and for one copy of the table.
 template <int DP, int MODE>
-struct GradQShape {
+struct QueryShape {
     static constexpr bool kCells = MODE == kGradQTable, kTight = kCells && DP == 128;
-    static constexpr int kStages = kTight ? 1 : 2;
-    static constexpr int kS = 0, kDP = kTcCols, kDQ = 2 * kTcCols, kCols = MODE == kDelta ? 128 : 256;
+    static constexpr int kBlocks = kCells || DP == 128 ? 1 : 2, kGroups = 4 / kBlocks;
+    static constexpr int kThreads = kTcRows * kGroups;
+    static constexpr int kStages = kTight ? 1 : 2, kPosStages = kCells && !kTight ? 4 : 2;
+    static constexpr int kS = 0, kDP = kTcCols, kDQ = 2 * kTcCols, kDS = kDQ + DP;
+    static constexpr int kCols = kCells ? 512 : MODE == kDelta ? 128 : 256;
     static constexpr uint32_t kQ = 0, kG = TcTile<DP>::bytes(128), kStage = TcTile<DP>::bytes(64),
                               kK = 2 * kG, kV = kK + kStages * kStage, kPos = kV + kStages * kStage,
-                              kBar = kPos + kStages * 3 * kTcCols * 4, kTable = kBar + 16;
-    static constexpr int kBlocks = kCells || DP == 128 ? 1 : MODE == kDelta && DP < 64 ? 3 : 2;
+                              kBar = kPos + kPosStages * 3 * kTcCols * 4, kTable = kBar + 64;
+    static constexpr int kTightEntries = 248;  // the table fits beside this many cells
     static __host__ __device__ constexpr int table_words(int entries) {
-        return kTight ? (entries + 3) / 4 * 4 : entries * 32;
+        return !kTight ? entries * 32 : entries > kTightEntries ? 0 : (entries + 3) / 4 * 4;
     }
     static size_t bytes(int entries) {
-        const size_t need = kTable + (size_t)table_words(entries) * 4 +
-                            (kCells ? (size_t)entries * 512 : 0) + 1024;
-        const size_t least = 233472 / (512 / kCols + 1);  // no more blocks than TMEM serves
+        size_t need = kTable + (size_t)table_words(entries) * 4 + (kCells ? (size_t)entries * 512 : 0) + 1024;
+        if (MODE == kDelta && need < kTable + 4 * 4 * kTcRows + 1024) need = kTable + 4 * 4 * kTcRows + 1024;
+        const size_t least = 233472 / (kBlocks + 1);  // no more blocks than the registers were cut for
         return need > least ? need : least;
     }
 };
 
-// Table gradient: every lane of every warp keeps its own cell of each entry
-// ([warp][entry][lane], its own bank: a plain read, add and write, no atomics).
 template <typename T, int DP, int BIAS, int MODE>
-__global__ void __launch_bounds__(kTcThreads, (GradQShape<DP, MODE>::kBlocks))
+__global__ void __launch_bounds__((QueryShape<DP, MODE>::kThreads), (QueryShape<DP, MODE>::kBlocks))
 attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ partial) {
-    using Shape = GradQShape<DP, MODE>;
-    constexpr int kStages = Shape::kStages;
+    using Shape = QueryShape<DP, MODE>;
+    constexpr int kStages = Shape::kStages, kThreads = Shape::kThreads, kPer = kTcCols / Shape::kGroups;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sb = smem_u32(smem);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, r = tid & 127, quarter = r >> 5, group = tid >> 7;
     const int h = blockIdx.y, hk = h / A.group;
     const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.q_tiles)[blockIdx.x];
-    const int p = t.first + tid, entries = A.a.axes * A.a.buckets;
+    const int p = t.first + r, entries = A.a.axes * A.a.buckets;
     int* kpos = reinterpret_cast<int*>(smem + Shape::kPos);
     float* table = reinterpret_cast<float*>(smem + Shape::kTable);
-    float* cells = table + Shape::table_words(entries) + warp * entries * 32;  // this warp's
+    float* cells = table + Shape::table_words(entries) + quarter * entries * 32;  // this quarter's
     uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kBar + 8);
+    unsigned* flags = reinterpret_cast<unsigned*>(smem + Shape::kBar + 16);  // rows to form again
 
     if (tid < 32) tmem_alloc(smem_u32(slot), Shape::kCols);
     if (tid == 0) mbar_init(sb + Shape::kBar);
+    if (tid < 4) flags[tid] = 0u;
     const KeySpan span = key_span(A, t.first, t.first + t.rows - 1, t.lk, kTcCols);
     const int tiles = span.count();
-    const bool live = tid < t.rows;
-    // Addresses are those of the cells where there are cells, else of the table.
+    const bool live = r < t.rows;
     BiasRow bias;
-    if (BIAS) bias.init(A, A.a.qpos, t.row, tid, live, Shape::kCells ? smem_u32(cells) : sb + Shape::kTable, 1);
-    const int to_table = (int)(sb + Shape::kTable - smem_u32(cells));
+    if (BIAS) bias.init(A, A.a.qpos, t.row, r, live, sb + Shape::kTable, 1);
     auto load_tile = [&](int i) {
         const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
         const int64_t row = (int64_t)t.other + k0;
         const uint32_t stage = (i % kStages) * Shape::kStage;
-        tc_load<T, DP, kTcCols>(sb + Shape::kK + stage, A.a.k, row, n, hk, A.a.k_row, A.a.k_head, A.a.dim);
-        tc_load<T, DP, kTcCols>(sb + Shape::kV + stage, A.a.v, row, n, hk, A.a.v_row, A.a.v_head, A.a.dim);
-        if (BIAS) tc_load_columns(kpos + (i % kStages) * 3 * kTcCols, A.a.kpos, row, n, A.a.axes, bias, 1);
+        tc_load<T, DP, kTcCols, kThreads>(sb + Shape::kK + stage, A.a.k, row, n, hk, A.a.k_row, A.a.k_head, A.a.dim);
+        tc_load<T, DP, kTcCols, kThreads>(sb + Shape::kV + stage, A.a.v, row, n, hk, A.a.v_row, A.a.v_head, A.a.dim);
+        if (BIAS)
+            tc_load_columns(kpos + (i % Shape::kPosStages) * 3 * kTcCols, A.a.kpos, row, n, A.a.axes, bias, 1);
     };
-    tc_load<T, DP, 128>(sb + Shape::kQ, A.a.q, t.row, t.rows, h, A.a.q_row, A.a.q_head, A.a.dim);
-    tc_load<T, DP, 128>(sb + Shape::kG, A.a.grad_out, t.row, t.rows, h,
-                        (int64_t)A.a.heads * A.a.dim, A.a.dim, A.a.dim);
+    tc_load<T, DP, 128, kThreads>(sb + Shape::kQ, A.a.q, t.row, t.rows, h, A.a.q_row, A.a.q_head, A.a.dim);
+    tc_load<T, DP, 128, kThreads>(sb + Shape::kG, A.a.grad_out, t.row, t.rows, h,
+                                  (int64_t)A.a.heads * A.a.dim, A.a.dim, A.a.dim);
     if (tiles > 0) load_tile(0);
-    const int64_t at = (((int64_t)t.row + tid) * A.a.heads + h) * A.a.dim;
-    float* delta_at = A.a.delta + (int64_t)h * A.a.q_rows + t.row + tid;
+    const int64_t at = (((int64_t)t.row + r) * A.a.heads + h) * A.a.dim;
+    float* delta_at = A.a.delta + (int64_t)h * A.a.q_rows + t.row + r;
     if (BIAS) {
-        if (Shape::kTight) {
-            for (int e = tid; e < entries; e += kTcThreads) table[e] = table_entry(A.a, e, h) * kLog2e;
-        } else {
+        if (!Shape::kTight) {
             tc_load_table(A, table, h);
+        } else if (entries <= Shape::kTightEntries) {
+            for (int e = tid; e < entries; e += kThreads) table[e] = table_entry(A.a, e, h) * kLog2e;
         }
     }
-    if (Shape::kCells)
-        for (int e = lane; e < entries * 32; e += 32) cells[e] = 0.f;
-    const float lse2 = live ? load_lse2(A, t.row + tid, h) : INFINITY;
+    if (Shape::kCells) {
+        float* all = table + Shape::table_words(entries);
+        for (int e = tid; e < entries * 128; e += kThreads) all[e] = 0.f;
+    }
+    const float lse2 = live ? load_lse2(A, t.row + r, h) : INFINITY;
     tc_load_done();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
-    const uint32_t mine = tmem + ((uint32_t)(tid & ~31) << 16);
+    const uint32_t mine = tmem + ((uint32_t)quarter << 21);  // lanes 32 quarter ..
     Waiter done(sb + Shape::kBar, A.a.status);
     if (tid == 0 && tiles > 0) {
         mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kQ, sb + Shape::kK);
         mma_scores<T, DP, kTcCols>(tmem + Shape::kDP, sb + Shape::kG, sb + Shape::kV);
         mma_commit(sb + Shape::kBar);
     }
-    float delta = 0.f;  // D; kDelta: its sum so far
+    float delta = 0.f;  // D; kDelta: this thread's columns of its sum so far
     if (MODE == kGradQTable) {
         if (live) delta = *delta_at;
     } else if (MODE == kGradQ && live) {
         for (int c = 0; c * 8 < A.a.dim; ++c) {
             float g[8], o[8];
-            Elem<T>::unpack(*reinterpret_cast<const uint4*>(smem + Shape::kG + TcTile<DP>::at(128, tid, c)), g);
+            Elem<T>::unpack(*reinterpret_cast<const uint4*>(smem + Shape::kG + TcTile<DP>::at(128, r, c)), g);
             Elem<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(A.a.out) + at + c * 8), o);
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = fmaf(g[e], o[e], delta);
         }
-        *delta_at = delta;
+        if (group == 0) *delta_at = delta;
     }
     const f32x2 scale2 = pack2(A.scale_log2, A.scale_log2), lse22 = pack2(-lse2, -lse2);
+    // Group a's cells of axis a: the bias addresses moved to this quarter's cells.
+    int cell_add = 0, cell_lo = 0, cell_hi = 0;
+    if (Shape::kCells) {
+        const int move = (int)smem_u32(cells) - (int)(sb + Shape::kTable);
+#pragma unroll
+        for (int a = 0; a < kAttnMaxAxes; ++a)
+            if (a == group) {
+                cell_add = bias.add[a] + move;
+                cell_lo = bias.lo[a] + move;
+                cell_hi = bias.hi[a] + move;
+            }
+    }
 
     for (int i = 0; i < tiles; ++i) {
         done.wait();
@@ -142,101 +165,88 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
                            all_visible(A, t.first, t.first + 127, k0, k0 + kTcCols - 1);
         uint64_t seen = whole ? ~0ull : live ? seen_keys(A, p, k0, n) : 0ull;
         if (BIAS && bias.far) seen = 0ull;
-        const bool all = __all_sync(FULL_MASK, seen == ~0ull);
-        const int* cols = kpos + (i % kStages) * 3 * kTcCols;
+        seen >>= group * kPer;
+        const uint64_t full = kPer == 64 ? ~0ull : (1ull << (kPer & 63)) - 1;
+        const bool all = __all_sync(FULL_MASK, (seen & full) == full);
+        const int* cols = kpos + (i % Shape::kPosStages) * 3 * kTcCols;
+        float s[kPer];
 #pragma unroll
-        for (int c = 0; c < kTcCols; c += 16) {
-            float s[16], dp[16];
-            tmem_ld16(mine + Shape::kS + c, s);
-            tmem_ld16(mine + Shape::kDP + c, dp);
+        for (int c = 0; c < kPer; c += 16) tmem_ld16(mine + Shape::kS + group * kPer + c, s + c);
+#pragma unroll
+        for (int c = 0; c < kPer; c += 16) {
+            float dp[16];
+            tmem_ld16(mine + Shape::kDP + group * kPer + c, dp);
             tmem_wait_ld();
-            tmem_use(s);
+            if (c == 0) tmem_use(s);
             tmem_use(dp);
-            int cell[kAttnMaxAxes][16];
             f32x2 b[8];
-            if (Shape::kCells) {
+            if (Shape::kTight) {
 #pragma unroll
                 for (int a = 0; a < kAttnMaxAxes; ++a)
                     if (a < A.a.axes) {
 #pragma unroll
-                        for (int e = 0; e < 16; e += 4) {
-                            const int4 c4 = *reinterpret_cast<const int4*>(cols + a * kTcCols + c + e);
-                            cell[a][e] = bias.address<BIAS == 2>(A, a, c4.x);
-                            cell[a][e + 1] = bias.address<BIAS == 2>(A, a, c4.y);
-                            cell[a][e + 2] = bias.address<BIAS == 2>(A, a, c4.z);
-                            cell[a][e + 3] = bias.address<BIAS == 2>(A, a, c4.w);
-                        }
-#pragma unroll
                         for (int e = 0; e < 16; e += 2) {
-                            const int x = Shape::kTight ? (int)(sb + Shape::kTable) + 4 * a * A.a.buckets +
-                                                              ((cell[a][e] - bias.lo[a]) >> 5)
-                                                        : cell[a][e] + to_table;
-                            const int y = Shape::kTight ? (int)(sb + Shape::kTable) + 4 * a * A.a.buckets +
-                                                              ((cell[a][e + 1] - bias.lo[a]) >> 5)
-                                                        : cell[a][e + 1] + to_table;
-                            const f32x2 v = pack2(lds_table(x), lds_table(y));
-                            b[e / 2] = a ? add2(b[e / 2], v) : v;
+                            float v[2];
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const int word = (bias.address<BIAS == 2>(
+                                                      A, a, cols[a * kTcCols + group * kPer + c + e + k]) -
+                                                  bias.lo[a]) >> 7;
+                                v[k] = entries <= Shape::kTightEntries
+                                           ? table[a * A.a.buckets + word]
+                                           : table_entry(A.a, a * A.a.buckets + word, h) * kLog2e;
+                            }
+                            const f32x2 x = pack2(v[0], v[1]);
+                            b[e / 2] = a ? add2(b[e / 2], x) : x;
                         }
                     }
             } else if (BIAS) {
-                bias16<BIAS == 2>(A, bias, cols + c, b);
+                bias16<BIAS == 2>(A, bias, cols + group * kPer + c, b);
             }
             const uint32_t bits = (uint32_t)(seen >> c);
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-                f32x2 x = fma2(pack2(s[e], s[e + 1]), scale2, lse22);
+                f32x2 x = fma2(pack2(s[c + e], s[c + e + 1]), scale2, lse22);
                 if (BIAS) x = add2(x, b[e / 2]);
                 float u, v;
                 unpack2(x, u, v);
                 u = exp2_sfu(u);
                 v = exp2_sfu(v);
                 if (MODE == kDelta) {
-                    s[e] = u * dp[e];
-                    s[e + 1] = v * dp[e + 1];
+                    s[c + e] = u * dp[e];
+                    s[c + e + 1] = v * dp[e + 1];
                 } else {
-                    s[e] = u * (dp[e] - delta);
-                    s[e + 1] = v * (dp[e + 1] - delta);
+                    s[c + e] = u * (dp[e] - delta);
+                    s[c + e + 1] = v * (dp[e + 1] - delta);
                 }
             }
             if (!all) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] = (bits >> e) & 1u ? s[e] : 0.f;
+                for (int e = 0; e < 16; ++e) s[c + e] = (bits >> e) & 1u ? s[c + e] : 0.f;
             }
             if (MODE == kDelta) {
-                f32x2 sum = pack2(s[0], s[1]);
+                f32x2 sum = pack2(s[c], s[c + 1]);
 #pragma unroll
-                for (int e = 2; e < 16; e += 2) sum = add2(sum, pack2(s[e], s[e + 1]));
+                for (int e = 2; e < 16; e += 2) sum = add2(sum, pack2(s[c + e], s[c + e + 1]));
                 float u, v;
                 unpack2(sum, u, v);
                 delta += u + v;
-                continue;
+            } else {
+                if (Shape::kCells)
+                    tmem_st16(mine + Shape::kDS + (i & 1) * kTcCols + group * kPer + c,
+                              reinterpret_cast<const uint32_t*>(s + c));
+                uint32_t w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = Elem<T>::two(s[c + 2 * e], s[c + 2 * e + 1]);
+                tmem_st8(mine + Shape::kS + group * kPer + c, w);
             }
-            if (Shape::kCells) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    // Cells of different axes are different: read the three, then write them.
-                    float v[kAttnMaxAxes];
-#pragma unroll
-                    for (int a = 0; a < kAttnMaxAxes; ++a)
-                        if (a < A.a.axes)
-                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[a]) : "r"(cell[a][e]));
-#pragma unroll
-                    for (int a = 0; a < kAttnMaxAxes; ++a)
-                        if (a < A.a.axes)
-                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(cell[a][e]), "f"(v[a] + s[e]));
-                }
-            }
-            uint32_t w[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = Elem<T>::two(s[2 * e], s[2 * e + 1]);
-            tmem_st8(mine + Shape::kS + c / 2, w);  // over columns already read
         }
-        tmem_wait_st();
+        if (MODE != kDelta) tmem_wait_st();
         tc_load_done();
         tc_fence_before();
         __syncthreads();
+        tc_fence_after();
         if (tid == 0) {
-            tc_fence_after();
             const uint32_t stage = (i % kStages) * Shape::kStage, next = Shape::kStage - stage;
             if (MODE != kDelta)
                 mma_weighted<T, DP, kTcCols>(tmem + Shape::kDQ, tmem + Shape::kS, sb + Shape::kK + stage, i > 0);
@@ -245,6 +255,39 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
                 mma_scores<T, DP, kTcCols>(tmem + Shape::kDP, sb + Shape::kG, sb + Shape::kV + next);
             }
             mma_commit(sb + Shape::kBar);
+        }
+        __syncwarp();
+        if (Shape::kCells && group < A.a.axes) {
+            const int* axis = cols + group * kTcCols;
+#pragma unroll
+            for (int c = 0; c < kTcCols; c += 16) {
+                float ds[16];
+                tmem_ld16(mine + Shape::kDS + (i & 1) * kTcCols + c, ds);
+                int at_cell[16];
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const int4 c4 = *reinterpret_cast<const int4*>(axis + c + e);
+                    at_cell[e] = max(__viaddmin_s32(c4.x, cell_add, cell_hi), cell_lo);
+                    at_cell[e + 1] = max(__viaddmin_s32(c4.y, cell_add, cell_hi), cell_lo);
+                    at_cell[e + 2] = max(__viaddmin_s32(c4.z, cell_add, cell_hi), cell_lo);
+                    at_cell[e + 3] = max(__viaddmin_s32(c4.w, cell_add, cell_hi), cell_lo);
+                }
+                if (BIAS == 2) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        at_cell[e] = cell_lo + 128 * min(max(__ldg(A.a.map + ((at_cell[e] - cell_lo) >> 7)), 0),
+                                                         A.a.buckets - 1);
+                }
+                tmem_wait_ld();
+                tmem_use(ds);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float v;
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at_cell[e]) : "memory");
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(at_cell[e]), "f"(v + ds[e]) : "memory");
+                }
+            }
+            tc_fence_before();
         }
         if (kStages == 1 && i + 1 < tiles) {
             done.wait();  // the keys are free
@@ -263,17 +306,25 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
     if (tiles > 0) done.wait();
     const bool far = BIAS && live && bias.far;
     if (MODE == kDelta) {
-        if (live) *delta_at = delta;
-        __syncwarp();
-        for (unsigned bad = __ballot_sync(FULL_MASK, far); bad; bad &= bad - 1) {
-            const int r = (tid & ~31) + __ffs(bad) - 1;
-            const float d = exact_delta_row<T>(A, (int64_t)t.row + r, t.first + r, t.other, t.lk, h);
-            if (r == tid) *delta_at = d;
+        // The groups' shares in order; the table's place is free now.
+        float* shares = table;
+        __syncthreads();
+        shares[tid] = delta;
+        __syncthreads();
+        if (group == 0) {
+            for (int g = 1; g < Shape::kGroups; ++g) delta += shares[g * kTcRows + r];
+            for (unsigned bad = __ballot_sync(FULL_MASK, far); bad; bad &= bad - 1) {
+                const int row = (r & ~31) + __ffs(bad) - 1;
+                const float d = exact_delta_row<T>(A, (int64_t)t.row + row, t.first + row, t.other, t.lk, h);
+                if (row == r) delta = d;
+            }
+            if (live) *delta_at = delta;
         }
     } else {
         bool nan = far;
 #pragma unroll
         for (int c = 0; c < DP; c += 16) {
+            if ((c / 16) % Shape::kGroups != group) continue;
             float o[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = 0.f;
@@ -293,13 +344,15 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
                 if (c + e < A.a.dim)
                     *reinterpret_cast<uint4*>(static_cast<T*>(A.a.grad_q) + at + c + e) = Elem<T>::pack(o + e);
         }
-        __syncwarp();
-        const unsigned apart = __ballot_sync(FULL_MASK, far);
-        for (unsigned bad = __ballot_sync(FULL_MASK, nan); bad; bad &= bad - 1) {
-            const int r = __ffs(bad) - 1;
-            exact_grad_q_row<T>(A, (int64_t)t.row + (tid & ~31) + r, t.first + (tid & ~31) + r, t.other, t.lk,
-                                h, Shape::kCells && ((apart >> r) & 1u) ? cells : nullptr);
-        }
+        const unsigned bad_here = __ballot_sync(FULL_MASK, nan), apart = __ballot_sync(FULL_MASK, far);
+        if (lane == 0 && bad_here) atomicOr(flags + quarter, bad_here);
+        __syncthreads();
+        if (group == 0)
+            for (unsigned bad = flags[quarter]; bad; bad &= bad - 1) {
+                const int b = __ffs(bad) - 1, row = (r & ~31) + b;
+                exact_grad_q_row<T>(A, (int64_t)t.row + row, t.first + row, t.other, t.lk, h,
+                                    Shape::kCells && ((apart >> b) & 1u) ? cells : nullptr);
+            }
     }
     tc_fence_before();
     __syncthreads();
@@ -308,7 +361,7 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
         tmem_free(tmem, Shape::kCols);
     }
     if (Shape::kCells)
-        for (int e = tid; e < entries; e += kTcThreads) {
+        for (int e = tid; e < entries; e += kThreads) {
             float v = 0.f;
             const float* all = table + Shape::table_words(entries);
             for (int w = 0; w < 4; ++w)
@@ -322,14 +375,15 @@ template <int DP>
 struct GradKvShape {
     static constexpr int kS = 0, kDP = kTcCols, kDK = 2 * kTcCols, kDV = kDK + DP;
     static constexpr int kCols = kDV + DP <= 256 ? 256 : 512;
-    static constexpr int kBlocks = 512 / kCols;
+    static constexpr int kBlocks = 512 / kCols, kGroups = 4 / kBlocks, kThreads = kTcRows * kGroups;
     static constexpr uint32_t kK = 0, kV = TcTile<DP>::bytes(128), kStage = TcTile<DP>::bytes(64),
                               kQ = 2 * kV, kG = kQ + 2 * kStage, kRow = kG + 2 * kStage,
                               kPos = kRow + 2 * 2 * kTcCols * 4, kBar = kPos + 2 * 3 * kTcCols * 4,
-                              kTable = kBar + 16;
+                              kTable = kBar + 64;
     static size_t bytes(int entries) {
         const size_t need = kTable + (size_t)entries * 128 + 1024;
-        return need > kTcPairBytes ? need : kTcPairBytes;
+        const size_t least = 233472 / (kBlocks + 1);
+        return need > least ? need : least;
     }
 };
 
@@ -338,18 +392,19 @@ struct GradKvShape {
 // ([cloud * sink tiles + tile][key head][share][dk, dv][128][dim], float32) for
 // the join kernel.  shares == 1: no block does.
 template <typename T, int DP, int BIAS>
-__global__ void __launch_bounds__(kTcThreads, (GradKvShape<DP>::kBlocks))
+__global__ void __launch_bounds__((GradKvShape<DP>::kThreads), (GradKvShape<DP>::kBlocks))
 attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __restrict__ partial) {
     using Shape = GradKvShape<DP>;
+    constexpr int kThreads = Shape::kThreads, kPer = kTcCols / Shape::kGroups;
     const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.k_tiles)[blockIdx.x];
     const bool shared = shares > 1 && t.first < A.a.sinks;
     if (!shared && blockIdx.z > 0) return;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sb = smem_u32(smem);
-    const int tid = threadIdx.x, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31, r = tid & 127, quarter = r >> 5, group = tid >> 7;
     const int hk = blockIdx.y, h0 = hk * A.group;
-    const int j = t.first + tid;
+    const int j = t.first + r;
     int* qpos = reinterpret_cast<int*>(smem + Shape::kPos);
     float* rows = reinterpret_cast<float*>(smem + Shape::kRow);  // [stage][-lse2, -D][64]
     const f32x2 scale2 = pack2(A.scale_log2, A.scale_log2);
@@ -358,6 +413,8 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
 
     if (tid < 32) tmem_alloc(smem_u32(slot), Shape::kCols);
     if (tid == 0) mbar_init(sb + Shape::kBar);
+    unsigned* flags = reinterpret_cast<unsigned*>(smem + Shape::kBar + 16);  // rows to form again
+    if (tid < 4) flags[tid] = 0u;
     int lo, hi;
     query_span(A, t.first, t.first + t.rows - 1, t.lq, t.lk, lo, hi);
     int first = 0, per = hi > lo ? (hi - lo + kTcCols - 1) / kTcCols : 0;
@@ -366,28 +423,28 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
         per = (int)((int64_t)per * (blockIdx.z + 1) / shares) - first;
     }
     const int tiles = per * A.group;
-    const bool live = tid < t.rows;
+    const bool live = r < t.rows;
     BiasRow bias;
-    if (BIAS) bias.init(A, A.a.kpos, t.row, tid, live, sb + Shape::kTable, -1);
+    if (BIAS) bias.init(A, A.a.kpos, t.row, r, live, sb + Shape::kTable, -1);
     auto query0 = [&](int i) { return lo + (first + i % per) * kTcCols; };
     auto load_tile = [&](int i) {
         const int i0 = query0(i), n = min(kTcCols, hi - i0), h = h0 + i / per;
         const int64_t row = (int64_t)t.other + i0;
         const uint32_t stage = (i & 1) * Shape::kStage;
-        tc_load<T, DP, kTcCols>(sb + Shape::kQ + stage, A.a.q, row, n, h, A.a.q_row, A.a.q_head, A.a.dim);
-        tc_load<T, DP, kTcCols>(sb + Shape::kG + stage, A.a.grad_out, row, n, h,
+        tc_load<T, DP, kTcCols, kThreads>(sb + Shape::kQ + stage, A.a.q, row, n, h, A.a.q_row, A.a.q_head, A.a.dim);
+        tc_load<T, DP, kTcCols, kThreads>(sb + Shape::kG + stage, A.a.grad_out, row, n, h,
                                 (int64_t)A.a.heads * A.a.dim, A.a.dim, A.a.dim);
         float* dst = rows + (i & 1) * 2 * kTcCols;
         if (tid < kTcCols) {
             dst[tid] = tid < n ? -load_lse2(A, row + tid, h) : -INFINITY;
-        } else {
-            const int r = tid - kTcCols;
-            dst[tid] = r < n ? -A.a.delta[(int64_t)h * A.a.q_rows + row + r] : 0.f;
+        } else if (tid < 2 * kTcCols) {
+            const int c = tid - kTcCols;
+            dst[tid] = c < n ? -A.a.delta[(int64_t)h * A.a.q_rows + row + c] : 0.f;
         }
         if (BIAS) tc_load_columns(qpos + (i & 1) * 3 * kTcCols, A.a.qpos, row, n, A.a.axes, bias, -1);
     };
-    tc_load<T, DP, 128>(sb + Shape::kK, A.a.k, t.row, t.rows, hk, A.a.k_row, A.a.k_head, A.a.dim);
-    tc_load<T, DP, 128>(sb + Shape::kV, A.a.v, t.row, t.rows, hk, A.a.v_row, A.a.v_head, A.a.dim);
+    tc_load<T, DP, 128, kThreads>(sb + Shape::kK, A.a.k, t.row, t.rows, hk, A.a.k_row, A.a.k_head, A.a.dim);
+    tc_load<T, DP, 128, kThreads>(sb + Shape::kV, A.a.v, t.row, t.rows, hk, A.a.v_row, A.a.v_head, A.a.dim);
     if (tiles > 0) load_tile(0);
     if (BIAS) tc_load_table(A, table, h0);
     tc_load_done();
@@ -395,7 +452,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
-    const uint32_t mine = tmem + ((uint32_t)(tid & ~31) << 16);
+    const uint32_t mine = tmem + ((uint32_t)quarter << 21);
     Waiter done(sb + Shape::kBar, A.a.status);
     if (tid == 0 && tiles > 0) {
         mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kK, sb + Shape::kQ);
@@ -414,12 +471,15 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
                            all_visible(A, p0, p0 + kTcCols - 1, t.first, t.first + 127);
         uint64_t seen = whole ? ~0ull : live ? seeing_queries(A, j, p0, n) : 0ull;
         if (BIAS && bias.far) seen = 0ull;
-        const bool all = __all_sync(FULL_MASK, seen == ~0ull);
+        seen >>= group * kPer;
+        const uint64_t full = (1ull << kPer) - 1;
+        const bool all = __all_sync(FULL_MASK, (seen & full) == full);
         const int* cols = qpos + (i & 1) * 3 * kTcCols;
         const float* row = rows + (i & 1) * 2 * kTcCols;
 #pragma unroll
-        for (int c = 0; c < kTcCols; c += 16) {
+        for (int cc = 0; cc < kPer; cc += 16) {
             float s[16], dp[16];
+            const int c = group * kPer + cc;
             tmem_ld16(mine + Shape::kS + c, s);
             tmem_ld16(mine + Shape::kDP + c, dp);
             tmem_wait_ld();
@@ -444,7 +504,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
                 unpack2(add2(pack2(dp[e], dp[e + 1]), d0), dp[e], dp[e + 1]);
                 unpack2(add2(pack2(dp[e + 2], dp[e + 3]), d1), dp[e + 2], dp[e + 3]);
             }
-            const uint32_t bits = (uint32_t)(seen >> c);
+            const uint32_t bits = (uint32_t)(seen >> cc);
             uint32_t w[8], g[8];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -464,8 +524,8 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
                 w[e] = Elem<T>::two(s[2 * e], s[2 * e + 1]);
                 g[e] = Elem<T>::two(dp[2 * e], dp[2 * e + 1]);
             }
-            tmem_st8(mine + Shape::kS + c / 2, w);
-            tmem_st8(mine + Shape::kDP + c / 2, g);
+            tmem_st8(mine + Shape::kS + c, w);
+            tmem_st8(mine + Shape::kDP + c, g);
         }
         tmem_wait_st();
         tc_load_done();
@@ -485,17 +545,18 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
     }
     if (tiles > 0) done.wait();
     bool nan = BIAS && live && bias.far;
-    const int64_t at = (((int64_t)t.row + tid) * A.a.kv_heads + hk) * A.a.dim;
+    const int64_t at = (((int64_t)t.row + r) * A.a.kv_heads + hk) * A.a.dim;
     const int sink_tiles = (A.a.sinks + kAttnTile - 1) / kAttnTile;
     float* sums = nullptr;
     if (shared) {
         const int64_t tile = (int64_t)t.cloud * sink_tiles + t.first / kAttnTile;
-        sums = partial + (((tile * A.a.kv_heads + hk) * shares + blockIdx.z) * 2 * kAttnTile + tid) * A.a.dim;
+        sums = partial + (((tile * A.a.kv_heads + hk) * shares + blockIdx.z) * 2 * kAttnTile + r) * A.a.dim;
     }
 #pragma unroll
     for (int which = 0; which < 2; ++which)
 #pragma unroll
         for (int c = 0; c < DP; c += 16) {
+            if ((c / 16) % Shape::kGroups != group) continue;
             float o[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = 0.f;
@@ -524,11 +585,13 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
                 }
             }
         }
-    __syncwarp();
-    if (!shared)
-        for (unsigned bad = __ballot_sync(FULL_MASK, nan); bad; bad &= bad - 1) {
-            const int r = (tid & ~31) + __ffs(bad) - 1;
-            exact_grad_kv_row<T>(A, t.base, t.first + r, t.other, t.lq, t.lk, hk);
+    const unsigned bad_here = __ballot_sync(FULL_MASK, nan);
+    if (lane == 0 && bad_here) atomicOr(flags + quarter, bad_here);
+    __syncthreads();
+    if (!shared && group == 0)
+        for (unsigned bad = flags[quarter]; bad; bad &= bad - 1) {
+            const int row = (r & ~31) + __ffs(bad) - 1;
+            exact_grad_kv_row<T>(A, t.base, t.first + row, t.other, t.lq, t.lk, hk);
         }
     tc_fence_before();
     __syncthreads();
@@ -583,11 +646,11 @@ size_t sink_bytes(const AttnArgs& A) {
 
 template <typename T, int DP, int BIAS, int MODE>
 int run_q(const AttnArgs& A, float* partial, cudaStream_t s) {
-    const size_t bytes = GradQShape<DP, MODE>::bytes(BIAS ? A.a.axes * A.a.buckets : 0);
+    const size_t bytes = QueryShape<DP, MODE>::bytes(BIAS ? A.a.axes * A.a.buckets : 0);
     const int st = tc_prepare(attn_tc_query_kernel<T, DP, BIAS, MODE>, bytes, "attn_tc_query_kernel");
     if (st != kOk) return st;
     const dim3 grid((unsigned)A.a.q_tile_count, (unsigned)A.a.heads);
-    attn_tc_query_kernel<T, DP, BIAS, MODE><<<grid, kTcThreads, bytes, s>>>(A, partial);
+    attn_tc_query_kernel<T, DP, BIAS, MODE><<<grid, QueryShape<DP, MODE>::kThreads, bytes, s>>>(A, partial);
     return check_launch("attn_tc_query_kernel");
 }
 template <typename T, int DP, int BIAS>
@@ -597,7 +660,7 @@ int run_kv(const AttnArgs& A, float* partial, cudaStream_t s) {
     if (st != kOk) return st;
     const int shares = sink_shares(A);
     dim3 grid((unsigned)A.a.k_tile_count, (unsigned)A.a.kv_heads, (unsigned)shares);
-    attn_tc_grad_kv_kernel<T, DP, BIAS><<<grid, kTcThreads, bytes, s>>>(A, shares, partial);
+    attn_tc_grad_kv_kernel<T, DP, BIAS><<<grid, GradKvShape<DP>::kThreads, bytes, s>>>(A, shares, partial);
     st = check_launch("attn_tc_grad_kv_kernel");
     if (st != kOk || shares == 1) return st;
     grid.z = kAttnTile / 8;

@@ -34,7 +34,7 @@ struct FwdShape {
 };
 
 template <typename T, int DP, int BIAS>
-__global__ void __launch_bounds__(kTcThreads, (BIAS && DP <= 64 ? 3 : FwdShape<DP>::kBlocks))
+__global__ void __launch_bounds__(kTcRows, (BIAS && DP <= 64 ? 3 : FwdShape<DP>::kBlocks))
 attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
     using Shape = FwdShape<DP>;
     extern __shared__ unsigned char smem_raw[];
@@ -58,11 +58,11 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
         const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
         const int64_t row = (int64_t)t.other + k0;
         const uint32_t stage = (i & 1) * Shape::kStage;
-        tc_load<T, DP, kTcCols>(sb + Shape::kK + stage, A.a.k, row, n, hk, A.a.k_row, A.a.k_head, A.a.dim);
-        tc_load<T, DP, kTcCols>(sb + Shape::kV + stage, A.a.v, row, n, hk, A.a.v_row, A.a.v_head, A.a.dim);
+        tc_load<T, DP, kTcCols, kTcRows>(sb + Shape::kK + stage, A.a.k, row, n, hk, A.a.k_row, A.a.k_head, A.a.dim);
+        tc_load<T, DP, kTcCols, kTcRows>(sb + Shape::kV + stage, A.a.v, row, n, hk, A.a.v_row, A.a.v_head, A.a.dim);
         if (BIAS) tc_load_columns(kpos + (i & 1) * 3 * kTcCols, A.a.kpos, row, n, A.a.axes, bias, 1);
     };
-    tc_load<T, DP, 128>(sb + Shape::kQ, A.a.q, t.row, t.rows, h, A.a.q_row, A.a.q_head, A.a.dim);
+    tc_load<T, DP, 128, kTcRows>(sb + Shape::kQ, A.a.q, t.row, t.rows, h, A.a.q_row, A.a.q_head, A.a.dim);
     if (tiles > 0) load_tile(0);
     if (BIAS) tc_load_table(A, table, h);
     tc_load_done();
@@ -159,7 +159,7 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
                 part[(e >> 1) & 1] = add2(part[(e >> 1) & 1], pack2(a, b));
                 w[e / 2] = Elem<T>::two(a, b);
             }
-            tmem_st8(mine + Shape::kS + c / 2, w);
+            tmem_st8(mine + Shape::kS + c, w);
         }
         {
             float a, b;
@@ -228,7 +228,7 @@ int run(const AttnArgs& A, cudaStream_t s) {
     const int st = tc_prepare(attn_tc_fwd_kernel<T, DP, BIAS>, bytes, "attn_tc_fwd_kernel");
     if (st != kOk) return st;
     const dim3 grid((unsigned)A.a.q_tile_count, (unsigned)A.a.heads);
-    attn_tc_fwd_kernel<T, DP, BIAS><<<grid, kTcThreads, bytes, s>>>(A);
+    attn_tc_fwd_kernel<T, DP, BIAS><<<grid, kTcRows, bytes, s>>>(A);
     return check_launch("attn_tc_fwd_kernel");
 }
 template <typename T, int DP>
