@@ -66,6 +66,16 @@ struct Waiter {
     }
 };
 
+// Two barriers used in turn: step i waits for what step i - 2 committed.
+struct WaiterPair {
+    Waiter even, odd;
+    __device__ __forceinline__ WaiterPair(uint32_t bars, int32_t* st) : even(bars, st), odd(bars + 8, st) {}
+    __device__ __forceinline__ void wait(int i) {
+        if (i & 1) odd.wait();
+        else even.wait();
+    }
+};
+
 // ---------------------------------------------------------------- TMEM
 __device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t cols) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot),
@@ -172,8 +182,12 @@ __device__ __forceinline__ void tc_load(uint32_t tile, const void* base, int64_t
                      : "memory");
     }
 }
-__device__ __forceinline__ void tc_load_done() {
-    asm volatile("cp.async.wait_all;" ::: "memory");
+// Closes a group of copies; waits until at most PENDING younger groups are open
+// and shows what has landed to the tensor core.
+__device__ __forceinline__ void tc_load_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void tc_load_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
@@ -294,19 +308,25 @@ struct BiasRow {
         return at;
     }
 };
-// Columns [r0, r0 + n) by axis: dst[axis * 64 + column].
-__device__ __forceinline__ void tc_load_columns(int* dst, const int32_t* pos, int64_t r0, int n, int axes,
-                                                const BiasRow& row, int sign) {
-    if (threadIdx.x < kTcCols) {
+// Positions of columns [r0, r0 + n) by axis, dst[axis * 64 + column]: fetched into
+// registers by the first 64 threads and stored later, past the latency.
+struct Columns {
+    int v[kAttnMaxAxes];
+    __device__ __forceinline__ void fetch(const int32_t* pos, int64_t r0, int n, int axes) {
 #pragma unroll
         for (int a = 0; a < kAttnMaxAxes; ++a)
-            if (a < axes)
-                dst[a * kTcCols + threadIdx.x] =
-                    threadIdx.x < n
-                        ? BiasRow::column(pos[(r0 + threadIdx.x) * axes + a], row.ref[a], sign)
-                        : 0;
+            if (a < axes && (int)threadIdx.x < n) v[a] = pos[(r0 + threadIdx.x) * axes + a];
     }
-}
+    __device__ __forceinline__ void store(int* dst, int n, int axes, const BiasRow& row, int sign) const {
+        if (threadIdx.x < kTcCols) {
+#pragma unroll
+            for (int a = 0; a < kAttnMaxAxes; ++a)
+                if (a < axes)
+                    dst[a * kTcCols + threadIdx.x] =
+                        (int)threadIdx.x < n ? BiasRow::column(v[a], row.ref[a], sign) : 0;
+        }
+    }
+};
 // The table does not change while columns are read: free to move.
 __device__ __forceinline__ float lds_table(int addr) {
     float v;
@@ -314,18 +334,25 @@ __device__ __forceinline__ float lds_table(int addr) {
     return v;
 }
 // Bias of 16 columns as pairs; cols: the staged columns of axis 0 at column c.
-template <bool MAPPED>
-__device__ __forceinline__ void bias16(const AttnArgs& A, const BiasRow& row, const int* cols, f32x2 (&t)[8]) {
+// ONE: the table has one copy, at `one` (null: read it from global memory, for
+// head h); addresses are then used as entry numbers.
+template <bool MAPPED, bool ONE>
+__device__ __forceinline__ void bias16(const AttnArgs& A, const BiasRow& row, const int* cols, f32x2 (&t)[8],
+                                       const float* one, int h) {
+    auto entry = [&](int a, int col) {
+        const int at = row.template address<MAPPED>(A, a, col);
+        if (!ONE) return lds_table(at);
+        const int e = a * A.a.buckets + ((at - row.lo[a]) >> 7);
+        return one ? one[e] : table_entry(A.a, e, h) * kLog2e;
+    };
 #pragma unroll
     for (int a = 0; a < kAttnMaxAxes; ++a)
         if (a < A.a.axes) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 const int4 c4 = *reinterpret_cast<const int4*>(cols + a * kTcCols + e);
-                const f32x2 x = pack2(lds_table(row.address<MAPPED>(A, a, c4.x)),
-                                      lds_table(row.address<MAPPED>(A, a, c4.y)));
-                const f32x2 y = pack2(lds_table(row.address<MAPPED>(A, a, c4.z)),
-                                      lds_table(row.address<MAPPED>(A, a, c4.w)));
+                const f32x2 x = pack2(entry(a, c4.x), entry(a, c4.y));
+                const f32x2 y = pack2(entry(a, c4.z), entry(a, c4.w));
                 t[e / 2] = a ? add2(t[e / 2], x) : x;
                 t[e / 2 + 1] = a ? add2(t[e / 2 + 1], y) : y;
             }

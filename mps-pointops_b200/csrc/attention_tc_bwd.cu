@@ -9,10 +9,9 @@
 // dP are formed twice, which the tensor cores have time for beside the
 // exponentials.
 //
-// Per tile of 64 columns the tensor core forms S and dP in TMEM, a thread turns
-// its row of them into 16-bit pairs of the score gradient (and of the weight)
-// over the same columns, and these are the left operands of the accumulating
-// products; those and the next tile's S and dP go out in one issue.
+// Per tile of 64 columns the tensor core forms S and dP in TMEM, the threads of a
+// row turn them into 16-bit pairs of the score gradient (and of the weight) over
+// the same columns, and these are the left operands of the accumulating products.
 #include <string>
 
 #include "attention_exact.cuh"
@@ -28,48 +27,56 @@ namespace {
 // stored and tensor-core results are off by 2e-3 and (sums rounded towards zero)
 // 3e-6 of it, always the same way for all pairs of a row.  kDelta forms D = sum
 // P dP in float32 first; kGradQTable then forms dq and the table's gradient.
+constexpr size_t kTcSmem = 232448;  // shared memory of a block at most
 enum QueryMode { kGradQ = 0, kDelta = 1, kGradQTable = 2 };
 
-// Threads: NG groups of 128; thread `row` of each group shares the row and takes
-// 64 / NG columns of every tile, so that 16 warps are on an SM (one thread per
+// Threads: four groups of 128; thread `row` of each group shares the row and
+// takes 16 columns of every tile, so that 16 warps are on an SM (one thread per
 // row left 4 to 8, and most of the time went to fixed latencies).
+//
+// S and dP have two buffers in TMEM.  At the end of step i the tensor core gets
+// dq += dS_i K_i and then, over the buffer that this frees, S and dP of tile
+// i + 2: those of tile i + 1 are ready when the step's barrier falls.
 //
 // Table gradient: a thread may only add to cells that no other adds to, so lane
 // l of quarter w (rows 32 w ..) has its own cell of each entry ([w][entry][l],
 // its own bank: a plain read, add and write, no atomics), and group a keeps
 // those of axis a: the groups leave their score gradients in TMEM as float32
 // (two buffers), and after the tile's barrier group a adds all 64 columns of
-// them to its axis while the tensor core forms the next tile's S and dP.  With
-// DP = 128 the cells (up to 128 KB) leave room for one stage of keys and values
-// and for one copy of the table.
+// them to its axis.  With DP = 128 the cells (up to 128 KB) leave room for one
+// stage of keys and values, one buffer of S and dP, and one copy of the table.
+constexpr int kBwdThreads = 4 * kTcRows, kBwdCols = kTcCols / 4;
 template <int DP, int MODE>
 struct QueryShape {
     static constexpr bool kCells = MODE == kGradQTable, kTight = kCells && DP == 128;
-    static constexpr int kBlocks = kCells || DP == 128 ? 1 : 2, kGroups = 4 / kBlocks;
-    static constexpr int kThreads = kTcRows * kGroups;
-    static constexpr int kStages = kTight ? 1 : 2, kPosStages = kCells && !kTight ? 4 : 2;
-    static constexpr int kS = 0, kDP = kTcCols, kDQ = 2 * kTcCols, kDS = kDQ + DP;
-    static constexpr int kCols = kCells ? 512 : MODE == kDelta ? 128 : 256;
+    // Keys serve S and dq of their tile, values dP alone.
+    static constexpr int kKStages = kTight ? 1 : 4, kVStages = kTight ? 1 : 2, kPosStages = kTight ? 2 : 4;
+    static constexpr int kS = 0, kDP = kTcCols, kBuffer = kTight ? 0 : 2 * kTcCols;  // TMEM columns
+    static constexpr int kDQ = 2 * kTcCols + kBuffer, kDS = kDQ + DP;
+    static constexpr int kCols = MODE == kDelta ? 256 : 512;
     static constexpr uint32_t kQ = 0, kG = TcTile<DP>::bytes(128), kStage = TcTile<DP>::bytes(64),
-                              kK = 2 * kG, kV = kK + kStages * kStage, kPos = kV + kStages * kStage,
+                              kK = 2 * kG, kV = kK + kKStages * kStage, kPos = kV + kVStages * kStage,
                               kBar = kPos + kPosStages * 3 * kTcCols * 4, kTable = kBar + 64;
-    static constexpr int kTightEntries = 248;  // the table fits beside this many cells
-    static __host__ __device__ constexpr int table_words(int entries) {
-        return !kTight ? entries * 32 : entries > kTightEntries ? 0 : (entries + 3) / 4 * 4;
+    static constexpr int kTightEntries = 248;  // the table fits beside this many cells (DP = 128)
+    static __host__ __device__ constexpr int table_words(int entries, bool one) {
+        return !one ? entries * 32 : kTight && entries > kTightEntries ? 0 : (entries + 3) / 4 * 4;
     }
-    static size_t bytes(int entries) {
-        size_t need = kTable + (size_t)table_words(entries) * 4 + (kCells ? (size_t)entries * 512 : 0) + 1024;
-        if (MODE == kDelta && need < kTable + 4 * 4 * kTcRows + 1024) need = kTable + 4 * 4 * kTcRows + 1024;
-        const size_t least = 233472 / (kBlocks + 1);  // no more blocks than the registers were cut for
-        return need > least ? need : least;
+    // One copy of the table where a copy per lane does not fit beside the cells.
+    static bool one_copy(int entries) {
+        return kTight || (kCells && kTable + (size_t)entries * 640 + 1024 > kTcSmem);
+    }
+    static size_t bytes(int entries, bool one) {
+        size_t need = kTable + (size_t)table_words(entries, one) * 4 + (kCells ? (size_t)entries * 512 : 0) + 1024;
+        if (MODE == kDelta && need < kTable + 4 * kBwdThreads + 1024) need = kTable + 4 * kBwdThreads + 1024;
+        return need > 233472 / 2 ? need : 233472 / 2;  // one block per SM: TMEM serves no second one
     }
 };
 
-template <typename T, int DP, int BIAS, int MODE>
-__global__ void __launch_bounds__((QueryShape<DP, MODE>::kThreads), (QueryShape<DP, MODE>::kBlocks))
+template <typename T, int DP, int BIAS, int MODE, bool ONE>
+__global__ void __launch_bounds__(kBwdThreads, 1)
 attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ partial) {
     using Shape = QueryShape<DP, MODE>;
-    constexpr int kStages = Shape::kStages, kThreads = Shape::kThreads, kPer = kTcCols / Shape::kGroups;
+    constexpr int kThreads = kBwdThreads;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sb = smem_u32(smem);
@@ -79,12 +86,15 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
     const int p = t.first + r, entries = A.a.axes * A.a.buckets;
     int* kpos = reinterpret_cast<int*>(smem + Shape::kPos);
     float* table = reinterpret_cast<float*>(smem + Shape::kTable);
-    float* cells = table + Shape::table_words(entries) + quarter * entries * 32;  // this quarter's
-    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kBar + 8);
-    unsigned* flags = reinterpret_cast<unsigned*>(smem + Shape::kBar + 16);  // rows to form again
+    float* cells = table + Shape::table_words(entries, ONE) + quarter * entries * 32;  // this quarter's
+    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kBar + 16);
+    unsigned* flags = reinterpret_cast<unsigned*>(smem + Shape::kBar + 32);  // rows to form again
 
     if (tid < 32) tmem_alloc(smem_u32(slot), Shape::kCols);
-    if (tid == 0) mbar_init(sb + Shape::kBar);
+    if (tid == 0) {
+        mbar_init(sb + Shape::kBar);
+        mbar_init(sb + Shape::kBar + 8);
+    }
     if (tid < 4) flags[tid] = 0u;
     const KeySpan span = key_span(A, t.first, t.first + t.rows - 1, t.lk, kTcCols);
     const int tiles = span.count();
@@ -92,44 +102,76 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
     BiasRow bias;
     if (BIAS) bias.init(A, A.a.qpos, t.row, r, live, sb + Shape::kTable, 1);
     auto load_tile = [&](int i) {
+        if (i >= tiles) return;
         const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
         const int64_t row = (int64_t)t.other + k0;
-        const uint32_t stage = (i % kStages) * Shape::kStage;
-        tc_load<T, DP, kTcCols, kThreads>(sb + Shape::kK + stage, A.a.k, row, n, hk, A.a.k_row, A.a.k_head, A.a.dim);
-        tc_load<T, DP, kTcCols, kThreads>(sb + Shape::kV + stage, A.a.v, row, n, hk, A.a.v_row, A.a.v_head, A.a.dim);
-        if (BIAS)
-            tc_load_columns(kpos + (i % Shape::kPosStages) * 3 * kTcCols, A.a.kpos, row, n, A.a.axes, bias, 1);
+        tc_load<T, DP, kTcCols, kThreads>(sb + Shape::kK + (i % Shape::kKStages) * Shape::kStage, A.a.k, row, n, hk,
+                                          A.a.k_row, A.a.k_head, A.a.dim);
+        tc_load<T, DP, kTcCols, kThreads>(sb + Shape::kV + (i % Shape::kVStages) * Shape::kStage, A.a.v, row, n, hk,
+                                          A.a.v_row, A.a.v_head, A.a.dim);
+    };
+    Columns columns;
+    auto fetch_columns = [&](int i) {
+        if (!BIAS || i >= tiles) return;
+        const int k0 = span.tile(i) * kTcCols;
+        columns.fetch(A.a.kpos, (int64_t)t.other + k0, min(kTcCols, t.lk - k0), A.a.axes);
+    };
+    auto store_columns = [&](int i) {
+        if (!BIAS || i >= tiles) return;
+        columns.store(kpos + (i % Shape::kPosStages) * 3 * kTcCols,
+                      min(kTcCols, t.lk - span.tile(i) * kTcCols), A.a.axes, bias, 1);
     };
     tc_load<T, DP, 128, kThreads>(sb + Shape::kQ, A.a.q, t.row, t.rows, h, A.a.q_row, A.a.q_head, A.a.dim);
     tc_load<T, DP, 128, kThreads>(sb + Shape::kG, A.a.grad_out, t.row, t.rows, h,
                                   (int64_t)A.a.heads * A.a.dim, A.a.dim, A.a.dim);
-    if (tiles > 0) load_tile(0);
+    load_tile(0);
+    tc_load_commit();
+    if (!Shape::kTight) load_tile(1);
+    tc_load_commit();
+    fetch_columns(0);
     const int64_t at = (((int64_t)t.row + r) * A.a.heads + h) * A.a.dim;
     float* delta_at = A.a.delta + (int64_t)h * A.a.q_rows + t.row + r;
     if (BIAS) {
-        if (!Shape::kTight) {
+        if (!ONE) {
             tc_load_table(A, table, h);
-        } else if (entries <= Shape::kTightEntries) {
+        } else if (!Shape::kTight || entries <= Shape::kTightEntries) {
             for (int e = tid; e < entries; e += kThreads) table[e] = table_entry(A.a, e, h) * kLog2e;
         }
     }
     if (Shape::kCells) {
-        float* all = table + Shape::table_words(entries);
+        float* all = table + Shape::table_words(entries, ONE);
         for (int e = tid; e < entries * 128; e += kThreads) all[e] = 0.f;
     }
     const float lse2 = live ? load_lse2(A, t.row + r, h) : INFINITY;
-    tc_load_done();
+    store_columns(0);
+    if (!Shape::kTight) {
+        fetch_columns(1);
+        store_columns(1);
+    }
+    tc_load_wait<0>();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
-    const uint32_t mine = tmem + ((uint32_t)quarter << 21);  // lanes 32 quarter ..
-    Waiter done(sb + Shape::kBar, A.a.status);
-    if (tid == 0 && tiles > 0) {
-        mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kQ, sb + Shape::kK);
-        mma_scores<T, DP, kTcCols>(tmem + Shape::kDP, sb + Shape::kG, sb + Shape::kV);
+    const uint32_t mine = tmem + ((uint32_t)quarter << 21) + kBwdCols * group;  // lanes 32 quarter .., own columns
+    WaiterPair done(sb + Shape::kBar, A.a.status);
+    auto scores = [&](int i) {  // S and dP of tile i into its buffer
+        if (i >= tiles) return;
+        const uint32_t buffer = tmem + (i & 1) * Shape::kBuffer;
+        mma_scores<T, DP, kTcCols>(buffer + Shape::kS, sb + Shape::kQ,
+                                   sb + Shape::kK + (i % Shape::kKStages) * Shape::kStage);
+        mma_scores<T, DP, kTcCols>(buffer + Shape::kDP, sb + Shape::kG,
+                                   sb + Shape::kV + (i % Shape::kVStages) * Shape::kStage);
+    };
+    if (tid == 0) {
+        scores(0);
         mma_commit(sb + Shape::kBar);
+        if (!Shape::kTight) {
+            scores(1);
+            mma_commit(sb + Shape::kBar + 8);
+        }
     }
+    __syncwarp();
     float delta = 0.f;  // D; kDelta: this thread's columns of its sum so far
     if (MODE == kGradQTable) {
         if (live) delta = *delta_at;
@@ -158,111 +200,91 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
     }
 
     for (int i = 0; i < tiles; ++i) {
-        done.wait();
-        if (kStages == 2 && i + 1 < tiles) load_tile(i + 1);
+        done.wait(i);
+        // dq of tile i - 2 and S and dP of tile i are done: the stages of keys i - 2 and of
+        // values i are free.
+        if (!Shape::kTight) {
+            load_tile(i + 2);
+            tc_load_commit();
+            fetch_columns(i + 2);
+        }
         const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
         const bool whole = n == kTcCols && t.rows == 128 &&
                            all_visible(A, t.first, t.first + 127, k0, k0 + kTcCols - 1);
-        uint64_t seen = whole ? ~0ull : live ? seen_keys(A, p, k0, n) : 0ull;
-        if (BIAS && bias.far) seen = 0ull;
-        seen >>= group * kPer;
-        const uint64_t full = kPer == 64 ? ~0ull : (1ull << (kPer & 63)) - 1;
-        const bool all = __all_sync(FULL_MASK, (seen & full) == full);
+        const int c0 = kBwdCols * group;  // this thread's columns
+        const uint32_t own = mine + (i & 1) * Shape::kBuffer;
+        float s[16], dp[16];
+        tmem_ld16(own + Shape::kS, s);
+        tmem_ld16(own + Shape::kDP, dp);
+        uint32_t bits = 0xffffu;
+        if (!whole) bits = live ? (uint32_t)(seen_keys(A, p, k0, n) >> c0) & 0xffffu : 0u;
+        if (BIAS && bias.far) bits = 0u;
+        const bool all = __all_sync(FULL_MASK, bits == 0xffffu);
         const int* cols = kpos + (i % Shape::kPosStages) * 3 * kTcCols;
-        float s[kPer];
+        f32x2 b[8];
+        if (BIAS)
+            bias16<BIAS == 2, ONE>(A, bias, cols + c0, b,
+                                   !Shape::kTight || entries <= Shape::kTightEntries ? table : nullptr, h);
+        tmem_wait_ld();
+        tmem_use(s);
+        tmem_use(dp);
 #pragma unroll
-        for (int c = 0; c < kPer; c += 16) tmem_ld16(mine + Shape::kS + group * kPer + c, s + c);
-#pragma unroll
-        for (int c = 0; c < kPer; c += 16) {
-            float dp[16];
-            tmem_ld16(mine + Shape::kDP + group * kPer + c, dp);
-            tmem_wait_ld();
-            if (c == 0) tmem_use(s);
-            tmem_use(dp);
-            f32x2 b[8];
-            if (Shape::kTight) {
-#pragma unroll
-                for (int a = 0; a < kAttnMaxAxes; ++a)
-                    if (a < A.a.axes) {
-#pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            float v[2];
-#pragma unroll
-                            for (int k = 0; k < 2; ++k) {
-                                const int word = (bias.address<BIAS == 2>(
-                                                      A, a, cols[a * kTcCols + group * kPer + c + e + k]) -
-                                                  bias.lo[a]) >> 7;
-                                v[k] = entries <= Shape::kTightEntries
-                                           ? table[a * A.a.buckets + word]
-                                           : table_entry(A.a, a * A.a.buckets + word, h) * kLog2e;
-                            }
-                            const f32x2 x = pack2(v[0], v[1]);
-                            b[e / 2] = a ? add2(b[e / 2], x) : x;
-                        }
-                    }
-            } else if (BIAS) {
-                bias16<BIAS == 2>(A, bias, cols + group * kPer + c, b);
-            }
-            const uint32_t bits = (uint32_t)(seen >> c);
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-                f32x2 x = fma2(pack2(s[c + e], s[c + e + 1]), scale2, lse22);
-                if (BIAS) x = add2(x, b[e / 2]);
-                float u, v;
-                unpack2(x, u, v);
-                u = exp2_sfu(u);
-                v = exp2_sfu(v);
-                if (MODE == kDelta) {
-                    s[c + e] = u * dp[e];
-                    s[c + e + 1] = v * dp[e + 1];
-                } else {
-                    s[c + e] = u * (dp[e] - delta);
-                    s[c + e + 1] = v * (dp[e + 1] - delta);
-                }
-            }
-            if (!all) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[c + e] = (bits >> e) & 1u ? s[c + e] : 0.f;
-            }
+        for (int e = 0; e < 16; e += 2) {
+            f32x2 x = fma2(pack2(s[e], s[e + 1]), scale2, lse22);
+            if (BIAS) x = add2(x, b[e / 2]);
+            float u, v;
+            unpack2(x, u, v);
+            u = exp2_sfu(u);
+            v = exp2_sfu(v);
             if (MODE == kDelta) {
-                f32x2 sum = pack2(s[c], s[c + 1]);
-#pragma unroll
-                for (int e = 2; e < 16; e += 2) sum = add2(sum, pack2(s[c + e], s[c + e + 1]));
-                float u, v;
-                unpack2(sum, u, v);
-                delta += u + v;
+                s[e] = u * dp[e];
+                s[e + 1] = v * dp[e + 1];
             } else {
-                if (Shape::kCells)
-                    tmem_st16(mine + Shape::kDS + (i & 1) * kTcCols + group * kPer + c,
-                              reinterpret_cast<const uint32_t*>(s + c));
-                uint32_t w[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = Elem<T>::two(s[c + 2 * e], s[c + 2 * e + 1]);
-                tmem_st8(mine + Shape::kS + group * kPer + c, w);
+                s[e] = u * (dp[e] - delta);
+                s[e + 1] = v * (dp[e + 1] - delta);
             }
         }
+        if (!all) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = (bits >> e) & 1u ? s[e] : 0.f;
+        }
+        if (MODE == kDelta) {
+            f32x2 sum = pack2(s[0], s[1]);
+#pragma unroll
+            for (int e = 2; e < 16; e += 2) sum = add2(sum, pack2(s[e], s[e + 1]));
+            float u, v;
+            unpack2(sum, u, v);
+            delta += u + v;
+        } else {
+            if (Shape::kCells)
+                tmem_st16(mine + Shape::kDS + (i & 1) * kTcCols, reinterpret_cast<const uint32_t*>(s));
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = Elem<T>::two(s[2 * e], s[2 * e + 1]);
+            tmem_st8(own + Shape::kS, w);
+        }
+        if (!Shape::kTight) store_columns(i + 2);
         if (MODE != kDelta) tmem_wait_st();
-        tc_load_done();
+        tc_load_wait<0>();
         tc_fence_before();
         __syncthreads();
         tc_fence_after();
         if (tid == 0) {
-            const uint32_t stage = (i % kStages) * Shape::kStage, next = Shape::kStage - stage;
             if (MODE != kDelta)
-                mma_weighted<T, DP, kTcCols>(tmem + Shape::kDQ, tmem + Shape::kS, sb + Shape::kK + stage, i > 0);
-            if (kStages == 2 && i + 1 < tiles) {
-                mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kQ, sb + Shape::kK + next);
-                mma_scores<T, DP, kTcCols>(tmem + Shape::kDP, sb + Shape::kG, sb + Shape::kV + next);
-            }
-            mma_commit(sb + Shape::kBar);
+                mma_weighted<T, DP, kTcCols>(tmem + Shape::kDQ, tmem + (i & 1) * Shape::kBuffer + Shape::kS,
+                                             sb + Shape::kK + (i % Shape::kKStages) * Shape::kStage, i > 0);
+            // Executed in order after it: the buffer may be overwritten.
+            if (!Shape::kTight) scores(i + 2);
+            mma_commit(sb + Shape::kBar + 8 * (i & 1));
         }
         __syncwarp();
         if (Shape::kCells && group < A.a.axes) {
             const int* axis = cols + group * kTcCols;
+            const uint32_t buffer = tmem + ((uint32_t)quarter << 21) + Shape::kDS + (i & 1) * kTcCols;
 #pragma unroll
             for (int c = 0; c < kTcCols; c += 16) {
                 float ds[16];
-                tmem_ld16(mine + Shape::kDS + (i & 1) * kTcCols + c, ds);
+                tmem_ld16(buffer + c, ds);
                 int at_cell[16];
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
@@ -289,21 +311,26 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
             }
             tc_fence_before();
         }
-        if (kStages == 1 && i + 1 < tiles) {
-            done.wait();  // the keys are free
+        if (Shape::kTight && i + 1 < tiles) {
+            done.wait(i);  // dq of this tile: its keys are free
             load_tile(i + 1);
-            tc_load_done();
+            tc_load_commit();
+            fetch_columns(i + 1);
+            store_columns(i + 1);
+            tc_load_wait<0>();
             tc_fence_before();
             __syncthreads();
             if (tid == 0) {
                 tc_fence_after();
-                mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kQ, sb + Shape::kK);
-                mma_scores<T, DP, kTcCols>(tmem + Shape::kDP, sb + Shape::kG, sb + Shape::kV);
-                mma_commit(sb + Shape::kBar);
+                scores(i + 1);
+                mma_commit(sb + Shape::kBar + 8 * ((i + 1) & 1));
             }
+            __syncwarp();
         }
     }
-    if (tiles > 0) done.wait();
+    // What was committed last: by steps tiles - 2 and tiles - 1 (tight: tiles - 1 alone).
+    if (!Shape::kTight) done.wait(tiles);
+    if (!Shape::kTight || tiles > 0) done.wait(tiles + 1);
     const bool far = BIAS && live && bias.far;
     if (MODE == kDelta) {
         // The groups' shares in order; the table's place is free now.
@@ -312,7 +339,7 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
         shares[tid] = delta;
         __syncthreads();
         if (group == 0) {
-            for (int g = 1; g < Shape::kGroups; ++g) delta += shares[g * kTcRows + r];
+            for (int g = 1; g < 4; ++g) delta += shares[g * kTcRows + r];
             for (unsigned bad = __ballot_sync(FULL_MASK, far); bad; bad &= bad - 1) {
                 const int row = (r & ~31) + __ffs(bad) - 1;
                 const float d = exact_delta_row<T>(A, (int64_t)t.row + row, t.first + row, t.other, t.lk, h);
@@ -324,12 +351,12 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
         bool nan = far;
 #pragma unroll
         for (int c = 0; c < DP; c += 16) {
-            if ((c / 16) % Shape::kGroups != group) continue;
+            if ((c / 16) % 4 != group) continue;
             float o[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = 0.f;
             if (tiles > 0) {
-                tmem_ld16(mine + Shape::kDQ + c, o);
+                tmem_ld16(mine - kBwdCols * group + Shape::kDQ + c, o);
                 tmem_wait_ld();
                 tmem_use(o);
             }
@@ -363,7 +390,7 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
     if (Shape::kCells)
         for (int e = tid; e < entries; e += kThreads) {
             float v = 0.f;
-            const float* all = table + Shape::table_words(entries);
+            const float* all = table + Shape::table_words(entries, ONE);
             for (int w = 0; w < 4; ++w)
                 for (int l = 0; l < 32; ++l) v += all[(w * entries + e) * 32 + ((l + e) & 31)];
             partial[((int64_t)blockIdx.x * A.a.heads + h) * entries + e] = v;
@@ -371,19 +398,20 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
 }
 
 // ---------------------------------------------------------------- keys and values
+// Pipeline and threads as in the query kernel: dv += P^T_i dO_i and dk += dS^T_i Q_i
+// are followed by S^T and dP^T of tile i + 2 over the same buffer.
 template <int DP>
 struct GradKvShape {
-    static constexpr int kS = 0, kDP = kTcCols, kDK = 2 * kTcCols, kDV = kDK + DP;
-    static constexpr int kCols = kDV + DP <= 256 ? 256 : 512;
-    static constexpr int kBlocks = 512 / kCols, kGroups = 4 / kBlocks, kThreads = kTcRows * kGroups;
+    static constexpr int kS = 0, kDP = kTcCols, kBuffer = 2 * kTcCols, kDK = 4 * kTcCols, kDV = kDK + DP;
+    static constexpr int kCols = 512;
     static constexpr uint32_t kK = 0, kV = TcTile<DP>::bytes(128), kStage = TcTile<DP>::bytes(64),
-                              kQ = 2 * kV, kG = kQ + 2 * kStage, kRow = kG + 2 * kStage,
-                              kPos = kRow + 2 * 2 * kTcCols * 4, kBar = kPos + 2 * 3 * kTcCols * 4,
+                              kQ = 2 * kV, kG = kQ + 4 * kStage, kRow = kG + 4 * kStage,
+                              kPos = kRow + 4 * 2 * kTcCols * 4, kBar = kPos + 4 * 3 * kTcCols * 4,
                               kTable = kBar + 64;
-    static size_t bytes(int entries) {
-        const size_t need = kTable + (size_t)entries * 128 + 1024;
-        const size_t least = 233472 / (kBlocks + 1);
-        return need > least ? need : least;
+    static bool one_copy(int entries) { return kTable + (size_t)entries * 128 + 1024 > kTcSmem; }
+    static size_t bytes(int entries, bool one) {
+        const size_t need = kTable + (size_t)entries * (one ? 4 : 128) + 1024;
+        return need > 233472 / 2 ? need : 233472 / 2;  // one block per SM: TMEM serves no second one
     }
 };
 
@@ -391,11 +419,11 @@ struct GradKvShape {
 // `shares` blocks divide those queries; each leaves its sums in `partial`
 // ([cloud * sink tiles + tile][key head][share][dk, dv][128][dim], float32) for
 // the join kernel.  shares == 1: no block does.
-template <typename T, int DP, int BIAS>
-__global__ void __launch_bounds__((GradKvShape<DP>::kThreads), (GradKvShape<DP>::kBlocks))
+template <typename T, int DP, int BIAS, bool ONE>
+__global__ void __launch_bounds__(kBwdThreads, 1)
 attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __restrict__ partial) {
     using Shape = GradKvShape<DP>;
-    constexpr int kThreads = Shape::kThreads, kPer = kTcCols / Shape::kGroups;
+    constexpr int kThreads = kBwdThreads;
     const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.k_tiles)[blockIdx.x];
     const bool shared = shares > 1 && t.first < A.a.sinks;
     if (!shared && blockIdx.z > 0) return;
@@ -409,11 +437,14 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
     float* rows = reinterpret_cast<float*>(smem + Shape::kRow);  // [stage][-lse2, -D][64]
     const f32x2 scale2 = pack2(A.scale_log2, A.scale_log2);
     float* table = reinterpret_cast<float*>(smem + Shape::kTable);
-    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kBar + 8);
+    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kBar + 16);
 
     if (tid < 32) tmem_alloc(smem_u32(slot), Shape::kCols);
-    if (tid == 0) mbar_init(sb + Shape::kBar);
-    unsigned* flags = reinterpret_cast<unsigned*>(smem + Shape::kBar + 16);  // rows to form again
+    if (tid == 0) {
+        mbar_init(sb + Shape::kBar);
+        mbar_init(sb + Shape::kBar + 8);
+    }
+    unsigned* flags = reinterpret_cast<unsigned*>(smem + Shape::kBar + 32);  // rows to form again
     if (tid < 4) flags[tid] = 0u;
     int lo, hi;
     query_span(A, t.first, t.first + t.rows - 1, t.lq, t.lk, lo, hi);
@@ -426,67 +457,100 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
     const bool live = r < t.rows;
     BiasRow bias;
     if (BIAS) bias.init(A, A.a.kpos, t.row, r, live, sb + Shape::kTable, -1);
+    auto load_table = [&](int h) {
+        if (!BIAS) return;
+        if (!ONE) tc_load_table(A, table, h);
+        else
+            for (int e = tid; e < A.a.axes * A.a.buckets; e += kThreads) table[e] = table_entry(A.a, e, h) * kLog2e;
+    };
     auto query0 = [&](int i) { return lo + (first + i % per) * kTcCols; };
     auto load_tile = [&](int i) {
+        if (i >= tiles) return;
         const int i0 = query0(i), n = min(kTcCols, hi - i0), h = h0 + i / per;
         const int64_t row = (int64_t)t.other + i0;
-        const uint32_t stage = (i & 1) * Shape::kStage;
+        const uint32_t stage = (i & 3) * Shape::kStage;
         tc_load<T, DP, kTcCols, kThreads>(sb + Shape::kQ + stage, A.a.q, row, n, h, A.a.q_row, A.a.q_head, A.a.dim);
         tc_load<T, DP, kTcCols, kThreads>(sb + Shape::kG + stage, A.a.grad_out, row, n, h,
-                                (int64_t)A.a.heads * A.a.dim, A.a.dim, A.a.dim);
-        float* dst = rows + (i & 1) * 2 * kTcCols;
-        if (tid < kTcCols) {
-            dst[tid] = tid < n ? -load_lse2(A, row + tid, h) : -INFINITY;
-        } else if (tid < 2 * kTcCols) {
-            const int c = tid - kTcCols;
-            dst[tid] = c < n ? -A.a.delta[(int64_t)h * A.a.q_rows + row + c] : 0.f;
-        }
-        if (BIAS) tc_load_columns(qpos + (i & 1) * 3 * kTcCols, A.a.qpos, row, n, A.a.axes, bias, -1);
+                                          (int64_t)A.a.heads * A.a.dim, A.a.dim, A.a.dim);
+    };
+    // What a thread fetches of a tile beside them and stores past the latency: -lse2 or
+    // -D of a query, and its position.
+    float stat = 0.f;
+    Columns columns;
+    auto fetch_columns = [&](int i) {
+        if (i >= tiles) return;
+        const int i0 = query0(i), n = min(kTcCols, hi - i0), h = h0 + i / per, c = tid & (kTcCols - 1);
+        const int64_t row = (int64_t)t.other + i0;
+        if (tid < kTcCols) stat = c < n ? -load_lse2(A, row + c, h) : -INFINITY;
+        else if (tid < 2 * kTcCols) stat = c < n ? -A.a.delta[(int64_t)h * A.a.q_rows + row + c] : 0.f;
+        if (BIAS) columns.fetch(A.a.qpos, row, n, A.a.axes);
+    };
+    auto store_columns = [&](int i) {
+        if (i >= tiles) return;
+        if (tid < 2 * kTcCols) rows[(i & 3) * 2 * kTcCols + tid] = stat;
+        if (BIAS)
+            columns.store(qpos + (i & 3) * 3 * kTcCols, min(kTcCols, hi - query0(i)), A.a.axes, bias, -1);
     };
     tc_load<T, DP, 128, kThreads>(sb + Shape::kK, A.a.k, t.row, t.rows, hk, A.a.k_row, A.a.k_head, A.a.dim);
     tc_load<T, DP, 128, kThreads>(sb + Shape::kV, A.a.v, t.row, t.rows, hk, A.a.v_row, A.a.v_head, A.a.dim);
-    if (tiles > 0) load_tile(0);
-    if (BIAS) tc_load_table(A, table, h0);
-    tc_load_done();
+    load_tile(0);
+    tc_load_commit();
+    load_tile(1);
+    tc_load_commit();
+    fetch_columns(0);
+    load_table(h0);
+    store_columns(0);
+    fetch_columns(1);
+    store_columns(1);
+    tc_load_wait<0>();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
     const uint32_t mine = tmem + ((uint32_t)quarter << 21);
-    Waiter done(sb + Shape::kBar, A.a.status);
-    if (tid == 0 && tiles > 0) {
-        mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kK, sb + Shape::kQ);
-        mma_scores<T, DP, kTcCols>(tmem + Shape::kDP, sb + Shape::kV, sb + Shape::kG);
+    WaiterPair done(sb + Shape::kBar, A.a.status);
+    auto scores = [&](int i) {  // S^T and dP^T of tile i into its buffer
+        if (i >= tiles) return;
+        const uint32_t buffer = tmem + (i & 1) * Shape::kBuffer, stage = (i & 3) * Shape::kStage;
+        mma_scores<T, DP, kTcCols>(buffer + Shape::kS, sb + Shape::kK, sb + Shape::kQ + stage);
+        mma_scores<T, DP, kTcCols>(buffer + Shape::kDP, sb + Shape::kV, sb + Shape::kG + stage);
+    };
+    if (tid == 0) {
+        scores(0);
         mma_commit(sb + Shape::kBar);
+        scores(1);
+        mma_commit(sb + Shape::kBar + 8);
     }
+    __syncwarp();
     for (int i = 0; i < tiles; ++i) {
         if (BIAS && i > 0 && i % per == 0) {  // the next query head's table
-            tc_load_table(A, table, h0 + i / per);
+            load_table(h0 + i / per);
             __syncthreads();
         }
-        done.wait();
-        if (i + 1 < tiles) load_tile(i + 1);
+        done.wait(i);
+        load_tile(i + 2);  // over tile i - 2, whose products are done
+        tc_load_commit();
+        fetch_columns(i + 2);
         const int i0 = query0(i), n = min(kTcCols, hi - i0), p0 = i0 + t.lk - t.lq;
         const bool whole = n == kTcCols && t.rows == 128 &&
                            all_visible(A, p0, p0 + kTcCols - 1, t.first, t.first + 127);
-        uint64_t seen = whole ? ~0ull : live ? seeing_queries(A, j, p0, n) : 0ull;
-        if (BIAS && bias.far) seen = 0ull;
-        seen >>= group * kPer;
-        const uint64_t full = (1ull << kPer) - 1;
-        const bool all = __all_sync(FULL_MASK, (seen & full) == full);
-        const int* cols = qpos + (i & 1) * 3 * kTcCols;
-        const float* row = rows + (i & 1) * 2 * kTcCols;
-#pragma unroll
-        for (int cc = 0; cc < kPer; cc += 16) {
+        const int c = kBwdCols * group;  // this thread's columns
+        const uint32_t own = mine + (i & 1) * Shape::kBuffer + c;
+        uint32_t bits = 0xffffu;
+        if (!whole) bits = live ? (uint32_t)(seeing_queries(A, j, p0, n) >> c) & 0xffffu : 0u;
+        if (BIAS && bias.far) bits = 0u;
+        const bool all = __all_sync(FULL_MASK, bits == 0xffffu);
+        const int* cols = qpos + (i & 3) * 3 * kTcCols;
+        const float* row = rows + (i & 3) * 2 * kTcCols;
+        {
             float s[16], dp[16];
-            const int c = group * kPer + cc;
-            tmem_ld16(mine + Shape::kS + c, s);
-            tmem_ld16(mine + Shape::kDP + c, dp);
+            tmem_ld16(own + Shape::kS, s);
+            tmem_ld16(own + Shape::kDP, dp);
+            f32x2 b[8];
+            if (BIAS) bias16<BIAS == 2, ONE>(A, bias, cols + c, b, table, h0 + i / per);
             tmem_wait_ld();
             tmem_use(s);
             tmem_use(dp);
-            f32x2 b[8];
-            if (BIAS) bias16<BIAS == 2>(A, bias, cols + c, b);
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 // Staged negated: -lse2 and -D.
@@ -504,7 +568,6 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
                 unpack2(add2(pack2(dp[e], dp[e + 1]), d0), dp[e], dp[e + 1]);
                 unpack2(add2(pack2(dp[e + 2], dp[e + 3]), d1), dp[e + 2], dp[e + 3]);
             }
-            const uint32_t bits = (uint32_t)(seen >> cc);
             uint32_t w[8], g[8];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -524,26 +587,26 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
                 w[e] = Elem<T>::two(s[2 * e], s[2 * e + 1]);
                 g[e] = Elem<T>::two(dp[2 * e], dp[2 * e + 1]);
             }
-            tmem_st8(mine + Shape::kS + c, w);
-            tmem_st8(mine + Shape::kDP + c, g);
+            tmem_st8(own + Shape::kS, w);
+            tmem_st8(own + Shape::kDP, g);
         }
+        store_columns(i + 2);
         tmem_wait_st();
-        tc_load_done();
+        tc_load_wait<0>();
         tc_fence_before();
         __syncthreads();
         if (tid == 0) {
             tc_fence_after();
-            const uint32_t stage = (i & 1) * Shape::kStage, next = Shape::kStage - stage;
-            mma_weighted<T, DP, kTcCols>(tmem + Shape::kDV, tmem + Shape::kS, sb + Shape::kG + stage, i > 0);
-            mma_weighted<T, DP, kTcCols>(tmem + Shape::kDK, tmem + Shape::kDP, sb + Shape::kQ + stage, i > 0);
-            if (i + 1 < tiles) {
-                mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kK, sb + Shape::kQ + next);
-                mma_scores<T, DP, kTcCols>(tmem + Shape::kDP, sb + Shape::kV, sb + Shape::kG + next);
-            }
-            mma_commit(sb + Shape::kBar);
+            const uint32_t stage = (i & 3) * Shape::kStage, buffer = tmem + (i & 1) * Shape::kBuffer;
+            mma_weighted<T, DP, kTcCols>(tmem + Shape::kDV, buffer + Shape::kS, sb + Shape::kG + stage, i > 0);
+            mma_weighted<T, DP, kTcCols>(tmem + Shape::kDK, buffer + Shape::kDP, sb + Shape::kQ + stage, i > 0);
+            scores(i + 2);
+            mma_commit(sb + Shape::kBar + 8 * (i & 1));
         }
+        __syncwarp();
     }
-    if (tiles > 0) done.wait();
+    done.wait(tiles);
+    done.wait(tiles + 1);
     bool nan = BIAS && live && bias.far;
     const int64_t at = (((int64_t)t.row + r) * A.a.kv_heads + hk) * A.a.dim;
     const int sink_tiles = (A.a.sinks + kAttnTile - 1) / kAttnTile;
@@ -556,7 +619,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
     for (int which = 0; which < 2; ++which)
 #pragma unroll
         for (int c = 0; c < DP; c += 16) {
-            if ((c / 16) % Shape::kGroups != group) continue;
+            if ((c / 16) % 4 != group) continue;
             float o[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = 0.f;
@@ -644,23 +707,32 @@ size_t sink_bytes(const AttnArgs& A) {
     return (size_t)(tiles * A.a.kv_heads * shares * 2 * kAttnTile * A.a.dim) * sizeof(float);
 }
 
-template <typename T, int DP, int BIAS, int MODE>
+template <typename T, int DP, int BIAS, int MODE, bool ONE = QueryShape<DP, MODE>::kTight>
 int run_q(const AttnArgs& A, float* partial, cudaStream_t s) {
-    const size_t bytes = QueryShape<DP, MODE>::bytes(BIAS ? A.a.axes * A.a.buckets : 0);
-    const int st = tc_prepare(attn_tc_query_kernel<T, DP, BIAS, MODE>, bytes, "attn_tc_query_kernel");
+    using Shape = QueryShape<DP, MODE>;
+    const int entries = BIAS ? A.a.axes * A.a.buckets : 0;
+    if constexpr (Shape::kCells && !Shape::kTight) {
+        if (!ONE && Shape::one_copy(entries)) return run_q<T, DP, BIAS, MODE, true>(A, partial, s);
+    }
+    const size_t bytes = Shape::bytes(entries, ONE);
+    const int st = tc_prepare(attn_tc_query_kernel<T, DP, BIAS, MODE, ONE>, bytes, "attn_tc_query_kernel");
     if (st != kOk) return st;
     const dim3 grid((unsigned)A.a.q_tile_count, (unsigned)A.a.heads);
-    attn_tc_query_kernel<T, DP, BIAS, MODE><<<grid, QueryShape<DP, MODE>::kThreads, bytes, s>>>(A, partial);
+    attn_tc_query_kernel<T, DP, BIAS, MODE, ONE><<<grid, kBwdThreads, bytes, s>>>(A, partial);
     return check_launch("attn_tc_query_kernel");
 }
-template <typename T, int DP, int BIAS>
+template <typename T, int DP, int BIAS, bool ONE = false>
 int run_kv(const AttnArgs& A, float* partial, cudaStream_t s) {
-    const size_t bytes = GradKvShape<DP>::bytes(BIAS ? A.a.axes * A.a.buckets : 0);
-    int st = tc_prepare(attn_tc_grad_kv_kernel<T, DP, BIAS>, bytes, "attn_tc_grad_kv_kernel");
+    const int entries = BIAS ? A.a.axes * A.a.buckets : 0;
+    if constexpr (BIAS != 0 && DP == 128) {  // narrower rows always leave room
+        if (!ONE && GradKvShape<DP>::one_copy(entries)) return run_kv<T, DP, BIAS, true>(A, partial, s);
+    }
+    const size_t bytes = GradKvShape<DP>::bytes(entries, ONE);
+    int st = tc_prepare(attn_tc_grad_kv_kernel<T, DP, BIAS, ONE>, bytes, "attn_tc_grad_kv_kernel");
     if (st != kOk) return st;
     const int shares = sink_shares(A);
     dim3 grid((unsigned)A.a.k_tile_count, (unsigned)A.a.kv_heads, (unsigned)shares);
-    attn_tc_grad_kv_kernel<T, DP, BIAS><<<grid, GradKvShape<DP>::kThreads, bytes, s>>>(A, shares, partial);
+    attn_tc_grad_kv_kernel<T, DP, BIAS, ONE><<<grid, kBwdThreads, bytes, s>>>(A, shares, partial);
     st = check_launch("attn_tc_grad_kv_kernel");
     if (st != kOk || shares == 1) return st;
     grid.z = kAttnTile / 8;

@@ -24,7 +24,7 @@ struct FwdShape {
     static constexpr int kBlocks = 512 / kCols;
     static constexpr uint32_t kQ = 0, kK = TcTile<DP>::bytes(128), kStage = TcTile<DP>::bytes(64),
                               kV = kK + 2 * kStage, kPos = kV + 2 * kStage,
-                              kBar = kPos + 2 * 3 * kTcCols * 4, kTable = kBar + 16;
+                              kBar = kPos + 3 * 3 * kTcCols * 4, kTable = kBar + 16;
     static size_t bytes(int entries) {
         // At least what keeps more blocks than TMEM serves off an SM (they would wait for it).
         const size_t need = kTable + (size_t)entries * 128 + 1024;
@@ -40,7 +40,7 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sb = smem_u32(smem);
-    const int tid = threadIdx.x, lane = tid & 31;
+    const int tid = threadIdx.x;
     const int h = blockIdx.y, hk = h / A.group;
     const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.q_tiles)[blockIdx.x];
     const int p = t.first + tid;
@@ -54,18 +54,49 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
     const int tiles = span.count();
     BiasRow bias;
     if (BIAS) bias.init(A, A.a.qpos, t.row, tid, tid < t.rows, sb + Shape::kTable, 1);
-    auto load_tile = [&](int i) {
-        const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
-        const int64_t row = (int64_t)t.other + k0;
-        const uint32_t stage = (i & 1) * Shape::kStage;
-        tc_load<T, DP, kTcCols, kTcRows>(sb + Shape::kK + stage, A.a.k, row, n, hk, A.a.k_row, A.a.k_head, A.a.dim);
-        tc_load<T, DP, kTcCols, kTcRows>(sb + Shape::kV + stage, A.a.v, row, n, hk, A.a.v_row, A.a.v_head, A.a.dim);
-        if (BIAS) tc_load_columns(kpos + (i & 1) * 3 * kTcCols, A.a.kpos, row, n, A.a.axes, bias, 1);
+    auto first_key = [&](int i, int& k0, int& n) {
+        k0 = span.tile(i) * kTcCols;
+        n = min(kTcCols, t.lk - k0);
+    };
+    auto load_keys = [&](int i) {
+        if (i >= tiles) return;
+        int k0, n;
+        first_key(i, k0, n);
+        tc_load<T, DP, kTcCols, kTcRows>(sb + Shape::kK + (i & 1) * Shape::kStage, A.a.k, (int64_t)t.other + k0, n,
+                                         hk, A.a.k_row, A.a.k_head, A.a.dim);
+    };
+    auto load_values = [&](int i) {
+        if (i >= tiles) return;
+        int k0, n;
+        first_key(i, k0, n);
+        tc_load<T, DP, kTcCols, kTcRows>(sb + Shape::kV + (i & 1) * Shape::kStage, A.a.v, (int64_t)t.other + k0, n,
+                                         hk, A.a.v_row, A.a.v_head, A.a.dim);
+    };
+    Columns columns;
+    auto fetch_columns = [&](int i) {
+        if (!BIAS || i >= tiles) return;
+        int k0, n;
+        first_key(i, k0, n);
+        columns.fetch(A.a.kpos, (int64_t)t.other + k0, n, A.a.axes);
+    };
+    auto store_columns = [&](int i) {
+        if (!BIAS || i >= tiles) return;
+        int k0, n;
+        first_key(i, k0, n);
+        columns.store(kpos + (i % 3) * 3 * kTcCols, n, A.a.axes, bias, 1);
     };
     tc_load<T, DP, 128, kTcRows>(sb + Shape::kQ, A.a.q, t.row, t.rows, h, A.a.q_row, A.a.q_head, A.a.dim);
-    if (tiles > 0) load_tile(0);
+    load_keys(0);
+    load_values(0);
+    tc_load_commit();
+    load_keys(1);
+    tc_load_commit();
+    fetch_columns(0);
     if (BIAS) tc_load_table(A, table, h);
-    tc_load_done();
+    store_columns(0);
+    fetch_columns(1);
+    store_columns(1);
+    tc_load_wait<1>();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -82,20 +113,26 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
     const float mul = BIAS ? 1.f : (A.scale_log2 > 0.f ? A.scale_log2 : 1.f);
     for (int i = 0; i < tiles; ++i) {
         done.wait();
-        if (i + 1 < tiles) load_tile(i + 1);
+        // S of tile i and P V of tile i - 1 are done: their operands' stages are free.
+        // Copies get until the end of the next iteration.
+        load_keys(i + 2);
+        load_values(i + 1);
+        tc_load_commit();
+        fetch_columns(i + 2);
         float s[kTcCols];
 #pragma unroll
         for (int c = 0; c < kTcCols; c += 16) tmem_ld16(mine + Shape::kS + c, s + c);
         tmem_wait_ld();
         tmem_use(s);
-        const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
+        int k0, n;
+        first_key(i, k0, n);
         if (BIAS) {
-            const int* cols = kpos + (i & 1) * 3 * kTcCols;
+            const int* cols = kpos + (i % 3) * 3 * kTcCols;
             const f32x2 scale2 = pack2(A.scale_log2, A.scale_log2);
 #pragma unroll
             for (int c = 0; c < kTcCols; c += 16) {
                 f32x2 b[8];
-                bias16<BIAS == 2>(A, bias, cols + c, b);
+                bias16<BIAS == 2, false>(A, bias, cols + c, b, nullptr, h);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     unpack2(fma2(pack2(s[c + 2 * e], s[c + 2 * e + 1]), scale2, b[e]), s[c + 2 * e],
@@ -166,8 +203,9 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
             unpack2(add2(part[0], part[1]), a, b);
             sum += a + b;
         }
+        store_columns(i + 2);
         tmem_wait_st();
-        tc_load_done();
+        tc_load_wait<1>();
         tc_fence_before();
         __syncthreads();
         if (tid == 0) {

@@ -462,3 +462,48 @@ def test_norm_rotate_gradient_against_differences(cuda_device):
         analytic = (got[i].double() * d).sum().item()
         bound = 2.0 ** -20 * sums[0][1] / (2 * h) + 4 * h * h * got[i].double().norm().item()
         assert abs(numeric - analytic) <= bound, i
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("D", [16, 64, 128])
+@pytest.mark.parametrize("reach,axes", [(42, 3), (127, 1), (41, 3), (113, 1), (0, 3)])
+def test_largest_tables(cuda_device, dtype, D, reach, axes):
+    """Tables of up to 256 entries, at the sizes where their copies in shared
+    memory change form, and of one bucket per axis."""
+    g = torch.Generator().manual_seed(21)
+    lens = [140, 37]
+    n, H = sum(lens), 2
+    q, k, v, grad = (rand(g, n, H, D, dtype=dtype).to(cuda_device) for _ in range(4))
+    pos = torch.randint(-2 * reach - 3, 2 * reach + 3, (n, axes), generator=g, dtype=torch.int32)
+    table = rand(g, axes, 2 * reach + 1, H, scale=0.5).to(cuda_device)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v, table)]
+    out = attention.window_attention(*leaves[:3], ends(lens, cuda_device), window=(60, 60), sinks=1,
+                                     bias_table=leaves[3], position=pos.to(cuda_device))
+    grads = torch.autograd.grad(out, leaves, grad)
+    want = C.attention(q, k, v, lens, lens, left=60, right=60, sinks=1, table=table, qpos=pos, kpos=pos,
+                       grad=grad)
+    for name, got in zip(("out", "dq", "dk", "dv", "dtable"), (out, *grads)):
+        C.check(got, want[name], name)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_rows_far_apart_in_one_tile(cuda_device, dtype):
+    """Clouds whose neighbours along the order are millions of cells apart:
+    forward, every gradient and the table's."""
+    g = torch.Generator().manual_seed(22)
+    lens, H, D = [150, 20], 2, 32
+    n = sum(lens)
+    q, k, v, grad = (rand(g, n, H, D, dtype=dtype).to(cuda_device) for _ in range(4))
+    far = torch.tensor([0, 3, 1 << 21, (1 << 21) + 2, 1 << 25, -(1 << 29), (1 << 29) + 1],
+                       dtype=torch.int32)
+    pos = far[torch.randint(0, len(far), (n, 3), generator=g)]
+    pos[20:90] = torch.randint(0, 9, (70, 3), generator=g, dtype=torch.int32)
+    table = rand(g, 3, 11, H, scale=0.5).to(cuda_device)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v, table)]
+    out = attention.window_attention(*leaves[:3], ends(lens, cuda_device), window=(40, 40), sinks=2,
+                                     bias_table=leaves[3], position=pos.to(cuda_device))
+    grads = torch.autograd.grad(out, leaves, grad)
+    want = C.attention(q, k, v, lens, lens, left=40, right=40, sinks=2, table=table, qpos=pos, kpos=pos,
+                       grad=grad)
+    for name, got in zip(("out", "dq", "dk", "dv", "dtable"), (out, *grads)):
+        C.check(got, want[name], name)
