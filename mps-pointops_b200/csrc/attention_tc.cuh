@@ -5,10 +5,14 @@
 // length: 32, 64 or 128 bytes; DP = 128 is two halves of 64 elements.  One
 // tile serves both ways: as a K-major operand (rows = M or N, elements = K)
 // for scores, and as an MN-major B operand (rows = K, elements = N) for the
-// products with the weights.  Rows are copied with 16-byte cp.async whose
-// source size is 0 past a cloud's end, so no value of another cloud enters a
-// product; a tensor-map copy could only bound the whole tensor.
+// products with the weights.  Tiles come by tensor-map copies (TMA) of 64 rows of
+// one head, which cost the computing warps nothing (as 16-byte cp.async they took
+// a third of a step).  A copy runs past a cloud's end into the next cloud's rows:
+// their weights are exact zeros, and a result row that a NaN or an infinity among
+// them turns into a NaN is formed again pair by pair (attention_exact.cuh).
 #pragma once
+
+#include <cuda.h>
 
 #include <string>
 
@@ -41,25 +45,33 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Wait of at most kTcWaitNs.  A thread whose wait ran out reports it, waits no
-// more and goes on through the same control flow (barriers of the block stay
-// matched, memory accesses do not depend on the data that failed to come).
+// Waits of at most kTcWaitNs.  A thread whose wait ran out reports it and goes on
+// through the same control flow (barriers of the block stay matched, memory
+// accesses do not depend on the data that failed to come).
+// One thread's waits: `dead` once one of them ran out; later ones are then cut
+// short, but still let copies in flight land.
+struct Patience {
+    int32_t* status;
+    bool dead = false;
+    __device__ __forceinline__ explicit Patience(int32_t* st) : status(st) {}
+    __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity) {
+        if (mbar_try(bar, parity)) return;
+        const unsigned long long t0 = globaltimer_ns(), limit = dead ? kTcWaitNs / 1000 : kTcWaitNs;
+        while (!mbar_try(bar, parity))
+            if (globaltimer_ns() - t0 > limit) {
+                dead = true;
+                if (status) *status = 1;
+                break;
+            }
+    }
+};
 struct Waiter {
     uint32_t bar;
     uint32_t phase = 0;
-    int32_t* status;
-    bool dead = false;
-    __device__ __forceinline__ Waiter(uint32_t b, int32_t* st) : bar(b), status(st) {}
+    Patience patience;
+    __device__ __forceinline__ Waiter(uint32_t b, int32_t* st) : bar(b), patience(st) {}
     __device__ __forceinline__ void wait() {
-        if (!dead && !mbar_try(bar, phase)) {
-            const unsigned long long t0 = globaltimer_ns();
-            while (!mbar_try(bar, phase))
-                if (globaltimer_ns() - t0 > kTcWaitNs) {
-                    dead = true;
-                    if (status) *status = 1;
-                    break;
-                }
-        }
+        patience.wait(bar, phase);
         phase ^= 1;
         __syncwarp();  // the TMEM accesses that follow are warp-wide
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -163,32 +175,29 @@ struct TcTile {
     }
 };
 
-// Rows [r0, r0 + n) of one head into a tile of ROWS rows, zeros past n and dim.
-template <typename T, int DP, int ROWS, int THREADS>
-__device__ __forceinline__ void tc_load(uint32_t tile, const void* base, int64_t r0, int n, int h,
-                                        int64_t row_stride, int64_t head_stride, int dim) {
-    using L = TcTile<DP>;
-    const T* src = attn_row<T>(base, r0, h, row_stride, head_stride);
-    constexpr int kStep = THREADS / L::kChunks;
-    constexpr int kPer = (ROWS + kStep - 1) / kStep;
-    const int c = threadIdx.x % L::kChunks;
-    int r = threadIdx.x / L::kChunks;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i, r += kStep) {
-        if (ROWS % kStep && r >= ROWS) break;
-        const bool live = r < n && c * 8 < dim;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tile + L::at(ROWS, r, c)),
-                     "l"(live ? src + r * row_stride + c * 8 : src), "r"(live ? 16 : 0)
-                     : "memory");
-    }
+// The maps of one call: queries, keys, values and the gradient of the result.
+struct TcMaps {
+    CUtensorMap q, k, v, g;
+};
+// Announces `bytes` on a barrier whose phase ends when they have come.
+__device__ __forceinline__ void tma_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+                 : "memory");
 }
-// Closes a group of copies; waits until at most PENDING younger groups are open
-// and shows what has landed to the tensor core.
-__device__ __forceinline__ void tc_load_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int PENDING>
-__device__ __forceinline__ void tc_load_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+// Rows [row, row + ROWS) of head h into a tile; rows past the tensor and elements
+// past dim are zeros.  The box starts at element 0 or 64: a multiple of 16 bytes.
+template <int DP, int ROWS>
+__device__ __forceinline__ void tma_rows(uint32_t tile, const CUtensorMap* map, int h, int row, uint32_t bar) {
+    using L = TcTile<DP>;
+#pragma unroll
+    for (int half = 0; half < L::kHalves; ++half)
+#pragma unroll
+        for (int r = 0; r < ROWS; r += 64)
+            asm volatile(
+                "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
+                "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(tile + (half * ROWS + r) * L::kRowBytes),
+                "l"(map), "r"(half * 64), "r"(h), "r"(row + r), "r"(bar)
+                : "memory");
 }
 
 // kind::f16 (both operands the same 16-bit type), float accumulators, M = 128.
@@ -274,8 +283,9 @@ __device__ __forceinline__ uint64_t seeing_queries(const AttnArgs& A, int j, int
 // a row beyond +-2^21 of it (`far`) could then be wrong, is left out of the tile
 // and formed pair by pair (attention_exact.cuh).
 constexpr int kNear = 1 << 21;
+// By the block's row threads (a multiple of 128).
 __device__ __forceinline__ void tc_load_table(const AttnArgs& A, float* table, int h) {
-    for (int e = threadIdx.x; e < A.a.axes * A.a.buckets * 32; e += blockDim.x)
+    for (int e = threadIdx.x; e < A.a.axes * A.a.buckets * 32; e += (blockDim.x & ~127u))
         table[e] = table_entry(A.a, e >> 5, h) * kLog2e;
 }
 struct BiasRow {
@@ -357,6 +367,53 @@ __device__ __forceinline__ void bias16(const AttnArgs& A, const BiasRow& row, co
                 t[e / 2 + 1] = a ? add2(t[e / 2 + 1], y) : y;
             }
         }
+}
+
+// Host: a map of (rows, heads, dim) for boxes of 64 rows of one head.
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                CUtensorMapFloatOOBfill);
+inline EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+template <int DP>
+int make_map(CUtensorMap* map, const AttnArgs& A, const void* base, int64_t rows, int heads, int64_t row_stride,
+             int64_t head_stride) {
+    if (rows == 0) return kOk;  // no tile reads it
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return fail(kCudaError, "window attention: cuTensorMapEncodeTiled is not available");
+    constexpr int kInner = DP < 64 ? DP : 64;
+    const cuuint64_t dims[3] = {(cuuint64_t)A.a.dim, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)row_stride * 2};
+    const cuuint32_t box[3] = {kInner, 1, 64}, steps[3] = {1, 1, 1};
+    const CUtensorMapSwizzle swizzle = kInner == 64   ? CU_TENSOR_MAP_SWIZZLE_128B
+                                       : kInner == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                      : CU_TENSOR_MAP_SWIZZLE_32B;
+    const CUresult r =
+        encode(map, A.a.dtype == MPO_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+               const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(kCudaError, "window attention: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+    return kOk;
+}
+template <int DP>
+int make_maps(TcMaps& M, const AttnArgs& A, bool backward) {
+    int st = make_map<DP>(&M.q, A, A.a.q, A.a.q_rows, A.a.heads, A.a.q_row, A.a.q_head);
+    if (st == kOk) st = make_map<DP>(&M.k, A, A.a.k, A.a.k_rows, A.a.kv_heads, A.a.k_row, A.a.k_head);
+    if (st == kOk) st = make_map<DP>(&M.v, A, A.a.v, A.a.k_rows, A.a.kv_heads, A.a.v_row, A.a.v_head);
+    if (st == kOk && backward)
+        st = make_map<DP>(&M.g, A, A.a.grad_out, A.a.q_rows, A.a.heads, (int64_t)A.a.heads * A.a.dim, A.a.dim);
+    return st;
 }
 
 template <typename K>

@@ -28,15 +28,22 @@ namespace {
 // 3e-6 of it, always the same way for all pairs of a row.  kDelta forms D = sum
 // P dP in float32 first; kGradQTable then forms dq and the table's gradient.
 constexpr size_t kTcSmem = 232448;  // shared memory of a block at most
+// Barrier of the computing threads alone.
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
+
 enum QueryMode { kGradQ = 0, kDelta = 1, kGradQTable = 2 };
 
 // Threads: four groups of 128; thread `row` of each group shares the row and
 // takes 16 columns of every tile, so that 16 warps are on an SM (one thread per
-// row left 4 to 8, and most of the time went to fixed latencies).
+// row left 4 to 8, and most of the time went to fixed latencies).  One thread of
+// a further warp issues the copies and the products: a computing warp that did
+// was held up by the tensor core's queue, 2400 of 4300 cycles of a step at D =
+// 128, and the others with it at the next barrier.
 //
 // S and dP have two buffers in TMEM.  At the end of step i the tensor core gets
 // dq += dS_i K_i and then, over the buffer that this frees, S and dP of tile
-// i + 2: those of tile i + 1 are ready when the step's barrier falls.
+// i + 2: those of tile i + 1 are ready when the step's barrier falls.  The tile
+// after those is copied as soon as the products of tile i - 1 are done.
 //
 // Table gradient: a thread may only add to cells that no other adds to, so lane
 // l of quarter w (rows 32 w ..) has its own cell of each entry ([w][entry][l],
@@ -45,38 +52,42 @@ enum QueryMode { kGradQ = 0, kDelta = 1, kGradQTable = 2 };
 // (two buffers), and after the tile's barrier group a adds all 64 columns of
 // them to its axis.  With DP = 128 the cells (up to 128 KB) leave room for one
 // stage of keys and values, one buffer of S and dP, and one copy of the table.
-constexpr int kBwdThreads = 4 * kTcRows, kBwdCols = kTcCols / 4;
+constexpr int kBwdCompute = 4 * kTcRows, kBwdThreads = kBwdCompute + 32, kBwdCols = kTcCols / 4;
 template <int DP, int MODE>
 struct QueryShape {
     static constexpr bool kCells = MODE == kGradQTable, kTight = kCells && DP == 128;
     // Keys serve S and dq of their tile, values dP alone.
-    static constexpr int kKStages = kTight ? 1 : 4, kVStages = kTight ? 1 : 2, kPosStages = kTight ? 2 : 4;
+    static constexpr int kKStages = kTight ? 1 : 4, kVStages = kTight ? 1 : 2, kPosStages = kTight ? 3 : 4;
     static constexpr int kS = 0, kDP = kTcCols, kBuffer = kTight ? 0 : 2 * kTcCols;  // TMEM columns
     static constexpr int kDQ = 2 * kTcCols + kBuffer, kDS = kDQ + DP;
     static constexpr int kCols = MODE == kDelta ? 256 : 512;
     static constexpr uint32_t kQ = 0, kG = TcTile<DP>::bytes(128), kStage = TcTile<DP>::bytes(64),
-                              kK = 2 * kG, kV = kK + kKStages * kStage, kPos = kV + kVStages * kStage,
-                              kBar = kPos + kPosStages * 3 * kTcCols * 4, kTable = kBar + 64;
+                              kK = 2 * kG, kV = kK + kKStages * kStage, kBar = kV + kVStages * kStage,
+                              kTable = kBar + 128;
+    // Barriers: products (2); stages of keys (4), values (2), Q and dO; then TMEM's address, row flags.
+    static constexpr uint32_t kFullK = kBar + 16, kFullV = kBar + 48, kFullQ = kBar + 64, kSlot = kBar + 72,
+                              kFlags = kBar + 80;
+    static constexpr int kAhead = kTight ? 1 : 2;  // steps from the fetch of a tile's positions to their use
     static constexpr int kTightEntries = 248;  // the table fits beside this many cells (DP = 128)
     static __host__ __device__ constexpr int table_words(int entries, bool one) {
         return !one ? entries * 32 : kTight && entries > kTightEntries ? 0 : (entries + 3) / 4 * 4;
     }
-    // One copy of the table where a copy per lane does not fit beside the cells.
-    static bool one_copy(int entries) {
-        return kTight || (kCells && kTable + (size_t)entries * 640 + 1024 > kTcSmem);
-    }
-    static size_t bytes(int entries, bool one) {
-        size_t need = kTable + (size_t)table_words(entries, one) * 4 + (kCells ? (size_t)entries * 512 : 0) + 1024;
-        if (MODE == kDelta && need < kTable + 4 * kBwdThreads + 1024) need = kTable + 4 * kBwdThreads + 1024;
+    static __host__ __device__ constexpr int pos_words(int axes) { return kPosStages * axes * kTcCols; }
+    static size_t bytes(int axes, int entries, bool one) {
+        size_t need = kTable + (size_t)(pos_words(axes) + table_words(entries, one)) * 4 +
+                      (kCells ? (size_t)entries * 512 : 0) + 1024;
+        if (MODE == kDelta && need < kTable + 4 * kBwdCompute + 1024) need = kTable + 4 * kBwdCompute + 1024;
         return need > 233472 / 2 ? need : 233472 / 2;  // one block per SM: TMEM serves no second one
     }
+    // One copy of the table where a copy per lane does not fit beside the cells.
+    static bool one_copy(int axes, int entries) { return kTight || bytes(axes, entries, false) > kTcSmem; }
 };
 
 template <typename T, int DP, int BIAS, int MODE, bool ONE>
 __global__ void __launch_bounds__(kBwdThreads, 1)
-attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ partial) {
+attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TcMaps M,
+                     float* __restrict__ partial) {
     using Shape = QueryShape<DP, MODE>;
-    constexpr int kThreads = kBwdThreads;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sb = smem_u32(smem);
@@ -84,32 +95,103 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
     const int h = blockIdx.y, hk = h / A.group;
     const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.q_tiles)[blockIdx.x];
     const int p = t.first + r, entries = A.a.axes * A.a.buckets;
-    int* kpos = reinterpret_cast<int*>(smem + Shape::kPos);
+    // After the barriers: the table, the cells ([quarter][entry][lane]), the columns' positions.
     float* table = reinterpret_cast<float*>(smem + Shape::kTable);
-    float* cells = table + Shape::table_words(entries, ONE) + quarter * entries * 32;  // this quarter's
-    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kBar + 16);
-    unsigned* flags = reinterpret_cast<unsigned*>(smem + Shape::kBar + 32);  // rows to form again
-
-    if (tid < 32) tmem_alloc(smem_u32(slot), Shape::kCols);
-    if (tid == 0) {
-        mbar_init(sb + Shape::kBar);
-        mbar_init(sb + Shape::kBar + 8);
-    }
-    if (tid < 4) flags[tid] = 0u;
+    float* all_cells = table + Shape::table_words(entries, ONE);
+    float* cells = all_cells + quarter * entries * 32;  // this quarter's
+    int* kpos = reinterpret_cast<int*>(all_cells + (Shape::kCells ? entries * 128 : 0));
+    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kSlot);
+    unsigned* flags = reinterpret_cast<unsigned*>(smem + Shape::kFlags);  // rows to form again
     const KeySpan span = key_span(A, t.first, t.first + t.rows - 1, t.lk, kTcCols);
     const int tiles = span.count();
+
+    if (tid >= kBwdCompute) {  // the warp that feeds the tensor core
+        tmem_alloc(smem_u32(slot), Shape::kCols);
+        auto full_k = [&](int i) { return sb + Shape::kFullK + 8 * (i % Shape::kKStages); };
+        auto full_v = [&](int i) { return sb + Shape::kFullV + 8 * (i % Shape::kVStages); };
+        auto load_tile = [&](int i) {
+            if (i >= tiles) return;
+            const int row = t.other + span.tile(i) * kTcCols;
+            tma_expect(full_k(i), Shape::kStage);
+            tma_rows<DP, kTcCols>(sb + Shape::kK + (i % Shape::kKStages) * Shape::kStage, &M.k, hk, row, full_k(i));
+            tma_expect(full_v(i), Shape::kStage);
+            tma_rows<DP, kTcCols>(sb + Shape::kV + (i % Shape::kVStages) * Shape::kStage, &M.v, hk, row, full_v(i));
+        };
+        Patience patience(A.a.status);
+        uint32_t tmem = 0;
+        auto scores = [&](int i) {  // S and dP of tile i into its buffer
+            if (i >= tiles) return;
+            const uint32_t buffer = tmem + (i & 1) * Shape::kBuffer;
+            patience.wait(full_k(i), (i / Shape::kKStages) & 1);
+            mma_scores<T, DP, kTcCols>(buffer + Shape::kS, sb + Shape::kQ,
+                                       sb + Shape::kK + (i % Shape::kKStages) * Shape::kStage);
+            patience.wait(full_v(i), (i / Shape::kVStages) & 1);
+            mma_scores<T, DP, kTcCols>(buffer + Shape::kDP, sb + Shape::kG,
+                                       sb + Shape::kV + (i % Shape::kVStages) * Shape::kStage);
+        };
+        // Step i commits to barrier i & 1; the prologue stands for steps -2 and -1.
+        auto products_done = [&](int i) { patience.wait(sb + Shape::kBar + 8 * (i & 1), ((i + 2) >> 1) & 1); };
+        if (lane == 0) {
+            for (int i = 0; i < 9; ++i) mbar_init(sb + Shape::kBar + 8 * i);
+            tma_expect(sb + Shape::kFullQ, 2 * Shape::kG);
+            tma_rows<DP, 128>(sb + Shape::kQ, &M.q, h, t.row, sb + Shape::kFullQ);
+            tma_rows<DP, 128>(sb + Shape::kG, &M.g, h, t.row, sb + Shape::kFullQ);
+            load_tile(0);
+            if (!Shape::kTight) load_tile(1);
+        }
+        __syncwarp();
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        tmem = *slot;
+        if (lane == 0) {
+            patience.wait(sb + Shape::kFullQ, 0);
+            scores(0);
+            mma_commit(sb + Shape::kBar);
+            if (!Shape::kTight) {
+                scores(1);
+                mma_commit(sb + Shape::kBar + 8);
+                products_done(-2);
+                load_tile(2);
+            }
+        }
+        __syncwarp();
+        for (int i = 0; i < tiles; ++i) {
+            __syncthreads();  // the score gradients of tile i are in TMEM
+            if (lane == 0) {
+                tc_fence_after();
+                if (MODE != kDelta)
+                    mma_weighted<T, DP, kTcCols>(tmem + Shape::kDQ, tmem + (i & 1) * Shape::kBuffer + Shape::kS,
+                                                 sb + Shape::kK + (i % Shape::kKStages) * Shape::kStage, i > 0);
+                if (!Shape::kTight) {
+                    scores(i + 2);  // executed in order: the buffer may be overwritten
+                    mma_commit(sb + Shape::kBar + 8 * (i & 1));
+                    products_done(i - 1);
+                    load_tile(i + 3);
+                } else {
+                    // One stage, one buffer: barrier 1 tells that it is free, barrier 0 that S is there.
+                    mma_commit(sb + Shape::kBar + 8);
+                    patience.wait(sb + Shape::kBar + 8, i & 1);
+                    if (i + 1 < tiles) {
+                        load_tile(i + 1);
+                        scores(i + 1);
+                        mma_commit(sb + Shape::kBar);
+                    }
+                }
+            }
+            __syncwarp();
+        }
+        tc_fence_before();
+        __syncthreads();  // the results have been read
+        tc_fence_after();
+        tmem_free(tmem, Shape::kCols);
+        return;
+    }
+
+    if (tid < 4) flags[tid] = 0u;
     const bool live = r < t.rows;
     BiasRow bias;
     if (BIAS) bias.init(A, A.a.qpos, t.row, r, live, sb + Shape::kTable, 1);
-    auto load_tile = [&](int i) {
-        if (i >= tiles) return;
-        const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
-        const int64_t row = (int64_t)t.other + k0;
-        tc_load<T, DP, kTcCols, kThreads>(sb + Shape::kK + (i % Shape::kKStages) * Shape::kStage, A.a.k, row, n, hk,
-                                          A.a.k_row, A.a.k_head, A.a.dim);
-        tc_load<T, DP, kTcCols, kThreads>(sb + Shape::kV + (i % Shape::kVStages) * Shape::kStage, A.a.v, row, n, hk,
-                                          A.a.v_row, A.a.v_head, A.a.dim);
-    };
     Columns columns;
     auto fetch_columns = [&](int i) {
         if (!BIAS || i >= tiles) return;
@@ -118,16 +200,9 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
     };
     auto store_columns = [&](int i) {
         if (!BIAS || i >= tiles) return;
-        columns.store(kpos + (i % Shape::kPosStages) * 3 * kTcCols,
+        columns.store(kpos + (i % Shape::kPosStages) * A.a.axes * kTcCols,
                       min(kTcCols, t.lk - span.tile(i) * kTcCols), A.a.axes, bias, 1);
     };
-    tc_load<T, DP, 128, kThreads>(sb + Shape::kQ, A.a.q, t.row, t.rows, h, A.a.q_row, A.a.q_head, A.a.dim);
-    tc_load<T, DP, 128, kThreads>(sb + Shape::kG, A.a.grad_out, t.row, t.rows, h,
-                                  (int64_t)A.a.heads * A.a.dim, A.a.dim, A.a.dim);
-    load_tile(0);
-    tc_load_commit();
-    if (!Shape::kTight) load_tile(1);
-    tc_load_commit();
     fetch_columns(0);
     const int64_t at = (((int64_t)t.row + r) * A.a.heads + h) * A.a.dim;
     float* delta_at = A.a.delta + (int64_t)h * A.a.q_rows + t.row + r;
@@ -135,55 +210,34 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
         if (!ONE) {
             tc_load_table(A, table, h);
         } else if (!Shape::kTight || entries <= Shape::kTightEntries) {
-            for (int e = tid; e < entries; e += kThreads) table[e] = table_entry(A.a, e, h) * kLog2e;
+            for (int e = tid; e < entries; e += kBwdCompute) table[e] = table_entry(A.a, e, h) * kLog2e;
         }
     }
-    if (Shape::kCells) {
-        float* all = table + Shape::table_words(entries, ONE);
-        for (int e = tid; e < entries * 128; e += kThreads) all[e] = 0.f;
-    }
+    if (Shape::kCells)
+        for (int e = tid; e < entries * 128; e += kBwdCompute) all_cells[e] = 0.f;
     const float lse2 = live ? load_lse2(A, t.row + r, h) : INFINITY;
     store_columns(0);
-    if (!Shape::kTight) {
-        fetch_columns(1);
-        store_columns(1);
-    }
-    tc_load_wait<0>();
+    fetch_columns(1);
+    store_columns(1);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
     const uint32_t mine = tmem + ((uint32_t)quarter << 21) + kBwdCols * group;  // lanes 32 quarter .., own columns
     WaiterPair done(sb + Shape::kBar, A.a.status);
-    auto scores = [&](int i) {  // S and dP of tile i into its buffer
-        if (i >= tiles) return;
-        const uint32_t buffer = tmem + (i & 1) * Shape::kBuffer;
-        mma_scores<T, DP, kTcCols>(buffer + Shape::kS, sb + Shape::kQ,
-                                   sb + Shape::kK + (i % Shape::kKStages) * Shape::kStage);
-        mma_scores<T, DP, kTcCols>(buffer + Shape::kDP, sb + Shape::kG,
-                                   sb + Shape::kV + (i % Shape::kVStages) * Shape::kStage);
-    };
-    if (tid == 0) {
-        scores(0);
-        mma_commit(sb + Shape::kBar);
-        if (!Shape::kTight) {
-            scores(1);
-            mma_commit(sb + Shape::kBar + 8);
-        }
-    }
-    __syncwarp();
     float delta = 0.f;  // D; kDelta: this thread's columns of its sum so far
     if (MODE == kGradQTable) {
         if (live) delta = *delta_at;
-    } else if (MODE == kGradQ && live) {
-        for (int c = 0; c * 8 < A.a.dim; ++c) {
+    } else if (MODE == kGradQ) {
+        Patience(A.a.status).wait(sb + Shape::kFullQ, 0);
+        for (int c = 0; live && c * 8 < A.a.dim; ++c) {
             float g[8], o[8];
             Elem<T>::unpack(*reinterpret_cast<const uint4*>(smem + Shape::kG + TcTile<DP>::at(128, r, c)), g);
             Elem<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(A.a.out) + at + c * 8), o);
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = fmaf(g[e], o[e], delta);
         }
-        if (group == 0) *delta_at = delta;
+        if (live && group == 0) *delta_at = delta;
     }
     const f32x2 scale2 = pack2(A.scale_log2, A.scale_log2), lse22 = pack2(-lse2, -lse2);
     // Group a's cells of axis a: the bias addresses moved to this quarter's cells.
@@ -200,14 +254,9 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
     }
 
     for (int i = 0; i < tiles; ++i) {
-        done.wait(i);
-        // dq of tile i - 2 and S and dP of tile i are done: the stages of keys i - 2 and of
-        // values i are free.
-        if (!Shape::kTight) {
-            load_tile(i + 2);
-            tc_load_commit();
-            fetch_columns(i + 2);
-        }
+        if (Shape::kTight) done.even.wait();
+        else done.wait(i);
+        fetch_columns(i + Shape::kAhead);
         const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
         const bool whole = n == kTcCols && t.rows == 128 &&
                            all_visible(A, t.first, t.first + 127, k0, k0 + kTcCols - 1);
@@ -220,7 +269,7 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
         if (!whole) bits = live ? (uint32_t)(seen_keys(A, p, k0, n) >> c0) & 0xffffu : 0u;
         if (BIAS && bias.far) bits = 0u;
         const bool all = __all_sync(FULL_MASK, bits == 0xffffu);
-        const int* cols = kpos + (i % Shape::kPosStages) * 3 * kTcCols;
+        const int* cols = kpos + (i % Shape::kPosStages) * A.a.axes * kTcCols;
         f32x2 b[8];
         if (BIAS)
             bias16<BIAS == 2, ONE>(A, bias, cols + c0, b,
@@ -263,21 +312,11 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
             for (int e = 0; e < 8; ++e) w[e] = Elem<T>::two(s[2 * e], s[2 * e + 1]);
             tmem_st8(own + Shape::kS, w);
         }
-        if (!Shape::kTight) store_columns(i + 2);
+        if (i + Shape::kAhead > 1) store_columns(i + Shape::kAhead);
         if (MODE != kDelta) tmem_wait_st();
-        tc_load_wait<0>();
         tc_fence_before();
         __syncthreads();
         tc_fence_after();
-        if (tid == 0) {
-            if (MODE != kDelta)
-                mma_weighted<T, DP, kTcCols>(tmem + Shape::kDQ, tmem + (i & 1) * Shape::kBuffer + Shape::kS,
-                                             sb + Shape::kK + (i % Shape::kKStages) * Shape::kStage, i > 0);
-            // Executed in order after it: the buffer may be overwritten.
-            if (!Shape::kTight) scores(i + 2);
-            mma_commit(sb + Shape::kBar + 8 * (i & 1));
-        }
-        __syncwarp();
         if (Shape::kCells && group < A.a.axes) {
             const int* axis = cols + group * kTcCols;
             const uint32_t buffer = tmem + ((uint32_t)quarter << 21) + Shape::kDS + (i & 1) * kTcCols;
@@ -311,33 +350,22 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
             }
             tc_fence_before();
         }
-        if (Shape::kTight && i + 1 < tiles) {
-            done.wait(i);  // dq of this tile: its keys are free
-            load_tile(i + 1);
-            tc_load_commit();
-            fetch_columns(i + 1);
-            store_columns(i + 1);
-            tc_load_wait<0>();
-            tc_fence_before();
-            __syncthreads();
-            if (tid == 0) {
-                tc_fence_after();
-                scores(i + 1);
-                mma_commit(sb + Shape::kBar + 8 * ((i + 1) & 1));
-            }
-            __syncwarp();
-        }
     }
-    // What was committed last: by steps tiles - 2 and tiles - 1 (tight: tiles - 1 alone).
-    if (!Shape::kTight) done.wait(tiles);
-    if (!Shape::kTight || tiles > 0) done.wait(tiles + 1);
+    // What was committed last: by steps tiles - 2 and tiles - 1.
+    if (!Shape::kTight) {
+        done.wait(tiles);
+        done.wait(tiles + 1);
+    } else if (tiles > 0) {
+        done.odd.phase = (tiles - 1) & 1;
+        done.odd.wait();
+    }
     const bool far = BIAS && live && bias.far;
     if (MODE == kDelta) {
         // The groups' shares in order; the table's place is free now.
         float* shares = table;
-        __syncthreads();
+        compute_sync();
         shares[tid] = delta;
-        __syncthreads();
+        compute_sync();
         if (group == 0) {
             for (int g = 1; g < 4; ++g) delta += shares[g * kTcRows + r];
             for (unsigned bad = __ballot_sync(FULL_MASK, far); bad; bad &= bad - 1) {
@@ -373,7 +401,7 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
         }
         const unsigned bad_here = __ballot_sync(FULL_MASK, nan), apart = __ballot_sync(FULL_MASK, far);
         if (lane == 0 && bad_here) atomicOr(flags + quarter, bad_here);
-        __syncthreads();
+        compute_sync();
         if (group == 0)
             for (unsigned bad = flags[quarter]; bad; bad &= bad - 1) {
                 const int b = __ffs(bad) - 1, row = (r & ~31) + b;
@@ -383,16 +411,11 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, float* __restrict__ par
     }
     tc_fence_before();
     __syncthreads();
-    if (tid < 32) {
-        tc_fence_after();
-        tmem_free(tmem, Shape::kCols);
-    }
     if (Shape::kCells)
-        for (int e = tid; e < entries; e += kThreads) {
+        for (int e = tid; e < entries; e += kBwdCompute) {
             float v = 0.f;
-            const float* all = table + Shape::table_words(entries, ONE);
             for (int w = 0; w < 4; ++w)
-                for (int l = 0; l < 32; ++l) v += all[(w * entries + e) * 32 + ((l + e) & 31)];
+                for (int l = 0; l < 32; ++l) v += all_cells[(w * entries + e) * 32 + ((l + e) & 31)];
             partial[((int64_t)blockIdx.x * A.a.heads + h) * entries + e] = v;
         }
 }
@@ -407,7 +430,9 @@ struct GradKvShape {
     static constexpr uint32_t kK = 0, kV = TcTile<DP>::bytes(128), kStage = TcTile<DP>::bytes(64),
                               kQ = 2 * kV, kG = kQ + 4 * kStage, kRow = kG + 4 * kStage,
                               kPos = kRow + 4 * 2 * kTcCols * 4, kBar = kPos + 4 * 3 * kTcCols * 4,
-                              kTable = kBar + 64;
+                              kTable = kBar + 128;
+    // Barriers: products (2); stages of queries and gradients (4), K and V; then TMEM's address, row flags.
+    static constexpr uint32_t kFull = kBar + 16, kFullK = kBar + 48, kSlot = kBar + 56, kFlags = kBar + 64;
     static bool one_copy(int entries) { return kTable + (size_t)entries * 128 + 1024 > kTcSmem; }
     static size_t bytes(int entries, bool one) {
         const size_t need = kTable + (size_t)entries * (one ? 4 : 128) + 1024;
@@ -421,9 +446,9 @@ struct GradKvShape {
 // the join kernel.  shares == 1: no block does.
 template <typename T, int DP, int BIAS, bool ONE>
 __global__ void __launch_bounds__(kBwdThreads, 1)
-attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __restrict__ partial) {
+attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TcMaps M, int shares,
+                       float* __restrict__ partial) {
     using Shape = GradKvShape<DP>;
-    constexpr int kThreads = kBwdThreads;
     const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.k_tiles)[blockIdx.x];
     const bool shared = shares > 1 && t.first < A.a.sinks;
     if (!shared && blockIdx.z > 0) return;
@@ -435,17 +460,10 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
     const int j = t.first + r;
     int* qpos = reinterpret_cast<int*>(smem + Shape::kPos);
     float* rows = reinterpret_cast<float*>(smem + Shape::kRow);  // [stage][-lse2, -D][64]
-    const f32x2 scale2 = pack2(A.scale_log2, A.scale_log2);
     float* table = reinterpret_cast<float*>(smem + Shape::kTable);
-    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kBar + 16);
+    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kSlot);
+    unsigned* flags = reinterpret_cast<unsigned*>(smem + Shape::kFlags);  // rows to form again
 
-    if (tid < 32) tmem_alloc(smem_u32(slot), Shape::kCols);
-    if (tid == 0) {
-        mbar_init(sb + Shape::kBar);
-        mbar_init(sb + Shape::kBar + 8);
-    }
-    unsigned* flags = reinterpret_cast<unsigned*>(smem + Shape::kBar + 32);  // rows to form again
-    if (tid < 4) flags[tid] = 0u;
     int lo, hi;
     query_span(A, t.first, t.first + t.rows - 1, t.lq, t.lk, lo, hi);
     int first = 0, per = hi > lo ? (hi - lo + kTcCols - 1) / kTcCols : 0;
@@ -454,6 +472,76 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
         per = (int)((int64_t)per * (blockIdx.z + 1) / shares) - first;
     }
     const int tiles = per * A.group;
+
+    if (tid >= kBwdCompute) {  // the warp that feeds the tensor core
+        tmem_alloc(smem_u32(slot), Shape::kCols);
+        auto full = [&](int i) { return sb + Shape::kFull + 8 * (i & 3); };
+        int next_head = h0, next_query = 0;  // of the tile to be copied next
+        auto load_next = [&](int i) {
+            if (i >= tiles) return;
+            const int row = t.other + lo + (first + next_query) * kTcCols;
+            const uint32_t stage = (i & 3) * Shape::kStage;
+            tma_expect(full(i), 2 * Shape::kStage);
+            tma_rows<DP, kTcCols>(sb + Shape::kQ + stage, &M.q, next_head, row, full(i));
+            tma_rows<DP, kTcCols>(sb + Shape::kG + stage, &M.g, next_head, row, full(i));
+            if (++next_query == per) {
+                next_query = 0;
+                ++next_head;
+            }
+        };
+        Patience patience(A.a.status);
+        uint32_t tmem = 0;
+        auto scores = [&](int i) {  // S^T and dP^T of tile i into its buffer
+            if (i >= tiles) return;
+            const uint32_t buffer = tmem + (i & 1) * Shape::kBuffer, stage = (i & 3) * Shape::kStage;
+            patience.wait(full(i), (i >> 2) & 1);
+            mma_scores<T, DP, kTcCols>(buffer + Shape::kS, sb + Shape::kK, sb + Shape::kQ + stage);
+            mma_scores<T, DP, kTcCols>(buffer + Shape::kDP, sb + Shape::kV, sb + Shape::kG + stage);
+        };
+        auto products_done = [&](int i) { patience.wait(sb + Shape::kBar + 8 * (i & 1), ((i + 2) >> 1) & 1); };
+        if (lane == 0) {
+            for (int i = 0; i < 7; ++i) mbar_init(sb + Shape::kBar + 8 * i);
+            tma_expect(sb + Shape::kFullK, 2 * Shape::kV);
+            tma_rows<DP, 128>(sb + Shape::kK, &M.k, hk, t.row, sb + Shape::kFullK);
+            tma_rows<DP, 128>(sb + Shape::kV, &M.v, hk, t.row, sb + Shape::kFullK);
+            for (int i = 0; i < 3; ++i) load_next(i);
+        }
+        __syncwarp();
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        tmem = *slot;
+        if (lane == 0) {
+            patience.wait(sb + Shape::kFullK, 0);
+            scores(0);
+            mma_commit(sb + Shape::kBar);
+            scores(1);
+            mma_commit(sb + Shape::kBar + 8);
+        }
+        __syncwarp();
+        for (int i = 0; i < tiles; ++i) {
+            __syncthreads();  // weights and score gradients of tile i are in TMEM
+            if (lane == 0) {
+                tc_fence_after();
+                const uint32_t stage = (i & 3) * Shape::kStage, buffer = tmem + (i & 1) * Shape::kBuffer;
+                mma_weighted<T, DP, kTcCols>(tmem + Shape::kDV, buffer + Shape::kS, sb + Shape::kG + stage, i > 0);
+                mma_weighted<T, DP, kTcCols>(tmem + Shape::kDK, buffer + Shape::kDP, sb + Shape::kQ + stage, i > 0);
+                scores(i + 2);  // executed in order: the buffer may be overwritten
+                mma_commit(sb + Shape::kBar + 8 * (i & 1));
+                products_done(i - 1);
+                load_next(i + 3);
+            }
+            __syncwarp();
+        }
+        tc_fence_before();
+        __syncthreads();  // the results have been read
+        tc_fence_after();
+        tmem_free(tmem, Shape::kCols);
+        return;
+    }
+
+    if (tid < 4) flags[tid] = 0u;
+    const f32x2 scale2 = pack2(A.scale_log2, A.scale_log2);
     const bool live = r < t.rows;
     BiasRow bias;
     if (BIAS) bias.init(A, A.a.kpos, t.row, r, live, sb + Shape::kTable, -1);
@@ -461,77 +549,51 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
         if (!BIAS) return;
         if (!ONE) tc_load_table(A, table, h);
         else
-            for (int e = tid; e < A.a.axes * A.a.buckets; e += kThreads) table[e] = table_entry(A.a, e, h) * kLog2e;
+            for (int e = tid; e < A.a.axes * A.a.buckets; e += kBwdCompute) table[e] = table_entry(A.a, e, h) * kLog2e;
     };
-    auto query0 = [&](int i) { return lo + (first + i % per) * kTcCols; };
-    auto load_tile = [&](int i) {
-        if (i >= tiles) return;
-        const int i0 = query0(i), n = min(kTcCols, hi - i0), h = h0 + i / per;
-        const int64_t row = (int64_t)t.other + i0;
-        const uint32_t stage = (i & 3) * Shape::kStage;
-        tc_load<T, DP, kTcCols, kThreads>(sb + Shape::kQ + stage, A.a.q, row, n, h, A.a.q_row, A.a.q_head, A.a.dim);
-        tc_load<T, DP, kTcCols, kThreads>(sb + Shape::kG + stage, A.a.grad_out, row, n, h,
-                                          (int64_t)A.a.heads * A.a.dim, A.a.dim, A.a.dim);
-    };
-    // What a thread fetches of a tile beside them and stores past the latency: -lse2 or
-    // -D of a query, and its position.
+    // What a thread fetches of a tile and stores past the latency: -lse2 or -D of a
+    // query, and its position.  The head and the first query of the tile fetched next.
+    int next_head = h0, next_query = 0;
     float stat = 0.f;
     Columns columns;
-    auto fetch_columns = [&](int i) {
+    auto fetch_next = [&](int i) {
         if (i >= tiles) return;
-        const int i0 = query0(i), n = min(kTcCols, hi - i0), h = h0 + i / per, c = tid & (kTcCols - 1);
+        const int i0 = lo + (first + next_query) * kTcCols, n = min(kTcCols, hi - i0), c = tid & (kTcCols - 1);
         const int64_t row = (int64_t)t.other + i0;
-        if (tid < kTcCols) stat = c < n ? -load_lse2(A, row + c, h) : -INFINITY;
-        else if (tid < 2 * kTcCols) stat = c < n ? -A.a.delta[(int64_t)h * A.a.q_rows + row + c] : 0.f;
+        if (tid < kTcCols) stat = c < n ? -load_lse2(A, row + c, next_head) : -INFINITY;
+        else if (tid < 2 * kTcCols) stat = c < n ? -A.a.delta[(int64_t)next_head * A.a.q_rows + row + c] : 0.f;
         if (BIAS) columns.fetch(A.a.qpos, row, n, A.a.axes);
     };
-    auto store_columns = [&](int i) {
+    auto store_next = [&](int i) {
         if (i >= tiles) return;
+        const int i0 = lo + (first + next_query) * kTcCols;
         if (tid < 2 * kTcCols) rows[(i & 3) * 2 * kTcCols + tid] = stat;
-        if (BIAS)
-            columns.store(qpos + (i & 3) * 3 * kTcCols, min(kTcCols, hi - query0(i)), A.a.axes, bias, -1);
+        if (BIAS) columns.store(qpos + (i & 3) * 3 * kTcCols, min(kTcCols, hi - i0), A.a.axes, bias, -1);
+        if (++next_query == per) {
+            next_query = 0;
+            ++next_head;
+        }
     };
-    tc_load<T, DP, 128, kThreads>(sb + Shape::kK, A.a.k, t.row, t.rows, hk, A.a.k_row, A.a.k_head, A.a.dim);
-    tc_load<T, DP, 128, kThreads>(sb + Shape::kV, A.a.v, t.row, t.rows, hk, A.a.v_row, A.a.v_head, A.a.dim);
-    load_tile(0);
-    tc_load_commit();
-    load_tile(1);
-    tc_load_commit();
-    fetch_columns(0);
+    fetch_next(0);
     load_table(h0);
-    store_columns(0);
-    fetch_columns(1);
-    store_columns(1);
-    tc_load_wait<0>();
+    store_next(0);
+    fetch_next(1);
+    store_next(1);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
     const uint32_t mine = tmem + ((uint32_t)quarter << 21);
     WaiterPair done(sb + Shape::kBar, A.a.status);
-    auto scores = [&](int i) {  // S^T and dP^T of tile i into its buffer
-        if (i >= tiles) return;
-        const uint32_t buffer = tmem + (i & 1) * Shape::kBuffer, stage = (i & 3) * Shape::kStage;
-        mma_scores<T, DP, kTcCols>(buffer + Shape::kS, sb + Shape::kK, sb + Shape::kQ + stage);
-        mma_scores<T, DP, kTcCols>(buffer + Shape::kDP, sb + Shape::kV, sb + Shape::kG + stage);
-    };
-    if (tid == 0) {
-        scores(0);
-        mma_commit(sb + Shape::kBar);
-        scores(1);
-        mma_commit(sb + Shape::kBar + 8);
-    }
-    __syncwarp();
+    int head = h0, query = 0;  // of the tile at hand
     for (int i = 0; i < tiles; ++i) {
-        if (BIAS && i > 0 && i % per == 0) {  // the next query head's table
-            load_table(h0 + i / per);
-            __syncthreads();
+        if (BIAS && query == 0 && i > 0) {  // the next query head's table
+            load_table(head);
+            compute_sync();
         }
         done.wait(i);
-        load_tile(i + 2);  // over tile i - 2, whose products are done
-        tc_load_commit();
-        fetch_columns(i + 2);
-        const int i0 = query0(i), n = min(kTcCols, hi - i0), p0 = i0 + t.lk - t.lq;
+        fetch_next(i + 2);
+        const int i0 = lo + (first + query) * kTcCols, n = min(kTcCols, hi - i0), p0 = i0 + t.lk - t.lq;
         const bool whole = n == kTcCols && t.rows == 128 &&
                            all_visible(A, p0, p0 + kTcCols - 1, t.first, t.first + 127);
         const int c = kBwdCols * group;  // this thread's columns
@@ -547,7 +609,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
             tmem_ld16(own + Shape::kS, s);
             tmem_ld16(own + Shape::kDP, dp);
             f32x2 b[8];
-            if (BIAS) bias16<BIAS == 2, ONE>(A, bias, cols + c, b, table, h0 + i / per);
+            if (BIAS) bias16<BIAS == 2, ONE>(A, bias, cols + c, b, table, head);
             tmem_wait_ld();
             tmem_use(s);
             tmem_use(dp);
@@ -590,20 +652,14 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
             tmem_st8(own + Shape::kS, w);
             tmem_st8(own + Shape::kDP, g);
         }
-        store_columns(i + 2);
+        store_next(i + 2);
         tmem_wait_st();
-        tc_load_wait<0>();
         tc_fence_before();
         __syncthreads();
-        if (tid == 0) {
-            tc_fence_after();
-            const uint32_t stage = (i & 3) * Shape::kStage, buffer = tmem + (i & 1) * Shape::kBuffer;
-            mma_weighted<T, DP, kTcCols>(tmem + Shape::kDV, buffer + Shape::kS, sb + Shape::kG + stage, i > 0);
-            mma_weighted<T, DP, kTcCols>(tmem + Shape::kDK, buffer + Shape::kDP, sb + Shape::kQ + stage, i > 0);
-            scores(i + 2);
-            mma_commit(sb + Shape::kBar + 8 * (i & 1));
+        if (++query == per) {
+            query = 0;
+            ++head;
         }
-        __syncwarp();
     }
     done.wait(tiles);
     done.wait(tiles + 1);
@@ -650,7 +706,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
         }
     const unsigned bad_here = __ballot_sync(FULL_MASK, nan);
     if (lane == 0 && bad_here) atomicOr(flags + quarter, bad_here);
-    __syncthreads();
+    compute_sync();
     if (!shared && group == 0)
         for (unsigned bad = flags[quarter]; bad; bad &= bad - 1) {
             const int row = (r & ~31) + __ffs(bad) - 1;
@@ -658,10 +714,6 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __
         }
     tc_fence_before();
     __syncthreads();
-    if (tid < 32) {
-        tc_fence_after();
-        tmem_free(tmem, Shape::kCols);
-    }
 }
 
 // grad_k and grad_v of the key tiles with sinks: the shares' sums in order.  A
@@ -708,31 +760,31 @@ size_t sink_bytes(const AttnArgs& A) {
 }
 
 template <typename T, int DP, int BIAS, int MODE, bool ONE = QueryShape<DP, MODE>::kTight>
-int run_q(const AttnArgs& A, float* partial, cudaStream_t s) {
+int run_q(const AttnArgs& A, const TcMaps& M, float* partial, cudaStream_t s) {
     using Shape = QueryShape<DP, MODE>;
-    const int entries = BIAS ? A.a.axes * A.a.buckets : 0;
+    const int axes = BIAS ? A.a.axes : 0, entries = axes * A.a.buckets;
     if constexpr (Shape::kCells && !Shape::kTight) {
-        if (!ONE && Shape::one_copy(entries)) return run_q<T, DP, BIAS, MODE, true>(A, partial, s);
+        if (!ONE && Shape::one_copy(axes, entries)) return run_q<T, DP, BIAS, MODE, true>(A, M, partial, s);
     }
-    const size_t bytes = Shape::bytes(entries, ONE);
+    const size_t bytes = Shape::bytes(axes, entries, ONE);
     const int st = tc_prepare(attn_tc_query_kernel<T, DP, BIAS, MODE, ONE>, bytes, "attn_tc_query_kernel");
     if (st != kOk) return st;
     const dim3 grid((unsigned)A.a.q_tile_count, (unsigned)A.a.heads);
-    attn_tc_query_kernel<T, DP, BIAS, MODE, ONE><<<grid, kBwdThreads, bytes, s>>>(A, partial);
+    attn_tc_query_kernel<T, DP, BIAS, MODE, ONE><<<grid, kBwdThreads, bytes, s>>>(A, M, partial);
     return check_launch("attn_tc_query_kernel");
 }
 template <typename T, int DP, int BIAS, bool ONE = false>
-int run_kv(const AttnArgs& A, float* partial, cudaStream_t s) {
+int run_kv(const AttnArgs& A, const TcMaps& M, float* partial, cudaStream_t s) {
     const int entries = BIAS ? A.a.axes * A.a.buckets : 0;
     if constexpr (BIAS != 0 && DP == 128) {  // narrower rows always leave room
-        if (!ONE && GradKvShape<DP>::one_copy(entries)) return run_kv<T, DP, BIAS, true>(A, partial, s);
+        if (!ONE && GradKvShape<DP>::one_copy(entries)) return run_kv<T, DP, BIAS, true>(A, M, partial, s);
     }
     const size_t bytes = GradKvShape<DP>::bytes(entries, ONE);
     int st = tc_prepare(attn_tc_grad_kv_kernel<T, DP, BIAS, ONE>, bytes, "attn_tc_grad_kv_kernel");
     if (st != kOk) return st;
     const int shares = sink_shares(A);
     dim3 grid((unsigned)A.a.k_tile_count, (unsigned)A.a.kv_heads, (unsigned)shares);
-    attn_tc_grad_kv_kernel<T, DP, BIAS, ONE><<<grid, kBwdThreads, bytes, s>>>(A, shares, partial);
+    attn_tc_grad_kv_kernel<T, DP, BIAS, ONE><<<grid, kBwdThreads, bytes, s>>>(A, M, shares, partial);
     st = check_launch("attn_tc_grad_kv_kernel");
     if (st != kOk || shares == 1) return st;
     grid.z = kAttnTile / 8;
@@ -742,21 +794,23 @@ int run_kv(const AttnArgs& A, float* partial, cudaStream_t s) {
 template <typename T, int DP, int BIAS>
 int run(const AttnArgs& A, cudaStream_t s) {
     float* sums = static_cast<float*>(A.a.workspace);
-    int st = kOk;
+    TcMaps M = {};
+    int st = make_maps<DP>(M, A, true);
+    if (st != kOk) return st;
     if (A.a.q_tile_count) {
         if constexpr (BIAS != 0) {
             float* partial = reinterpret_cast<float*>(static_cast<unsigned char*>(A.a.workspace) + sink_bytes(A));
             if (A.a.grad_table) {
-                st = run_q<T, DP, BIAS, kDelta>(A, nullptr, s);
-                if (st == kOk) st = run_q<T, DP, BIAS, kGradQTable>(A, partial, s);
+                st = run_q<T, DP, BIAS, kDelta>(A, M, nullptr, s);
+                if (st == kOk) st = run_q<T, DP, BIAS, kGradQTable>(A, M, partial, s);
             } else {
-                st = run_q<T, DP, BIAS, kGradQ>(A, nullptr, s);
+                st = run_q<T, DP, BIAS, kGradQ>(A, M, nullptr, s);
             }
         } else {
-            st = run_q<T, DP, BIAS, kGradQ>(A, nullptr, s);
+            st = run_q<T, DP, BIAS, kGradQ>(A, M, nullptr, s);
         }
     }
-    if (st == kOk && A.a.k_tile_count) st = run_kv<T, DP, BIAS>(A, sums, s);
+    if (st == kOk && A.a.k_tile_count) st = run_kv<T, DP, BIAS>(A, M, sums, s);
     return st;
 }
 template <typename T, int DP>

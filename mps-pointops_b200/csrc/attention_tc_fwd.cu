@@ -24,7 +24,9 @@ struct FwdShape {
     static constexpr int kBlocks = 512 / kCols;
     static constexpr uint32_t kQ = 0, kK = TcTile<DP>::bytes(128), kStage = TcTile<DP>::bytes(64),
                               kV = kK + 2 * kStage, kPos = kV + 2 * kStage,
-                              kBar = kPos + 3 * 3 * kTcCols * 4, kTable = kBar + 16;
+                              kBar = kPos + 3 * 3 * kTcCols * 4, kTable = kBar + 64;
+    // Barriers: products; stages of keys (2) and values (2), the first keys with Q.
+    static constexpr uint32_t kFullK = kBar + 8, kFullV = kBar + 24, kSlot = kBar + 40;
     static size_t bytes(int entries) {
         // At least what keeps more blocks than TMEM serves off an SM (they would wait for it).
         const size_t need = kTable + (size_t)entries * 128 + 1024;
@@ -35,7 +37,7 @@ struct FwdShape {
 
 template <typename T, int DP, int BIAS>
 __global__ void __launch_bounds__(kTcRows, (BIAS && DP <= 64 ? 3 : FwdShape<DP>::kBlocks))
-attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
+attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TcMaps M) {
     using Shape = FwdShape<DP>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -46,31 +48,43 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
     const int p = t.first + tid;
     int* kpos = reinterpret_cast<int*>(smem + Shape::kPos);
     float* table = reinterpret_cast<float*>(smem + Shape::kTable);
-    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kBar + 8);
+    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kSlot);
 
     if (tid < 32) tmem_alloc(smem_u32(slot), Shape::kCols);
-    if (tid == 0) mbar_init(sb + Shape::kBar);
+    if (tid == 0)
+        for (int i = 0; i < 5; ++i) mbar_init(sb + Shape::kBar + 8 * i);
     const KeySpan span = key_span(A, t.first, t.first + t.rows - 1, t.lk, kTcCols);
     const int tiles = span.count();
+    // Thread 0 issues the copies and the products.
+    auto load_keys = [&](int i) {
+        if (i >= tiles) return;
+        const uint32_t bar = sb + Shape::kFullK + 8 * (i & 1);
+        tma_expect(bar, Shape::kStage + (i == 0 ? Shape::kK : 0));
+        if (i == 0) tma_rows<DP, 128>(sb + Shape::kQ, &M.q, h, t.row, bar);
+        tma_rows<DP, kTcCols>(sb + Shape::kK + (i & 1) * Shape::kStage, &M.k, hk, t.other + span.tile(i) * kTcCols, bar);
+    };
+    auto load_values = [&](int i) {
+        if (i >= tiles) return;
+        const uint32_t bar = sb + Shape::kFullV + 8 * (i & 1);
+        tma_expect(bar, Shape::kStage);
+        tma_rows<DP, kTcCols>(sb + Shape::kV + (i & 1) * Shape::kStage, &M.v, hk, t.other + span.tile(i) * kTcCols, bar);
+    };
+    Patience patience(A.a.status);
+    auto scores = [&](int i) {
+        patience.wait(sb + Shape::kFullK + 8 * (i & 1), (i >> 1) & 1);
+        mma_scores<T, DP, kTcCols>(*slot + Shape::kS, sb + Shape::kQ, sb + Shape::kK + (i & 1) * Shape::kStage);
+    };
+    if (tid == 0) {
+        load_keys(0);
+        load_values(0);
+        load_keys(1);
+    }
+    __syncwarp();
     BiasRow bias;
     if (BIAS) bias.init(A, A.a.qpos, t.row, tid, tid < t.rows, sb + Shape::kTable, 1);
     auto first_key = [&](int i, int& k0, int& n) {
         k0 = span.tile(i) * kTcCols;
         n = min(kTcCols, t.lk - k0);
-    };
-    auto load_keys = [&](int i) {
-        if (i >= tiles) return;
-        int k0, n;
-        first_key(i, k0, n);
-        tc_load<T, DP, kTcCols, kTcRows>(sb + Shape::kK + (i & 1) * Shape::kStage, A.a.k, (int64_t)t.other + k0, n,
-                                         hk, A.a.k_row, A.a.k_head, A.a.dim);
-    };
-    auto load_values = [&](int i) {
-        if (i >= tiles) return;
-        int k0, n;
-        first_key(i, k0, n);
-        tc_load<T, DP, kTcCols, kTcRows>(sb + Shape::kV + (i & 1) * Shape::kStage, A.a.v, (int64_t)t.other + k0, n,
-                                         hk, A.a.v_row, A.a.v_head, A.a.dim);
     };
     Columns columns;
     auto fetch_columns = [&](int i) {
@@ -85,18 +99,11 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
         first_key(i, k0, n);
         columns.store(kpos + (i % 3) * 3 * kTcCols, n, A.a.axes, bias, 1);
     };
-    tc_load<T, DP, 128, kTcRows>(sb + Shape::kQ, A.a.q, t.row, t.rows, h, A.a.q_row, A.a.q_head, A.a.dim);
-    load_keys(0);
-    load_values(0);
-    tc_load_commit();
-    load_keys(1);
-    tc_load_commit();
     fetch_columns(0);
     if (BIAS) tc_load_table(A, table, h);
     store_columns(0);
     fetch_columns(1);
     store_columns(1);
-    tc_load_wait<1>();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -104,9 +111,10 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
     const uint32_t mine = tmem + ((uint32_t)(tid & ~31) << 16);  // this warp's lanes
     Waiter done(sb + Shape::kBar, A.a.status);
     if (tid == 0 && tiles > 0) {
-        mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kQ, sb + Shape::kK);
+        scores(0);
         mma_commit(sb + Shape::kBar);
     }
+    __syncwarp();
 
     // Running maximum in units of s2 = S * mul + bias (log2), as of the last rescale.
     float top = -INFINITY, sum = 0.f;
@@ -114,10 +122,11 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
     for (int i = 0; i < tiles; ++i) {
         done.wait();
         // S of tile i and P V of tile i - 1 are done: their operands' stages are free.
-        // Copies get until the end of the next iteration.
-        load_keys(i + 2);
-        load_values(i + 1);
-        tc_load_commit();
+        if (tid == 0) {
+            load_keys(i + 2);
+            load_values(i + 1);
+        }
+        __syncwarp();
         fetch_columns(i + 2);
         float s[kTcCols];
 #pragma unroll
@@ -205,19 +214,18 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A) {
         }
         store_columns(i + 2);
         tmem_wait_st();
-        tc_load_wait<1>();
         tc_fence_before();
         __syncthreads();
         if (tid == 0) {
             tc_fence_after();
             const uint32_t stage = (i & 1) * Shape::kStage;
+            patience.wait(sb + Shape::kFullV + 8 * (i & 1), (i >> 1) & 1);
             mma_weighted<T, DP, kTcCols>(tmem + Shape::kO, tmem + Shape::kS, sb + Shape::kV + stage, i > 0);
             // Issued after P V and executed in order after it: S may overwrite the weights.
-            if (i + 1 < tiles)
-                mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kQ,
-                                           sb + Shape::kK + (Shape::kStage - stage));
+            if (i + 1 < tiles) scores(i + 1);
             mma_commit(sb + Shape::kBar);
         }
+        __syncwarp();
     }
     if (tiles > 0) done.wait();
     const bool live = tid < t.rows;
@@ -265,8 +273,11 @@ int run(const AttnArgs& A, cudaStream_t s) {
     const size_t bytes = FwdShape<DP>::bytes(BIAS ? A.a.axes * A.a.buckets : 0);
     const int st = tc_prepare(attn_tc_fwd_kernel<T, DP, BIAS>, bytes, "attn_tc_fwd_kernel");
     if (st != kOk) return st;
+    TcMaps maps = {};
+    const int mapped = make_maps<DP>(maps, A, false);
+    if (mapped != kOk) return mapped;
     const dim3 grid((unsigned)A.a.q_tile_count, (unsigned)A.a.heads);
-    attn_tc_fwd_kernel<T, DP, BIAS><<<grid, kTcRows, bytes, s>>>(A);
+    attn_tc_fwd_kernel<T, DP, BIAS><<<grid, kTcRows, bytes, s>>>(A, maps);
     return check_launch("attn_tc_fwd_kernel");
 }
 template <typename T, int DP>
