@@ -160,18 +160,24 @@ struct TcTile {
         const int turn = kRowBytes == 128 ? (r & 7) : kRowBytes == 64 ? ((r >> 1) & 3) : ((r >> 2) & 1);
         return half * rows * kRowBytes + r * kRowBytes + ((cc ^ turn) << 4);
     }
-    static __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo) {
-        return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
-               ((uint64_t)(8 * kRowBytes >> 4) << 32) | (1ull << 46) | (kSwizzle << 61);
+    // Matrix descriptors: the low word holds the address and the leading offset (in 16-byte
+    // units; shared memory ends below 2^18, so neither runs into the other), the high word
+    // the stride of eight rows, the version and the swizzle.  The low word of a tile is formed
+    // once; a product's operand is a constant away from it.
+    static constexpr uint32_t kHigh = (8 * kRowBytes >> 4) | (1u << 14) | ((uint32_t)kSwizzle << 29);
+    static __device__ __forceinline__ uint64_t desc(uint32_t low) {
+        uint64_t d;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(low), "r"(kHigh));
+        return d;
     }
-    // K-major operand, elements 16 k .. 16 k + 15 of every row.
+    // K-major operand of `rows` rows, elements 16 k .. 16 k + 15 of every row.
     static __device__ __forceinline__ uint64_t k_major(uint32_t tile, int rows, int k) {
         const int half = k / (kRowBytes / 32), kk = k % (kRowBytes / 32);
-        return desc(tile + half * rows * kRowBytes + kk * 32, 16);
+        return desc(((tile >> 4) | (1u << 16)) + ((half * rows * kRowBytes + kk * 32) >> 4));
     }
     // MN-major operand, rows 16 k .. 16 k + 15, all DP elements.
     static __device__ __forceinline__ uint64_t mn_major(uint32_t tile, int rows, int k) {
-        return desc(tile + k * 16 * kRowBytes, rows * kRowBytes);
+        return desc(((tile >> 4) | ((uint32_t)(rows * kRowBytes >> 4) << 16)) + (k * 16 * kRowBytes >> 4));
     }
 };
 
@@ -210,16 +216,16 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(0u)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
         : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(0u)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
         : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
@@ -277,44 +283,62 @@ __device__ __forceinline__ uint64_t seeing_queries(const AttnArgs& A, int j, int
 // costs one wavefront whatever the buckets (one shared copy: about three, for
 // neighbouring points that differ).
 //
-// Positions are staged relative to the tile's first row and times 128, so that
-// column + row, clamped to the axis' entries, is the address: two instructions
-// per pair and axis.  Columns beyond +-2^22 of the first row are clamped there;
-// a row beyond +-2^21 of it (`far`) could then be wrong, is left out of the tile
-// and formed pair by pair (attention_exact.cuh).
-constexpr int kNear = 1 << 21;
+// The address of a pair's entry takes two multiply-adds: integer instructions run
+// at half their rate and bound the first form of this.  Positions are staged as
+// floats relative to the tile's first row; with d = key - query, the saturating
+//   t = sat(d / 2R + 1/2)         (d split into the column's and the row's part)
+// clamps to the axis' 2 R + 1 entries for nothing, and
+//   t * (2R * 128) + first entry  in units of 2^-149, the spacing of denormals,
+// is a float whose bits are the address.  Rounding: the row's part is below
+// 2^15 / 2R + 1 and off by 2^-25 of its power of two, t by 2^-25, so the address
+// before its rounding to an integer is off by at most 0.26 (R = 1; every R was
+// gone through) and comes out exact.  Columns beyond +-2^16 of the first row are
+// clamped there (t saturates all the same); a row beyond +-2^15 of it (`far`) is
+// left out of the tile and formed pair by pair (attention_exact.cuh).
+constexpr int kNear = 1 << 15;
 // By the block's row threads (a multiple of 128).
 __device__ __forceinline__ void tc_load_table(const AttnArgs& A, float* table, int h) {
     for (int e = threadIdx.x; e < A.a.axes * A.a.buckets * 32; e += (blockDim.x & ~127u))
         table[e] = table_entry(A.a, e >> 5, h) * kLog2e;
 }
 struct BiasRow {
-    int add[kAttnMaxAxes], lo[kAttnMaxAxes], hi[kAttnMaxAxes];
+    float part[kAttnMaxAxes];  // 1/2 - row / 2R (or + row / 2R)
+    float first[kAttnMaxAxes]; // address of this lane's first entry, as bits
+    float inv, span;           // 1 / 2R; 256 R as bits
     int ref[kAttnMaxAxes];
     bool far = false;
     // sign 1: rows are queries, columns keys (key - query = column - row); -1: the reverse.
-    __device__ __forceinline__ void init(const AttnArgs& A, const int32_t* pos, int64_t first, int row,
+    __device__ __forceinline__ void init(const AttnArgs& A, const int32_t* pos, int64_t base, int row,
                                          bool live, uint32_t table, int sign) {
+        inv = A.a.reach ? 1.f / (float)(2 * A.a.reach) : 0.f;
+        span = __int_as_float(256 * A.a.reach);
 #pragma unroll
         for (int a = 0; a < kAttnMaxAxes; ++a) {
-            add[a] = lo[a] = hi[a] = ref[a] = 0;
+            part[a] = first[a] = 0.f;
+            ref[a] = 0;
             if (a >= A.a.axes) continue;
-            ref[a] = pos[first * A.a.axes + a];
-            const int d = live ? pos[(first + row) * A.a.axes + a] - ref[a] : 0;
-            if (d > kNear || d < -kNear) far = true;
-            lo[a] = (int)table + a * A.a.buckets * 128 + (threadIdx.x & 31) * 4;
-            hi[a] = lo[a] + 256 * A.a.reach;
-            add[a] = lo[a] + 128 * A.a.reach - (far ? 0 : sign * d * 128);
+            ref[a] = pos[base * A.a.axes + a];
+            const int d = live ? pos[(base + row) * A.a.axes + a] - ref[a] : 0;
+            const bool beyond = d > kNear || d < -kNear;
+            far |= beyond;
+            part[a] = (float)(0.5 - (double)(beyond ? 0 : sign * d) * (double)inv);
+            first[a] = __int_as_float((int)table + a * A.a.buckets * 128 + (threadIdx.x & 31) * 4);
         }
     }
     // Staged value of a column.
-    static __device__ __forceinline__ int column(int pos, int ref, int sign) {
-        return sign * max(min(pos - ref, 2 * kNear), -2 * kNear) * 128;
+    static __device__ __forceinline__ float column(int pos, int ref, int sign) {
+        return (float)(sign * max(min(pos - ref, 2 * kNear), -2 * kNear));
     }
+    // Address of the entry (or of the cell, with `from` the first) of a column, `row` being
+    // the row's part.
     template <bool MAPPED>
-    __device__ __forceinline__ int address(const AttnArgs& A, int a, int col) const {
-        int at = max(__viaddmin_s32(col, add[a], hi[a]), lo[a]);
-        if (MAPPED) at = lo[a] + 128 * min(max(__ldg(A.a.map + ((at - lo[a]) >> 7)), 0), A.a.buckets - 1);
+    __device__ __forceinline__ int address(const AttnArgs& A, float row, float col, float from) const {
+        const float t = __saturatef(fmaf(col, inv, row));
+        int at = __float_as_int(fmaf(t, span, from));
+        if (MAPPED) {
+            const int lo = __float_as_int(from);
+            at = lo + 128 * min(max(__ldg(A.a.map + ((at - lo) >> 7)), 0), A.a.buckets - 1);
+        }
         return at;
     }
 };
@@ -327,13 +351,13 @@ struct Columns {
         for (int a = 0; a < kAttnMaxAxes; ++a)
             if (a < axes && (int)threadIdx.x < n) v[a] = pos[(r0 + threadIdx.x) * axes + a];
     }
-    __device__ __forceinline__ void store(int* dst, int n, int axes, const BiasRow& row, int sign) const {
+    __device__ __forceinline__ void store(float* dst, int n, int axes, const BiasRow& row, int sign) const {
         if (threadIdx.x < kTcCols) {
 #pragma unroll
             for (int a = 0; a < kAttnMaxAxes; ++a)
                 if (a < axes)
                     dst[a * kTcCols + threadIdx.x] =
-                        (int)threadIdx.x < n ? BiasRow::column(v[a], row.ref[a], sign) : 0;
+                        (int)threadIdx.x < n ? BiasRow::column(v[a], row.ref[a], sign) : 0.f;
         }
     }
 };
@@ -347,12 +371,12 @@ __device__ __forceinline__ float lds_table(int addr) {
 // ONE: the table has one copy, at `one` (null: read it from global memory, for
 // head h); addresses are then used as entry numbers.
 template <bool MAPPED, bool ONE>
-__device__ __forceinline__ void bias16(const AttnArgs& A, const BiasRow& row, const int* cols, f32x2 (&t)[8],
+__device__ __forceinline__ void bias16(const AttnArgs& A, const BiasRow& row, const float* cols, f32x2 (&t)[8],
                                        const float* one, int h) {
-    auto entry = [&](int a, int col) {
-        const int at = row.template address<MAPPED>(A, a, col);
+    auto entry = [&](int a, float col) {
+        const int at = row.template address<MAPPED>(A, row.part[a], col, row.first[a]);
         if (!ONE) return lds_table(at);
-        const int e = a * A.a.buckets + ((at - row.lo[a]) >> 7);
+        const int e = a * A.a.buckets + ((at - __float_as_int(row.first[a])) >> 7);
         return one ? one[e] : table_entry(A.a, e, h) * kLog2e;
     };
 #pragma unroll
@@ -360,7 +384,7 @@ __device__ __forceinline__ void bias16(const AttnArgs& A, const BiasRow& row, co
         if (a < A.a.axes) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
-                const int4 c4 = *reinterpret_cast<const int4*>(cols + a * kTcCols + e);
+                const float4 c4 = *reinterpret_cast<const float4*>(cols + a * kTcCols + e);
                 const f32x2 x = pack2(entry(a, c4.x), entry(a, c4.y));
                 const f32x2 y = pack2(entry(a, c4.z), entry(a, c4.w));
                 t[e / 2] = a ? add2(t[e / 2], x) : x;

@@ -99,7 +99,7 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
     float* table = reinterpret_cast<float*>(smem + Shape::kTable);
     float* all_cells = table + Shape::table_words(entries, ONE);
     float* cells = all_cells + quarter * entries * 32;  // this quarter's
-    int* kpos = reinterpret_cast<int*>(all_cells + (Shape::kCells ? entries * 128 : 0));
+    float* kpos = reinterpret_cast<float*>(all_cells + (Shape::kCells ? entries * 128 : 0));
     uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kSlot);
     unsigned* flags = reinterpret_cast<unsigned*>(smem + Shape::kFlags);  // rows to form again
     const KeySpan span = key_span(A, t.first, t.first + t.rows - 1, t.lk, kTcCols);
@@ -240,18 +240,9 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         if (live && group == 0) *delta_at = delta;
     }
     const f32x2 scale2 = pack2(A.scale_log2, A.scale_log2), lse22 = pack2(-lse2, -lse2);
-    // Group a's cells of axis a: the bias addresses moved to this quarter's cells.
-    int cell_add = 0, cell_lo = 0, cell_hi = 0;
-    if (Shape::kCells) {
-        const int move = (int)smem_u32(cells) - (int)(sb + Shape::kTable);
-#pragma unroll
-        for (int a = 0; a < kAttnMaxAxes; ++a)
-            if (a == group) {
-                cell_add = bias.add[a] + move;
-                cell_lo = bias.lo[a] + move;
-                cell_hi = bias.hi[a] + move;
-            }
-    }
+    // Group a's cells of axis a: this lane's first.
+    const float cell_first =
+        __int_as_float((int)smem_u32(cells) + min(group, 2) * A.a.buckets * 128 + lane * 4);
 
     for (int i = 0; i < tiles; ++i) {
         if (Shape::kTight) done.even.wait();
@@ -269,7 +260,7 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         if (!whole) bits = live ? (uint32_t)(seen_keys(A, p, k0, n) >> c0) & 0xffffu : 0u;
         if (BIAS && bias.far) bits = 0u;
         const bool all = __all_sync(FULL_MASK, bits == 0xffffu);
-        const int* cols = kpos + (i % Shape::kPosStages) * A.a.axes * kTcCols;
+        const float* cols = kpos + (i % Shape::kPosStages) * A.a.axes * kTcCols;
         f32x2 b[8];
         if (BIAS)
             bias16<BIAS == 2, ONE>(A, bias, cols + c0, b,
@@ -318,7 +309,8 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         __syncthreads();
         tc_fence_after();
         if (Shape::kCells && group < A.a.axes) {
-            const int* axis = cols + group * kTcCols;
+            const float* axis = cols + group * kTcCols;
+            const float part = group == 0 ? bias.part[0] : group == 1 ? bias.part[1] : bias.part[2];
             const uint32_t buffer = tmem + ((uint32_t)quarter << 21) + Shape::kDS + (i & 1) * kTcCols;
 #pragma unroll
             for (int c = 0; c < kTcCols; c += 16) {
@@ -327,17 +319,11 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
                 int at_cell[16];
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
-                    const int4 c4 = *reinterpret_cast<const int4*>(axis + c + e);
-                    at_cell[e] = max(__viaddmin_s32(c4.x, cell_add, cell_hi), cell_lo);
-                    at_cell[e + 1] = max(__viaddmin_s32(c4.y, cell_add, cell_hi), cell_lo);
-                    at_cell[e + 2] = max(__viaddmin_s32(c4.z, cell_add, cell_hi), cell_lo);
-                    at_cell[e + 3] = max(__viaddmin_s32(c4.w, cell_add, cell_hi), cell_lo);
-                }
-                if (BIAS == 2) {
+                    const float4 c4 = *reinterpret_cast<const float4*>(axis + c + e);
+                    const float col[4] = {c4.x, c4.y, c4.z, c4.w};
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        at_cell[e] = cell_lo + 128 * min(max(__ldg(A.a.map + ((at_cell[e] - cell_lo) >> 7)), 0),
-                                                         A.a.buckets - 1);
+                    for (int k = 0; k < 4; ++k)
+                        at_cell[e + k] = bias.address<BIAS == 2>(A, part, col[k], cell_first);
                 }
                 tmem_wait_ld();
                 tmem_use(ds);
@@ -458,7 +444,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
     const int tid = threadIdx.x, lane = tid & 31, r = tid & 127, quarter = r >> 5, group = tid >> 7;
     const int hk = blockIdx.y, h0 = hk * A.group;
     const int j = t.first + r;
-    int* qpos = reinterpret_cast<int*>(smem + Shape::kPos);
+    float* qpos = reinterpret_cast<float*>(smem + Shape::kPos);
     float* rows = reinterpret_cast<float*>(smem + Shape::kRow);  // [stage][-lse2, -D][64]
     float* table = reinterpret_cast<float*>(smem + Shape::kTable);
     uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kSlot);
@@ -551,8 +537,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
         else
             for (int e = tid; e < A.a.axes * A.a.buckets; e += kBwdCompute) table[e] = table_entry(A.a, e, h) * kLog2e;
     };
-    // What a thread fetches of a tile and stores past the latency: -lse2 or -D of a
-    // query, and its position.  The head and the first query of the tile fetched next.
+    // What a thread fetches of a tile and stores (-lse2, -D, the position) past the latency.  The head and the first query of the tile fetched next.
     int next_head = h0, next_query = 0;
     float stat = 0.f;
     Columns columns;
@@ -560,14 +545,18 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
         if (i >= tiles) return;
         const int i0 = lo + (first + next_query) * kTcCols, n = min(kTcCols, hi - i0), c = tid & (kTcCols - 1);
         const int64_t row = (int64_t)t.other + i0;
-        if (tid < kTcCols) stat = c < n ? -load_lse2(A, row + c, next_head) : -INFINITY;
-        else if (tid < 2 * kTcCols) stat = c < n ? -A.a.delta[(int64_t)next_head * A.a.q_rows + row + c] : 0.f;
+        if (tid < 2 * kTcCols && c < n)
+            stat = (tid < kTcCols ? A.a.lse : A.a.delta)[(int64_t)next_head * A.a.q_rows + row + c];
         if (BIAS) columns.fetch(A.a.qpos, row, n, A.a.axes);
     };
     auto store_next = [&](int i) {
         if (i >= tiles) return;
         const int i0 = lo + (first + next_query) * kTcCols;
-        if (tid < 2 * kTcCols) rows[(i & 3) * 2 * kTcCols + tid] = stat;
+        if (tid < 2 * kTcCols) {
+            const bool on = (tid & (kTcCols - 1)) < hi - i0;
+            rows[(i & 3) * 2 * kTcCols + tid] =
+                tid < kTcCols ? (on && stat != -INFINITY ? -stat * kLog2e : -INFINITY) : (on ? -stat : 0.f);
+        }
         if (BIAS) columns.store(qpos + (i & 3) * 3 * kTcCols, min(kTcCols, hi - i0), A.a.axes, bias, -1);
         if (++next_query == per) {
             next_query = 0;
@@ -602,7 +591,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
         if (!whole) bits = live ? (uint32_t)(seeing_queries(A, j, p0, n) >> c) & 0xffffu : 0u;
         if (BIAS && bias.far) bits = 0u;
         const bool all = __all_sync(FULL_MASK, bits == 0xffffu);
-        const int* cols = qpos + (i & 3) * 3 * kTcCols;
+        const float* cols = qpos + (i & 3) * 3 * kTcCols;
         const float* row = rows + (i & 3) * 2 * kTcCols;
         {
             float s[16], dp[16];

@@ -1,7 +1,8 @@
 // Forward attention of serialised clouds for 16-bit types on the tensor cores
 // (definitions: attention_common.cuh; operands: attention_tc.cuh).
 //
-// A block owns 128 query rows of one head, one thread per row.  It streams the
+// A block owns 128 query rows of one head, one thread per row, and a warp that
+// issues copies and products.  It streams the
 // visible key tiles (64 keys) through two shared-memory stages.  Per tile the
 // tensor core forms S = Q K^T into TMEM; a thread reads its row of scores,
 // carries the running maximum and sum of the softmax, writes its weights back
@@ -17,6 +18,7 @@
 namespace mpo {
 namespace {
 
+constexpr int kFwdThreads = kTcRows + 32;
 template <int DP>
 struct FwdShape {
     static constexpr int kS = 0, kO = kTcCols;  // TMEM columns
@@ -36,7 +38,7 @@ struct FwdShape {
 };
 
 template <typename T, int DP, int BIAS>
-__global__ void __launch_bounds__(kTcRows, (BIAS && DP <= 64 ? 3 : FwdShape<DP>::kBlocks))
+__global__ void __launch_bounds__(kFwdThreads, (BIAS && DP <= 64 ? 3 : FwdShape<DP>::kBlocks))
 attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TcMaps M) {
     using Shape = FwdShape<DP>;
     extern __shared__ unsigned char smem_raw[];
@@ -46,40 +48,81 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
     const int h = blockIdx.y, hk = h / A.group;
     const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.q_tiles)[blockIdx.x];
     const int p = t.first + tid;
-    int* kpos = reinterpret_cast<int*>(smem + Shape::kPos);
+    float* kpos = reinterpret_cast<float*>(smem + Shape::kPos);
     float* table = reinterpret_cast<float*>(smem + Shape::kTable);
     uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kSlot);
 
-    if (tid < 32) tmem_alloc(smem_u32(slot), Shape::kCols);
-    if (tid == 0)
-        for (int i = 0; i < 5; ++i) mbar_init(sb + Shape::kBar + 8 * i);
     const KeySpan span = key_span(A, t.first, t.first + t.rows - 1, t.lk, kTcCols);
     const int tiles = span.count();
-    // Thread 0 issues the copies and the products.
-    auto load_keys = [&](int i) {
-        if (i >= tiles) return;
-        const uint32_t bar = sb + Shape::kFullK + 8 * (i & 1);
-        tma_expect(bar, Shape::kStage + (i == 0 ? Shape::kK : 0));
-        if (i == 0) tma_rows<DP, 128>(sb + Shape::kQ, &M.q, h, t.row, bar);
-        tma_rows<DP, kTcCols>(sb + Shape::kK + (i & 1) * Shape::kStage, &M.k, hk, t.other + span.tile(i) * kTcCols, bar);
-    };
-    auto load_values = [&](int i) {
-        if (i >= tiles) return;
-        const uint32_t bar = sb + Shape::kFullV + 8 * (i & 1);
-        tma_expect(bar, Shape::kStage);
-        tma_rows<DP, kTcCols>(sb + Shape::kV + (i & 1) * Shape::kStage, &M.v, hk, t.other + span.tile(i) * kTcCols, bar);
-    };
-    Patience patience(A.a.status);
-    auto scores = [&](int i) {
-        patience.wait(sb + Shape::kFullK + 8 * (i & 1), (i >> 1) & 1);
-        mma_scores<T, DP, kTcCols>(*slot + Shape::kS, sb + Shape::kQ, sb + Shape::kK + (i & 1) * Shape::kStage);
-    };
-    if (tid == 0) {
-        load_keys(0);
-        load_values(0);
-        load_keys(1);
+
+    if (tid >= kTcRows) {  // the warp that feeds the tensor core
+        tmem_alloc(smem_u32(slot), Shape::kCols);
+        auto load_keys = [&](int i) {
+            if (i >= tiles) return;
+            const uint32_t bar = sb + Shape::kFullK + 8 * (i & 1);
+            tma_expect(bar, Shape::kStage + (i == 0 ? Shape::kK : 0));
+            if (i == 0) tma_rows<DP, 128>(sb + Shape::kQ, &M.q, h, t.row, bar);
+            tma_rows<DP, kTcCols>(sb + Shape::kK + (i & 1) * Shape::kStage, &M.k, hk,
+                                  t.other + span.tile(i) * kTcCols, bar);
+        };
+        auto load_values = [&](int i) {
+            if (i >= tiles) return;
+            const uint32_t bar = sb + Shape::kFullV + 8 * (i & 1);
+            tma_expect(bar, Shape::kStage);
+            tma_rows<DP, kTcCols>(sb + Shape::kV + (i & 1) * Shape::kStage, &M.v, hk,
+                                  t.other + span.tile(i) * kTcCols, bar);
+        };
+        Patience patience(A.a.status);
+        uint32_t tmem = 0;
+        auto scores = [&](int i) {
+            if (i >= tiles) return;
+            patience.wait(sb + Shape::kFullK + 8 * (i & 1), (i >> 1) & 1);
+            mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kQ, sb + Shape::kK + (i & 1) * Shape::kStage);
+        };
+        if ((tid & 31) == 0) {
+            for (int i = 0; i < 5; ++i) mbar_init(sb + Shape::kBar + 8 * i);
+            load_keys(0);
+            load_values(0);
+            load_keys(1);
+        }
+        __syncwarp();
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        tmem = *slot;
+        if ((tid & 31) == 0) {
+            scores(0);
+            mma_commit(sb + Shape::kBar);
+            patience.wait(sb + Shape::kBar, 0);  // S of tile 0: the first keys' stage is free
+            load_keys(2);
+            load_values(1);
+        }
+        __syncwarp();
+        for (int i = 0; i < tiles; ++i) {
+            __syncthreads();  // the weights of tile i are in TMEM
+            if ((tid & 31) == 0) {
+                tc_fence_after();
+                patience.wait(sb + Shape::kFullV + 8 * (i & 1), (i >> 1) & 1);
+                mma_weighted<T, DP, kTcCols>(tmem + Shape::kO, tmem + Shape::kS,
+                                             sb + Shape::kV + (i & 1) * Shape::kStage, i > 0);
+                // Issued after P V and executed in order after it: S may overwrite the weights.
+                scores(i + 1);
+                mma_commit(sb + Shape::kBar);
+                // S of tile i + 1 and P V of tile i are done: their operands' stages are free.
+                // Copies get until the end of the next step.
+                patience.wait(sb + Shape::kBar, (i + 1) & 1);
+                load_keys(i + 3);
+                load_values(i + 2);
+            }
+            __syncwarp();
+        }
+        tc_fence_before();
+        __syncthreads();  // the rows have been read
+        tc_fence_after();
+        tmem_free(tmem, Shape::kCols);
+        return;
     }
-    __syncwarp();
+
     BiasRow bias;
     if (BIAS) bias.init(A, A.a.qpos, t.row, tid, tid < t.rows, sb + Shape::kTable, 1);
     auto first_key = [&](int i, int& k0, int& n) {
@@ -110,23 +153,12 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
     const uint32_t tmem = *slot;
     const uint32_t mine = tmem + ((uint32_t)(tid & ~31) << 16);  // this warp's lanes
     Waiter done(sb + Shape::kBar, A.a.status);
-    if (tid == 0 && tiles > 0) {
-        scores(0);
-        mma_commit(sb + Shape::kBar);
-    }
-    __syncwarp();
 
     // Running maximum in units of s2 = S * mul + bias (log2), as of the last rescale.
     float top = -INFINITY, sum = 0.f;
     const float mul = BIAS ? 1.f : (A.scale_log2 > 0.f ? A.scale_log2 : 1.f);
     for (int i = 0; i < tiles; ++i) {
         done.wait();
-        // S of tile i and P V of tile i - 1 are done: their operands' stages are free.
-        if (tid == 0) {
-            load_keys(i + 2);
-            load_values(i + 1);
-        }
-        __syncwarp();
         fetch_columns(i + 2);
         float s[kTcCols];
 #pragma unroll
@@ -136,7 +168,7 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
         int k0, n;
         first_key(i, k0, n);
         if (BIAS) {
-            const int* cols = kpos + (i % 3) * 3 * kTcCols;
+            const float* cols = kpos + (i % 3) * 3 * kTcCols;
             const f32x2 scale2 = pack2(A.scale_log2, A.scale_log2);
 #pragma unroll
             for (int c = 0; c < kTcCols; c += 16) {
@@ -216,16 +248,6 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
         tmem_wait_st();
         tc_fence_before();
         __syncthreads();
-        if (tid == 0) {
-            tc_fence_after();
-            const uint32_t stage = (i & 1) * Shape::kStage;
-            patience.wait(sb + Shape::kFullV + 8 * (i & 1), (i >> 1) & 1);
-            mma_weighted<T, DP, kTcCols>(tmem + Shape::kO, tmem + Shape::kS, sb + Shape::kV + stage, i > 0);
-            // Issued after P V and executed in order after it: S may overwrite the weights.
-            if (i + 1 < tiles) scores(i + 1);
-            mma_commit(sb + Shape::kBar);
-        }
-        __syncwarp();
     }
     if (tiles > 0) done.wait();
     const bool live = tid < t.rows;
@@ -262,10 +284,6 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
     }
     tc_fence_before();
     __syncthreads();
-    if (tid < 32) {
-        tc_fence_after();
-        tmem_free(tmem, Shape::kCols);
-    }
 }
 
 template <typename T, int DP, int BIAS>
@@ -277,7 +295,7 @@ int run(const AttnArgs& A, cudaStream_t s) {
     const int mapped = make_maps<DP>(maps, A, false);
     if (mapped != kOk) return mapped;
     const dim3 grid((unsigned)A.a.q_tile_count, (unsigned)A.a.heads);
-    attn_tc_fwd_kernel<T, DP, BIAS><<<grid, kTcRows, bytes, s>>>(A, maps);
+    attn_tc_fwd_kernel<T, DP, BIAS><<<grid, kFwdThreads, bytes, s>>>(A, maps);
     return check_launch("attn_tc_fwd_kernel");
 }
 template <typename T, int DP>
