@@ -29,6 +29,9 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return (uint32_t)__cvta_generic_to_shared(p);
 }
 
+// A value that is the same in every lane, for the uniform registers.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(FULL_MASK, v); }
+
 // ---------------------------------------------------------------- barriers
 __device__ __forceinline__ void mbar_init(uint32_t bar) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
@@ -54,7 +57,12 @@ struct Patience {
     int32_t* status;
     bool dead = false;
     __device__ __forceinline__ explicit Patience(int32_t* st) : status(st) {}
+    // By a converged warp.
     __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity) {
+        poll(bar, parity);
+        __syncwarp();
+    }
+    __device__ __forceinline__ void poll(uint32_t bar, uint32_t parity) {
         if (mbar_try(bar, parity)) return;
         const unsigned long long t0 = globaltimer_ns(), limit = dead ? kTcWaitNs / 1000 : kTcWaitNs;
         while (!mbar_try(bar, parity))
@@ -73,17 +81,17 @@ struct Waiter {
     __device__ __forceinline__ void wait() {
         patience.wait(bar, phase);
         phase ^= 1;
-        __syncwarp();  // the TMEM accesses that follow are warp-wide
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     }
 };
 
-// Two barriers used in turn: step i waits for what step i - 2 committed.
-struct WaiterPair {
+// B barriers used in turn: step i waits for what step i - B committed.
+template <int B>
+struct Waiters {
     Waiter even, odd;
-    __device__ __forceinline__ WaiterPair(uint32_t bars, int32_t* st) : even(bars, st), odd(bars + 8, st) {}
+    __device__ __forceinline__ Waiters(uint32_t bars, int32_t* st) : even(bars, st), odd(bars + 8, st) {}
     __device__ __forceinline__ void wait(int i) {
-        if (i & 1) odd.wait();
+        if (B == 2 && (i & 1)) odd.wait();
         else even.wait();
     }
 };
@@ -185,9 +193,14 @@ struct TcTile {
 struct TcMaps {
     CUtensorMap q, k, v, g;
 };
+// What follows is called by a whole converged warp and issued by one elected
+// lane, the same one every time: the operands then stay in uniform registers
+// (under a branch on the lane each product took 90 cycles to issue, twice what
+// it takes to run).
+#define MPO_ELECTED "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e "
 // Announces `bytes` on a barrier whose phase ends when they have come.
 __device__ __forceinline__ void tma_expect(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+    asm volatile(MPO_ELECTED "mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes)
                  : "memory");
 }
 // Rows [row, row + ROWS) of head h into a tile; rows past the tensor and elements
@@ -200,8 +213,8 @@ __device__ __forceinline__ void tma_rows(uint32_t tile, const CUtensorMap* map, 
 #pragma unroll
         for (int r = 0; r < ROWS; r += 64)
             asm volatile(
-                "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
-                "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(tile + (half * ROWS + r) * L::kRowBytes),
+                MPO_ELECTED "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
+                "[%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(tile + (half * ROWS + r) * L::kRowBytes),
                 "l"(map), "r"(half * 64), "r"(h), "r"(row + r), "r"(bar)
                 : "memory");
 }
@@ -214,23 +227,25 @@ __device__ __forceinline__ constexpr uint32_t tc_idesc(int n, bool b_mn) {
 }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
         : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
         : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile(
-        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+        MPO_ELECTED "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
         : "memory");
 }
 // D (128 x NB) = A (128 rows of tile a) . B (NB rows of tile b)^T over DP elements.

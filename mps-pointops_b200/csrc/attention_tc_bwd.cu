@@ -29,21 +29,25 @@ namespace {
 // P dP in float32 first; kGradQTable then forms dq and the table's gradient.
 constexpr size_t kTcSmem = 232448;  // shared memory of a block at most
 // Barrier of the computing threads alone.
-__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
+template <int THREADS>
+__device__ __forceinline__ void compute_sync() {
+    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+}
 
 enum QueryMode { kGradQ = 0, kDelta = 1, kGradQTable = 2 };
 
-// Threads: four groups of 128; thread `row` of each group shares the row and
-// takes 16 columns of every tile, so that 16 warps are on an SM (one thread per
-// row left 4 to 8, and most of the time went to fixed latencies).  One thread of
-// a further warp issues the copies and the products: a computing warp that did
-// was held up by the tensor core's queue, 2400 of 4300 cycles of a step at D =
-// 128, and the others with it at the next barrier.
+// Threads: NG groups of 128; thread `row` of each group shares the row and takes
+// 64 / NG columns of every tile, so that 16 warps are on an SM (one thread per
+// row left 4 to 8, and most of the time went to fixed latencies).  A further warp
+// issues the copies and the products: a computing warp that did was held up by
+// the tensor core's queue, 2400 of 4300 cycles of a step at D = 128, and the
+// others with it at the next barrier.
 //
-// S and dP have two buffers in TMEM.  At the end of step i the tensor core gets
-// dq += dS_i K_i and then, over the buffer that this frees, S and dP of tile
-// i + 2: those of tile i + 1 are ready when the step's barrier falls.  The tile
-// after those is copied as soon as the products of tile i - 1 are done.
+// Where shared memory and TMEM serve two blocks per SM (DP <= 64, no cells), each
+// has NG = 2 and one buffer of S and dP, and the blocks fill each other's gaps.
+// Else one block has NG = 4 and two buffers: at the end of step i the tensor core
+// gets dq += dS_i K_i and then, over the buffer that this frees, S and dP of tile
+// i + 2, so those of tile i + 1 are ready when the step's barrier falls.
 //
 // Table gradient: a thread may only add to cells that no other adds to, so lane
 // l of quarter w (rows 32 w ..) has its own cell of each entry ([w][entry][l],
@@ -52,15 +56,18 @@ enum QueryMode { kGradQ = 0, kDelta = 1, kGradQTable = 2 };
 // (two buffers), and after the tile's barrier group a adds all 64 columns of
 // them to its axis.  With DP = 128 the cells (up to 128 KB) leave room for one
 // stage of keys and values, one buffer of S and dP, and one copy of the table.
-constexpr int kBwdCompute = 4 * kTcRows, kBwdThreads = kBwdCompute + 32, kBwdCols = kTcCols / 4;
 template <int DP, int MODE>
 struct QueryShape {
     static constexpr bool kCells = MODE == kGradQTable, kTight = kCells && DP == 128;
+    static constexpr int kBlocks = kCells || DP == 128 ? 1 : 2, kGroups = 4 / kBlocks;
+    static constexpr int kCompute = kGroups * kTcRows, kThreads = kCompute + 32, kPer = kTcCols / kGroups;
+    static constexpr int kBuffers = kTight || kBlocks == 2 ? 1 : 2;
     // Keys serve S and dq of their tile, values dP alone.
-    static constexpr int kKStages = kTight ? 1 : 4, kVStages = kTight ? 1 : 2, kPosStages = kTight ? 3 : 4;
-    static constexpr int kS = 0, kDP = kTcCols, kBuffer = kTight ? 0 : 2 * kTcCols;  // TMEM columns
+    static constexpr int kKStages = kTight ? 1 : 2 + kBuffers, kVStages = kTight ? 1 : 2;
+    static constexpr int kPosStages = kTight ? 3 : 4;
+    static constexpr int kS = 0, kDP = kTcCols, kBuffer = (kBuffers - 1) * 2 * kTcCols;  // TMEM columns
     static constexpr int kDQ = 2 * kTcCols + kBuffer, kDS = kDQ + DP;
-    static constexpr int kCols = MODE == kDelta ? 256 : 512;
+    static constexpr int kCols = kBlocks == 2 ? 256 : 512;
     static constexpr uint32_t kQ = 0, kG = TcTile<DP>::bytes(128), kStage = TcTile<DP>::bytes(64),
                               kK = 2 * kG, kV = kK + kKStages * kStage, kBar = kV + kVStages * kStage,
                               kTable = kBar + 128;
@@ -76,18 +83,20 @@ struct QueryShape {
     static size_t bytes(int axes, int entries, bool one) {
         size_t need = kTable + (size_t)(pos_words(axes) + table_words(entries, one)) * 4 +
                       (kCells ? (size_t)entries * 512 : 0) + 1024;
-        if (MODE == kDelta && need < kTable + 4 * kBwdCompute + 1024) need = kTable + 4 * kBwdCompute + 1024;
-        return need > 233472 / 2 ? need : 233472 / 2;  // one block per SM: TMEM serves no second one
+        if (MODE == kDelta && need < kTable + 4 * kCompute + 1024) need = kTable + 4 * kCompute + 1024;
+        const size_t least = 233472 / (kBlocks + 1);  // no more blocks than TMEM serves
+        return need > least ? need : least;
     }
     // One copy of the table where a copy per lane does not fit beside the cells.
     static bool one_copy(int axes, int entries) { return kTight || bytes(axes, entries, false) > kTcSmem; }
 };
 
 template <typename T, int DP, int BIAS, int MODE, bool ONE>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__((QueryShape<DP, MODE>::kThreads), (QueryShape<DP, MODE>::kBlocks))
 attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TcMaps M,
                      float* __restrict__ partial) {
     using Shape = QueryShape<DP, MODE>;
+    constexpr int kPer = Shape::kPer, kBuffers = Shape::kBuffers;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sb = smem_u32(smem);
@@ -103,9 +112,9 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
     uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kSlot);
     unsigned* flags = reinterpret_cast<unsigned*>(smem + Shape::kFlags);  // rows to form again
     const KeySpan span = key_span(A, t.first, t.first + t.rows - 1, t.lk, kTcCols);
-    const int tiles = span.count();
+    const int tiles = (int)uniform((uint32_t)span.count());
 
-    if (tid >= kBwdCompute) {  // the warp that feeds the tensor core
+    if (tid >= Shape::kCompute) {  // the warp that feeds the tensor core
         tmem_alloc(smem_u32(slot), Shape::kCols);
         auto full_k = [&](int i) { return sb + Shape::kFullK + 8 * (i % Shape::kKStages); };
         auto full_v = [&](int i) { return sb + Shape::kFullV + 8 * (i % Shape::kVStages); };
@@ -121,7 +130,7 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         uint32_t tmem = 0;
         auto scores = [&](int i) {  // S and dP of tile i into its buffer
             if (i >= tiles) return;
-            const uint32_t buffer = tmem + (i & 1) * Shape::kBuffer;
+            const uint32_t buffer = tmem + (i & (kBuffers - 1)) * Shape::kBuffer;
             patience.wait(full_k(i), (i / Shape::kKStages) & 1);
             mma_scores<T, DP, kTcCols>(buffer + Shape::kS, sb + Shape::kQ,
                                        sb + Shape::kK + (i % Shape::kKStages) * Shape::kStage);
@@ -129,57 +138,53 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
             mma_scores<T, DP, kTcCols>(buffer + Shape::kDP, sb + Shape::kG,
                                        sb + Shape::kV + (i % Shape::kVStages) * Shape::kStage);
         };
-        // Step i commits to barrier i & 1; the prologue stands for steps -2 and -1.
-        auto products_done = [&](int i) { patience.wait(sb + Shape::kBar + 8 * (i & 1), ((i + 2) >> 1) & 1); };
-        if (lane == 0) {
+        if (lane == 0)
             for (int i = 0; i < 9; ++i) mbar_init(sb + Shape::kBar + 8 * i);
-            tma_expect(sb + Shape::kFullQ, 2 * Shape::kG);
-            tma_rows<DP, 128>(sb + Shape::kQ, &M.q, h, t.row, sb + Shape::kFullQ);
-            tma_rows<DP, 128>(sb + Shape::kG, &M.g, h, t.row, sb + Shape::kFullQ);
-            load_tile(0);
-            if (!Shape::kTight) load_tile(1);
-        }
         __syncwarp();
+        tma_expect(sb + Shape::kFullQ, 2 * Shape::kG);
+        tma_rows<DP, 128>(sb + Shape::kQ, &M.q, h, t.row, sb + Shape::kFullQ);
+        tma_rows<DP, 128>(sb + Shape::kG, &M.g, h, t.row, sb + Shape::kFullQ);
+        load_tile(0);
+        if (!Shape::kTight) load_tile(1);
         tc_fence_before();
         __syncthreads();
         tc_fence_after();
-        tmem = *slot;
-        if (lane == 0) {
-            patience.wait(sb + Shape::kFullQ, 0);
-            scores(0);
-            mma_commit(sb + Shape::kBar);
-            if (!Shape::kTight) {
-                scores(1);
-                mma_commit(sb + Shape::kBar + 8);
-                products_done(-2);
-                load_tile(2);
-            }
+        tmem = uniform(*slot);
+        patience.wait(sb + Shape::kFullQ, 0);
+        // Step i commits to barrier i mod kBuffers; the prologue stands for the kBuffers steps
+        // before step 0.
+        scores(0);
+        mma_commit(sb + Shape::kBar);
+        if (kBuffers == 2) {
+            scores(1);
+            mma_commit(sb + Shape::kBar + 8);
+            patience.wait(sb + Shape::kBar, 0);
+            load_tile(2);
         }
-        __syncwarp();
         for (int i = 0; i < tiles; ++i) {
             __syncthreads();  // the score gradients of tile i are in TMEM
-            if (lane == 0) {
-                tc_fence_after();
-                if (MODE != kDelta)
-                    mma_weighted<T, DP, kTcCols>(tmem + Shape::kDQ, tmem + (i & 1) * Shape::kBuffer + Shape::kS,
-                                                 sb + Shape::kK + (i % Shape::kKStages) * Shape::kStage, i > 0);
-                if (!Shape::kTight) {
-                    scores(i + 2);  // executed in order: the buffer may be overwritten
-                    mma_commit(sb + Shape::kBar + 8 * (i & 1));
-                    products_done(i - 1);
-                    load_tile(i + 3);
-                } else {
-                    // One stage, one buffer: barrier 1 tells that it is free, barrier 0 that S is there.
-                    mma_commit(sb + Shape::kBar + 8);
-                    patience.wait(sb + Shape::kBar + 8, i & 1);
-                    if (i + 1 < tiles) {
-                        load_tile(i + 1);
-                        scores(i + 1);
-                        mma_commit(sb + Shape::kBar);
-                    }
+            tc_fence_after();
+            if (MODE != kDelta)
+                mma_weighted<T, DP, kTcCols>(tmem + Shape::kDQ,
+                                             tmem + (i & (kBuffers - 1)) * Shape::kBuffer + Shape::kS,
+                                             sb + Shape::kK + (i % Shape::kKStages) * Shape::kStage, i > 0);
+            if (Shape::kTight) {
+                // One stage, one buffer: barrier 1 tells that it is free, barrier 0 that S is there.
+                mma_commit(sb + Shape::kBar + 8);
+                patience.wait(sb + Shape::kBar + 8, i & 1);
+                if (i + 1 < tiles) {
+                    load_tile(i + 1);
+                    scores(i + 1);
+                    mma_commit(sb + Shape::kBar);
                 }
+            } else {
+                scores(i + kBuffers);  // executed in order: the buffer may be overwritten
+                mma_commit(sb + Shape::kBar + 8 * (i & (kBuffers - 1)));
+                // The products of step i - 1 are done (one buffer: the others waited for them):
+                // keys i - 1 and values i + kBuffers - 1 are free.
+                if (kBuffers == 2) patience.wait(sb + Shape::kBar + 8 * ((i - 1) & 1), ((i + 1) >> 1) & 1);
+                load_tile(i + kBuffers + 1);
             }
-            __syncwarp();
         }
         tc_fence_before();
         __syncthreads();  // the results have been read
@@ -210,11 +215,11 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         if (!ONE) {
             tc_load_table(A, table, h);
         } else if (!Shape::kTight || entries <= Shape::kTightEntries) {
-            for (int e = tid; e < entries; e += kBwdCompute) table[e] = table_entry(A.a, e, h) * kLog2e;
+            for (int e = tid; e < entries; e += Shape::kCompute) table[e] = table_entry(A.a, e, h) * kLog2e;
         }
     }
     if (Shape::kCells)
-        for (int e = tid; e < entries * 128; e += kBwdCompute) all_cells[e] = 0.f;
+        for (int e = tid; e < entries * 128; e += Shape::kCompute) all_cells[e] = 0.f;
     const float lse2 = live ? load_lse2(A, t.row + r, h) : INFINITY;
     store_columns(0);
     fetch_columns(1);
@@ -223,8 +228,8 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
-    const uint32_t mine = tmem + ((uint32_t)quarter << 21) + kBwdCols * group;  // lanes 32 quarter .., own columns
-    WaiterPair done(sb + Shape::kBar, A.a.status);
+    const uint32_t mine = tmem + ((uint32_t)quarter << 21) + kPer * group;  // lanes 32 quarter .., own columns
+    Waiters<kBuffers> done(sb + Shape::kBar, A.a.status);
     float delta = 0.f;  // D; kDelta: this thread's columns of its sum so far
     if (MODE == kGradQTable) {
         if (live) delta = *delta_at;
@@ -245,22 +250,24 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         __int_as_float((int)smem_u32(cells) + min(group, 2) * A.a.buckets * 128 + lane * 4);
 
     for (int i = 0; i < tiles; ++i) {
-        if (Shape::kTight) done.even.wait();
-        else done.wait(i);
+        done.wait(i);
         fetch_columns(i + Shape::kAhead);
         const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
         const bool whole = n == kTcCols && t.rows == 128 &&
                            all_visible(A, t.first, t.first + 127, k0, k0 + kTcCols - 1);
-        const int c0 = kBwdCols * group;  // this thread's columns
-        const uint32_t own = mine + (i & 1) * Shape::kBuffer;
+        uint32_t bits = ~0u;  // of this thread's columns
+        if (!whole) bits = live ? (uint32_t)(seen_keys(A, p, k0, n) >> (kPer * group)) : 0u;
+        if (BIAS && bias.far) bits = 0u;
+        constexpr uint32_t kFull = kPer == 32 ? ~0u : (1u << (kPer & 31)) - 1;
+        const bool all = __all_sync(FULL_MASK, (bits & kFull) == kFull);
+        const float* cols = kpos + (i % Shape::kPosStages) * A.a.axes * kTcCols;
+#pragma unroll
+        for (int cc = 0; cc < kPer; cc += 16) {
+        const int c0 = kPer * group + cc;
+        const uint32_t own = mine + (i & (kBuffers - 1)) * Shape::kBuffer + cc;
         float s[16], dp[16];
         tmem_ld16(own + Shape::kS, s);
         tmem_ld16(own + Shape::kDP, dp);
-        uint32_t bits = 0xffffu;
-        if (!whole) bits = live ? (uint32_t)(seen_keys(A, p, k0, n) >> c0) & 0xffffu : 0u;
-        if (BIAS && bias.far) bits = 0u;
-        const bool all = __all_sync(FULL_MASK, bits == 0xffffu);
-        const float* cols = kpos + (i % Shape::kPosStages) * A.a.axes * kTcCols;
         f32x2 b[8];
         if (BIAS)
             bias16<BIAS == 2, ONE>(A, bias, cols + c0, b,
@@ -286,7 +293,7 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         }
         if (!all) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = (bits >> e) & 1u ? s[e] : 0.f;
+            for (int e = 0; e < 16; ++e) s[e] = (bits >> (cc + e)) & 1u ? s[e] : 0.f;
         }
         if (MODE == kDelta) {
             f32x2 sum = pack2(s[0], s[1]);
@@ -297,11 +304,12 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
             delta += u + v;
         } else {
             if (Shape::kCells)
-                tmem_st16(mine + Shape::kDS + (i & 1) * kTcCols, reinterpret_cast<const uint32_t*>(s));
+                tmem_st16(mine + Shape::kDS + (i & 1) * kTcCols + cc, reinterpret_cast<const uint32_t*>(s));
             uint32_t w[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = Elem<T>::two(s[2 * e], s[2 * e + 1]);
             tmem_st8(own + Shape::kS, w);
+        }
         }
         if (i + Shape::kAhead > 1) store_columns(i + Shape::kAhead);
         if (MODE != kDelta) tmem_wait_st();
@@ -337,10 +345,10 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
             tc_fence_before();
         }
     }
-    // What was committed last: by steps tiles - 2 and tiles - 1.
+    // What was committed last.
     if (!Shape::kTight) {
         done.wait(tiles);
-        done.wait(tiles + 1);
+        if (kBuffers == 2) done.wait(tiles + 1);
     } else if (tiles > 0) {
         done.odd.phase = (tiles - 1) & 1;
         done.odd.wait();
@@ -349,11 +357,11 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
     if (MODE == kDelta) {
         // The groups' shares in order; the table's place is free now.
         float* shares = table;
-        compute_sync();
+        compute_sync<Shape::kCompute>();
         shares[tid] = delta;
-        compute_sync();
+        compute_sync<Shape::kCompute>();
         if (group == 0) {
-            for (int g = 1; g < 4; ++g) delta += shares[g * kTcRows + r];
+            for (int g = 1; g < Shape::kGroups; ++g) delta += shares[g * kTcRows + r];
             for (unsigned bad = __ballot_sync(FULL_MASK, far); bad; bad &= bad - 1) {
                 const int row = (r & ~31) + __ffs(bad) - 1;
                 const float d = exact_delta_row<T>(A, (int64_t)t.row + row, t.first + row, t.other, t.lk, h);
@@ -365,12 +373,12 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         bool nan = far;
 #pragma unroll
         for (int c = 0; c < DP; c += 16) {
-            if ((c / 16) % 4 != group) continue;
+            if ((c / 16) % Shape::kGroups != group) continue;
             float o[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = 0.f;
             if (tiles > 0) {
-                tmem_ld16(mine - kBwdCols * group + Shape::kDQ + c, o);
+                tmem_ld16(mine - kPer * group + Shape::kDQ + c, o);
                 tmem_wait_ld();
                 tmem_use(o);
             }
@@ -387,7 +395,7 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         }
         const unsigned bad_here = __ballot_sync(FULL_MASK, nan), apart = __ballot_sync(FULL_MASK, far);
         if (lane == 0 && bad_here) atomicOr(flags + quarter, bad_here);
-        compute_sync();
+        compute_sync<Shape::kCompute>();
         if (group == 0)
             for (unsigned bad = flags[quarter]; bad; bad &= bad - 1) {
                 const int b = __ffs(bad) - 1, row = (r & ~31) + b;
@@ -398,7 +406,7 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
     tc_fence_before();
     __syncthreads();
     if (Shape::kCells)
-        for (int e = tid; e < entries; e += kBwdCompute) {
+        for (int e = tid; e < entries; e += Shape::kCompute) {
             float v = 0.f;
             for (int w = 0; w < 4; ++w)
                 for (int l = 0; l < 32; ++l) v += all_cells[(w * entries + e) * 32 + ((l + e) & 31)];
@@ -411,18 +419,22 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
 // are followed by S^T and dP^T of tile i + 2 over the same buffer.
 template <int DP>
 struct GradKvShape {
-    static constexpr int kS = 0, kDP = kTcCols, kBuffer = 2 * kTcCols, kDK = 4 * kTcCols, kDV = kDK + DP;
-    static constexpr int kCols = 512;
+    static constexpr int kBlocks = DP == 128 ? 1 : 2, kGroups = 4 / kBlocks, kBuffers = 3 - kBlocks;
+    static constexpr int kCompute = kGroups * kTcRows, kThreads = kCompute + 32, kPer = kTcCols / kGroups;
+    static constexpr int kStages = 2 + kBuffers, kRowStages = 4;
+    static constexpr int kS = 0, kDP = kTcCols, kBuffer = (kBuffers - 1) * 2 * kTcCols;
+    static constexpr int kDK = 2 * kTcCols + kBuffer, kDV = kDK + DP, kCols = 512 / kBlocks;
     static constexpr uint32_t kK = 0, kV = TcTile<DP>::bytes(128), kStage = TcTile<DP>::bytes(64),
-                              kQ = 2 * kV, kG = kQ + 4 * kStage, kRow = kG + 4 * kStage,
-                              kPos = kRow + 4 * 2 * kTcCols * 4, kBar = kPos + 4 * 3 * kTcCols * 4,
-                              kTable = kBar + 128;
+                              kQ = 2 * kV, kG = kQ + kStages * kStage, kRow = kG + kStages * kStage,
+                              kPos = kRow + kRowStages * 2 * kTcCols * 4,
+                              kBar = kPos + kRowStages * 3 * kTcCols * 4, kTable = kBar + 128;
     // Barriers: products (2); stages of queries and gradients (4), K and V; then TMEM's address, row flags.
     static constexpr uint32_t kFull = kBar + 16, kFullK = kBar + 48, kSlot = kBar + 56, kFlags = kBar + 64;
     static bool one_copy(int entries) { return kTable + (size_t)entries * 128 + 1024 > kTcSmem; }
     static size_t bytes(int entries, bool one) {
         const size_t need = kTable + (size_t)entries * (one ? 4 : 128) + 1024;
-        return need > 233472 / 2 ? need : 233472 / 2;  // one block per SM: TMEM serves no second one
+        const size_t least = 233472 / (kBlocks + 1);  // no more blocks than TMEM serves
+        return need > least ? need : least;
     }
 };
 
@@ -431,10 +443,11 @@ struct GradKvShape {
 // ([cloud * sink tiles + tile][key head][share][dk, dv][128][dim], float32) for
 // the join kernel.  shares == 1: no block does.
 template <typename T, int DP, int BIAS, bool ONE>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__((GradKvShape<DP>::kThreads), (GradKvShape<DP>::kBlocks))
 attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TcMaps M, int shares,
                        float* __restrict__ partial) {
     using Shape = GradKvShape<DP>;
+    constexpr int kPer = Shape::kPer, kBuffers = Shape::kBuffers;
     const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.k_tiles)[blockIdx.x];
     const bool shared = shares > 1 && t.first < A.a.sinks;
     if (!shared && blockIdx.z > 0) return;
@@ -457,16 +470,16 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
         first = (int)((int64_t)per * blockIdx.z / shares);
         per = (int)((int64_t)per * (blockIdx.z + 1) / shares) - first;
     }
-    const int tiles = per * A.group;
+    const int tiles = (int)uniform((uint32_t)(per * A.group));
 
-    if (tid >= kBwdCompute) {  // the warp that feeds the tensor core
+    if (tid >= Shape::kCompute) {  // the warp that feeds the tensor core
         tmem_alloc(smem_u32(slot), Shape::kCols);
-        auto full = [&](int i) { return sb + Shape::kFull + 8 * (i & 3); };
+        auto full = [&](int i) { return sb + Shape::kFull + 8 * (i % Shape::kStages); };
         int next_head = h0, next_query = 0;  // of the tile to be copied next
         auto load_next = [&](int i) {
             if (i >= tiles) return;
             const int row = t.other + lo + (first + next_query) * kTcCols;
-            const uint32_t stage = (i & 3) * Shape::kStage;
+            const uint32_t stage = (i % Shape::kStages) * Shape::kStage;
             tma_expect(full(i), 2 * Shape::kStage);
             tma_rows<DP, kTcCols>(sb + Shape::kQ + stage, &M.q, next_head, row, full(i));
             tma_rows<DP, kTcCols>(sb + Shape::kG + stage, &M.g, next_head, row, full(i));
@@ -479,45 +492,42 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
         uint32_t tmem = 0;
         auto scores = [&](int i) {  // S^T and dP^T of tile i into its buffer
             if (i >= tiles) return;
-            const uint32_t buffer = tmem + (i & 1) * Shape::kBuffer, stage = (i & 3) * Shape::kStage;
-            patience.wait(full(i), (i >> 2) & 1);
+            const uint32_t buffer = tmem + (i & (kBuffers - 1)) * Shape::kBuffer;
+            const uint32_t stage = (i % Shape::kStages) * Shape::kStage;
+            patience.wait(full(i), (i / Shape::kStages) & 1);
             mma_scores<T, DP, kTcCols>(buffer + Shape::kS, sb + Shape::kK, sb + Shape::kQ + stage);
             mma_scores<T, DP, kTcCols>(buffer + Shape::kDP, sb + Shape::kV, sb + Shape::kG + stage);
         };
-        auto products_done = [&](int i) { patience.wait(sb + Shape::kBar + 8 * (i & 1), ((i + 2) >> 1) & 1); };
-        if (lane == 0) {
+        if (lane == 0)
             for (int i = 0; i < 7; ++i) mbar_init(sb + Shape::kBar + 8 * i);
-            tma_expect(sb + Shape::kFullK, 2 * Shape::kV);
-            tma_rows<DP, 128>(sb + Shape::kK, &M.k, hk, t.row, sb + Shape::kFullK);
-            tma_rows<DP, 128>(sb + Shape::kV, &M.v, hk, t.row, sb + Shape::kFullK);
-            for (int i = 0; i < 3; ++i) load_next(i);
-        }
         __syncwarp();
+        tma_expect(sb + Shape::kFullK, 2 * Shape::kV);
+        tma_rows<DP, 128>(sb + Shape::kK, &M.k, hk, t.row, sb + Shape::kFullK);
+        tma_rows<DP, 128>(sb + Shape::kV, &M.v, hk, t.row, sb + Shape::kFullK);
+        for (int i = 0; i <= kBuffers; ++i) load_next(i);
         tc_fence_before();
         __syncthreads();
         tc_fence_after();
-        tmem = *slot;
-        if (lane == 0) {
-            patience.wait(sb + Shape::kFullK, 0);
-            scores(0);
-            mma_commit(sb + Shape::kBar);
+        tmem = uniform(*slot);
+        patience.wait(sb + Shape::kFullK, 0);
+        scores(0);
+        mma_commit(sb + Shape::kBar);
+        if (kBuffers == 2) {
             scores(1);
             mma_commit(sb + Shape::kBar + 8);
         }
-        __syncwarp();
         for (int i = 0; i < tiles; ++i) {
             __syncthreads();  // weights and score gradients of tile i are in TMEM
-            if (lane == 0) {
-                tc_fence_after();
-                const uint32_t stage = (i & 3) * Shape::kStage, buffer = tmem + (i & 1) * Shape::kBuffer;
-                mma_weighted<T, DP, kTcCols>(tmem + Shape::kDV, buffer + Shape::kS, sb + Shape::kG + stage, i > 0);
-                mma_weighted<T, DP, kTcCols>(tmem + Shape::kDK, buffer + Shape::kDP, sb + Shape::kQ + stage, i > 0);
-                scores(i + 2);  // executed in order: the buffer may be overwritten
-                mma_commit(sb + Shape::kBar + 8 * (i & 1));
-                products_done(i - 1);
-                load_next(i + 3);
-            }
-            __syncwarp();
+            tc_fence_after();
+            const uint32_t stage = (i % Shape::kStages) * Shape::kStage;
+            const uint32_t buffer = tmem + (i & (kBuffers - 1)) * Shape::kBuffer;
+            mma_weighted<T, DP, kTcCols>(tmem + Shape::kDV, buffer + Shape::kS, sb + Shape::kG + stage, i > 0);
+            mma_weighted<T, DP, kTcCols>(tmem + Shape::kDK, buffer + Shape::kDP, sb + Shape::kQ + stage, i > 0);
+            scores(i + kBuffers);  // executed in order: the buffer may be overwritten
+            mma_commit(sb + Shape::kBar + 8 * (i & (kBuffers - 1)));
+            // The products of step i - 1 are done (one buffer: the others waited for them).
+            if (kBuffers == 2) patience.wait(sb + Shape::kBar + 8 * ((i - 1) & 1), ((i + 1) >> 1) & 1);
+            load_next(i + kBuffers + 1);
         }
         tc_fence_before();
         __syncthreads();  // the results have been read
@@ -535,7 +545,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
         if (!BIAS) return;
         if (!ONE) tc_load_table(A, table, h);
         else
-            for (int e = tid; e < A.a.axes * A.a.buckets; e += kBwdCompute) table[e] = table_entry(A.a, e, h) * kLog2e;
+            for (int e = tid; e < A.a.axes * A.a.buckets; e += Shape::kCompute) table[e] = table_entry(A.a, e, h) * kLog2e;
     };
     // What a thread fetches of a tile and stores (-lse2, -D, the position) past the latency.  The head and the first query of the tile fetched next.
     int next_head = h0, next_query = 0;
@@ -573,27 +583,29 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
     tc_fence_after();
     const uint32_t tmem = *slot;
     const uint32_t mine = tmem + ((uint32_t)quarter << 21);
-    WaiterPair done(sb + Shape::kBar, A.a.status);
+    Waiters<kBuffers> done(sb + Shape::kBar, A.a.status);
     int head = h0, query = 0;  // of the tile at hand
     for (int i = 0; i < tiles; ++i) {
         if (BIAS && query == 0 && i > 0) {  // the next query head's table
             load_table(head);
-            compute_sync();
+            compute_sync<Shape::kCompute>();
         }
         done.wait(i);
         fetch_next(i + 2);
         const int i0 = lo + (first + query) * kTcCols, n = min(kTcCols, hi - i0), p0 = i0 + t.lk - t.lq;
         const bool whole = n == kTcCols && t.rows == 128 &&
                            all_visible(A, p0, p0 + kTcCols - 1, t.first, t.first + 127);
-        const int c = kBwdCols * group;  // this thread's columns
-        const uint32_t own = mine + (i & 1) * Shape::kBuffer + c;
-        uint32_t bits = 0xffffu;
-        if (!whole) bits = live ? (uint32_t)(seeing_queries(A, j, p0, n) >> c) & 0xffffu : 0u;
+        uint32_t bits = ~0u;  // of this thread's columns
+        if (!whole) bits = live ? (uint32_t)(seeing_queries(A, j, p0, n) >> (kPer * group)) : 0u;
         if (BIAS && bias.far) bits = 0u;
-        const bool all = __all_sync(FULL_MASK, bits == 0xffffu);
+        constexpr uint32_t kFull = kPer == 32 ? ~0u : (1u << (kPer & 31)) - 1;
+        const bool all = __all_sync(FULL_MASK, (bits & kFull) == kFull);
         const float* cols = qpos + (i & 3) * 3 * kTcCols;
         const float* row = rows + (i & 3) * 2 * kTcCols;
-        {
+#pragma unroll
+        for (int cc = 0; cc < kPer; cc += 16) {
+            const int c = kPer * group + cc;
+            const uint32_t own = mine + (i & (kBuffers - 1)) * Shape::kBuffer + c;
             float s[16], dp[16];
             tmem_ld16(own + Shape::kS, s);
             tmem_ld16(own + Shape::kDP, dp);
@@ -628,7 +640,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
             if (!all) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const bool on = (bits >> e) & 1u;
+                    const bool on = (bits >> (cc + e)) & 1u;
                     s[e] = on ? s[e] : 0.f;
                     dp[e] = on ? dp[e] : 0.f;
                 }
@@ -651,7 +663,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
         }
     }
     done.wait(tiles);
-    done.wait(tiles + 1);
+    if (kBuffers == 2) done.wait(tiles + 1);
     bool nan = BIAS && live && bias.far;
     const int64_t at = (((int64_t)t.row + r) * A.a.kv_heads + hk) * A.a.dim;
     const int sink_tiles = (A.a.sinks + kAttnTile - 1) / kAttnTile;
@@ -664,7 +676,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
     for (int which = 0; which < 2; ++which)
 #pragma unroll
         for (int c = 0; c < DP; c += 16) {
-            if ((c / 16) % 4 != group) continue;
+            if ((c / 16) % Shape::kGroups != group) continue;
             float o[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = 0.f;
@@ -695,7 +707,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
         }
     const unsigned bad_here = __ballot_sync(FULL_MASK, nan);
     if (lane == 0 && bad_here) atomicOr(flags + quarter, bad_here);
-    compute_sync();
+    compute_sync<Shape::kCompute>();
     if (!shared && group == 0)
         for (unsigned bad = flags[quarter]; bad; bad &= bad - 1) {
             const int row = (r & ~31) + __ffs(bad) - 1;
@@ -759,7 +771,7 @@ int run_q(const AttnArgs& A, const TcMaps& M, float* partial, cudaStream_t s) {
     const int st = tc_prepare(attn_tc_query_kernel<T, DP, BIAS, MODE, ONE>, bytes, "attn_tc_query_kernel");
     if (st != kOk) return st;
     const dim3 grid((unsigned)A.a.q_tile_count, (unsigned)A.a.heads);
-    attn_tc_query_kernel<T, DP, BIAS, MODE, ONE><<<grid, kBwdThreads, bytes, s>>>(A, M, partial);
+    attn_tc_query_kernel<T, DP, BIAS, MODE, ONE><<<grid, Shape::kThreads, bytes, s>>>(A, M, partial);
     return check_launch("attn_tc_query_kernel");
 }
 template <typename T, int DP, int BIAS, bool ONE = false>
@@ -773,7 +785,7 @@ int run_kv(const AttnArgs& A, const TcMaps& M, float* partial, cudaStream_t s) {
     if (st != kOk) return st;
     const int shares = sink_shares(A);
     dim3 grid((unsigned)A.a.k_tile_count, (unsigned)A.a.kv_heads, (unsigned)shares);
-    attn_tc_grad_kv_kernel<T, DP, BIAS, ONE><<<grid, kBwdThreads, bytes, s>>>(A, M, shares, partial);
+    attn_tc_grad_kv_kernel<T, DP, BIAS, ONE><<<grid, GradKvShape<DP>::kThreads, bytes, s>>>(A, M, shares, partial);
     st = check_launch("attn_tc_grad_kv_kernel");
     if (st != kOk || shares == 1) return st;
     grid.z = kAttnTile / 8;

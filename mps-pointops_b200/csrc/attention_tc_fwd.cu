@@ -53,7 +53,7 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
     uint32_t* slot = reinterpret_cast<uint32_t*>(smem + Shape::kSlot);
 
     const KeySpan span = key_span(A, t.first, t.first + t.rows - 1, t.lk, kTcCols);
-    const int tiles = span.count();
+    const int tiles = (int)uniform((uint32_t)span.count());
 
     if (tid >= kTcRows) {  // the warp that feeds the tensor core
         tmem_alloc(smem_u32(slot), Shape::kCols);
@@ -79,42 +79,35 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
             patience.wait(sb + Shape::kFullK + 8 * (i & 1), (i >> 1) & 1);
             mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kQ, sb + Shape::kK + (i & 1) * Shape::kStage);
         };
-        if ((tid & 31) == 0) {
+        if ((tid & 31) == 0)
             for (int i = 0; i < 5; ++i) mbar_init(sb + Shape::kBar + 8 * i);
-            load_keys(0);
-            load_values(0);
-            load_keys(1);
-        }
         __syncwarp();
+        load_keys(0);
+        load_values(0);
+        load_keys(1);
         tc_fence_before();
         __syncthreads();
         tc_fence_after();
-        tmem = *slot;
-        if ((tid & 31) == 0) {
-            scores(0);
-            mma_commit(sb + Shape::kBar);
-            patience.wait(sb + Shape::kBar, 0);  // S of tile 0: the first keys' stage is free
-            load_keys(2);
-            load_values(1);
-        }
-        __syncwarp();
+        tmem = uniform(*slot);
+        scores(0);
+        mma_commit(sb + Shape::kBar);
+        patience.wait(sb + Shape::kBar, 0);  // S of tile 0: the first keys' stage is free
+        load_keys(2);
+        load_values(1);
         for (int i = 0; i < tiles; ++i) {
             __syncthreads();  // the weights of tile i are in TMEM
-            if ((tid & 31) == 0) {
-                tc_fence_after();
-                patience.wait(sb + Shape::kFullV + 8 * (i & 1), (i >> 1) & 1);
-                mma_weighted<T, DP, kTcCols>(tmem + Shape::kO, tmem + Shape::kS,
-                                             sb + Shape::kV + (i & 1) * Shape::kStage, i > 0);
-                // Issued after P V and executed in order after it: S may overwrite the weights.
-                scores(i + 1);
-                mma_commit(sb + Shape::kBar);
-                // S of tile i + 1 and P V of tile i are done: their operands' stages are free.
-                // Copies get until the end of the next step.
-                patience.wait(sb + Shape::kBar, (i + 1) & 1);
-                load_keys(i + 3);
-                load_values(i + 2);
-            }
-            __syncwarp();
+            tc_fence_after();
+            patience.wait(sb + Shape::kFullV + 8 * (i & 1), (i >> 1) & 1);
+            mma_weighted<T, DP, kTcCols>(tmem + Shape::kO, tmem + Shape::kS,
+                                         sb + Shape::kV + (i & 1) * Shape::kStage, i > 0);
+            // Issued after P V and executed in order after it: S may overwrite the weights.
+            scores(i + 1);
+            mma_commit(sb + Shape::kBar);
+            // S of tile i + 1 and P V of tile i are done: their operands' stages are free.
+            // Copies get until the end of the next step.
+            patience.wait(sb + Shape::kBar, (i + 1) & 1);
+            load_keys(i + 3);
+            load_values(i + 2);
         }
         tc_fence_before();
         __syncthreads();  // the rows have been read
