@@ -204,7 +204,6 @@ __device__ __forceinline__ float table_entry(const mpo_attention& a, int e, int 
 // ---------------------------------------------------------------- launchers
 // attention_tc_fwd.cu, attention_tc_bwd.cu: 16-bit types on the tensor cores.
 int attn_tc_forward(const AttnArgs& A, cudaStream_t s);
-size_t attn_tc_backward_bytes(const AttnArgs& A);
 int attn_tc_backward(const AttnArgs& A, cudaStream_t s);
 // attention_rows.cu: few query rows per cloud.
 bool attn_rows_eligible(const AttnArgs& A);

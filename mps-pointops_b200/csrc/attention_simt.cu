@@ -9,7 +9,7 @@
 // time: the FP32 pipes bound it.
 #include <string>
 
-#include "attention_exact.cuh"
+#include "attention_sinks.cuh"
 
 namespace mpo {
 namespace {
@@ -361,18 +361,24 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_q_kernel(const __grid
         product_nn<DP>(dq, S.w, S.rows[2]);
         if (partial) {
             __syncthreads();
-            if (threadIdx.x < 64) {
-                // One row per thread, columns in a rotated order (spreads the banks); cell
-                // (entry, thread) belongs to this thread alone.
-                const int r = threadIdx.x;
-                for (int c = 0; c < kTR; ++c) {
-                    const int col = (c + r) & 63;
-                    const float v = S.w[r * kPS + col];
-                    for (int a = 0; a < A.a.axes; ++a) {
-                        const int b = bias_bucket(S.cpos[a * kTR + col], S.rpos[a * kTR + r],
-                                                  A.a.reach, A.a.map ? S.map : nullptr);
-                        S.hist[(a * A.a.buckets + b) * 64 + r] += v;
-                    }
+            // A row per thread and half block, columns in a rotated order (spreads the banks);
+            // even axes by the first 64 threads, odd ones by the others, so cell (entry, row)
+            // belongs to one thread.  Two columns at a time: where both meet in one cell the
+            // second sum carries the first, and is written last.
+            const int r = threadIdx.x & 63;
+            for (int a = threadIdx.x >> 6; a < A.a.axes; a += 2) {
+                float* cells = S.hist + (size_t)a * A.a.buckets * 64 + r;
+                const int rp = S.rpos[a * kTR + r];
+                const uint8_t* map = A.a.map ? S.map : nullptr;
+#pragma unroll 4
+                for (int c = 0; c < kTR; c += 2) {
+                    const int c0 = (c + r) & 63, c1 = (c + 1 + r) & 63;
+                    const int x = bias_bucket(S.cpos[a * kTR + c0], rp, A.a.reach, map) * 64;
+                    const int y = bias_bucket(S.cpos[a * kTR + c1], rp, A.a.reach, map) * 64;
+                    const float u = cells[x] + S.w[r * kPS + c0];
+                    const float v = (x == y ? u : cells[y]) + S.w[r * kPS + c1];
+                    cells[x] = u;
+                    cells[y] = v;
                 }
             }
         }
@@ -410,13 +416,16 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_q_kernel(const __grid
 
 // ---------------------------------------------------------------- backward: keys and values
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __grid_constant__ AttnArgs A) {
+__global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __restrict__ partial) {
     extern __shared__ __align__(16) unsigned char smem[];
     const SimtSmem S(smem, DP, 4);
     constexpr int W = DP / 16;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, hk = blockIdx.y;
     Half H;  // p0: index of the first key
     if (!H.load(A.a.k_tiles)) return;
+    // The planned tile decides: both of its halves are shared out or neither is.
+    const bool shared = shares > 1 && H.t.first < A.a.sinks;
+    if (!shared && blockIdx.z > 0) return;
     const int64_t o_row = (int64_t)A.a.heads * A.a.dim;
     load_rows<T, DP>(S.rows[0], A.a.k, H.row, H.rows, hk, A.a.k_row, A.a.k_head, A.a.dim);
     load_rows<T, DP>(S.rows[1], A.a.v, H.row, H.rows, hk, A.a.v_row, A.a.v_head, A.a.dim);
@@ -428,6 +437,11 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __gri
         for (int e = 0; e < W; ++e) dk[i][e] = dv[i][e] = 0.f;
     int lo, hi;
     query_span(A, H.p0, H.p0 + H.rows - 1, H.t.lq, H.t.lk, lo, hi);
+    if (shared) {
+        const int n = max(0, hi - lo), base = lo;
+        lo = base + (int)((int64_t)n * blockIdx.z / shares);
+        hi = base + (int)((int64_t)n * (blockIdx.z + 1) / shares);
+    }
     for (int h = hk * A.group; h < (hk + 1) * A.group; ++h) {
         __syncthreads();
         if (A.a.table) load_bias(A, S, h);
@@ -478,10 +492,16 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __gri
         bool nan = false;
         if (r < H.rows) {
             const int64_t at = ((H.row + r) * A.a.kv_heads + hk) * A.a.dim + tx * W;
+            float* sums =
+                shared ? sink_sums(A, partial, H.t.cloud, H.p0 + r, hk, shares, blockIdx.z) + tx * W : nullptr;
 #pragma unroll
             for (int e = 0; e < W; ++e) {
                 nan |= isnan(dk[i][e]) | isnan(dv[i][e]);
-                if (tx * W + e < A.a.dim) {
+                if (tx * W + e >= A.a.dim) continue;
+                if (sums) {
+                    sums[e] = dk[i][e] * A.a.scale;
+                    sums[(int64_t)kAttnTile * A.a.dim + e] = dv[i][e];
+                } else {
                     static_cast<T*>(A.a.grad_k)[at + e] = Elem<T>::from(dk[i][e] * A.a.scale);
                     static_cast<T*>(A.a.grad_v)[at + e] = Elem<T>::from(dv[i][e]);
                 }
@@ -492,7 +512,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __gri
         if (b >> 16) bad |= 1u << (8 + i);
     }
     __syncwarp();
-    for (; bad; bad &= bad - 1) {
+    for (; bad && !shared; bad &= bad - 1) {
         const int r = (threadIdx.x >> 5) * 16 + __ffs(bad) - 1;
         exact_grad_kv_row<T>(A, (int64_t)H.t.base, H.p0 + r, H.t.other, H.t.lq, H.t.lk, hk);
     }
@@ -518,7 +538,10 @@ int run_fwd(const AttnArgs& A, cudaStream_t s) {
 template <typename T, int DP>
 int run_bwd(const AttnArgs& A, cudaStream_t s) {
     const int entries = A.a.axes * A.a.buckets;
-    float* partial = A.a.grad_table ? static_cast<float*>(A.a.workspace) : nullptr;
+    float* sums = static_cast<float*>(A.a.workspace);
+    float* partial = A.a.grad_table ? reinterpret_cast<float*>(
+                                          static_cast<unsigned char*>(A.a.workspace) + sink_bytes(A))
+                                    : nullptr;
     const size_t qb = SimtSmem::bytes(DP, 4, partial ? entries : 0);
     const size_t kb = SimtSmem::bytes(DP, 4, 0);
     int st = prepare(attn_simt_grad_q_kernel<T, DP>, qb, "attn_simt_grad_q_kernel");
@@ -531,9 +554,11 @@ int run_bwd(const AttnArgs& A, cudaStream_t s) {
         if (st != kOk) return st;
     }
     if (A.a.k_tile_count) {
-        const dim3 grid((unsigned)(2 * A.a.k_tile_count), (unsigned)A.a.kv_heads);
-        attn_simt_grad_kv_kernel<T, DP><<<grid, kThreads, kb, s>>>(A);
+        const int shares = sink_shares(A);
+        const dim3 grid((unsigned)(2 * A.a.k_tile_count), (unsigned)A.a.kv_heads, (unsigned)shares);
+        attn_simt_grad_kv_kernel<T, DP><<<grid, kThreads, kb, s>>>(A, shares, sums);
         st = check_launch("attn_simt_grad_kv_kernel");
+        if (st == kOk && shares > 1) st = join_sinks<T>(A, shares, sums, s);
     }
     return st;
 }

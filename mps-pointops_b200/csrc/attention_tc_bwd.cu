@@ -14,7 +14,7 @@
 // the same columns, and these are the left operands of the accumulating products.
 #include <string>
 
-#include "attention_exact.cuh"
+#include "attention_sinks.cuh"
 #include "attention_tc.cuh"
 
 namespace mpo {
@@ -335,11 +335,17 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
                 }
                 tmem_wait_ld();
                 tmem_use(ds);
+                // Two columns at a time, for half the round trips: where both meet in one cell the
+                // second sum carries the first, and is written last.
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float v;
-                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at_cell[e]) : "memory");
-                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(at_cell[e]), "f"(v + ds[e]) : "memory");
+                for (int e = 0; e < 16; e += 2) {
+                    float u, v;
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(u) : "r"(at_cell[e]) : "memory");
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at_cell[e + 1]) : "memory");
+                    u += ds[e];
+                    v = (at_cell[e] == at_cell[e + 1] ? u : v) + ds[e + 1];
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(at_cell[e]), "f"(u) : "memory");
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(at_cell[e + 1]), "f"(v) : "memory");
                 }
             }
             tc_fence_before();
@@ -438,10 +444,7 @@ struct GradKvShape {
     }
 };
 
-// Key tiles that hold sinks are seen by every later query of their cloud.
-// `shares` blocks divide those queries; each leaves its sums in `partial`
-// ([cloud * sink tiles + tile][key head][share][dk, dv][128][dim], float32) for
-// the join kernel.  shares == 1: no block does.
+// Key tiles that hold sinks are shared out: attention_sinks.cuh.
 template <typename T, int DP, int BIAS, bool ONE>
 __global__ void __launch_bounds__((GradKvShape<DP>::kThreads), (GradKvShape<DP>::kBlocks))
 attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TcMaps M, int shares,
@@ -666,12 +669,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
     if (kBuffers == 2) done.wait(tiles + 1);
     bool nan = BIAS && live && bias.far;
     const int64_t at = (((int64_t)t.row + r) * A.a.kv_heads + hk) * A.a.dim;
-    const int sink_tiles = (A.a.sinks + kAttnTile - 1) / kAttnTile;
-    float* sums = nullptr;
-    if (shared) {
-        const int64_t tile = (int64_t)t.cloud * sink_tiles + t.first / kAttnTile;
-        sums = partial + (((tile * A.a.kv_heads + hk) * shares + blockIdx.z) * 2 * kAttnTile + r) * A.a.dim;
-    }
+    float* sums = shared ? sink_sums(A, partial, t.cloud, j, hk, shares, blockIdx.z) : nullptr;
 #pragma unroll
     for (int which = 0; which < 2; ++which)
 #pragma unroll
@@ -717,49 +715,6 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
     __syncthreads();
 }
 
-// grad_k and grad_v of the key tiles with sinks: the shares' sums in order.  A
-// warp per key row.
-template <typename T>
-__global__ void __launch_bounds__(256)
-attn_tc_join_kv_kernel(const __grid_constant__ AttnArgs A, int shares, const float* __restrict__ partial) {
-    const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.k_tiles)[blockIdx.x];
-    if (t.first >= A.a.sinks) return;
-    const int r = blockIdx.z * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, hk = blockIdx.y;
-    if (r >= t.rows) return;
-    const int sink_tiles = (A.a.sinks + kAttnTile - 1) / kAttnTile;
-    const int64_t tile = (int64_t)t.cloud * sink_tiles + t.first / kAttnTile;
-    const float* src = partial + (((tile * A.a.kv_heads + hk) * shares) * 2 * kAttnTile + r) * A.a.dim;
-    const int64_t at = (((int64_t)t.row + r) * A.a.kv_heads + hk) * A.a.dim, half = (int64_t)kAttnTile * A.a.dim;
-    bool nan = false;
-    for (int d = lane; d < A.a.dim; d += 32) {
-        float dk = 0.f, dv = 0.f;
-        for (int z = 0; z < shares; ++z) {
-            dk += src[z * 2 * half + d];
-            dv += src[(z * 2 + 1) * half + d];
-        }
-        nan |= isnan(dk) | isnan(dv);
-        static_cast<T*>(A.a.grad_k)[at + d] = Elem<T>::from(dk);
-        static_cast<T*>(A.a.grad_v)[at + d] = Elem<T>::from(dv);
-    }
-    if (__any_sync(FULL_MASK, nan))
-        exact_grad_kv_row<T>(A, t.base, t.first + r, t.other, t.lq, t.lk, hk);
-}
-
-// Blocks that share a key tile with sinks: each about as many queries as see
-// any other key tile, but no more blocks than fill the GPU (eight per SM).
-int sink_shares(const AttnArgs& A) {
-    if (A.a.sinks == 0) return 1;
-    const int64_t window = (int64_t)A.left + A.right + kAttnTile;
-    const int64_t tiles = (int64_t)A.a.clouds * ceil_div(A.a.sinks, kAttnTile) * A.a.kv_heads;
-    return (int)max64(1, min64(A.a.max_rows / window, ceil_div(8 * sm_count(), max64(tiles, 1))));
-}
-size_t sink_bytes(const AttnArgs& A) {
-    const int shares = sink_shares(A);
-    if (shares == 1) return 0;
-    const int64_t tiles = (int64_t)A.a.clouds * ceil_div(A.a.sinks, kAttnTile);
-    return (size_t)(tiles * A.a.kv_heads * shares * 2 * kAttnTile * A.a.dim) * sizeof(float);
-}
-
 template <typename T, int DP, int BIAS, int MODE, bool ONE = QueryShape<DP, MODE>::kTight>
 int run_q(const AttnArgs& A, const TcMaps& M, float* partial, cudaStream_t s) {
     using Shape = QueryShape<DP, MODE>;
@@ -788,9 +743,7 @@ int run_kv(const AttnArgs& A, const TcMaps& M, float* partial, cudaStream_t s) {
     attn_tc_grad_kv_kernel<T, DP, BIAS, ONE><<<grid, GradKvShape<DP>::kThreads, bytes, s>>>(A, M, shares, partial);
     st = check_launch("attn_tc_grad_kv_kernel");
     if (st != kOk || shares == 1) return st;
-    grid.z = kAttnTile / 8;
-    attn_tc_join_kv_kernel<T><<<grid, 256, 0, s>>>(A, shares, partial);
-    return check_launch("attn_tc_join_kv_kernel");
+    return join_sinks<T>(A, shares, partial, s);
 }
 template <typename T, int DP, int BIAS>
 int run(const AttnArgs& A, cudaStream_t s) {
@@ -829,7 +782,6 @@ int by_dim(const AttnArgs& A, cudaStream_t s) {
 
 }  // namespace
 
-size_t attn_tc_backward_bytes(const AttnArgs& A) { return sink_bytes(A); }
 int attn_tc_backward(const AttnArgs& A, cudaStream_t s) {
     return A.a.dtype == MPO_F16 ? by_dim<__half>(A, s) : by_dim<__nv_bfloat16>(A, s);
 }

@@ -85,13 +85,6 @@ struct Raw {  // eight elements as loaded
     typename Four<T>::V lo, hi;
 };
 template <typename T>
-__device__ __forceinline__ Raw<T> load_raw(const T* p, const Lane& L) {
-    Raw<T> r;
-    r.lo = *reinterpret_cast<const typename Four<T>::V*>(p + L.lo);
-    r.hi = *reinterpret_cast<const typename Four<T>::V*>(p + L.hi);
-    return r;
-}
-template <typename T>
 __device__ __forceinline__ Eight unpack(const Raw<T>& r, bool interleaved) {
     float x[8];
     Four<T>::get(r.lo, x);
@@ -109,7 +102,7 @@ __device__ __forceinline__ Eight unpack(const Raw<T>& r, bool interleaved) {
     return e;
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const Lane& L, const Eight& e, bool interleaved) {
+__device__ __forceinline__ void store8(T* p, int apart, const Eight& e, bool interleaved) {
     float x[8];
     if (interleaved) {
         unpack2(e.v[0], x[0], x[2]);
@@ -120,8 +113,8 @@ __device__ __forceinline__ void store8(T* p, const Lane& L, const Eight& e, bool
 #pragma unroll
         for (int i = 0; i < 4; ++i) unpack2(e.v[i], x[2 * i], x[2 * i + 1]);
     }
-    *reinterpret_cast<typename Four<T>::V*>(p + L.lo) = Four<T>::put(x);
-    *reinterpret_cast<typename Four<T>::V*>(p + L.hi) = Four<T>::put(x + 4);
+    *reinterpret_cast<typename Four<T>::V*>(p) = Four<T>::put(x);
+    *reinterpret_cast<typename Four<T>::V*>(p + apart) = Four<T>::put(x + 4);
 }
 // Weights of q and k in shared memory, by chunk in the order of an Eight (ones
 // where none is given).
@@ -163,19 +156,17 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
     for (int o = lanes >> 1; o; o >>= 1) v += __shfl_xor_sync(FULL_MASK, v, o);
     return v;
 }
-__device__ __forceinline__ f32x2 neg2(f32x2 a) { return a ^ 0x8000000080000000ull; }
-
-// Cosines and sines of the lane's four pairs.
+// Cosines and sines of the lane's four pairs, and the sines negated.
 struct Turn {
-    f32x2 c[2], s[2];
-    // (u, v) -> (u c - v s, u s + v c); back: by -theta.
-    __device__ __forceinline__ void apply(Eight& e, bool back) const {
+    f32x2 c[2], s[2], n[2];
+    // (u, v) -> (u c - v s, u s + v c); BACK: by -theta.
+    template <bool BACK>
+    __device__ __forceinline__ void apply(Eight& e) const {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const f32x2 sn = back ? neg2(s[i]) : s[i];
             const f32x2 u = e.v[i], v = e.v[2 + i];
-            e.v[i] = fma2(u, c[i], neg2(mul2(v, sn)));
-            e.v[2 + i] = fma2(u, sn, mul2(v, c[i]));
+            e.v[i] = fma2(u, c[i], mul2(v, BACK ? s[i] : n[i]));
+            e.v[2 + i] = fma2(u, BACK ? n[i] : s[i], mul2(v, c[i]));
         }
     }
 };
@@ -211,24 +202,62 @@ __device__ __forceinline__ Turn read_turn(const float* cs, int chunk) {
     t.c[1] = pack2(c.z, c.w);
     t.s[0] = pack2(s.x, s.y);
     t.s[1] = pack2(s.z, s.w);
+    t.n[0] = pack2(-s.x, -s.y);
+    t.n[1] = pack2(-s.z, -s.w);
     return t;
 }
 
-// Units of work: (row, share of the row's q and k heads); a warp takes units
-// in grid strides.  A round serves 32 / lanes heads; U rounds of loads are in
-// flight, as loaded (packed), and the first of them go out before the row's
-// angles are formed.
-template <typename T, int U>
+// Units of work: (row, share of the row's rounds); a warp takes units in grid
+// strides.  A round serves 32 / lanes heads of q or of k; q's rounds come first.
+// U rounds of loads are in flight, as loaded (packed), and the first of them go
+// out before the row's angles are formed.
+struct Rounds {
+    int step, q, total;  // heads of a round; q's rounds; all rounds
+    __device__ __forceinline__ Rounds(const mpo_rotate& a, int lanes) {
+        step = 32 / lanes;
+        q = (a.heads + step - 1) / step;
+        total = q + (a.kv_heads + step - 1) / step;
+    }
+    // Does this lane have a head in round r?
+    __device__ __forceinline__ bool has(const mpo_rotate& a, int r, int sub) const {
+        return r < q ? r * step + sub < a.heads : (r - q) * step + sub < a.kv_heads;
+    }
+};
+// Walks a lane's head through the rounds: one addition per round.
+template <typename T>
+struct Walk {
+    T* at;
+    T* k0;             // the lane's head in k's first round
+    int64_t dq, dk;    // strides of a round
+    __device__ __forceinline__ Walk(T* q, T* k, int64_t q_head, int64_t k_head, const Rounds& R, int sub, int lo,
+                                    int r) {
+        dq = q_head * R.step;
+        dk = k_head * R.step;
+        k0 = k + sub * k_head + lo;
+        at = r < R.q ? q + sub * q_head + lo + r * dq : k0 + (r - R.q) * dk;
+    }
+    // From round r to r + 1.
+    __device__ __forceinline__ void next(const Rounds& R, int r) { at = r + 1 == R.q ? k0 : at + (r < R.q ? dq : dk); }
+};
+template <typename T>
+__device__ __forceinline__ Raw<T> load_at(const T* p, int apart) {
+    Raw<T> r;
+    r.lo = *reinterpret_cast<const typename Four<T>::V*>(p);
+    r.hi = *reinterpret_cast<const typename Four<T>::V*>(p + apart);
+    return r;
+}
+
+template <typename T, int U, bool IL>
 __global__ void __launch_bounds__(kRotThreads, kFwdBlocksPerSm)
-norm_rotate_kernel(const mpo_rotate a, int lanes, int shares) {
+norm_rotate_kernel(const __grid_constant__ mpo_rotate a, int lanes, int shares) {
     __shared__ __align__(16) float angles[kRotWarps][2 * kMaxPairs];
     __shared__ __align__(16) float weights[2][32][8];
     float* cs = angles[threadIdx.x >> 5];
     const int lane = threadIdx.x & 31, chunk = lane & (lanes - 1), sub = lane / lanes;
-    const int step = 32 / lanes, total = a.heads + a.kv_heads;
-    const int rounds = (total + step - 1) / step;
+    const Rounds R(a, lanes);
     const Lane L(a, chunk);
-    const bool il = a.interleaved && L.turns;
+    const bool il = IL && L.turns;
+    const int apart = L.hi - L.lo;
     stage_weights(a, weights, lanes);
     __syncthreads();
     const float inv = 1.f / (float)a.dim;
@@ -236,25 +265,25 @@ norm_rotate_kernel(const mpo_rotate a, int lanes, int shares) {
     for (int64_t u = (int64_t)blockIdx.x * kRotWarps + (threadIdx.x >> 5); u < units;
          u += (int64_t)gridDim.x * kRotWarps) {
         const int64_t row = shares == 1 ? u : u / shares;
-        int r0 = 0, r1 = rounds;
+        int r0 = 0, r1 = R.total;
         if (shares > 1) {
             const int share = (int)(u - row * shares);
-            r0 = rounds * share / shares;
-            r1 = rounds * (share + 1) / shares;
+            r0 = R.total * share / shares;
+            r1 = R.total * (share + 1) / shares;
         }
-        const T* q = static_cast<const T*>(a.q) + row * a.q_row;
-        const T* k = static_cast<const T*>(a.k) + row * a.k_row;
-        T* oq = static_cast<T*>(a.out_q) + row * a.heads * a.dim;
-        T* ok = static_cast<T*>(a.out_k) + row * a.kv_heads * a.dim;
+        Walk<const T> in(static_cast<const T*>(a.q) + row * a.q_row, static_cast<const T*>(a.k) + row * a.k_row,
+                         a.q_head, a.k_head, R, sub, L.lo, r0);
+        Walk<T> out(static_cast<T*>(a.out_q) + row * a.heads * a.dim,
+                    static_cast<T*>(a.out_k) + row * a.kv_heads * a.dim, a.dim, a.dim, R, sub, L.lo, r0);
         Raw<T> raw[U] = {};
-        auto fetch = [&](int r) {
-            const int h = r * step + sub;
-            if (L.live && r < r1 && h < total)
-                return load_raw<T>(h < a.heads ? q + h * a.q_head : k + (h - a.heads) * a.k_head, L);
-            return Raw<T>{};
+        auto fetch = [&](int r, Raw<T>& x) {
+            x = Raw<T>{};
+            if (r >= r1) return;
+            if (L.live && R.has(a, r, sub)) x = load_at<T>(in.at, apart);
+            in.next(R, r);
         };
 #pragma unroll
-        for (int i = 0; i < U; ++i) raw[i] = fetch(r0 + i);
+        for (int i = 0; i < U; ++i) fetch(r0 + i, raw[i]);
         Turn turn;
         if (a.pairs) {
             row_angles(a, row, cs);
@@ -264,19 +293,17 @@ norm_rotate_kernel(const mpo_rotate a, int lanes, int shares) {
 #pragma unroll
             for (int i = 0; i < U; ++i) {
                 if (r + i < r1) {  // uniform over the warp
-                    const int h = (r + i) * step + sub;
-                    const bool is_q = h < a.heads;
                     Eight x = unpack<T>(raw[i], il);
-                    raw[i] = fetch(r + i + U);
+                    fetch(r + i + U, raw[i]);
                     const float ss = lanes_sum(dot8(x, x), lanes);
                     const float rs = rsqrtf(fmaf(ss, inv, a.eps));
                     const f32x2 rs2 = pack2(rs, rs);
-                    const Eight w = read_weight(weights[is_q ? 0 : 1][chunk]);
+                    const Eight w = read_weight(weights[r + i < R.q ? 0 : 1][chunk]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x.v[e] = mul2(mul2(x.v[e], rs2), w.v[e]);
-                    if (L.turns) turn.apply(x, false);
-                    if (L.live && h < total)
-                        store8<T>(is_q ? oq + h * a.dim : ok + (h - a.heads) * a.dim, L, x, il);
+                    if (L.turns) turn.apply<false>(x);
+                    if (L.live && R.has(a, r + i, sub)) store8<T>(out.at, apart, x, il);
+                    out.next(R, r + i);
                 }
             }
         }
@@ -286,9 +313,9 @@ norm_rotate_kernel(const mpo_rotate a, int lanes, int shares) {
 // Backward.  A lane keeps the weight gradients of its eight elements over all
 // of its units; the block's warps and head slots join in shared memory in a
 // fixed order and each block writes one partial (2, dim) row.
-template <typename T, int U>
+template <typename T, int U, bool IL>
 __global__ void __launch_bounds__(kRotThreads, kBwdBlocksPerSm)
-norm_rotate_bwd_kernel(const mpo_rotate a, int lanes, int shares, float* __restrict__ partial) {
+norm_rotate_bwd_kernel(const __grid_constant__ mpo_rotate a, int lanes, int shares, float* __restrict__ partial) {
     __shared__ __align__(16) union {
         float angles[kRotWarps][2 * kMaxPairs];
         float sums[kRotWarps][32][17];
@@ -296,10 +323,10 @@ norm_rotate_bwd_kernel(const mpo_rotate a, int lanes, int shares, float* __restr
     __shared__ __align__(16) float weights[2][32][8];
     float* cs = sh.angles[threadIdx.x >> 5];
     const int lane = threadIdx.x & 31, chunk = lane & (lanes - 1), sub = lane / lanes;
-    const int step = 32 / lanes, total = a.heads + a.kv_heads;
-    const int rounds = (total + step - 1) / step;
+    const Rounds R(a, lanes);
     const Lane L(a, chunk);
-    const bool il = a.interleaved && L.turns;
+    const bool il = IL && L.turns;
+    const int apart = L.hi - L.lo;
     stage_weights(a, weights, lanes);
     __syncthreads();
     Eight gq, gk;
@@ -310,28 +337,29 @@ norm_rotate_bwd_kernel(const mpo_rotate a, int lanes, int shares, float* __restr
     for (int64_t u = (int64_t)blockIdx.x * kRotWarps + (threadIdx.x >> 5); u < units;
          u += (int64_t)gridDim.x * kRotWarps) {
         const int64_t row = shares == 1 ? u : u / shares;
-        int r0 = 0, r1 = rounds;
+        int r0 = 0, r1 = R.total;
         if (shares > 1) {
             const int share = (int)(u - row * shares);
-            r0 = rounds * share / shares;
-            r1 = rounds * (share + 1) / shares;
+            r0 = R.total * share / shares;
+            r1 = R.total * (share + 1) / shares;
         }
-        const T* q = static_cast<const T*>(a.q) + row * a.q_row;
-        const T* k = static_cast<const T*>(a.k) + row * a.k_row;
+        Walk<const T> in(static_cast<const T*>(a.q) + row * a.q_row, static_cast<const T*>(a.k) + row * a.k_row,
+                         a.q_head, a.k_head, R, sub, L.lo, r0);
         const int64_t dq = row * a.heads * a.dim, dk = row * a.kv_heads * a.dim;
-        const T* gyq = static_cast<const T*>(a.grad_q) + dq;
-        const T* gyk = static_cast<const T*>(a.grad_k) + dk;
+        Walk<const T> gin(static_cast<const T*>(a.grad_q) + dq, static_cast<const T*>(a.grad_k) + dk, a.dim, a.dim, R,
+                          sub, L.lo, r0);
+        Walk<T> out(static_cast<T*>(a.out_q) + dq, static_cast<T*>(a.out_k) + dk, a.dim, a.dim, R, sub, L.lo, r0);
         Raw<T> rx[U] = {}, rg[U] = {};
         auto fetch = [&](int r, Raw<T>& x, Raw<T>& g) {
-            const int h = r * step + sub;
             x = Raw<T>{};
             g = Raw<T>{};
-            if (L.live && r < r1 && h < total) {
-                const bool is_q = h < a.heads;
-                const int hk = h - a.heads;
-                x = load_raw<T>(is_q ? q + h * a.q_head : k + hk * a.k_head, L);
-                g = load_raw<T>(is_q ? gyq + h * a.dim : gyk + hk * a.dim, L);
+            if (r >= r1) return;
+            if (L.live && R.has(a, r, sub)) {
+                x = load_at<T>(in.at, apart);
+                g = load_at<T>(gin.at, apart);
             }
+            in.next(R, r);
+            gin.next(R, r);
         };
 #pragma unroll
         for (int i = 0; i < U; ++i) fetch(r0 + i, rx[i], rg[i]);
@@ -344,11 +372,10 @@ norm_rotate_bwd_kernel(const mpo_rotate a, int lanes, int shares, float* __restr
 #pragma unroll
             for (int i = 0; i < U; ++i) {
                 if (r + i < r1) {
-                    const int h = (r + i) * step + sub;
-                    const bool is_q = h < a.heads;
+                    const bool is_q = r + i < R.q;  // uniform over the warp
                     Eight y = unpack<T>(rx[i], il), b = unpack<T>(rg[i], il), hw;
                     fetch(r + i + U, rx[i], rg[i]);
-                    if (L.turns) turn.apply(b, true);
+                    if (L.turns) turn.apply<true>(b);
                     const Eight w = read_weight(weights[is_q ? 0 : 1][chunk]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) hw.v[e] = mul2(b.v[e], w.v[e]);
@@ -357,20 +384,18 @@ norm_rotate_bwd_kernel(const mpo_rotate a, int lanes, int shares, float* __restr
                     const float rs = rsqrtf(fmaf(ss, inv, a.eps));
                     const float back = -(hx * inv * rs * rs * rs);
                     const f32x2 rs2 = pack2(rs, rs), back2 = pack2(back, back);
-                    if (h < total) {
+                    // A lane without a head holds zeros: it adds nothing.
+                    if (is_q) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const f32x2 xr = mul2(y.v[e], rs2);
-                            if (is_q) gq.v[e] = fma2(b.v[e], xr, gq.v[e]);
-                            else gk.v[e] = fma2(b.v[e], xr, gk.v[e]);
-                        }
+                        for (int e = 0; e < 4; ++e) gq.v[e] = fma2(b.v[e], mul2(y.v[e], rs2), gq.v[e]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) gk.v[e] = fma2(b.v[e], mul2(y.v[e], rs2), gk.v[e]);
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) y.v[e] = fma2(y.v[e], back2, mul2(rs2, hw.v[e]));
-                    if (L.live && h < total)
-                        store8<T>(is_q ? static_cast<T*>(a.out_q) + dq + h * a.dim
-                                       : static_cast<T*>(a.out_k) + dk + (h - a.heads) * a.dim,
-                                  L, y, il);
+                    if (L.live && R.has(a, r + i, sub)) store8<T>(out.at, apart, y, il);
+                    out.next(R, r + i);
                 }
             }
         }
@@ -399,7 +424,7 @@ norm_rotate_bwd_kernel(const mpo_rotate a, int lanes, int shares, float* __restr
         if (c * 8 >= a.dim) continue;
         float v = 0.f;
         for (int w = 0; w < kRotWarps; ++w)
-            for (int sl = 0; sl < step; ++sl) v += sh.sums[w][sl * lanes + c][e];
+            for (int sl = 0; sl < R.step; ++sl) v += sh.sums[w][sl * lanes + c][e];
         const Lane at(a, c);
         const int el = (e & 7) < 4 ? at.lo + (e & 3) : at.hi + (e & 3);
         partial[((int64_t)blockIdx.x * 2 + (e >> 3)) * a.dim + el] = v;
@@ -441,7 +466,7 @@ struct RotateGrid {
 RotateGrid rotate_grid(const mpo_rotate& a, int per_sm) {
     RotateGrid g;
     g.lanes = rotate_lanes(a.dim);
-    const int64_t rounds = ceil_div(a.heads + a.kv_heads, 32 / g.lanes);
+    const int64_t rounds = ceil_div(a.heads, 32 / g.lanes) + ceil_div(a.kv_heads, 32 / g.lanes);
     const int64_t warps = (int64_t)sm_count() * per_sm * kRotWarps;
     g.shares = (int)max64(1, min64(rounds, warps / (2 * max64(a.rows, 1))));
     g.blocks = (unsigned)max64(1, min64(ceil_div(a.rows * g.shares, kRotWarps),
@@ -485,7 +510,10 @@ template <typename T>
 int run_rotate(const mpo_rotate& a, cudaStream_t s) {
     constexpr int kDepth = sizeof(T) == 2 ? 4 : 2;
     const RotateGrid g = rotate_grid(a, kFwdBlocksPerSm);
-    norm_rotate_kernel<T, kDepth><<<g.blocks, kRotThreads, 0, s>>>(a, g.lanes, g.shares);
+    if (a.interleaved)
+        norm_rotate_kernel<T, kDepth, true><<<g.blocks, kRotThreads, 0, s>>>(a, g.lanes, g.shares);
+    else
+        norm_rotate_kernel<T, kDepth, false><<<g.blocks, kRotThreads, 0, s>>>(a, g.lanes, g.shares);
     return check_launch("norm_rotate_kernel");
 }
 template <typename T>
@@ -494,7 +522,10 @@ int run_rotate_bwd(const mpo_rotate& a, cudaStream_t s) {
     const RotateGrid g = rotate_grid(a, kBwdBlocksPerSm);
     const bool weights = a.grad_q_weight || a.grad_k_weight;
     float* partial = weights ? static_cast<float*>(a.workspace) : nullptr;
-    norm_rotate_bwd_kernel<T, kDepth><<<g.blocks, kRotThreads, 0, s>>>(a, g.lanes, g.shares, partial);
+    if (a.interleaved)
+        norm_rotate_bwd_kernel<T, kDepth, true><<<g.blocks, kRotThreads, 0, s>>>(a, g.lanes, g.shares, partial);
+    else
+        norm_rotate_bwd_kernel<T, kDepth, false><<<g.blocks, kRotThreads, 0, s>>>(a, g.lanes, g.shares, partial);
     int st = check_launch("norm_rotate_bwd_kernel");
     if (st != kOk || !weights) return st;
     norm_weight_reduce_kernel<<<(unsigned)ceil_div(2 * a.dim, 32), 1024, 0, s>>>(
