@@ -155,15 +155,52 @@ attn_rows_kernel(const __grid_constant__ AttnArgs A, int per, int units, int spl
     constexpr int NB = DP / 32;                 // 32-element blocks of a dot product
     constexpr int NV = DP / 64 < 1 ? 1 : DP / 64;  // value blocks of 8 (lane groups) x 8 elements
     constexpr int kPitch = DP + 4;
-    __shared__ float sh[kRowsWarps * 16 * kPitch];
+    // The warps' rows at the end; before that the heads' tables ([entry][head], times log2 e)
+    // and each warp's bias of 16 rows x 16 keys.
+    constexpr int kJoin = kRowsWarps * 16 * kPitch, kBiasWords = kAttnMaxEntries * 16 + kRowsWarps * 256;
+    __shared__ float sh[BIAS && kBiasWords > kJoin ? kBiasWords : kJoin];
     Unit U;
     if (!rows_unit(A, per, units, 16, splits, U)) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int rows = U.rows * U.gc;             // of the 16
+    float* tile = sh + kAttnMaxEntries * 16 + warp * 256;
+    // Bias: lane l forms that of key l % 16 and rows l / 16, l / 16 + 2, ..
+    const int kl = lane & 15;
+    int kp[kAttnMaxAxes] = {0, 0, 0};
+    if (BIAS) {
+        for (int e = threadIdx.x; e < A.a.axes * A.a.buckets * U.gc; e += kRowsThreads)
+            sh[e / U.gc * 16 + e % U.gc] = table_entry(A.a, e / U.gc, U.h0 + e % U.gc) * kLog2e;
+        __syncthreads();
+    }
+    auto load_key_pos = [&](int c) {
+        if (!BIAS || c + kl >= U.c1) return;
+        const int64_t k = (int64_t)U.t.other + U.key(c + kl);
+        for (int a = 0; a < A.a.axes; ++a) kp[a] = A.a.kpos[k * A.a.axes + a];
+    };
+    auto form_bias = [&]() {  // of the keys whose positions are at hand
+        if (!BIAS) return;
+        __syncwarp();
+        int i_old = -1, bucket[kAttnMaxAxes] = {0, 0, 0};
+        for (int r = lane >> 4; r < rows; r += 2) {
+            const int i = r / U.gc, hh = r - i * U.gc;
+            if (i != i_old) {  // the heads of a query row share its buckets
+                i_old = i;
+                const int64_t q = (int64_t)U.t.row + U.row0 + i;
+                for (int a = 0; a < A.a.axes; ++a) {
+                    int b = bias_bucket(kp[a], A.a.qpos[q * A.a.axes + a], A.a.reach, nullptr);
+                    if (A.a.map) b = min(max(__ldg(A.a.map + b), 0), A.a.buckets - 1);
+                    bucket[a] = (a * A.a.buckets + b) * 16;
+                }
+            }
+            float x = 0.f;
+            for (int a = 0; a < A.a.axes; ++a) x += sh[bucket[a] + hh];
+            tile[r * 16 + kl] = x;
+        }
+        __syncwarp();
+    };
     // Queries: rows g and g + 8.
     uint32_t qf[2 * NB][4];
     int pos[2], head[2];
-    int qp[2][3] = {{0, 0, 0}, {0, 0, 0}};
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         const int r = g + 8 * half;
@@ -182,8 +219,6 @@ attn_rows_kernel(const __grid_constant__ AttnArgs A, int per, int units, int spl
             qf[2 * b + 1][half] = u.z;
             qf[2 * b + 1][half + 2] = u.w;
         }
-        if (BIAS)
-            for (int a = 0; a < A.a.axes; ++a) qp[half][a] = A.a.qpos[q * A.a.axes + a];
         if (!on) head[half] = -1;
     }
     float o[8 * NV][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -206,8 +241,13 @@ attn_rows_kernel(const __grid_constant__ AttnArgs A, int per, int units, int spl
         }
     };
     int c = U.c0 + 16 * warp;
-    if (c < U.c1) load_keys(c);
+    if (c < U.c1) {
+        load_keys(c);
+        load_key_pos(c);
+    }
     for (; c < U.c1; c += kStep) {
+        form_bias();
+        load_key_pos(c + kStep);
         // Values of keys 2t, 2t + 1, 2t + 8, 2t + 9.
         uint4 vf[4][NV];
 #pragma unroll
@@ -239,13 +279,7 @@ attn_rows_kernel(const __grid_constant__ AttnArgs A, int per, int units, int spl
                 float x = -INFINITY;
                 if (head[row] >= 0 && cc < U.c1 && attn_visible(A, pos[row], j)) {
                     x = s[half][e] * A.scale_log2;
-                    if (BIAS)
-                        for (int a = 0; a < A.a.axes; ++a) {
-                            int b = bias_bucket(A.a.kpos[((int64_t)U.t.other + j) * A.a.axes + a],
-                                                qp[row][a], A.a.reach, nullptr);
-                            if (A.a.map) b = min(max(__ldg(A.a.map + b), 0), A.a.buckets - 1);
-                            x += table_entry(A.a, a * A.a.buckets + b, head[row]) * kLog2e;
-                        }
+                    if (BIAS) x += tile[(g + 8 * row) * 16 + 8 * half + 2 * t + (e & 1)];
                 }
                 s[half][e] = x;
             }
@@ -294,6 +328,7 @@ attn_rows_kernel(const __grid_constant__ AttnArgs A, int per, int units, int spl
             }
         }
     }
+    if (BIAS) __syncthreads();  // the tables and tiles have been read
     // Column n of product j of block b is element 64 b + 8 n + j.
 #pragma unroll
     for (int row = 0; row < 2; ++row) {

@@ -16,6 +16,7 @@
 // x frequency / pi is summed in double and reduced to one turn there (positions
 // of 10^5 would cost a float sum 2 decimal digits), then sincospif.
 #include <string>
+#include <type_traits>
 
 #include "attention_common.cuh"
 
@@ -152,10 +153,13 @@ __device__ __forceinline__ float dot8(const Eight& a, const Eight& b) {
     const f32x2 q = fma2(a.v[3], b.v[3], mul2(a.v[1], b.v[1]));
     return pair_sum(p, q);
 }
-__device__ __forceinline__ float lanes_sum(float v, int lanes) {
-    for (int o = lanes >> 1; o; o >>= 1) v += __shfl_xor_sync(FULL_MASK, v, o);
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int o = LANES >> 1; o; o >>= 1) v += __shfl_xor_sync(FULL_MASK, v, o);
     return v;
 }
+
 // Cosines and sines of the lane's four pairs, and the sines negated.
 struct Turn {
     f32x2 c[2], s[2], n[2];
@@ -207,127 +211,99 @@ __device__ __forceinline__ Turn read_turn(const float* cs, int chunk) {
     return t;
 }
 
-// Units of work: (row, share of the row's rounds); a warp takes units in grid
-// strides.  A round serves 32 / lanes heads of q or of k; q's rounds come first.
-// U rounds of loads are in flight, as loaded (packed), and the first of them go
-// out before the row's angles are formed.
-struct Rounds {
-    int step, q, total;  // heads of a round; q's rounds; all rounds
-    __device__ __forceinline__ Rounds(const mpo_rotate& a, int lanes) {
-        step = 32 / lanes;
-        q = (a.heads + step - 1) / step;
-        total = q + (a.kv_heads + step - 1) / step;
-    }
-    // Does this lane have a head in round r?
-    __device__ __forceinline__ bool has(const mpo_rotate& a, int r, int sub) const {
-        return r < q ? r * step + sub < a.heads : (r - q) * step + sub < a.kv_heads;
-    }
-};
-// Walks a lane's head through the rounds: one addition per round.
+// Units of work: (row, share of the row's heads); a warp takes units in grid
+// strides.  A round serves 32 / LANES heads of q or of k; U rounds of loads of
+// each are in flight, as loaded (packed), and the first of them go out before
+// the row's angles are formed.  A lane past the last head loads that head again
+// and stores nothing.
 template <typename T>
-struct Walk {
-    T* at;
-    T* k0;             // the lane's head in k's first round
-    int64_t dq, dk;    // strides of a round
-    __device__ __forceinline__ Walk(T* q, T* k, int64_t q_head, int64_t k_head, const Rounds& R, int sub, int lo,
-                                    int r) {
-        dq = q_head * R.step;
-        dk = k_head * R.step;
-        k0 = k + sub * k_head + lo;
-        at = r < R.q ? q + sub * q_head + lo + r * dq : k0 + (r - R.q) * dk;
-    }
-    // From round r to r + 1.
-    __device__ __forceinline__ void next(const Rounds& R, int r) { at = r + 1 == R.q ? k0 : at + (r < R.q ? dq : dk); }
-};
-template <typename T>
-__device__ __forceinline__ Raw<T> load_at(const T* p, int apart) {
+__device__ __forceinline__ Raw<T> load_at(const T* base, int head, int stride, int apart) {
+    const T* p = base + (int64_t)head * stride;
     Raw<T> r;
     r.lo = *reinterpret_cast<const typename Four<T>::V*>(p);
     r.hi = *reinterpret_cast<const typename Four<T>::V*>(p + apart);
     return r;
 }
+// Runs f(this lane's head, ring slot) over the rounds of `heads` heads from `first`.
+template <int U, typename F>
+__device__ __forceinline__ void over_rounds(int sub, int first, int step, int heads, F&& f) {
+    for (int h = first; h < heads; h += U * step) {  // uniform over the warp
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (h + i * step < heads) f(h + i * step + sub, i);
+    }
+}
 
-template <typename T, int U, bool IL>
+template <typename T, int U, bool IL, int LANES>
 __global__ void __launch_bounds__(kRotThreads, kFwdBlocksPerSm)
-norm_rotate_kernel(const __grid_constant__ mpo_rotate a, int lanes, int shares) {
+norm_rotate_kernel(const __grid_constant__ mpo_rotate a, int shares) {
+    constexpr int kHeads = 32 / LANES;
     __shared__ __align__(16) float angles[kRotWarps][2 * kMaxPairs];
     __shared__ __align__(16) float weights[2][32][8];
     float* cs = angles[threadIdx.x >> 5];
-    const int lane = threadIdx.x & 31, chunk = lane & (lanes - 1), sub = lane / lanes;
-    const Rounds R(a, lanes);
+    const int lane = threadIdx.x & 31, chunk = lane % LANES, sub = lane / LANES;
     const Lane L(a, chunk);
     const bool il = IL && L.turns;
-    const int apart = L.hi - L.lo;
-    stage_weights(a, weights, lanes);
+    const int apart = L.hi - L.lo, lo = L.live ? L.lo : 0, step = kHeads * shares;
+    stage_weights(a, weights, LANES);
     __syncthreads();
     const float inv = 1.f / (float)a.dim;
     const int64_t units = a.rows * shares;
     for (int64_t u = (int64_t)blockIdx.x * kRotWarps + (threadIdx.x >> 5); u < units;
          u += (int64_t)gridDim.x * kRotWarps) {
         const int64_t row = shares == 1 ? u : u / shares;
-        int r0 = 0, r1 = R.total;
-        if (shares > 1) {
-            const int share = (int)(u - row * shares);
-            r0 = R.total * share / shares;
-            r1 = R.total * (share + 1) / shares;
-        }
-        Walk<const T> in(static_cast<const T*>(a.q) + row * a.q_row, static_cast<const T*>(a.k) + row * a.k_row,
-                         a.q_head, a.k_head, R, sub, L.lo, r0);
-        Walk<T> out(static_cast<T*>(a.out_q) + row * a.heads * a.dim,
-                    static_cast<T*>(a.out_k) + row * a.kv_heads * a.dim, a.dim, a.dim, R, sub, L.lo, r0);
-        Raw<T> raw[U] = {};
-        auto fetch = [&](int r, Raw<T>& x) {
-            x = Raw<T>{};
-            if (r >= r1) return;
-            if (L.live && R.has(a, r, sub)) x = load_at<T>(in.at, apart);
-            in.next(R, r);
-        };
+        const int first = shares == 1 ? 0 : (int)(u - row * shares) * kHeads;
+        const T* q = static_cast<const T*>(a.q) + row * a.q_row + lo;
+        const T* k = static_cast<const T*>(a.k) + row * a.k_row + lo;
+        Raw<T> rq[U], rk[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) fetch(r0 + i, raw[i]);
+        for (int i = 0; i < U; ++i) {
+            rq[i] = load_at<T>(q, min(first + i * step + sub, a.heads - 1), (int)a.q_head, apart);
+            rk[i] = load_at<T>(k, min(first + i * step + sub, a.kv_heads - 1), (int)a.k_head, apart);
+        }
         Turn turn;
         if (a.pairs) {
             row_angles(a, row, cs);
             if (L.turns) turn = read_turn(cs, chunk);
         }
-        for (int r = r0; r < r1; r += U) {
+        auto all = [&](const T* in, int stride, T* out, int heads, Raw<T>(&raw)[U], const float* weight) {
+            over_rounds<U>(sub, first, step, heads, [&](int h, int i) {
+                Eight x = unpack<T>(raw[i], il);
+                if (h - sub + U * step < heads) raw[i] = load_at<T>(in, min(h + U * step, heads - 1), stride, apart);
+                if (!L.live) x = Eight{};
+                const float rs = rsqrtf(fmaf(lanes_sum<LANES>(dot8(x, x)), inv, a.eps));
+                const f32x2 rs2 = pack2(rs, rs);
+                const Eight w = read_weight(weight);
 #pragma unroll
-            for (int i = 0; i < U; ++i) {
-                if (r + i < r1) {  // uniform over the warp
-                    Eight x = unpack<T>(raw[i], il);
-                    fetch(r + i + U, raw[i]);
-                    const float ss = lanes_sum(dot8(x, x), lanes);
-                    const float rs = rsqrtf(fmaf(ss, inv, a.eps));
-                    const f32x2 rs2 = pack2(rs, rs);
-                    const Eight w = read_weight(weights[r + i < R.q ? 0 : 1][chunk]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x.v[e] = mul2(mul2(x.v[e], rs2), w.v[e]);
-                    if (L.turns) turn.apply<false>(x);
-                    if (L.live && R.has(a, r + i, sub)) store8<T>(out.at, apart, x, il);
-                    out.next(R, r + i);
-                }
-            }
-        }
+                for (int e = 0; e < 4; ++e) x.v[e] = mul2(mul2(x.v[e], rs2), w.v[e]);
+                if (L.turns) turn.template apply<false>(x);
+                if (L.live && h < heads) store8<T>(out + h * a.dim, apart, x, il);
+            });
+        };
+        all(q, (int)a.q_head, static_cast<T*>(a.out_q) + row * a.heads * a.dim + lo, a.heads, rq, weights[0][chunk]);
+        all(k, (int)a.k_head, static_cast<T*>(a.out_k) + row * a.kv_heads * a.dim + lo, a.kv_heads, rk,
+            weights[1][chunk]);
     }
 }
 
 // Backward.  A lane keeps the weight gradients of its eight elements over all
 // of its units; the block's warps and head slots join in shared memory in a
 // fixed order and each block writes one partial (2, dim) row.
-template <typename T, int U, bool IL>
+template <typename T, int U, bool IL, int LANES>
 __global__ void __launch_bounds__(kRotThreads, kBwdBlocksPerSm)
-norm_rotate_bwd_kernel(const __grid_constant__ mpo_rotate a, int lanes, int shares, float* __restrict__ partial) {
+norm_rotate_bwd_kernel(const __grid_constant__ mpo_rotate a, int shares, float* __restrict__ partial) {
+    constexpr int kHeads = 32 / LANES;
     __shared__ __align__(16) union {
         float angles[kRotWarps][2 * kMaxPairs];
         float sums[kRotWarps][32][17];
     } sh;
     __shared__ __align__(16) float weights[2][32][8];
     float* cs = sh.angles[threadIdx.x >> 5];
-    const int lane = threadIdx.x & 31, chunk = lane & (lanes - 1), sub = lane / lanes;
-    const Rounds R(a, lanes);
+    const int lane = threadIdx.x & 31, chunk = lane % LANES, sub = lane / LANES;
     const Lane L(a, chunk);
     const bool il = IL && L.turns;
-    const int apart = L.hi - L.lo;
-    stage_weights(a, weights, lanes);
+    const int apart = L.hi - L.lo, lo = L.live ? L.lo : 0, step = kHeads * shares;
+    stage_weights(a, weights, LANES);
     __syncthreads();
     Eight gq, gk;
 #pragma unroll
@@ -337,68 +313,55 @@ norm_rotate_bwd_kernel(const __grid_constant__ mpo_rotate a, int lanes, int shar
     for (int64_t u = (int64_t)blockIdx.x * kRotWarps + (threadIdx.x >> 5); u < units;
          u += (int64_t)gridDim.x * kRotWarps) {
         const int64_t row = shares == 1 ? u : u / shares;
-        int r0 = 0, r1 = R.total;
-        if (shares > 1) {
-            const int share = (int)(u - row * shares);
-            r0 = R.total * share / shares;
-            r1 = R.total * (share + 1) / shares;
-        }
-        Walk<const T> in(static_cast<const T*>(a.q) + row * a.q_row, static_cast<const T*>(a.k) + row * a.k_row,
-                         a.q_head, a.k_head, R, sub, L.lo, r0);
-        const int64_t dq = row * a.heads * a.dim, dk = row * a.kv_heads * a.dim;
-        Walk<const T> gin(static_cast<const T*>(a.grad_q) + dq, static_cast<const T*>(a.grad_k) + dk, a.dim, a.dim, R,
-                          sub, L.lo, r0);
-        Walk<T> out(static_cast<T*>(a.out_q) + dq, static_cast<T*>(a.out_k) + dk, a.dim, a.dim, R, sub, L.lo, r0);
-        Raw<T> rx[U] = {}, rg[U] = {};
-        auto fetch = [&](int r, Raw<T>& x, Raw<T>& g) {
-            x = Raw<T>{};
-            g = Raw<T>{};
-            if (r >= r1) return;
-            if (L.live && R.has(a, r, sub)) {
-                x = load_at<T>(in.at, apart);
-                g = load_at<T>(gin.at, apart);
-            }
-            in.next(R, r);
-            gin.next(R, r);
-        };
+        const int first = shares == 1 ? 0 : (int)(u - row * shares) * kHeads;
+        const T* q = static_cast<const T*>(a.q) + row * a.q_row + lo;
+        const T* k = static_cast<const T*>(a.k) + row * a.k_row + lo;
+        const int64_t dq = row * a.heads * a.dim + lo, dk = row * a.kv_heads * a.dim + lo;
+        const T* gyq = static_cast<const T*>(a.grad_q) + dq;
+        const T* gyk = static_cast<const T*>(a.grad_k) + dk;
+        Raw<T> rq[U], rk[U], rgq[U], rgk[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) fetch(r0 + i, rx[i], rg[i]);
+        for (int i = 0; i < U; ++i) {
+            const int hq = min(first + i * step + sub, a.heads - 1), hk = min(first + i * step + sub, a.kv_heads - 1);
+            rq[i] = load_at<T>(q, hq, (int)a.q_head, apart);
+            rgq[i] = load_at<T>(gyq, hq, a.dim, apart);
+            rk[i] = load_at<T>(k, hk, (int)a.k_head, apart);
+            rgk[i] = load_at<T>(gyk, hk, a.dim, apart);
+        }
         Turn turn;
         if (a.pairs) {
             row_angles(a, row, cs);
             if (L.turns) turn = read_turn(cs, chunk);
         }
-        for (int r = r0; r < r1; r += U) {
-#pragma unroll
-            for (int i = 0; i < U; ++i) {
-                if (r + i < r1) {
-                    const bool is_q = r + i < R.q;  // uniform over the warp
-                    Eight y = unpack<T>(rx[i], il), b = unpack<T>(rg[i], il), hw;
-                    fetch(r + i + U, rx[i], rg[i]);
-                    if (L.turns) turn.apply<true>(b);
-                    const Eight w = read_weight(weights[is_q ? 0 : 1][chunk]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) hw.v[e] = mul2(b.v[e], w.v[e]);
-                    const float ss = lanes_sum(dot8(y, y), lanes);
-                    const float hx = lanes_sum(dot8(hw, y), lanes);
-                    const float rs = rsqrtf(fmaf(ss, inv, a.eps));
-                    const float back = -(hx * inv * rs * rs * rs);
-                    const f32x2 rs2 = pack2(rs, rs), back2 = pack2(back, back);
-                    // A lane without a head holds zeros: it adds nothing.
-                    if (is_q) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) gq.v[e] = fma2(b.v[e], mul2(y.v[e], rs2), gq.v[e]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) gk.v[e] = fma2(b.v[e], mul2(y.v[e], rs2), gk.v[e]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y.v[e] = fma2(y.v[e], back2, mul2(rs2, hw.v[e]));
-                    if (L.live && R.has(a, r + i, sub)) store8<T>(out.at, apart, y, il);
-                    out.next(R, r + i);
+        auto all = [&](const T* in, int stride, const T* gin, T* out, int heads, Raw<T>(&raw)[U], Raw<T>(&rg)[U],
+                       const float* weight, Eight& gw) {
+            over_rounds<U>(sub, first, step, heads, [&](int h, int i) {
+                Eight y = unpack<T>(raw[i], il), b = unpack<T>(rg[i], il), hw;
+                if (h - sub + U * step < heads) {
+                    const int next = min(h + U * step, heads - 1);
+                    raw[i] = load_at<T>(in, next, stride, apart);
+                    rg[i] = load_at<T>(gin, next, a.dim, apart);
                 }
-            }
-        }
+                const bool on = L.live && h < heads;
+                if (!on) y = b = Eight{};  // adds nothing to the weights' gradients
+                if (L.turns) turn.template apply<true>(b);
+                const Eight w = read_weight(weight);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) hw.v[e] = mul2(b.v[e], w.v[e]);
+                const float ss = lanes_sum<LANES>(dot8(y, y)), hx = lanes_sum<LANES>(dot8(hw, y));
+                const float rs = rsqrtf(fmaf(ss, inv, a.eps));
+                const float back = -(hx * inv * rs * rs * rs);
+                const f32x2 rs2 = pack2(rs, rs), back2 = pack2(back, back);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    gw.v[e] = fma2(b.v[e], mul2(y.v[e], rs2), gw.v[e]);
+                    y.v[e] = fma2(y.v[e], back2, mul2(rs2, hw.v[e]));
+                }
+                if (on) store8<T>(out + h * a.dim, apart, y, il);
+            });
+        };
+        all(q, (int)a.q_head, gyq, static_cast<T*>(a.out_q) + dq, a.heads, rq, rgq, weights[0][chunk], gq);
+        all(k, (int)a.k_head, gyk, static_cast<T*>(a.out_k) + dk, a.kv_heads, rk, rgk, weights[1][chunk], gk);
     }
     if (!partial) return;
     __syncthreads();
@@ -419,12 +382,12 @@ norm_rotate_bwd_kernel(const __grid_constant__ mpo_rotate a, int lanes, int shar
     }
     __syncthreads();
     // Element e of chunk c: over the warps, then the head slots.
-    for (int t = threadIdx.x; t < 16 * lanes; t += kRotThreads) {
+    for (int t = threadIdx.x; t < 16 * LANES; t += kRotThreads) {
         const int c = t >> 4, e = t & 15;
         if (c * 8 >= a.dim) continue;
         float v = 0.f;
         for (int w = 0; w < kRotWarps; ++w)
-            for (int sl = 0; sl < R.step; ++sl) v += sh.sums[w][sl * lanes + c][e];
+            for (int sl = 0; sl < kHeads; ++sl) v += sh.sums[w][sl * LANES + c][e];
         const Lane at(a, c);
         const int el = (e & 7) < 4 ? at.lo + (e & 3) : at.hi + (e & 3);
         partial[((int64_t)blockIdx.x * 2 + (e >> 3)) * a.dim + el] = v;
@@ -466,7 +429,7 @@ struct RotateGrid {
 RotateGrid rotate_grid(const mpo_rotate& a, int per_sm) {
     RotateGrid g;
     g.lanes = rotate_lanes(a.dim);
-    const int64_t rounds = ceil_div(a.heads, 32 / g.lanes) + ceil_div(a.kv_heads, 32 / g.lanes);
+    const int64_t rounds = ceil_div(a.heads > a.kv_heads ? a.heads : a.kv_heads, 32 / g.lanes);
     const int64_t warps = (int64_t)sm_count() * per_sm * kRotWarps;
     g.shares = (int)max64(1, min64(rounds, warps / (2 * max64(a.rows, 1))));
     g.blocks = (unsigned)max64(1, min64(ceil_div(a.rows * g.shares, kRotWarps),
@@ -488,6 +451,8 @@ int check_rotate(const mpo_rotate* a, bool backward, const char* what) {
     if (a->pairs < 0 || a->pairs % 4 || 2 * a->pairs > a->dim)
         return bad("pairs must be a multiple of 4 with 2 * pairs <= dim");
     if (a->pairs && (a->axes < 1 || a->axes > kAttnMaxAxes)) return bad("axes must be in [1, 3]");
+    if (a->q_head < 0 || a->k_head < 0 || a->q_head > INT32_MAX || a->k_head > INT32_MAX)
+        return bad("head strides must be in [0, 2^31)");
     if (a->rows == 0) return kOk;
     if (!a->q || !a->k || !a->out_q || !a->out_k) return bad("null pointer");
     if (a->pairs && (!a->position || !a->freqs)) return bad("null pointer");
@@ -506,27 +471,43 @@ int check_rotate(const mpo_rotate* a, bool backward, const char* what) {
     return kOk;
 }
 
+// Calls f with the lane count as a compile-time constant.
+template <typename F>
+int with_lanes(int lanes, F&& f) {
+    switch (lanes) {
+        case 1: return f(std::integral_constant<int, 1>());
+        case 2: return f(std::integral_constant<int, 2>());
+        case 4: return f(std::integral_constant<int, 4>());
+        case 8: return f(std::integral_constant<int, 8>());
+        case 16: return f(std::integral_constant<int, 16>());
+        default: return f(std::integral_constant<int, 32>());
+    }
+}
 template <typename T>
 int run_rotate(const mpo_rotate& a, cudaStream_t s) {
-    constexpr int kDepth = sizeof(T) == 2 ? 4 : 2;
+    constexpr int kDepth = sizeof(T) == 2 ? 2 : 1;
     const RotateGrid g = rotate_grid(a, kFwdBlocksPerSm);
-    if (a.interleaved)
-        norm_rotate_kernel<T, kDepth, true><<<g.blocks, kRotThreads, 0, s>>>(a, g.lanes, g.shares);
-    else
-        norm_rotate_kernel<T, kDepth, false><<<g.blocks, kRotThreads, 0, s>>>(a, g.lanes, g.shares);
-    return check_launch("norm_rotate_kernel");
+    return with_lanes(g.lanes, [&](auto lanes) {
+        constexpr int L = decltype(lanes)::value;
+        if (a.interleaved) norm_rotate_kernel<T, kDepth, true, L><<<g.blocks, kRotThreads, 0, s>>>(a, g.shares);
+        else norm_rotate_kernel<T, kDepth, false, L><<<g.blocks, kRotThreads, 0, s>>>(a, g.shares);
+        return check_launch("norm_rotate_kernel");
+    });
 }
 template <typename T>
 int run_rotate_bwd(const mpo_rotate& a, cudaStream_t s) {
-    constexpr int kDepth = sizeof(T) == 2 ? 4 : 2;
+    constexpr int kDepth = sizeof(T) == 2 ? 2 : 1;
     const RotateGrid g = rotate_grid(a, kBwdBlocksPerSm);
     const bool weights = a.grad_q_weight || a.grad_k_weight;
     float* partial = weights ? static_cast<float*>(a.workspace) : nullptr;
-    if (a.interleaved)
-        norm_rotate_bwd_kernel<T, kDepth, true><<<g.blocks, kRotThreads, 0, s>>>(a, g.lanes, g.shares, partial);
-    else
-        norm_rotate_bwd_kernel<T, kDepth, false><<<g.blocks, kRotThreads, 0, s>>>(a, g.lanes, g.shares, partial);
-    int st = check_launch("norm_rotate_bwd_kernel");
+    const int st = with_lanes(g.lanes, [&](auto lanes) {
+        constexpr int L = decltype(lanes)::value;
+        if (a.interleaved)
+            norm_rotate_bwd_kernel<T, kDepth, true, L><<<g.blocks, kRotThreads, 0, s>>>(a, g.shares, partial);
+        else
+            norm_rotate_bwd_kernel<T, kDepth, false, L><<<g.blocks, kRotThreads, 0, s>>>(a, g.shares, partial);
+        return check_launch("norm_rotate_bwd_kernel");
+    });
     if (st != kOk || !weights) return st;
     norm_weight_reduce_kernel<<<(unsigned)ceil_div(2 * a.dim, 32), 1024, 0, s>>>(
         partial, (int)g.blocks, a.dim, a.grad_q_weight, a.grad_k_weight);
