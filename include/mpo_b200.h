@@ -549,9 +549,12 @@ MPO_API int mpo_allreduce_sum_f32_p2p(const float* value, float scale, float* ou
  *   (2t, 2t + 1) when interleaved.  dim is a multiple of 8 up to 256, pairs a
  *   multiple of 4 with 2 * pairs <= dim (0: no rotation).
  *   position (rows, axes <= 3) dense, int32 or (position_float) float32; freqs
- *   (axes, pairs) float32; q_weight / k_weight (dim) float32, nullable (ones).
- * Theta is formed in double and reduced before the sine; the rest is float32,
- * rounded once to the output's type. */
+ *   (axes, pairs) float32 or (freqs_double) float64; q_weight / k_weight (dim)
+ *   float32, nullable (ones).
+ * Theta is formed in the type of freqs, each product and sum rounded, axis 0
+ * first (float32 frequencies: what elementary float32 operations give), and
+ * reduced in double before its sine; the rest is float32, rounded once to the
+ * output's type. */
 typedef struct {
     const void *q, *k;
     int64_t q_row, q_head, k_row, k_head; /* strides, elements */
@@ -560,13 +563,13 @@ typedef struct {
     const float *q_weight, *k_weight;
     float *grad_q_weight, *grad_k_weight; /* backward: (dim), nullable */
     const void* position;
-    const float* freqs;
+    const void* freqs;
     void* workspace; /* backward */
     size_t workspace_bytes;
     int64_t rows;
     int32_t heads, kv_heads, dim, pairs, axes, position_float, interleaved, dtype;
     float eps;
-    int32_t reserved;
+    int32_t freqs_double;
 } mpo_rotate;
 MPO_API int mpo_norm_rotate(const mpo_rotate* args, void* stream);
 MPO_API size_t mpo_norm_rotate_workspace_bytes(const mpo_rotate* args);

@@ -163,7 +163,7 @@ attn_rows_kernel(const __grid_constant__ AttnArgs A, int per, int units, int spl
     if (!rows_unit(A, per, units, 16, splits, U)) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int rows = U.rows * U.gc;             // of the 16
-    float* tile = sh + kAttnMaxEntries * 16 + warp * 256;
+    float* tile = sh + (BIAS ? kAttnMaxEntries * 16 + warp * 256 : 0);
     // Bias: lane l forms that of key l % 16 and rows l / 16, l / 16 + 2, ..
     const int kl = lane & 15;
     int kp[kAttnMaxAxes] = {0, 0, 0};
@@ -175,7 +175,9 @@ attn_rows_kernel(const __grid_constant__ AttnArgs A, int per, int units, int spl
     auto load_key_pos = [&](int c) {
         if (!BIAS || c + kl >= U.c1) return;
         const int64_t k = (int64_t)U.t.other + U.key(c + kl);
-        for (int a = 0; a < A.a.axes; ++a) kp[a] = A.a.kpos[k * A.a.axes + a];
+#pragma unroll
+        for (int a = 0; a < kAttnMaxAxes; ++a)
+            if (a < A.a.axes) kp[a] = A.a.kpos[k * A.a.axes + a];
     };
     auto form_bias = [&]() {  // of the keys whose positions are at hand
         if (!BIAS) return;
@@ -186,14 +188,18 @@ attn_rows_kernel(const __grid_constant__ AttnArgs A, int per, int units, int spl
             if (i != i_old) {  // the heads of a query row share its buckets
                 i_old = i;
                 const int64_t q = (int64_t)U.t.row + U.row0 + i;
-                for (int a = 0; a < A.a.axes; ++a) {
-                    int b = bias_bucket(kp[a], A.a.qpos[q * A.a.axes + a], A.a.reach, nullptr);
-                    if (A.a.map) b = min(max(__ldg(A.a.map + b), 0), A.a.buckets - 1);
-                    bucket[a] = (a * A.a.buckets + b) * 16;
-                }
+#pragma unroll
+                for (int a = 0; a < kAttnMaxAxes; ++a)
+                    if (a < A.a.axes) {
+                        int b = bias_bucket(kp[a], A.a.qpos[q * A.a.axes + a], A.a.reach, nullptr);
+                        if (A.a.map) b = min(max(__ldg(A.a.map + b), 0), A.a.buckets - 1);
+                        bucket[a] = (a * A.a.buckets + b) * 16;
+                    }
             }
             float x = 0.f;
-            for (int a = 0; a < A.a.axes; ++a) x += sh[bucket[a] + hh];
+#pragma unroll
+            for (int a = 0; a < kAttnMaxAxes; ++a)
+                if (a < A.a.axes) x += sh[bucket[a] + hh];
             tile[r * 16 + kl] = x;
         }
         __syncwarp();
@@ -240,16 +246,12 @@ attn_rows_kernel(const __grid_constant__ AttnArgs A, int per, int units, int spl
                 kf[half][b] = load16(src + 32 * b, cc < U.c1 && 32 * b + 8 * t < A.a.dim);
         }
     };
-    int c = U.c0 + 16 * warp;
-    if (c < U.c1) {
-        load_keys(c);
-        load_key_pos(c);
-    }
-    for (; c < U.c1; c += kStep) {
-        form_bias();
-        load_key_pos(c + kStep);
-        // Values of keys 2t, 2t + 1, 2t + 8, 2t + 9.
-        uint4 vf[4][NV];
+    // Values of keys 2t, 2t + 1, 2t + 8, 2t + 9: a step ahead for narrow heads, where there are
+    // registers and fewer bytes in flight (53 -> 47 us for 32 streams of 2047 keys, D = 64; at D =
+    // 128 the same costs 287 -> 338 us for 64 streams of 8192).
+    constexpr bool kValuesAhead = DP <= 64;
+    uint4 vf[4][NV];
+    auto load_values = [&](int c) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int cc = c + 2 * t + (e & 1) + 8 * (e >> 1);
@@ -258,6 +260,17 @@ attn_rows_kernel(const __grid_constant__ AttnArgs A, int per, int units, int spl
             for (int b = 0; b < NV; ++b)
                 vf[e][b] = load16(src + 64 * b, cc < U.c1 && 64 * b + 8 * g < A.a.dim);
         }
+    };
+    int c = U.c0 + 16 * warp;
+    if (c < U.c1) {
+        load_keys(c);
+        if (kValuesAhead) load_values(c);
+        load_key_pos(c);
+    }
+    for (; c < U.c1; c += kStep) {
+        form_bias();
+        load_key_pos(c + kStep);
+        if (!kValuesAhead) load_values(c);
         float s[2][4];  // keys 2t, 2t + 1 of the half: rows g (0, 1) and g + 8 (2, 3)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -327,6 +340,7 @@ attn_rows_kernel(const __grid_constant__ AttnArgs A, int per, int units, int spl
                 mma16816<T>(o[8 * b + 2 * w + 1], pf, high_pair(v0[w], v1[w]), high_pair(v2[w], v3[w]));
             }
         }
+        if (kValuesAhead && c + kStep < U.c1) load_values(c + kStep);
     }
     if (BIAS) __syncthreads();  // the tables and tiles have been read
     // Column n of product j of block b is element 64 b + 8 n + j.
@@ -485,9 +499,10 @@ RowsPlan rows_plan(const AttnArgs& A) {
     P.units = (int)ceil_div(min64(A.a.max_rows, kAttnTile), P.per);
     const int64_t blocks = A.a.q_tile_count * P.units * A.a.kv_heads * ceil_div(A.group, P.heads_per);
     const int64_t span = min64(A.a.max_keys, (int64_t)A.left + A.right + 1 + A.a.sinks + P.per);
-    // Twelve blocks per SM (four rounds of what is resident) even out clouds of
-    // different lengths; a split keeps at least 256 keys, four per lane group.
-    P.splits = (int)max64(1, min64(min64(ceil_div(12 * sm_count(), max64(blocks, 1)), span / 256), 64));
+    // Twelve blocks per SM (several rounds of what is resident) even out clouds of
+    // different lengths; a split keeps at least 512 keys, eight steps of its warps,
+    // beside which its start and its join are short.
+    P.splits = (int)max64(1, min64(min64(ceil_div(12 * sm_count(), max64(blocks, 1)), span / 512), 64));
     return P;
 }
 

@@ -12,9 +12,10 @@
 // few, a share of one row's heads), so the angles of a row are formed once for
 // all of its heads, one pair per lane; `lanes` = dim / 8 rounded up to a power
 // of two serve one head, each holding the two halves of four pairs as two
-// vectors of four, so the rotation needs no exchange and the sums one butterfly.  Angles: position
-// x frequency / pi is summed in double and reduced to one turn there (positions
-// of 10^5 would cost a float sum 2 decimal digits), then sincospif.
+// vectors of four, so the rotation needs no exchange and the sums one butterfly.  Angles are formed in
+// the type of the frequencies (float32: as elementary float32 operations give
+// them; float64 for positions whose float32 angle would be off by too much),
+// reduced to one turn in double, then sincospif.
 #include <string>
 #include <type_traits>
 
@@ -189,9 +190,19 @@ __device__ __forceinline__ void row_angles(const mpo_rotate& a, int64_t row, flo
     __syncwarp();  // the previous row's angles have been read
     for (int t = threadIdx.x & 31; t < a.pairs; t += 32) {
         double theta = 0.;
+        if (a.freqs_double) {
 #pragma unroll
-        for (int ax = 0; ax < kAttnMaxAxes; ++ax)
-            if (ax < a.axes) theta = fma(pos[ax], (double)a.freqs[ax * a.pairs + t], theta);
+            for (int ax = 0; ax < kAttnMaxAxes; ++ax)
+                if (ax < a.axes)
+                    theta = __dadd_rn(theta, __dmul_rn(pos[ax], static_cast<const double*>(a.freqs)[ax * a.pairs + t]));
+        } else {
+            float sum = 0.f;
+#pragma unroll
+            for (int ax = 0; ax < kAttnMaxAxes; ++ax)
+                if (ax < a.axes)
+                    sum = __fadd_rn(sum, __fmul_rn((float)pos[ax], static_cast<const float*>(a.freqs)[ax * a.pairs + t]));
+            theta = (double)sum;
+        }
         const double half_turns = theta * 0.31830988618379067154;  // / pi
         const double whole = 2.0 * rint(half_turns * 0.5);
         sincospif((float)(half_turns - whole), cs + kMaxPairs + t, cs + t);

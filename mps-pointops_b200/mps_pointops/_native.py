@@ -62,7 +62,7 @@ class RotateArgs(ctypes.Structure):
               "freqs workspace"),
         (_sz, "workspace_bytes"), (_i64, "rows"),
         (_i32, "heads kv_heads dim pairs axes position_float interleaved dtype"), (_f32, "eps"),
-        (_i32, "reserved"))
+        (_i32, "freqs_double"))
 
 
 class AttentionArgs(ctypes.Structure):

@@ -191,7 +191,8 @@ def _rotate_call(backward: bool, q, k, wq, wk, position, freqs, eps, interleaved
             _address(freqs), _address(ws), nbytes, q.shape[0], q.shape[1], k.shape[1], q.shape[2],
             0 if freqs is None else freqs.shape[1], 0 if freqs is None else freqs.shape[0],
             int(position is not None and position.dtype == torch.float32), int(interleaved),
-            _DTYPES[q.dtype], eps, 0)
+            _DTYPES[q.dtype], eps,
+            int(freqs is not None and freqs.dtype == torch.float64))
 
     with N.on_device(device):
         lib = N.lib()
@@ -243,7 +244,8 @@ def norm_rotate(q: Tensor, k: Tensor, position: Tensor | None, freqs: Tensor | N
     ``interleaved`` (2t, 2t + 1), turns by ``sum_a position[n, a] * freqs[a, t]``;
     elements beyond 2P are left as they are.  ``position`` is (N, A) or (N,),
     integers or float32, A up to 3 (grid coordinates, say, or a row index);
-    ``freqs`` is (A, P) float32, P a multiple of 4.  Both None: no rotation.
+    ``freqs`` is (A, P), P a multiple of 4, float32 or float64: the angle is formed
+    in its type (float64 where positions are large).  Both None: no rotation.
     D is a multiple of 8 up to 256.  q and k may be strided views (of a packed
     projection); results are dense.  Gradients reach q, k and the weights, not
     the positions or frequencies.
@@ -263,8 +265,9 @@ def norm_rotate(q: Tensor, k: Tensor, position: Tensor | None, freqs: Tensor | N
     if not (math.isfinite(eps) and eps >= 0):
         raise ValueError("eps must be finite and not negative")
     if freqs is not None:
-        if not isinstance(freqs, Tensor) or freqs.ndim != 2 or freqs.dtype != torch.float32:
-            raise ValueError("freqs must be a float32 tensor of shape (A, P)")
+        if not isinstance(freqs, Tensor) or freqs.ndim != 2 or freqs.dtype not in (torch.float32,
+                                                                                   torch.float64):
+            raise ValueError("freqs must be a float32 or float64 tensor of shape (A, P)")
         axes, pairs = freqs.shape
         if not 1 <= axes <= 3:
             raise ValueError("freqs must have 1 to 3 axes")

@@ -120,7 +120,7 @@ def test_norm_rotate_refusals():
     refused("row count", q, k[:9], None, None)
     refused("like q", q, k.half(), None, None, error=TypeError)
     refused("multiple of 8", q[..., :12], k[..., :12], None, None)
-    refused("float32 tensor", q, k, pos, freqs.double())
+    refused("float32 or float64", q, k, pos, freqs.half())
     refused("multiple of 4", q, k, pos, torch.zeros(1, 6))
     refused("at most half", q, k, pos, torch.zeros(1, 20))
     refused("1 to 3 axes", q, k, torch.zeros(10, 4, dtype=torch.int32), torch.zeros(4, 16))

@@ -356,7 +356,12 @@ def rotate_reference(x, w, position, freqs, eps, interleaved, grad):
     y = x * r * w
     if freqs is not None:
         P = freqs.shape[1]
-        theta = (position.cpu().double() @ freqs.cpu().double())[:, None]
+        # The angle is formed in the type of the frequencies, axis 0 first.
+        f, p = freqs.cpu(), position.cpu().to(freqs.dtype)
+        theta = p[:, :1] * f[:1]
+        for ax in range(1, f.shape[0]):
+            theta = theta + p[:, ax:ax + 1] * f[ax:ax + 1]
+        theta = theta.double()[:, None]
         c, s = theta.cos(), theta.sin()
         if interleaved:
             a, b = y[..., 0:2 * P:2], y[..., 1:2 * P:2]
@@ -369,12 +374,13 @@ def rotate_reference(x, w, position, freqs, eps, interleaved, grad):
     return y.detach(), dx, dw
 
 
+@pytest.mark.parametrize("angle", [torch.float32, torch.float64])
 @pytest.mark.parametrize("dtype", [FP, BF, HF])
 @pytest.mark.parametrize("n,H,K,D,P,A,interleaved", [
     (1, 1, 1, 8, 4, 1, False), (1, 32, 8, 128, 64, 1, False), (63, 4, 4, 64, 24, 3, False),
     (257, 6, 2, 48, 12, 1, True), (100, 3, 1, 24, 12, 2, True), (65, 2, 2, 256, 128, 3, False),
     (3001, 8, 8, 64, 32, 3, False), (50, 5, 5, 80, 0, 0, False), (40, 2, 1, 16, 4, 2, False)])
-def test_norm_rotate(cuda_device, dtype, n, H, K, D, P, A, interleaved):
+def test_norm_rotate(cuda_device, dtype, n, H, K, D, P, A, interleaved, angle):
     """Values to a few roundings of float32 and one of the type; weight
     gradients to n H 2^-24 of the sum of magnitudes."""
     g = torch.Generator().manual_seed(n + D)
@@ -384,7 +390,7 @@ def test_norm_rotate(cuda_device, dtype, n, H, K, D, P, A, interleaved):
     pos = freqs = None
     if P:
         pos = torch.randint(-100000, 100000, (n, A), generator=g, dtype=torch.int32).to(cuda_device)
-        freqs = torch.rand(A, P, generator=g).to(cuda_device)
+        freqs = torch.rand(A, P, generator=g).to(cuda_device, angle)
     gq, gk = rand(g, n, H, D, dtype=dtype).to(cuda_device), rand(g, n, K, D, dtype=dtype).to(cuda_device)
     leaves = [x.detach().requires_grad_() for x in (q, k, wq, wk)]
     yq, yk = attention.norm_rotate(leaves[0], leaves[1], pos, freqs, q_weight=leaves[2],
