@@ -513,3 +513,18 @@ def test_rows_far_apart_in_one_tile(cuda_device, dtype):
                        grad=grad)
     for name, got in zip(("out", "dq", "dk", "dv", "dtable"), (out, *grads)):
         C.check(got, want[name], name)
+
+
+def test_example_trains_and_serves(cuda_device):
+    """The operators together: the loss falls, and rows over cached keys are those of
+    the whole cloud up to the rounding of weights and results (values of size 4 at
+    most: two roundings of 2^-8 of each)."""
+    import importlib.util
+
+    path = Path(__file__).resolve().parent.parent / "examples" / "denoise_serial_attention.py"
+    spec = importlib.util.spec_from_file_location("denoise_serial_attention", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses = example.train(20, cuda_device)
+    assert losses[-1] < 0.8 * losses[0]
+    assert example.cached_rows(cuda_device) <= 4 * 2 * 2 * 2.0 ** -8
