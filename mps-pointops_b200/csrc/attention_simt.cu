@@ -152,27 +152,42 @@ __device__ __forceinline__ void product_nn(float (&acc)[8][DP / 16], const float
 }
 
 // Scores of a tile in units of log2, -inf where invisible.  Rows are queries
-// (TRANSPOSED: keys) of the resident side.
+// (TRANSPOSED: keys) of the resident side, columns the streamed side's.  `whole`:
+// every pair of the tile is visible.
 template <bool TRANSPOSED>
 __device__ __forceinline__ void finish_scores(const AttnArgs& A, const SimtSmem& S, float (&s)[8][4],
-                                              int p0, int rows, int j0, int cols) {
+                                              int p0, int rows, int j0, int cols, bool whole) {
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[i][c] *= A.scale_log2;
+    for (int a = 0; a < A.a.axes; ++a) {
+        const float* table = S.table + a * A.a.buckets;
+        int cp[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) cp[c] = S.cpos[a * kTR + tx + 16 * c];
+        const int4 lo = *reinterpret_cast<const int4*>(S.rpos + a * kTR + 8 * ty);
+        const int4 hi = *reinterpret_cast<const int4*>(S.rpos + a * kTR + 8 * ty + 4);
+        const int rp[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int d = TRANSPOSED ? rp[i] - cp[c] : cp[c] - rp[i];
+                int b = min(max(d, -A.a.reach), A.a.reach) + A.a.reach;
+                if (A.a.map) b = S.map[b];
+                s[i][c] += table[b];
+            }
+    }
+    if (whole) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const int r = 8 * ty + i, col = tx + 16 * c;
-            float b = 0.f;
-            if (A.a.table)
-                for (int a = 0; a < A.a.axes; ++a) {
-                    const int rp = S.rpos[a * kTR + r], cp = S.cpos[a * kTR + col];
-                    b += S.table[a * A.a.buckets +
-                                 bias_bucket(TRANSPOSED ? rp : cp, TRANSPOSED ? cp : rp, A.a.reach,
-                                             A.a.map ? S.map : nullptr)];
-                }
             const int p = TRANSPOSED ? j0 + col : p0 + r, j = TRANSPOSED ? p0 + r : j0 + col;
-            const bool seen = r < rows && col < cols && attn_visible(A, p, j);
-            s[i][c] = seen ? fmaf(s[i][c], A.scale_log2, b) : -INFINITY;
+            if (!(r < rows && col < cols && attn_visible(A, p, j))) s[i][c] = -INFINITY;
         }
 }
 __device__ __forceinline__ float half_warp_max(float v) {
@@ -234,7 +249,8 @@ __global__ void __launch_bounds__(kThreads) attn_simt_fwd_kernel(const __grid_co
         __syncthreads();
         float s[8][4];
         product_nt<DP>(s, S.rows[0], S.rows[1]);
-        finish_scores<false>(A, S, s, H.p0, H.rows, k0, n);
+        finish_scores<false>(A, S, s, H.p0, H.rows, k0, n,
+                             n == kTR && H.rows == kTR && all_visible(A, H.p0, H.p0 + kTR - 1, k0, k0 + kTR - 1));
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float top = half_warp_max(fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3])));
@@ -346,7 +362,8 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_q_kernel(const __grid
         __syncthreads();
         float s[8][4], dp[8][4];
         product_nt<DP>(s, S.rows[0], S.rows[2]);
-        finish_scores<false>(A, S, s, H.p0, H.rows, k0, n);
+        finish_scores<false>(A, S, s, H.p0, H.rows, k0, n,
+                             n == kTR && H.rows == kTR && all_visible(A, H.p0, H.p0 + kTR - 1, k0, k0 + kTR - 1));
         product_nt<DP>(dp, S.rows[1], S.rows[3]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -460,7 +477,9 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __gri
             __syncthreads();
             float s[8][4];
             product_nt<DP>(s, S.rows[0], S.rows[2]);
-            finish_scores<true>(A, S, s, H.p0, H.rows, i0 + H.t.lk - H.t.lq, n);
+            const int q0 = i0 + H.t.lk - H.t.lq;
+            finish_scores<true>(A, S, s, H.p0, H.rows, q0, n,
+                                n == kTR && H.rows == kTR && all_visible(A, q0, q0 + kTR - 1, H.p0, H.p0 + kTR - 1));
             unsigned seen = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i)

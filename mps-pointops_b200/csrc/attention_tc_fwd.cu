@@ -21,14 +21,17 @@ namespace {
 constexpr int kFwdThreads = kTcRows + 32;
 template <int DP>
 struct FwdShape {
-    static constexpr int kS = 0, kO = kTcCols;  // TMEM columns
+    // Rows of 128 elements leave TMEM for a second buffer of S at the same two blocks per SM:
+    // S of tile i + 1 is then formed beside the softmax of tile i.
+    static constexpr int kBuffers = DP == 128 ? 2 : 1;
+    static constexpr int kS = 0, kO = kBuffers * kTcCols;  // TMEM columns
     static constexpr int kCols = kO + DP <= 128 ? 128 : 256;
     static constexpr int kBlocks = 512 / kCols;
     static constexpr uint32_t kQ = 0, kK = TcTile<DP>::bytes(128), kStage = TcTile<DP>::bytes(64),
                               kV = kK + 2 * kStage, kPos = kV + 2 * kStage,
                               kBar = kPos + 3 * 3 * kTcCols * 4, kTable = kBar + 64;
-    // Barriers: products; stages of keys (2) and values (2), the first keys with Q.
-    static constexpr uint32_t kFullK = kBar + 8, kFullV = kBar + 24, kSlot = kBar + 40;
+    // Barriers: products (2); stages of keys (2) and values (2), the first keys with Q.
+    static constexpr uint32_t kFullK = kBar + 16, kFullV = kBar + 32, kSlot = kBar + 48;
     static size_t bytes(int entries) {
         // At least what keeps more blocks than TMEM serves off an SM (they would wait for it).
         const size_t need = kTable + (size_t)entries * 128 + 1024;
@@ -41,6 +44,7 @@ template <typename T, int DP, int BIAS>
 __global__ void __launch_bounds__(kFwdThreads, (BIAS && DP <= 64 ? 3 : FwdShape<DP>::kBlocks))
 attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TcMaps M) {
     using Shape = FwdShape<DP>;
+    constexpr int kBuffers = Shape::kBuffers;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sb = smem_u32(smem);
@@ -77,10 +81,11 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
         auto scores = [&](int i) {
             if (i >= tiles) return;
             patience.wait(sb + Shape::kFullK + 8 * (i & 1), (i >> 1) & 1);
-            mma_scores<T, DP, kTcCols>(tmem + Shape::kS, sb + Shape::kQ, sb + Shape::kK + (i & 1) * Shape::kStage);
+            mma_scores<T, DP, kTcCols>(tmem + Shape::kS + (i & (kBuffers - 1)) * kTcCols, sb + Shape::kQ,
+                                       sb + Shape::kK + (i & 1) * Shape::kStage);
         };
         if ((tid & 31) == 0)
-            for (int i = 0; i < 5; ++i) mbar_init(sb + Shape::kBar + 8 * i);
+            for (int i = 0; i < 6; ++i) mbar_init(sb + Shape::kBar + 8 * i);
         __syncwarp();
         load_keys(0);
         load_values(0);
@@ -89,8 +94,14 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
         __syncthreads();
         tc_fence_after();
         tmem = uniform(*slot);
+        // Step i commits to barrier i mod kBuffers; the prologue stands for the kBuffers steps
+        // before step 0.
         scores(0);
         mma_commit(sb + Shape::kBar);
+        if (kBuffers == 2) {
+            scores(1);
+            mma_commit(sb + Shape::kBar + 8);
+        }
         patience.wait(sb + Shape::kBar, 0);  // S of tile 0: the first keys' stage is free
         load_keys(2);
         load_values(1);
@@ -98,16 +109,23 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
             __syncthreads();  // the weights of tile i are in TMEM
             tc_fence_after();
             patience.wait(sb + Shape::kFullV + 8 * (i & 1), (i >> 1) & 1);
-            mma_weighted<T, DP, kTcCols>(tmem + Shape::kO, tmem + Shape::kS,
+            mma_weighted<T, DP, kTcCols>(tmem + Shape::kO, tmem + Shape::kS + (i & (kBuffers - 1)) * kTcCols,
                                          sb + Shape::kV + (i & 1) * Shape::kStage, i > 0);
             // Issued after P V and executed in order after it: S may overwrite the weights.
-            scores(i + 1);
-            mma_commit(sb + Shape::kBar);
-            // S of tile i + 1 and P V of tile i are done: their operands' stages are free.
-            // Copies get until the end of the next step.
-            patience.wait(sb + Shape::kBar, (i + 1) & 1);
-            load_keys(i + 3);
-            load_values(i + 2);
+            scores(i + kBuffers);
+            mma_commit(sb + Shape::kBar + 8 * (i & (kBuffers - 1)));
+            if (kBuffers == 1) {
+                // S of tile i + 1 and P V of tile i are done: their operands' stages are free.
+                // Copies get until the end of the next step.
+                patience.wait(sb + Shape::kBar, (i + 1) & 1);
+                load_keys(i + 3);
+                load_values(i + 2);
+            } else {
+                // Those of step i - 1: S of tile i + 1 and P V of tile i - 1.
+                patience.wait(sb + Shape::kBar + 8 * ((i - 1) & 1), ((i + 1) >> 1) & 1);
+                load_keys(i + 3);
+                if (i > 0) load_values(i + 1);
+            }
         }
         tc_fence_before();
         __syncthreads();  // the rows have been read
@@ -145,17 +163,18 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
     tc_fence_after();
     const uint32_t tmem = *slot;
     const uint32_t mine = tmem + ((uint32_t)(tid & ~31) << 16);  // this warp's lanes
-    Waiter done(sb + Shape::kBar, A.a.status);
+    Waiters<kBuffers> done(sb + Shape::kBar, A.a.status);
 
     // Running maximum in units of s2 = S * mul + bias (log2), as of the last rescale.
     float top = -INFINITY, sum = 0.f;
     const float mul = BIAS ? 1.f : (A.scale_log2 > 0.f ? A.scale_log2 : 1.f);
     for (int i = 0; i < tiles; ++i) {
-        done.wait();
+        done.wait(i);
         fetch_columns(i + 2);
+        const uint32_t scored = mine + Shape::kS + (i & (kBuffers - 1)) * kTcCols;
         float s[kTcCols];
 #pragma unroll
-        for (int c = 0; c < kTcCols; c += 16) tmem_ld16(mine + Shape::kS + c, s + c);
+        for (int c = 0; c < kTcCols; c += 16) tmem_ld16(scored + c, s + c);
         tmem_wait_ld();
         tmem_use(s);
         int k0, n;
@@ -203,6 +222,10 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
                 sum *= f;
             }
             if (i > 0) {
+                if (kBuffers == 2) {  // P V of tile i - 1 still adds to the rows
+                    done.even.patience.wait(sb + Shape::kBar + 8 * ((i - 1) & 1), ((i + 1) >> 1) & 1);
+                    tc_fence_after();
+                }
 #pragma unroll
                 for (int c = 0; c < DP; c += 16) {
                     float o[16];
@@ -230,7 +253,7 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
                 part[(e >> 1) & 1] = add2(part[(e >> 1) & 1], pack2(a, b));
                 w[e / 2] = Elem<T>::two(a, b);
             }
-            tmem_st8(mine + Shape::kS + c, w);
+            tmem_st8(scored + c, w);
         }
         {
             float a, b;
@@ -242,7 +265,8 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
         tc_fence_before();
         __syncthreads();
     }
-    if (tiles > 0) done.wait();
+    done.wait(tiles);
+    if (kBuffers == 2) done.wait(tiles + 1);
     const bool live = tid < t.rows;
     bool nan = BIAS && live && bias.far;
     const int64_t at = (((int64_t)t.row + tid) * A.a.heads + h) * A.a.dim;
