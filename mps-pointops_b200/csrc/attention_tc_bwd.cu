@@ -27,13 +27,6 @@ namespace {
 // stored and tensor-core results are off by 2e-3 and (sums rounded towards zero)
 // 3e-6 of it, always the same way for all pairs of a row.  kDelta forms D = sum
 // P dP in float32 first; kGradQTable then forms dq and the table's gradient.
-constexpr size_t kTcSmem = 232448;  // shared memory of a block at most
-// Barrier of the computing threads alone.
-template <int THREADS>
-__device__ __forceinline__ void compute_sync() {
-    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
-}
-
 enum QueryMode { kGradQ = 0, kDelta = 1, kGradQTable = 2 };
 
 // Threads: NG groups of 128; thread `row` of each group shares the row and takes
@@ -723,7 +716,7 @@ int run_q(const AttnArgs& A, const TcMaps& M, float* partial, cudaStream_t s) {
         if (!ONE && Shape::one_copy(axes, entries)) return run_q<T, DP, BIAS, MODE, true>(A, M, partial, s);
     }
     const size_t bytes = Shape::bytes(axes, entries, ONE);
-    const int st = tc_prepare(attn_tc_query_kernel<T, DP, BIAS, MODE, ONE>, bytes, "attn_tc_query_kernel");
+    const int st = tc_prepare<&attn_tc_query_kernel<T, DP, BIAS, MODE, ONE>>("attn_tc_query_kernel");
     if (st != kOk) return st;
     const dim3 grid((unsigned)A.a.q_tile_count, (unsigned)A.a.heads);
     attn_tc_query_kernel<T, DP, BIAS, MODE, ONE><<<grid, Shape::kThreads, bytes, s>>>(A, M, partial);
@@ -736,7 +729,7 @@ int run_kv(const AttnArgs& A, const TcMaps& M, float* partial, cudaStream_t s) {
         if (!ONE && GradKvShape<DP>::one_copy(entries)) return run_kv<T, DP, BIAS, true>(A, M, partial, s);
     }
     const size_t bytes = GradKvShape<DP>::bytes(entries, ONE);
-    int st = tc_prepare(attn_tc_grad_kv_kernel<T, DP, BIAS, ONE>, bytes, "attn_tc_grad_kv_kernel");
+    int st = tc_prepare<&attn_tc_grad_kv_kernel<T, DP, BIAS, ONE>>("attn_tc_grad_kv_kernel");
     if (st != kOk) return st;
     const int shares = sink_shares(A);
     dim3 grid((unsigned)A.a.k_tile_count, (unsigned)A.a.kv_heads, (unsigned)shares);
