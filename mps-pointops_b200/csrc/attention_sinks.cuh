@@ -30,28 +30,33 @@ __global__ void __launch_bounds__(256)
 attn_join_sinks_kernel(const __grid_constant__ AttnArgs A, int shares, const float* __restrict__ partial) {
     const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.k_tiles)[blockIdx.x];
     if (t.first >= A.a.sinks) return;
-    const int r = blockIdx.z * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, hk = blockIdx.y;
-    if (r >= t.rows) return;
-    const float* src = sink_sums(A, const_cast<float*>(partial), t.cloud, t.first + r, hk, shares, 0);
-    const int64_t at = (((int64_t)t.row + r) * A.a.kv_heads + hk) * A.a.dim, half = (int64_t)kAttnTile * A.a.dim;
-    bool nan = false;
-    for (int d = lane; d < A.a.dim; d += 32) {
-        float dk = 0.f, dv = 0.f;
-        for (int z = 0; z < shares; ++z) {
-            dk += src[z * 2 * half + d];
-            dv += src[(z * 2 + 1) * half + d];
+    const int lane = threadIdx.x & 31, hk = blockIdx.y;
+    for (int r = blockIdx.z * 8 + (threadIdx.x >> 5); r < t.rows; r += 8 * gridDim.z) {
+        const float* src = sink_sums(A, const_cast<float*>(partial), t.cloud, t.first + r, hk, shares, 0);
+        const int64_t at = (((int64_t)t.row + r) * A.a.kv_heads + hk) * A.a.dim;
+        const int64_t half = (int64_t)kAttnTile * A.a.dim;
+        bool nan = false;
+        for (int d = lane; d < A.a.dim; d += 32) {
+            float dk = 0.f, dv = 0.f;
+            for (int z = 0; z < shares; ++z) {
+                dk += src[z * 2 * half + d];
+                dv += src[(z * 2 + 1) * half + d];
+            }
+            nan |= isnan(dk) | isnan(dv);
+            static_cast<T*>(A.a.grad_k)[at + d] = Elem<T>::from(dk);
+            static_cast<T*>(A.a.grad_v)[at + d] = Elem<T>::from(dv);
         }
-        nan |= isnan(dk) | isnan(dv);
-        static_cast<T*>(A.a.grad_k)[at + d] = Elem<T>::from(dk);
-        static_cast<T*>(A.a.grad_v)[at + d] = Elem<T>::from(dv);
+        if (__any_sync(FULL_MASK, nan)) {
+            __syncwarp();
+            exact_grad_kv_row<T>(A, t.base, t.first + r, t.other, t.lq, t.lk, hk);
+        }
     }
-    if (__any_sync(FULL_MASK, nan))
-        exact_grad_kv_row<T>(A, t.base, t.first + r, t.other, t.lq, t.lk, hk);
 }
 
 template <typename T>
 int join_sinks(const AttnArgs& A, int shares, const float* partial, cudaStream_t s) {
-    const dim3 grid((unsigned)A.a.k_tile_count, (unsigned)A.a.kv_heads, kAttnTile / 8);
+    // Most blocks find no sink in their tile and end: four of them per tile, not one per 8 rows.
+    const dim3 grid((unsigned)A.a.k_tile_count, (unsigned)A.a.kv_heads, 4);
     attn_join_sinks_kernel<T><<<grid, 256, 0, s>>>(A, shares, partial);
     return check_launch("attn_join_sinks_kernel");
 }

@@ -138,6 +138,17 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
           "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -259,14 +270,14 @@ __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b) {
                tc_idesc<T>(NB, false), k > 0);
 }
 // D (128 x DP) += weights (128 x NB) . B (NB rows of tile b).  The weights are 16-bit
-// pairs in TMEM: those of columns 16 k .. lie in the first 8 of the 16 columns
-// from a + 16 k, over the scores that they come from, so a thread overwrites
-// nothing but what it has read itself.
-template <typename T, int DP, int NB>
+// pairs in TMEM, those of columns 16 k .. in 8 columns from a + STRIDE k.  STRIDE
+// 16: in the first half of the scores that they come from, so a thread that forms
+// 16 columns overwrites nothing but what it has read itself.
+template <typename T, int DP, int NB, int STRIDE = 16>
 __device__ __forceinline__ void mma_weighted(uint32_t d, uint32_t a, uint32_t b, bool acc) {
 #pragma unroll
     for (int k = 0; k < NB / 16; ++k)
-        mma_ts(d, a + 16 * k, TcTile<DP>::mn_major(b, NB, k), tc_idesc<T>(DP, true), acc || k > 0);
+        mma_ts(d, a + STRIDE * k, TcTile<DP>::mn_major(b, NB, k), tc_idesc<T>(DP, true), acc || k > 0);
 }
 
 // ---------------------------------------------------------------- masks
@@ -384,11 +395,11 @@ __device__ __forceinline__ float lds_table(int addr) {
     asm("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
     return v;
 }
-// Bias of 16 columns as pairs; cols: the staged columns of axis 0 at column c.
+// Bias of N columns as pairs; cols: the staged columns of axis 0 at column c.
 // ONE: the table has one copy, at `one` (null: read it from global memory, for
 // head h); addresses are then used as entry numbers.
-template <bool MAPPED, bool ONE>
-__device__ __forceinline__ void bias16(const AttnArgs& A, const BiasRow& row, const float* cols, f32x2 (&t)[8],
+template <bool MAPPED, bool ONE, int N>
+__device__ __forceinline__ void bias_of(const AttnArgs& A, const BiasRow& row, const float* cols, f32x2 (&t)[N / 2],
                                        const float* one, int h) {
     auto entry = [&](int a, float col) {
         const int at = row.template address<MAPPED>(A, row.part[a], col, row.first[a]);
@@ -400,7 +411,7 @@ __device__ __forceinline__ void bias16(const AttnArgs& A, const BiasRow& row, co
     for (int a = 0; a < kAttnMaxAxes; ++a)
         if (a < A.a.axes) {
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
+            for (int e = 0; e < N; e += 4) {
                 const float4 c4 = *reinterpret_cast<const float4*>(cols + a * kTcCols + e);
                 const f32x2 x = pack2(entry(a, c4.x), entry(a, c4.y));
                 const f32x2 y = pack2(entry(a, c4.z), entry(a, c4.w));

@@ -47,7 +47,9 @@ enum QueryMode { kGradQ = 0, kDelta = 1, kGradQTable = 2 };
 // its own bank: a plain read, add and write, no atomics), and group a keeps
 // those of axis a: the groups leave their score gradients in TMEM as float32
 // (two buffers), and after the tile's barrier group a adds all 64 columns of
-// them to its axis.  With DP = 128 the cells (up to 128 KB) leave room for one
+// them to its axis.  A group that keeps cells forms 8 columns of a tile itself, the
+// others the rest, so that both take about as long; the pairs then have columns of
+// their own in TMEM.  With DP = 128 the cells (up to 128 KB) leave room for one
 // stage of keys and values, one buffer of S and dP, and one copy of the table.
 template <int DP, int MODE>
 struct QueryShape {
@@ -59,8 +61,10 @@ struct QueryShape {
     static constexpr int kKStages = kTight ? 1 : 2 + kBuffers, kVStages = kTight ? 1 : 2;
     static constexpr int kPosStages = kTight ? 3 : 4;
     static constexpr int kS = 0, kDP = kTcCols, kBuffer = (kBuffers - 1) * 2 * kTcCols;  // TMEM columns
-    static constexpr int kDQ = 2 * kTcCols + kBuffer, kDS = kDQ + DP;
+    static constexpr int kDQ = 2 * kTcCols + kBuffer;
+    static constexpr int kDS = kDQ + DP, kP = kDS + 2 * kTcCols;  // cells: two buffers each
     static constexpr int kCols = kBlocks == 2 ? 256 : 512;
+    static_assert(!kCells || kP + kTcCols <= kCols, "TMEM");
     static constexpr uint32_t kQ = 0, kG = TcTile<DP>::bytes(128), kStage = TcTile<DP>::bytes(64),
                               kK = 2 * kG, kV = kK + kKStages * kStage, kBar = kV + kVStages * kStage,
                               kTable = kBar + 128;
@@ -157,10 +161,12 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         for (int i = 0; i < tiles; ++i) {
             __syncthreads();  // the score gradients of tile i are in TMEM
             tc_fence_after();
-            if (MODE != kDelta)
-                mma_weighted<T, DP, kTcCols>(tmem + Shape::kDQ,
-                                             tmem + (i & (kBuffers - 1)) * Shape::kBuffer + Shape::kS,
-                                             sb + Shape::kK + (i % Shape::kKStages) * Shape::kStage, i > 0);
+            const uint32_t keys = sb + Shape::kK + (i % Shape::kKStages) * Shape::kStage;
+            if (Shape::kCells)
+                mma_weighted<T, DP, kTcCols, 8>(tmem + Shape::kDQ, tmem + Shape::kP + (i & 1) * (kTcCols / 2), keys, i > 0);
+            else if (MODE == kGradQ)
+                mma_weighted<T, DP, kTcCols>(tmem + Shape::kDQ, tmem + (i & (kBuffers - 1)) * Shape::kBuffer + Shape::kS,
+                                             keys, i > 0);
             if (Shape::kTight) {
                 // One stage, one buffer: barrier 1 tells that it is free, barrier 0 that S is there.
                 mma_commit(sb + Shape::kBar + 8);
@@ -221,7 +227,17 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
-    const uint32_t mine = tmem + ((uint32_t)quarter << 21) + kPer * group;  // lanes 32 quarter .., own columns
+    const uint32_t lanes = tmem + ((uint32_t)quarter << 21);  // 32 quarter ..
+    // Columns of a tile that this thread forms, in units.  With cells, a group that keeps those
+    // of an axis forms one unit of 8 columns and the others divide the rest.
+    constexpr int kUnit = Shape::kCells ? 8 : 16;
+    int first_column = 0, last_column = 0;
+    if (Shape::kCells) {
+        const int axes = A.a.axes, rest = kTcCols / kUnit - axes, others = Shape::kGroups - axes;
+        auto begin = [&](int g) { return g <= axes ? g : axes + rest * (g - axes) / others; };
+        first_column = kUnit * begin(group);
+        last_column = kUnit * begin(group + 1);
+    }
     Waiters<kBuffers> done(sb + Shape::kBar, A.a.status);
     float delta = 0.f;  // D; kDelta: this thread's columns of its sum so far
     if (MODE == kGradQTable) {
@@ -248,61 +264,74 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         const int k0 = span.tile(i) * kTcCols, n = min(kTcCols, t.lk - k0);
         const bool whole = n == kTcCols && t.rows == 128 &&
                            all_visible(A, t.first, t.first + 127, k0, k0 + kTcCols - 1);
-        uint32_t bits = ~0u;  // of this thread's columns
-        if (!whole) bits = live ? (uint32_t)(seen_keys(A, p, k0, n) >> (kPer * group)) : 0u;
-        if (BIAS && bias.far) bits = 0u;
-        constexpr uint32_t kFull = kPer == 32 ? ~0u : (1u << (kPer & 31)) - 1;
-        const bool all = __all_sync(FULL_MASK, (bits & kFull) == kFull);
+        uint64_t seen = ~0ull;
+        if (!whole) seen = live ? seen_keys(A, p, k0, n) : 0ull;
+        if (BIAS && bias.far) seen = 0ull;
+        const bool all = __all_sync(FULL_MASK, seen == ~0ull);
         const float* cols = kpos + (i % Shape::kPosStages) * A.a.axes * kTcCols;
-#pragma unroll
-        for (int cc = 0; cc < kPer; cc += 16) {
-        const int c0 = kPer * group + cc;
-        const uint32_t own = mine + (i & (kBuffers - 1)) * Shape::kBuffer + cc;
-        float s[16], dp[16];
-        tmem_ld16(own + Shape::kS, s);
-        tmem_ld16(own + Shape::kDP, dp);
-        f32x2 b[8];
-        if (BIAS)
-            bias16<BIAS == 2, ONE>(A, bias, cols + c0, b,
-                                   !Shape::kTight || entries <= Shape::kTightEntries ? table : nullptr, h);
-        tmem_wait_ld();
-        tmem_use(s);
-        tmem_use(dp);
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-            f32x2 x = fma2(pack2(s[e], s[e + 1]), scale2, lse22);
-            if (BIAS) x = add2(x, b[e / 2]);
-            float u, v;
-            unpack2(x, u, v);
-            u = exp2_sfu(u);
-            v = exp2_sfu(v);
-            if (MODE == kDelta) {
-                s[e] = u * dp[e];
-                s[e + 1] = v * dp[e + 1];
+        // kUnit columns from c0.
+        auto unit = [&](int c0) {
+            const uint32_t own = lanes + (i & (kBuffers - 1)) * Shape::kBuffer + c0;
+            const uint32_t pairs = Shape::kCells ? lanes + Shape::kP + (i & 1) * (kTcCols / 2) + c0 / 2 : own + Shape::kS;
+            float s[kUnit], dp[kUnit];
+            if constexpr (kUnit == 16) {
+                tmem_ld16(own + Shape::kS, s);
+                tmem_ld16(own + Shape::kDP, dp);
             } else {
-                s[e] = u * (dp[e] - delta);
-                s[e + 1] = v * (dp[e + 1] - delta);
+                tmem_ld8(own + Shape::kS, s);
+                tmem_ld8(own + Shape::kDP, dp);
             }
-        }
-        if (!all) {
+            f32x2 b[kUnit / 2];
+            if (BIAS)
+                bias_of<BIAS == 2, ONE, kUnit>(
+                    A, bias, cols + c0, b, !Shape::kTight || entries <= Shape::kTightEntries ? table : nullptr, h);
+            tmem_wait_ld();
+            tmem_use(s);
+            tmem_use(dp);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = (bits >> (cc + e)) & 1u ? s[e] : 0.f;
-        }
-        if (MODE == kDelta) {
-            f32x2 sum = pack2(s[0], s[1]);
+            for (int e = 0; e < kUnit; e += 2) {
+                f32x2 x = fma2(pack2(s[e], s[e + 1]), scale2, lse22);
+                if (BIAS) x = add2(x, b[e / 2]);
+                float u, v;
+                unpack2(x, u, v);
+                u = exp2_sfu(u);
+                v = exp2_sfu(v);
+                if (MODE == kDelta) {
+                    s[e] = u * dp[e];
+                    s[e + 1] = v * dp[e + 1];
+                } else {
+                    s[e] = u * (dp[e] - delta);
+                    s[e + 1] = v * (dp[e + 1] - delta);
+                }
+            }
+            if (!all) {
 #pragma unroll
-            for (int e = 2; e < 16; e += 2) sum = add2(sum, pack2(s[e], s[e + 1]));
-            float u, v;
-            unpack2(sum, u, v);
-            delta += u + v;
+                for (int e = 0; e < kUnit; ++e) s[e] = (uint32_t)(seen >> (c0 + e)) & 1u ? s[e] : 0.f;
+            }
+            if (MODE == kDelta) {
+                f32x2 sum = pack2(s[0], s[1]);
+#pragma unroll
+                for (int e = 2; e < kUnit; e += 2) sum = add2(sum, pack2(s[e], s[e + 1]));
+                float u, v;
+                unpack2(sum, u, v);
+                delta += u + v;
+            } else {
+                uint32_t w[kUnit / 2];
+#pragma unroll
+                for (int e = 0; e < kUnit / 2; ++e) w[e] = Elem<T>::two(s[2 * e], s[2 * e + 1]);
+                if constexpr (kUnit == 8) {
+                    tmem_st8(lanes + Shape::kDS + (i & 1) * kTcCols + c0, reinterpret_cast<const uint32_t*>(s));
+                    tmem_st4(pairs, w);
+                } else {
+                    tmem_st8(pairs, w);
+                }
+            }
+        };
+        if constexpr (Shape::kCells) {
+            for (int c0 = first_column; c0 < last_column; c0 += kUnit) unit(c0);
         } else {
-            if (Shape::kCells)
-                tmem_st16(mine + Shape::kDS + (i & 1) * kTcCols + cc, reinterpret_cast<const uint32_t*>(s));
-            uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = Elem<T>::two(s[2 * e], s[2 * e + 1]);
-            tmem_st8(own + Shape::kS, w);
-        }
+            for (int c0 = 0; c0 < kPer; c0 += kUnit) unit(kPer * group + c0);
         }
         if (i + Shape::kAhead > 1) store_columns(i + Shape::kAhead);
         if (MODE != kDelta) tmem_wait_st();
@@ -312,7 +341,7 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         if (Shape::kCells && group < A.a.axes) {
             const float* axis = cols + group * kTcCols;
             const float part = group == 0 ? bias.part[0] : group == 1 ? bias.part[1] : bias.part[2];
-            const uint32_t buffer = tmem + ((uint32_t)quarter << 21) + Shape::kDS + (i & 1) * kTcCols;
+            const uint32_t buffer = lanes + Shape::kDS + (i & 1) * kTcCols;
 #pragma unroll
             for (int c = 0; c < kTcCols; c += 16) {
                 float ds[16];
@@ -377,7 +406,7 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = 0.f;
             if (tiles > 0) {
-                tmem_ld16(mine - kPer * group + Shape::kDQ + c, o);
+                tmem_ld16(lanes + Shape::kDQ + c, o);
                 tmem_wait_ld();
                 tmem_use(o);
             }
@@ -606,7 +635,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
             tmem_ld16(own + Shape::kS, s);
             tmem_ld16(own + Shape::kDP, dp);
             f32x2 b[8];
-            if (BIAS) bias16<BIAS == 2, ONE>(A, bias, cols + c, b, table, head);
+            if (BIAS) bias_of<BIAS == 2, ONE, 16>(A, bias, cols + c, b, table, head);
             tmem_wait_ld();
             tmem_use(s);
             tmem_use(dp);

@@ -189,7 +189,7 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
 #pragma unroll
             for (int c = 0; c < kTcCols; c += 16) {
                 f32x2 b[8];
-                bias16<BIAS == 2, false>(A, bias, cols + c, b, nullptr, h);
+                bias_of<BIAS == 2, false, 16>(A, bias, cols + c, b, nullptr, h);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     unpack2(fma2(pack2(s[c + 2 * e], s[c + 2 * e + 1]), scale2, b[e]), s[c + 2 * e],

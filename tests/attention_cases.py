@@ -6,8 +6,8 @@ first order:
   out   the stored value and, for 16-bit types, each weight round: u (|o| + sum P |v|);
   dv    as out: u (|dv| + sum P |do|);
   D     formed from the stored out: e_i = sum_d |do| u (|o| + sum P |v|); where the
-        table's gradient is wanted, from a result whose weights keep at least 15 bits
-        (u replaced by 2^-15);
+        table's gradient is wanted, in float32 from the pairs themselves (allowed here:
+        u replaced by 2^-15);
   dq    sum_j (u |dS| + P e_i) |k| scale + u |dq|; dk likewise over i;
   dT    sum over the pairs of a bucket of P e_i.
 Float32 arithmetic adds to every score (64-term sums of exact products, the
