@@ -4,8 +4,10 @@
 // The tile kernels multiply whole tiles, in which an invisible pair counts as
 // a weight of 0; a NaN or an infinity among values that a row may not see then
 // turns its 0 into a NaN.  A tile kernel therefore sends each result row that
-// holds a NaN through these functions before it stores it: the row comes out
+// holds a NaN through these functions after it has stored it: the row comes out
 // with the contributions of its visible pairs alone.  No cost where no NaN is.
+// (The backward sends infinities too: a score gradient may leave float16's range
+// although its products with the rows do not.)
 #pragma once
 
 #include "attention_common.cuh"

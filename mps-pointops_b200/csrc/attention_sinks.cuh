@@ -42,7 +42,7 @@ attn_join_sinks_kernel(const __grid_constant__ AttnArgs A, int shares, const flo
                 dk += src[z * 2 * half + d];
                 dv += src[(z * 2 + 1) * half + d];
             }
-            nan |= isnan(dk) | isnan(dv);
+            nan |= !isfinite(dk) | !isfinite(dv);
             static_cast<T*>(A.a.grad_k)[at + d] = Elem<T>::from(dk);
             static_cast<T*>(A.a.grad_v)[at + d] = Elem<T>::from(dv);
         }

@@ -414,7 +414,7 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 o[e] *= A.a.scale;
-                nan |= isnan(o[e]);
+                nan |= !isfinite(o[e]);  // a float16 score gradient may have overflowed
             }
 #pragma unroll
             for (int e = 0; e < 16; e += 8)
@@ -709,7 +709,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 if (!which) o[e] *= A.a.scale;
-                nan |= isnan(o[e]);
+                nan |= !isfinite(o[e]);  // a float16 score gradient may have overflowed
                 if (BIAS && bias.far) o[e] = __int_as_float(0x7fffffff);  // for the join: form it again
             }
 #pragma unroll

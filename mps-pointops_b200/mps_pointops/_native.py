@@ -44,8 +44,7 @@ def packer(block: type[ctypes.Structure]):
     one call instead of one attribute store per field (None is a null pointer)."""
     codes = {_vp: "P", _i64: "q", _sz: "N", _i32: "i", _f32: "f"}
     layout = struct.Struct("".join(codes[kind] for _, kind in block._fields_))
-    assert layout.size == ctypes.sizeof(block) or ctypes.sizeof(block) - layout.size < 8
-    pad = b"\0" * (ctypes.sizeof(block) - layout.size)
+    pad = b"\0" * (ctypes.sizeof(block) - layout.size)  # struct does not pad the end
 
     def pack(*values) -> bytes:
         return layout.pack(*values) + pad

@@ -150,10 +150,11 @@ def _same(value: Tensor, like: Tensor, name: str) -> None:
 
 
 def _rows(x: Tensor, elements: int) -> Tensor:
-    """``x`` itself where its innermost axis is dense and each row starts on a
-    multiple of ``elements`` elements, else a dense copy."""
-    if (x.stride(2) == 1 and x.stride(0) % elements == 0 and x.stride(1) % elements == 0
-            and x.data_ptr() % (elements * x.element_size()) == 0) or x.numel() == 0:
+    """``x`` itself where its innermost axis is dense, each row starts on a multiple
+    of ``elements`` elements and no axis is broadcast, else a dense copy."""
+    rows, heads, inner = x.stride()
+    if (inner == 1 and rows > 0 and heads > 0 and rows % elements == 0 and heads % elements == 0
+            and heads < 1 << 31 and x.data_ptr() % (elements * x.element_size()) == 0) or x.numel() == 0:
         return x
     return x.clone(memory_format=torch.contiguous_format)
 

@@ -221,3 +221,25 @@ def test_argument_blocks_match_the_header(tmp_path):
     want = [ctypes.sizeof(N.RotateArgs), N.RotateArgs.eps.offset, ctypes.sizeof(N.AttentionArgs),
             N.AttentionArgs.workspace.offset, N.AttentionArgs.scale.offset]
     assert [int(x) for x in out.stdout.split()] == want
+
+
+def test_entry_addresses_of_the_tensor_core_kernels():
+    """The kernels form the address of a pair's table entry by two float32
+    multiply-adds, t = sat(column / 2R + part) and t * 256 R + first in denormals.
+    Their roundings leave every address exact for rows within 2^15 of the tile's
+    first and columns clamped at 2^16 (float64 carries the products exactly)."""
+    import numpy as np
+
+    f = np.float32
+    rng = np.random.default_rng(0)
+    for reach in [0, 1, 2, 3, 7, 15, 31, 42, 63, 127, 128, 500, 1023, 1024]:
+        inv = f(1) / f(2 * reach) if reach else f(0)
+        d = np.concatenate([np.arange(-reach - 2, reach + 3), [-65536, 65536, -40000, 40000]])
+        for row in [0, 1, -1, 32768, -32768, 32767, *rng.integers(-32768, 32769, 200)]:
+            part = f(0.5 - float(row) * float(inv))
+            column = np.clip(d + row, -65536, 65536)
+            t = np.clip((column * float(inv) + float(part)).astype(f), f(0), f(1))
+            for first in (1028, 200004):
+                address = np.rint(t.astype(np.float64) * (256 * reach) + first)
+                want = first + 128 * (np.clip(column - row, -reach, reach) + reach)
+                assert (address == want).all(), (reach, row)

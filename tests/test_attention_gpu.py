@@ -169,6 +169,41 @@ def test_packed_and_unaligned_views(cuda_device, dtype):
         C.check(got, want[name], name)
 
 
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_broadcast_inputs(cuda_device, dtype):
+    """Keys broadcast over heads and a query row broadcast over rows: values, and
+    gradients summed back."""
+    g = torch.Generator().manual_seed(17)
+    lens, n = [60, 41], 101
+    q1, k1, v = (rand(g, *s, dtype=dtype).to(cuda_device) for s in ((1, 4, 32), (n, 1, 32), (n, 4, 32)))
+    grad = rand(g, n, 4, 32, dtype=dtype).to(cuda_device)
+    leaves = [x.clone().requires_grad_() for x in (q1, k1, v)]
+    out = attention.window_attention(leaves[0].expand(n, 4, 32), leaves[1].expand(n, 4, 32), leaves[2],
+                                     ends(lens, cuda_device), window=(15, 15))
+    grads = torch.autograd.grad(out, leaves, grad)
+    want = C.attention(q1.expand(n, 4, 32), k1.expand(n, 4, 32), v, lens, lens, left=15, right=15, grad=grad)
+    C.check(out, want["out"], "out")
+    C.check(grads[2], want["dv"], "dv")
+    # The sums over rows and heads are torch's, of stored gradients: one more rounding of the
+    # result and n 2^-23 of the sum of magnitudes.
+    u = C.UNIT[dtype]
+    for got, name, axis in ((grads[0], "dq", 0), (grads[1], "dk", 1)):
+        value, bound = want[name]
+        total = value.sum(axis, keepdim=True)
+        allowed = bound.sum(axis, keepdim=True) + u * total.abs() + n * 2.0 ** -23 * value.abs().sum(axis, keepdim=True)
+        C.check(got, (total, allowed), name)
+
+
+def test_float16_gradients_past_its_range(cuda_device):
+    """Score gradients of some 10^5, beyond float16, between values within it."""
+    def edit(q, k, v, grad, table):
+        v.mul_(200)
+        grad.mul_(200)
+        k.mul_(2.0 ** -8)
+        q.mul_(2.0 ** -8)
+    run(cuda_device, HF, 1, 1, 64, [40], left=3, right=3, edit=edit)
+
+
 @pytest.mark.parametrize("dtype", [FP, BF, HF])
 def test_table_types_and_negative_scale(cuda_device, dtype):
     run(cuda_device, dtype, 2, 2, 32, [100], bias="grid", table_dtype=BF, scale=-0.3)
