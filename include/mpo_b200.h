@@ -580,8 +580,10 @@ MPO_API int mpo_norm_rotate_backward(const mpo_rotate* args, void* stream);
  * and of the other side.  Each cloud's rows on the owning side are cut into
  * tiles of 128 rows; a tile is eight int32 words {row, rows, first, other, lq,
  * lk, base, cloud}, `first` being the position i + Lk - Lq of its first row
- * (keys == 0: queries own) or its index in the cloud (keys != 0).  Returns the
- * tile count, writing at most `capacity` of them to `tiles` (nullable: count
+ * (keys == 0: queries own) or its index in the cloud (keys != 0).  Query tiles
+ * come in the order of their rows, key tiles by `first`, then by cloud (the
+ * backward divides the work of tiles that hold sinks, which it expects at the
+ * head of the list).  Returns the tile count, writing at most `capacity` of them to `tiles` (nullable: count
  * only), or -1 with mpo_last_error set when an offset decreases, is negative
  * or does not fit 30 bits. */
 MPO_API int64_t mpo_attention_plan(const int64_t* ends, const int64_t* other_ends, int64_t segs,

@@ -1,6 +1,7 @@
 // C entry points of the attention of serialised clouds: the tiles of a ragged
 // batch, the checks of arguments, the choice of kernels and the reduction of
 // the table's gradient (definitions: attention_common.cuh).
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -145,6 +146,12 @@ int64_t mpo_attention_plan(const int64_t* ends, const int64_t* other_ends, int64
         }
         base = ends[b];
         other = other_ends[b];
+    }
+    if (keys && tiles) {  // the tiles that may hold sinks to the head of the list
+        AttnTile* list = reinterpret_cast<AttnTile*>(tiles);
+        std::sort(list, list + max64(0, min64(count, capacity)), [](const AttnTile& x, const AttnTile& y) {
+            return x.first != y.first ? x.first < y.first : x.cloud < y.cloud;
+        });
     }
     return count;
 }

@@ -206,9 +206,9 @@ struct Half {
     AttnTile t;
     int rows, p0;
     int64_t row;
-    __device__ __forceinline__ bool load(const int32_t* tiles) {
-        t = reinterpret_cast<const AttnTile*>(tiles)[blockIdx.x >> 1];
-        const int off = (blockIdx.x & 1) * kTR;
+    __device__ __forceinline__ bool load(const int32_t* tiles, int half) {
+        t = reinterpret_cast<const AttnTile*>(tiles)[half >> 1];
+        const int off = (half & 1) * kTR;
         rows = min(kTR, t.rows - off);
         p0 = t.first + off;
         row = (int64_t)t.row + off;
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_fwd_kernel(const __grid_co
     constexpr int W = DP / 16;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, h = blockIdx.y, hk = h / A.group;
     Half H;
-    if (!H.load(A.a.q_tiles)) return;
+    if (!H.load(A.a.q_tiles, blockIdx.x)) return;
     load_rows<T, DP>(S.rows[0], A.a.q, H.row, H.rows, h, A.a.q_row, A.a.q_head, A.a.dim);
     if (A.a.table) {
         load_bias(A, S, h);
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_q_kernel(const __grid
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, h = blockIdx.y, hk = h / A.group;
     const int entries = A.a.axes * A.a.buckets;
     Half H;
-    const bool mine = H.load(A.a.q_tiles);
+    const bool mine = H.load(A.a.q_tiles, blockIdx.x);
     if (!mine) {
         if (partial)
             for (int e = threadIdx.x; e < entries; e += kThreads)
@@ -433,16 +433,18 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_q_kernel(const __grid
 
 // ---------------------------------------------------------------- backward: keys and values
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __grid_constant__ AttnArgs A, int shares, float* __restrict__ partial) {
+__global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __grid_constant__ AttnArgs A, int divided,
+                         int shares, float* __restrict__ partial) {
     extern __shared__ __align__(16) unsigned char smem[];
     const SimtSmem S(smem, DP, 4);
     constexpr int W = DP / 16;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, hk = blockIdx.y;
     Half H;  // p0: index of the first key
-    if (!H.load(A.a.k_tiles)) return;
+    const SinkBlock block = sink_block(blockIdx.x >> 1, divided, shares);
+    if (!H.load(A.a.k_tiles, 2 * block.tile + ((int)blockIdx.x & 1))) return;
     // The planned tile decides: both of its halves are shared out or neither is.
-    const bool shared = shares > 1 && H.t.first < A.a.sinks;
-    if (!shared && blockIdx.z > 0) return;
+    const bool shared = block.divided && H.t.first < A.a.sinks;
+    if (!shared && block.share > 0) return;
     const int64_t o_row = (int64_t)A.a.heads * A.a.dim;
     load_rows<T, DP>(S.rows[0], A.a.k, H.row, H.rows, hk, A.a.k_row, A.a.k_head, A.a.dim);
     load_rows<T, DP>(S.rows[1], A.a.v, H.row, H.rows, hk, A.a.v_row, A.a.v_head, A.a.dim);
@@ -456,8 +458,8 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __gri
     query_span(A, H.p0, H.p0 + H.rows - 1, H.t.lq, H.t.lk, lo, hi);
     if (shared) {
         const int n = max(0, hi - lo), base = lo;
-        lo = base + (int)((int64_t)n * blockIdx.z / shares);
-        hi = base + (int)((int64_t)n * (blockIdx.z + 1) / shares);
+        lo = base + (int)((int64_t)n * block.share / shares);
+        hi = base + (int)((int64_t)n * (block.share + 1) / shares);
     }
     for (int h = hk * A.group; h < (hk + 1) * A.group; ++h) {
         __syncthreads();
@@ -512,7 +514,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __gri
         if (r < H.rows) {
             const int64_t at = ((H.row + r) * A.a.kv_heads + hk) * A.a.dim + tx * W;
             float* sums =
-                shared ? sink_sums(A, partial, H.t.cloud, H.p0 + r, hk, shares, blockIdx.z) + tx * W : nullptr;
+                shared ? sink_sums(A, partial, H.t.cloud, H.p0 + r, hk, shares, block.share) + tx * W : nullptr;
 #pragma unroll
             for (int e = 0; e < W; ++e) {
                 nan |= isnan(dk[i][e]) | isnan(dv[i][e]);
@@ -573,11 +575,11 @@ int run_bwd(const AttnArgs& A, cudaStream_t s) {
         if (st != kOk) return st;
     }
     if (A.a.k_tile_count) {
-        const int shares = sink_shares(A);
-        const dim3 grid((unsigned)(2 * A.a.k_tile_count), (unsigned)A.a.kv_heads, (unsigned)shares);
-        attn_simt_grad_kv_kernel<T, DP><<<grid, kThreads, kb, s>>>(A, shares, sums);
+        const int shares = sink_shares(A), divided = sink_divided(A, shares);
+        const dim3 grid((unsigned)(2 * (A.a.k_tile_count + divided * (shares - 1))), (unsigned)A.a.kv_heads);
+        attn_simt_grad_kv_kernel<T, DP><<<grid, kThreads, kb, s>>>(A, divided, shares, sums);
         st = check_launch("attn_simt_grad_kv_kernel");
-        if (st == kOk && shares > 1) st = join_sinks<T>(A, shares, sums, s);
+        if (st == kOk && shares > 1) st = join_sinks<T>(A, divided, shares, sums, s);
     }
     return st;
 }

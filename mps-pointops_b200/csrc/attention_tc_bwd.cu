@@ -469,13 +469,14 @@ struct GradKvShape {
 // Key tiles that hold sinks are shared out: attention_sinks.cuh.
 template <typename T, int DP, int BIAS, bool ONE>
 __global__ void __launch_bounds__((GradKvShape<DP>::kThreads), (GradKvShape<DP>::kBlocks))
-attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TcMaps M, int shares,
-                       float* __restrict__ partial) {
+attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TcMaps M, int divided,
+                       int shares, float* __restrict__ partial) {
     using Shape = GradKvShape<DP>;
     constexpr int kPer = Shape::kPer, kBuffers = Shape::kBuffers;
-    const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.k_tiles)[blockIdx.x];
-    const bool shared = shares > 1 && t.first < A.a.sinks;
-    if (!shared && blockIdx.z > 0) return;
+    const SinkBlock block = sink_block(blockIdx.x, divided, shares);
+    const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.k_tiles)[block.tile];
+    const bool shared = block.divided && t.first < A.a.sinks;
+    if (!shared && block.share > 0) return;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sb = smem_u32(smem);
@@ -492,8 +493,8 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
     query_span(A, t.first, t.first + t.rows - 1, t.lq, t.lk, lo, hi);
     int first = 0, per = hi > lo ? (hi - lo + kTcCols - 1) / kTcCols : 0;
     if (shared) {
-        first = (int)((int64_t)per * blockIdx.z / shares);
-        per = (int)((int64_t)per * (blockIdx.z + 1) / shares) - first;
+        first = (int)((int64_t)per * block.share / shares);
+        per = (int)((int64_t)per * (block.share + 1) / shares) - first;
     }
     const int tiles = (int)uniform((uint32_t)(per * A.group));
 
@@ -691,7 +692,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
     if (kBuffers == 2) done.wait(tiles + 1);
     bool nan = BIAS && live && bias.far;
     const int64_t at = (((int64_t)t.row + r) * A.a.kv_heads + hk) * A.a.dim;
-    float* sums = shared ? sink_sums(A, partial, t.cloud, j, hk, shares, blockIdx.z) : nullptr;
+    float* sums = shared ? sink_sums(A, partial, t.cloud, j, hk, shares, block.share) : nullptr;
 #pragma unroll
     for (int which = 0; which < 2; ++which)
 #pragma unroll
@@ -760,12 +761,12 @@ int run_kv(const AttnArgs& A, const TcMaps& M, float* partial, cudaStream_t s) {
     const size_t bytes = GradKvShape<DP>::bytes(entries, ONE);
     int st = tc_prepare<&attn_tc_grad_kv_kernel<T, DP, BIAS, ONE>>("attn_tc_grad_kv_kernel");
     if (st != kOk) return st;
-    const int shares = sink_shares(A);
-    dim3 grid((unsigned)A.a.k_tile_count, (unsigned)A.a.kv_heads, (unsigned)shares);
-    attn_tc_grad_kv_kernel<T, DP, BIAS, ONE><<<grid, GradKvShape<DP>::kThreads, bytes, s>>>(A, M, shares, partial);
+    const int shares = sink_shares(A), divided = sink_divided(A, shares);
+    const dim3 grid((unsigned)(A.a.k_tile_count + divided * (shares - 1)), (unsigned)A.a.kv_heads);
+    attn_tc_grad_kv_kernel<T, DP, BIAS, ONE><<<grid, GradKvShape<DP>::kThreads, bytes, s>>>(A, M, divided, shares, partial);
     st = check_launch("attn_tc_grad_kv_kernel");
     if (st != kOk || shares == 1) return st;
-    return join_sinks<T>(A, shares, partial, s);
+    return join_sinks<T>(A, divided, shares, partial, s);
 }
 template <typename T, int DP, int BIAS>
 int run(const AttnArgs& A, cudaStream_t s) {

@@ -148,11 +148,13 @@ def test_tiles_cover_each_row_once():
         assert first == row - start + lk - lq
         covered += range(row, row + rows)
     assert covered == list(range(386))
-    covered = []
+    covered, order = [], []
     for row, rows, first, other, lq, lk, base, cloud in plan(key_ends, ends, 1):
         assert first == row - base
         covered += range(row, row + rows)
-    assert covered == list(range(400))
+        order.append((first, cloud))
+    assert sorted(covered) == list(range(400))
+    assert order == sorted(order)  # first tiles of all clouds, then second ones
     assert plan([], [], 0) == []
 
 
