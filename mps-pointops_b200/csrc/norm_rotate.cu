@@ -179,28 +179,28 @@ struct Turn {
 // the warp shares them through `cs` (cosines, then sines, kMaxPairs each).
 constexpr int kMaxPairs = 128;
 __device__ __forceinline__ void row_angles(const mpo_rotate& a, int64_t row, float* cs) {
-    double pos[kAttnMaxAxes];
+    int32_t word[kAttnMaxAxes];
 #pragma unroll
     for (int ax = 0; ax < kAttnMaxAxes; ++ax)
-        if (ax < a.axes) {
-            const int64_t at = row * a.axes + ax;
-            pos[ax] = a.position_float ? (double)static_cast<const float*>(a.position)[at]
-                                       : (double)static_cast<const int32_t*>(a.position)[at];
-        }
+        word[ax] = ax < a.axes ? static_cast<const int32_t*>(a.position)[row * a.axes + ax] : 0;
     __syncwarp();  // the previous row's angles have been read
     for (int t = threadIdx.x & 31; t < a.pairs; t += 32) {
         double theta = 0.;
         if (a.freqs_double) {
 #pragma unroll
             for (int ax = 0; ax < kAttnMaxAxes; ++ax)
-                if (ax < a.axes)
-                    theta = __dadd_rn(theta, __dmul_rn(pos[ax], static_cast<const double*>(a.freqs)[ax * a.pairs + t]));
+                if (ax < a.axes) {
+                    const double pos = a.position_float ? (double)__int_as_float(word[ax]) : (double)word[ax];
+                    theta = __dadd_rn(theta, __dmul_rn(pos, static_cast<const double*>(a.freqs)[ax * a.pairs + t]));
+                }
         } else {
             float sum = 0.f;
 #pragma unroll
             for (int ax = 0; ax < kAttnMaxAxes; ++ax)
-                if (ax < a.axes)
-                    sum = __fadd_rn(sum, __fmul_rn((float)pos[ax], static_cast<const float*>(a.freqs)[ax * a.pairs + t]));
+                if (ax < a.axes) {
+                    const float pos = a.position_float ? __int_as_float(word[ax]) : (float)word[ax];
+                    sum = __fadd_rn(sum, __fmul_rn(pos, static_cast<const float*>(a.freqs)[ax * a.pairs + t]));
+                }
             theta = (double)sum;
         }
         const double half_turns = theta * 0.31830988618379067154;  // / pi
