@@ -339,6 +339,23 @@ def test_many_queries_see_the_sinks(cuda_device, dtype):
     run(cuda_device, dtype, 2, 1, 16, [5000, 300], left=8, right=8, sinks=130)
 
 
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("backwards", [False, True])
+def test_sinks_of_short_clouds_and_any_order_of_tiles(cuda_device, dtype, backwards, monkeypatch):
+    """Clouds with no, fewer and more key tiles than the sinks reach into; the key tiles' order
+    decides which of them are divided, not the results."""
+    plan = attention.Segments._plan
+
+    def other_order(own, other, keys):
+        tiles = plan(own, other, keys)
+        return tiles.flip(0).contiguous() if keys else tiles
+
+    if backwards:
+        monkeypatch.setattr(attention.Segments, "_plan", staticmethod(other_order))
+    run(cuda_device, dtype, 2, 1, 64, [90, 3000, 0, 1, 129, 700], left=30, right=20, sinks=140)
+    run(cuda_device, dtype, 2, 2, 128, [20, 2100], [300, 2100], left=100, right=0, sinks=9, causal=True)
+
+
 @pytest.mark.parametrize("bias", [None, "grid"])
 def test_gradients_against_differences(cuda_device, bias):
     """Along a random direction, (L(x + h d) - L(x - h d)) / 2h in 64-bit sums of float32
