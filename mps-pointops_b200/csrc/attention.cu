@@ -5,7 +5,7 @@
 #include <cmath>
 #include <string>
 
-#include "attention_sinks.cuh"
+#include "attention_shares.cuh"
 
 namespace mpo {
 namespace {
@@ -106,9 +106,9 @@ AttnArgs derive(const mpo_attention& a) {
     return A;
 }
 
-// Backward workspace: the sinks' sums, then the table's partials.
+// Backward workspace: the shares' sums, then the table's partials.
 size_t workspace_bytes(const AttnArgs& A, bool backward) {
-    if (backward) return sink_bytes(A) + table_partial_bytes(A.a);
+    if (backward) return share_bytes(A) + table_partial_bytes(A.a);
     return A.a.q_tile_count && attn_rows_eligible(A) ? attn_rows_workspace(A) : 0;
 }
 
@@ -192,7 +192,7 @@ int mpo_window_attention_backward(const mpo_attention* args, void* stream) {
     if (st != kOk || !A.a.grad_table) return st;
     const int entries = A.a.axes * A.a.buckets;
     attn_table_reduce_kernel<<<dim3((unsigned)ceil_div(entries, 32), (unsigned)A.a.heads), 256, 0, s>>>(
-        reinterpret_cast<const float*>(static_cast<const unsigned char*>(A.a.workspace) + sink_bytes(A)),
+        reinterpret_cast<const float*>(static_cast<const unsigned char*>(A.a.workspace) + share_bytes(A)),
         A.a.q_tile_count * partial_blocks_per_tile(A.a), A.a.heads, entries, A.a.grad_table);
     return check_launch("attn_table_reduce_kernel");
 }

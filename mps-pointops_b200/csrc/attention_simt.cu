@@ -13,7 +13,7 @@
 // 768 blocks of 64 rows, of unequal clouds.
 #include <string>
 
-#include "attention_sinks.cuh"
+#include "attention_shares.cuh"
 
 namespace mpo {
 namespace {
@@ -437,17 +437,17 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_q_kernel(const __grid
 
 // ---------------------------------------------------------------- backward: keys and values
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __grid_constant__ AttnArgs A, int divided,
-                         int shares, float* __restrict__ partial) {
+__global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __grid_constant__ AttnArgs A, const KeyShares K,
+                         float* __restrict__ partial) {
     extern __shared__ __align__(16) unsigned char smem[];
     const SimtSmem S(smem, DP, 4);
     constexpr int W = DP / 16;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, hk = blockIdx.y;
     Half H;  // p0: index of the first key
-    const SinkBlock block = sink_block(blockIdx.x >> 1, divided, shares);
+    const ShareBlock block = share_block(blockIdx.x >> 1, K);
     if (!H.load(A.a.k_tiles, 2 * block.tile + ((int)blockIdx.x & 1))) return;
     // The planned tile decides: both of its halves are shared out or neither is.
-    const bool shared = block.divided && H.t.first < A.a.sinks;
+    const bool shared = block.divided && H.t.first < K.limit;
     if (!shared && block.share > 0) return;
     const int64_t o_row = (int64_t)A.a.heads * A.a.dim;
     load_rows<T, DP>(S.rows[0], A.a.k, H.row, H.rows, hk, A.a.k_row, A.a.k_head, A.a.dim);
@@ -462,8 +462,8 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __gri
     query_span(A, H.p0, H.p0 + H.rows - 1, H.t.lq, H.t.lk, lo, hi);
     if (shared) {
         const int n = max(0, hi - lo), base = lo;
-        lo = base + (int)((int64_t)n * block.share / shares);
-        hi = base + (int)((int64_t)n * (block.share + 1) / shares);
+        lo = base + (int)((int64_t)n * block.share / K.shares);
+        hi = base + (int)((int64_t)n * (block.share + 1) / K.shares);
     }
     for (int h = hk * A.group; h < (hk + 1) * A.group; ++h) {
         __syncthreads();
@@ -518,7 +518,8 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __gri
         if (r < H.rows) {
             const int64_t at = ((H.row + r) * A.a.kv_heads + hk) * A.a.dim + tx * W;
             float* sums =
-                shared ? sink_sums(A, partial, H.t.cloud, H.p0 + r, hk, shares, block.share) + tx * W : nullptr;
+                shared ? share_sums(A, partial, block.tile, H.p0 - H.t.first + r, hk, K.shares, block.share) + tx * W
+                       : nullptr;
 #pragma unroll
             for (int e = 0; e < W; ++e) {
                 nan |= isnan(dk[i][e]) | isnan(dv[i][e]);
@@ -565,7 +566,7 @@ int run_bwd(const AttnArgs& A, cudaStream_t s) {
     const int entries = A.a.axes * A.a.buckets;
     float* sums = static_cast<float*>(A.a.workspace);
     float* partial = A.a.grad_table ? reinterpret_cast<float*>(
-                                          static_cast<unsigned char*>(A.a.workspace) + sink_bytes(A))
+                                          static_cast<unsigned char*>(A.a.workspace) + share_bytes(A))
                                     : nullptr;
     const size_t qb = SimtSmem::bytes(DP, 4, partial ? entries : 0);
     const size_t kb = SimtSmem::bytes(DP, 4, 0);
@@ -579,11 +580,11 @@ int run_bwd(const AttnArgs& A, cudaStream_t s) {
         if (st != kOk) return st;
     }
     if (A.a.k_tile_count) {
-        const int shares = sink_shares(A), divided = sink_divided(A, shares);
-        const dim3 grid((unsigned)(2 * (A.a.k_tile_count + divided * (shares - 1))), (unsigned)A.a.kv_heads);
-        attn_simt_grad_kv_kernel<T, DP><<<grid, kThreads, kb, s>>>(A, divided, shares, sums);
+        const KeyShares K = key_shares(A);
+        const dim3 grid((unsigned)(2 * key_blocks(A, K)), (unsigned)A.a.kv_heads);
+        attn_simt_grad_kv_kernel<T, DP><<<grid, kThreads, kb, s>>>(A, K, sums);
         st = check_launch("attn_simt_grad_kv_kernel");
-        if (st == kOk && shares > 1) st = join_sinks<T>(A, divided, shares, sums, s);
+        if (st == kOk && K.shares > 1) st = join_shares<T>(A, K, sums, s);
     }
     return st;
 }

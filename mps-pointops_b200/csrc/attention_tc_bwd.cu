@@ -21,7 +21,7 @@
 // counting what they stall); latency at one block per SM binds.
 #include <string>
 
-#include "attention_sinks.cuh"
+#include "attention_shares.cuh"
 #include "attention_tc.cuh"
 
 namespace mpo {
@@ -493,16 +493,16 @@ struct GradKvShape {
     }
 };
 
-// Key tiles that hold sinks are shared out: attention_sinks.cuh.
+// Key tiles that hold sinks are shared out: attention_shares.cuh.
 template <typename T, int DP, int BIAS, bool ONE>
 __global__ void __launch_bounds__((GradKvShape<DP>::kThreads), (GradKvShape<DP>::kBlocks))
-attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TcMaps M, int divided,
-                       int shares, float* __restrict__ partial) {
+attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TcMaps M, const KeyShares K,
+                       float* __restrict__ partial) {
     using Shape = GradKvShape<DP>;
     constexpr int kPer = Shape::kPer, kBuffers = Shape::kBuffers;
-    const SinkBlock block = sink_block(blockIdx.x, divided, shares);
+    const ShareBlock block = share_block(blockIdx.x, K);
     const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.k_tiles)[block.tile];
-    const bool shared = block.divided && t.first < A.a.sinks;
+    const bool shared = block.divided && t.first < K.limit;
     if (!shared && block.share > 0) return;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -520,8 +520,8 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
     query_span(A, t.first, t.first + t.rows - 1, t.lq, t.lk, lo, hi);
     int first = 0, per = hi > lo ? (hi - lo + kTcCols - 1) / kTcCols : 0;
     if (shared) {
-        first = (int)((int64_t)per * block.share / shares);
-        per = (int)((int64_t)per * (block.share + 1) / shares) - first;
+        first = (int)((int64_t)per * block.share / K.shares);
+        per = (int)((int64_t)per * (block.share + 1) / K.shares) - first;
     }
     const int tiles = (int)uniform((uint32_t)(per * A.group));
 
@@ -719,7 +719,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
     if (kBuffers == 2) done.wait(tiles + 1);
     bool nan = BIAS && live && bias.far;
     const int64_t at = (((int64_t)t.row + r) * A.a.kv_heads + hk) * A.a.dim;
-    float* sums = shared ? sink_sums(A, partial, t.cloud, j, hk, shares, block.share) : nullptr;
+    float* sums = shared ? share_sums(A, partial, block.tile, r, hk, K.shares, block.share) : nullptr;
 #pragma unroll
     for (int which = 0; which < 2; ++which)
 #pragma unroll
@@ -788,12 +788,12 @@ int run_kv(const AttnArgs& A, const TcMaps& M, float* partial, cudaStream_t s) {
     const size_t bytes = GradKvShape<DP>::bytes(entries, ONE);
     int st = tc_prepare<&attn_tc_grad_kv_kernel<T, DP, BIAS, ONE>>("attn_tc_grad_kv_kernel");
     if (st != kOk) return st;
-    const int shares = sink_shares(A), divided = sink_divided(A, shares);
-    const dim3 grid((unsigned)(A.a.k_tile_count + divided * (shares - 1)), (unsigned)A.a.kv_heads);
-    attn_tc_grad_kv_kernel<T, DP, BIAS, ONE><<<grid, GradKvShape<DP>::kThreads, bytes, s>>>(A, M, divided, shares, partial);
+    const KeyShares K = key_shares(A);
+    const dim3 grid((unsigned)key_blocks(A, K), (unsigned)A.a.kv_heads);
+    attn_tc_grad_kv_kernel<T, DP, BIAS, ONE><<<grid, GradKvShape<DP>::kThreads, bytes, s>>>(A, M, K, partial);
     st = check_launch("attn_tc_grad_kv_kernel");
-    if (st != kOk || shares == 1) return st;
-    return join_sinks<T>(A, divided, shares, partial, s);
+    if (st != kOk || K.shares == 1) return st;
+    return join_shares<T>(A, K, partial, s);
 }
 template <typename T, int DP, int BIAS>
 int run(const AttnArgs& A, cudaStream_t s) {
@@ -803,7 +803,7 @@ int run(const AttnArgs& A, cudaStream_t s) {
     if (st != kOk) return st;
     if (A.a.q_tile_count) {
         if constexpr (BIAS != 0) {
-            float* partial = reinterpret_cast<float*>(static_cast<unsigned char*>(A.a.workspace) + sink_bytes(A));
+            float* partial = reinterpret_cast<float*>(static_cast<unsigned char*>(A.a.workspace) + share_bytes(A));
             if (A.a.grad_table) {
                 st = run_q<T, DP, BIAS, kDelta>(A, M, nullptr, s);
                 if (st == kOk) st = run_q<T, DP, BIAS, kGradQTable>(A, M, partial, s);
