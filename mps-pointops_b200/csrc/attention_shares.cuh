@@ -80,16 +80,18 @@ int join_shares(const AttnArgs& A, const KeyShares& K, const float* partial, cud
 // sinks would outlast all others (5 times the kernel's time on clouds of 4096 points
 // and a window of 512).  All tiles: where there are fewer blocks than half of the SMs,
 // as many as fill them, of 64 queries or more (undivided against divided and joined, us:
-// float32, clouds of 304, 200 and 100 points, 4 heads of 128 over 1: 446, 191; 700 and 300
-// points, 8 heads of 64 over 2, window 400: 619, 180; bf16, 1024 and 900 points, 8 over 2:
+// float32, clouds of 304, 200 and 100 points, 4 heads of 128 over 1: 446, 71; 700 and 300
+// points, 8 heads of 64 over 2, window 400: 619, 169; bf16, 1024 and 900 points, 8 over 2:
 // 61, 26; 2048 points, 16 heads of 128 over 4, causal: 119, 80; one cloud of 1024 points, 4
-// heads of 32, window 256: 10.5, 10.6).
+// heads of 32, window 256: 10.5, 10.6).  float32 divides the query heads of a key head too;
+// with 16-bit types that gave the first of these cases 23 against 20 us and took the
+// registers of the table's kernel (987 against 897 us at 8 x 8192 points).
 inline KeyShares key_shares(const AttnArgs& A) {
     const int64_t rows = A.a.max_rows, window = (int64_t)A.left + A.right + kAttnTile;
     const int64_t blocks = (int64_t)A.a.k_tile_count * A.a.kv_heads * (A.a.dtype == MPO_F32 ? 2 : 1);
     KeyShares K = {0, 0, 1};
     if (2 * blocks <= sm_count()) {
-        const int64_t seen = A.a.sinks ? rows : min64(rows, window);
+        const int64_t seen = (A.a.dtype == MPO_F32 ? A.group : 1) * (A.a.sinks ? rows : min64(rows, window));
         K.shares = (int)max64(1, min64(seen / 64, sm_count() / max64(blocks, 1)));
         if (K.shares > 1) {
             K.tiles = (int)A.a.k_tile_count;

@@ -460,15 +460,18 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __gri
         for (int e = 0; e < W; ++e) dk[i][e] = dv[i][e] = 0.f;
     int lo, hi;
     query_span(A, H.p0, H.p0 + H.rows - 1, H.t.lq, H.t.lk, lo, hi);
+    // `count` tiles of queries for each query head in turn, of which this block takes its share.
+    const int count = hi > lo ? (hi - lo + kTR - 1) / kTR : 0;
+    int begin = 0, end = count * A.group;
     if (shared) {
-        const int n = max(0, hi - lo), base = lo;
-        lo = base + (int)((int64_t)n * block.share / K.shares);
-        hi = base + (int)((int64_t)n * (block.share + 1) / K.shares);
+        begin = (int)((int64_t)count * A.group * block.share / K.shares);
+        end = (int)((int64_t)count * A.group * (block.share + 1) / K.shares);
     }
-    for (int h = hk * A.group; h < (hk + 1) * A.group; ++h) {
+    for (int h = hk * A.group; h < (hk + 1) * A.group; ++h, begin -= count, end -= count) {
+        if (begin >= count || end <= 0) continue;
         __syncthreads();
         if (A.a.table) load_bias(A, S, h);
-        for (int i0 = lo; i0 < hi; i0 += kTR) {
+        for (int i0 = lo + max(begin, 0) * kTR; i0 < min(hi, lo + end * kTR); i0 += kTR) {
             const int n = min(kTR, hi - i0);
             const int64_t qr = (int64_t)H.t.other + i0;
             __syncthreads();

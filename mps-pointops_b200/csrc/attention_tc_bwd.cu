@@ -17,8 +17,8 @@
 // keys and values 900 us, D alone 738 us, dq and the table 1616 us (880 of them its
 // cells: shared memory at 59 % and the issue slots at 57 % of their peaks bind).
 // Without a table, 5 ragged clouds of up to 4099 points, 16 heads of 128 over 4:
-// keys and values 288 us, queries 285 us, tensor cores busy 39 % of the former (59 %
-// counting what they stall); latency at one block per SM binds.
+// keys and values 288 us, queries 285 us, tensor cores at 39 % of their rate in the
+// former; latency at one block per SM binds.
 #include <string>
 
 #include "attention_shares.cuh"

@@ -15,9 +15,9 @@
 // exponentials behind it (60 % of their unit): 131 us for 8 clouds of 4096
 // points, 8 heads of 64, window 1024 (490 TFLOP/s; the products alone 38 us, the
 // exponentials 56).  With a table its look-ups bind, 45 % of shared memory and of
-// the issue slots at once: 728 us for 8 x 8192.  At 128 elements one block per SM
-// holds two buffers of S (183 us with one, 159 with two: 5 ragged clouds of up to
-// 4099 points, 16 heads over 4, window 1024).
+// the issue slots at once: 728 us for 8 x 8192.  At 128 elements two buffers of S hide
+// more of the latency: 183 us with one, 159 with two (5 ragged clouds of up to 4099
+// points, 16 heads over 4, window 1024, causal).
 #include <string>
 
 #include "attention_exact.cuh"
