@@ -329,29 +329,31 @@ def _status(device: torch.device) -> int:
 class _Options:
     """What a call of ``window_attention`` fixes besides its tensors."""
 
-    __slots__ = ("segments", "left", "right", "sinks", "causal", "scale", "qpos", "kpos", "map",
-                 "reach", "train", "want_lse")
+    __slots__ = ("segments", "left", "right", "sinks", "causal", "scale", "reach", "train",
+                 "want_lse")
 
 
 _pack_attention = N.packer(N.AttentionArgs)
 
 
-def _attention_call(backward: bool, o: _Options, q, k, v, table, out, lse, grad=None,
+def _attention_call(backward: bool, o: _Options, q, k, v, bias, out, lse, grad=None,
                     delta=None, dq=None, dk=None, dv=None, dtable=None) -> None:
+    """``bias``: the table, the positions of queries and keys and the bucket map (or None)."""
     seg, device = o.segments, q.device
-    bias = (0,) * 4 if table is None else (_DTYPES[table.dtype], table.shape[0], table.shape[1],
-                                           o.reach)
+    table, qpos, kpos, mapping = bias
+    shape = (0,) * 4 if table is None else (_DTYPES[table.dtype], table.shape[0], table.shape[1],
+                                            o.reach)
 
     def pack(ws, nbytes):
         return _pack_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0),
             k.stride(1), v.stride(0), v.stride(1), out.data_ptr(), _address(lse),
             _address(grad), _address(delta), _address(dq), _address(dk),
-            _address(dv), _address(table), _address(dtable), _address(o.qpos), _address(o.kpos),
-            _address(o.map), seg.query_tiles.data_ptr(), seg.key_tiles.data_ptr(),
+            _address(dv), _address(table), _address(dtable), _address(qpos), _address(kpos),
+            _address(mapping), seg.query_tiles.data_ptr(), seg.key_tiles.data_ptr(),
             _status(device), seg.query_tiles.shape[0], seg.key_tiles.shape[0], q.shape[0],
             k.shape[0], _address(ws), nbytes, q.shape[1], k.shape[1], q.shape[2],
-            _DTYPES[q.dtype], *bias, o.left, o.right, o.sinks, o.causal, seg.max_rows,
+            _DTYPES[q.dtype], *shape, o.left, o.right, o.sinks, o.causal, seg.max_rows,
             seg.max_keys, seg.clouds, o.scale, int(backward))
 
     with N.on_device(device):
@@ -368,23 +370,25 @@ def _attention_call(backward: bool, o: _Options, q, k, v, table, out, lse, grad=
         N.check(call(args, stream), "window_attention backward" if backward else "window_attention")
 
 
-def _forward(q, k, v, table, o: _Options):
+def _forward(q, k, v, bias, o: _Options):
     device = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=device)
     lse = None
     if o.train or o.want_lse:
         lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=device)
-    _attention_call(False, o, q, k, v, table, out, lse)
+    _attention_call(False, o, q, k, v, bias, out, lse)
     return out, lse
 
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, o: _Options):
+    def forward(ctx, q, k, v, o: _Options, *bias):
         vec = 16 // q.element_size()
         q, k, v = _rows(q, vec), _rows(k, vec), _rows(v, vec)
-        out, lse = _forward(q, k, v, table, o)
-        ctx.save_for_backward(q, k, v, table, out, lse)
+        out, lse = _forward(q, k, v, bias, o)
+        # Positions and map among them: the backward forms the bias again, and autograd
+        # refuses it if the caller has changed them since.
+        ctx.save_for_backward(q, k, v, out, lse, *bias)
         ctx.options = o
         ctx.mark_non_differentiable(lse)
         return out, lse
@@ -392,8 +396,8 @@ class _WindowAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, _):
-        q, k, v, table, out, lse = ctx.saved_tensors
-        o = ctx.options
+        q, k, v, out, lse, *bias = ctx.saved_tensors
+        o, table = ctx.options, bias[0]
         device = q.device
         grad = _dense(grad)
         dq = torch.empty(q.shape, dtype=q.dtype, device=device)
@@ -401,12 +405,12 @@ class _WindowAttention(torch.autograd.Function):
         dv = torch.empty(v.shape, dtype=v.dtype, device=device)
         delta = torch.empty_like(lse)
         dtable = None
-        if table is not None and ctx.needs_input_grad[3]:
+        if table is not None and ctx.needs_input_grad[4]:
             dtable = torch.empty(table.shape, dtype=torch.float32, device=device)
-        _attention_call(True, o, q, k, v, table, out, lse, grad, delta, dq, dk, dv, dtable)
+        _attention_call(True, o, q, k, v, bias, out, lse, grad, delta, dq, dk, dv, dtable)
         if dtable is not None:
             dtable = dtable.to(table.dtype)
-        return dq, dk, dv, dtable, None
+        return dq, dk, dv, None, dtable, None, None, None
 
 
 def _limit(value, name: str) -> int:
@@ -485,7 +489,6 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, segments: Segments | Tenso
     if segments.device != q.device:
         raise ValueError(f"segments must be on {q.device}")
     o.segments = segments
-    o.qpos = o.kpos = o.map = None
     o.reach = 0
     if bias_table is None:
         if position is not None or key_position is not None or buckets is not None:
@@ -510,29 +513,29 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, segments: Segments | Tenso
         if span % 2 == 0 or span > 2 * _MAX_REACH + 1:
             raise ValueError("an axis must span 2 R + 1 differences, R at most 1024")
         o.reach = span // 2
-        o.qpos = _positions(position, q.shape[0], axes, q, "position")
+        qpos = _positions(position, q.shape[0], axes, q, "position")
         if key_position is None:
             if q.shape[0] != k.shape[0]:
                 raise ValueError("key_position is needed where keys are not the queries' rows")
-            o.kpos = o.qpos
+            kpos = qpos
         else:
-            o.kpos = _positions(key_position, k.shape[0], axes, q, "key_position")
+            kpos = _positions(key_position, k.shape[0], axes, q, "key_position")
     N.require_cuda(q, "attention.window_attention")
+    bias = (None,) * 4
     if bias_table is not None:
-        same = o.kpos is o.qpos
-        o.qpos = o.qpos.to(torch.int32).contiguous()
-        o.kpos = o.qpos if same else o.kpos.to(torch.int32).contiguous()
-        o.map = None if buckets is None else buckets.contiguous()
-        bias_table = bias_table.contiguous()
+        same = kpos is qpos
+        qpos = qpos.to(torch.int32).contiguous()
+        kpos = qpos if same else kpos.to(torch.int32).contiguous()
+        bias = (bias_table.contiguous(), qpos, kpos, None if buckets is None else buckets.contiguous())
     grad = torch.is_grad_enabled()
     o.train = grad and (q.requires_grad or k.requires_grad or v.requires_grad or
                         (bias_table is not None and bias_table.requires_grad))
     o.want_lse = bool(return_lse)
     if o.train:
-        out, lse = _WindowAttention.apply(q, k, v, bias_table, o)
+        out, lse = _WindowAttention.apply(q, k, v, o, *bias)
     else:
         vec = 16 // q.element_size()
-        out, lse = _forward(_rows(q, vec), _rows(k, vec), _rows(v, vec), bias_table, o)
+        out, lse = _forward(_rows(q, vec), _rows(k, vec), _rows(v, vec), bias, o)
     return (out, lse) if return_lse else out
 
 

@@ -245,3 +245,36 @@ def test_entry_addresses_of_the_tensor_core_kernels():
                 address = np.rint(t.astype(np.float64) * (256 * reach) + first)
                 want = first + 128 * (np.clip(column - row, -reach, reach) + reach)
                 assert (address == want).all(), (reach, row)
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    """The native calls replaced by ones that note their arguments and leave zeros, so
+    that what the Python side does runs on CPU tensors."""
+    calls = []
+
+    def attention_call(backward, *args):
+        calls.append((backward, args))
+        for x in args[-4:] if backward else args[-2:]:  # dq, dk, dv, dtable; out, lse
+            if x is not None:
+                x.zero_()
+
+    monkeypatch.setattr(N, "require_cuda", lambda t, what: None)
+    monkeypatch.setattr(attention, "_attention_call", attention_call)
+    return calls
+
+
+@pytest.mark.parametrize("which", ["position", "key_position", "buckets"])
+def test_positions_changed_before_the_backward_are_refused(recorder, which):
+    """The backward forms the bias again: a position or map that the caller has
+    refilled since the forward is an error, as it is for every other saved input."""
+    q, k, v = (x.requires_grad_() for x in qkv())
+    kw = dict(position=torch.zeros(10, 1, dtype=torch.int32),
+              key_position=torch.zeros(10, 1, dtype=torch.int32),
+              buckets=torch.zeros(9, dtype=torch.int32))
+    out = call(q, k, v, bias_table=torch.zeros(1, 5, 4), **kw)
+    out.sum().backward(retain_graph=True)
+    assert [backward for backward, _ in recorder] == [False, True]
+    kw[which].fill_(3)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
