@@ -539,6 +539,10 @@ MPO_API int mpo_allreduce_sum_f32_p2p(const float* value, float scale, float* ou
 #define MPO_F32 0
 #define MPO_F16 1
 #define MPO_BF16 2
+/* Types of the positions that rotate (mpo_rotate.position_float). */
+#define MPO_POSITION_I32 0
+#define MPO_POSITION_F32 1
+#define MPO_POSITION_I64 2
 
 /* Norms of queries and keys for each head, then the rotation by position.
  *   q (rows, heads, dim) and k (rows, kv_heads, dim) of `dtype`, innermost
@@ -548,9 +552,9 @@ MPO_API int mpo_allreduce_sum_f32_p2p(const float* value, float scale, float* ou
  *   (u, v) -> (u cos - v sin, u sin + v cos).  Pairs are (t, pairs + t), or
  *   (2t, 2t + 1) when interleaved.  dim is a multiple of 8 up to 256, pairs a
  *   multiple of 4 with 2 * pairs <= dim (0: no rotation).
- *   position (rows, axes <= 3) dense, int32 or (position_float) float32; freqs
- *   (axes, pairs) float32 or (freqs_double) float64; q_weight / k_weight (dim)
- *   float32, nullable (ones).
+ *   position (rows, axes <= 3) dense, its type by position_float (int32,
+ *   float32 or int64: MPO_POSITION_*); freqs (axes, pairs) float32 or
+ *   (freqs_double) float64; q_weight / k_weight (dim) float32, nullable (ones).
  * Theta is formed in the type of freqs, each product and sum rounded, axis 0
  * first (float32 frequencies: what elementary float32 operations give), and
  * reduced in double before its sine; the rest is float32, rounded once to the

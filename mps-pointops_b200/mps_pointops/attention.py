@@ -178,6 +178,7 @@ def _stream(device: torch.device) -> int:
 # ----------------------------------------------------------------------------- norm and rotation
 
 _pack_rotate = N.packer(N.RotateArgs)
+_POSITIONS = {torch.int32: 0, torch.float32: 1, torch.int64: 2}
 
 
 def _rotate_call(backward: bool, q, k, wq, wk, position, freqs, eps, interleaved, out_q, out_k,
@@ -191,7 +192,7 @@ def _rotate_call(backward: bool, q, k, wq, wk, position, freqs, eps, interleaved
             _address(wk), _address(grad_wq), _address(grad_wk), _address(position),
             _address(freqs), _address(ws), nbytes, q.shape[0], q.shape[1], k.shape[1], q.shape[2],
             0 if freqs is None else freqs.shape[1], 0 if freqs is None else freqs.shape[0],
-            int(position is not None and position.dtype == torch.float32), int(interleaved),
+            0 if position is None else _POSITIONS[position.dtype], int(interleaved),
             _DTYPES[q.dtype], eps,
             int(freqs is not None and freqs.dtype == torch.float64))
 
@@ -244,9 +245,9 @@ def norm_rotate(q: Tensor, k: Tensor, position: Tensor | None, freqs: Tensor | N
     Pair t of the first 2P elements of a head, (t, P + t) or with
     ``interleaved`` (2t, 2t + 1), turns by ``sum_a position[n, a] * freqs[a, t]``;
     elements beyond 2P are left as they are.  ``position`` is (N, A) or (N,),
-    integers or float32, A up to 3 (grid coordinates, say, or a row index);
-    ``freqs`` is (A, P), P a multiple of 4, float32 or float64: the angle is formed
-    in its type (float64 where positions are large).  Both None: no rotation.
+    int32, int64 or float32, A up to 3 (grid coordinates, say, or a row index);
+    ``freqs`` is (A, P), P a multiple of 4, float32 or float64: positions go to its
+    type and the angle is formed in it (float64 where positions are large).  Both None: no rotation.
     D is a multiple of 8 up to 256.  q and k may be strided views (of a packed
     projection); results are dense.  Gradients reach q, k and the weights, not
     the positions or frequencies.
@@ -274,8 +275,7 @@ def norm_rotate(q: Tensor, k: Tensor, position: Tensor | None, freqs: Tensor | N
             raise ValueError("freqs must have 1 to 3 axes")
         if pairs % 4 or 2 * pairs > dim:
             raise ValueError("freqs must have a multiple of 4 pairs, at most half of the head size")
-        if not isinstance(position, Tensor) or position.dtype not in (torch.int32, torch.int64,
-                                                                      torch.float32):
+        if not isinstance(position, Tensor) or position.dtype not in _POSITIONS:
             raise ValueError("position must be an int32, int64 or float32 tensor")
         if position.ndim == 1:
             position = position.unsqueeze(1)
@@ -294,10 +294,7 @@ def norm_rotate(q: Tensor, k: Tensor, position: Tensor | None, freqs: Tensor | N
         weights.append(w)
     N.require_cuda(q, "attention.norm_rotate")
     if freqs is not None:
-        position = position.detach()
-        if position.dtype == torch.int64:
-            position = position.to(torch.int32)
-        position, freqs = position.contiguous(), _dense(freqs.detach())
+        position, freqs = position.detach().contiguous(), _dense(freqs.detach())
         if freqs.shape[1] == 0:
             position = freqs = None
     args = (*weights, position, freqs, float(eps), bool(interleaved))

@@ -3,6 +3,7 @@ of a ragged batch, the bucket maps and the checks at the C entries."""
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import pytest
@@ -278,3 +279,38 @@ def test_positions_changed_before_the_backward_are_refused(recorder, which):
     kw[which].fill_(3)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.sum().backward()
+
+
+def test_long_positions_reach_the_kernel_whole(monkeypatch):
+    """int64 positions go to norm_rotate's kernel as they are, not cut to 32 bits."""
+    seen = {}
+
+    def pack(*values):
+        args = dict(zip((name for name, _ in N.RotateArgs._fields_), values))
+        kind = {0: ctypes.c_int32, 1: ctypes.c_float, 2: ctypes.c_int64}[args["position_float"]]
+        seen["position"] = list((kind * 10).from_address(args["position"]))
+        return b""
+
+    class Library:
+        def mpo_norm_rotate(self, args, stream):
+            return 0
+
+    monkeypatch.setattr(N, "require_cuda", lambda t, what: None)
+    monkeypatch.setattr(N, "lib", Library)
+    monkeypatch.setattr(N, "on_device", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(attention, "_pack_rotate", pack)
+    monkeypatch.setattr(attention, "_stream", lambda device: 0)
+    q, k, _ = qkv()
+    want = [(1 << 32) + 3, -(1 << 40), 7, *range(7)]
+    attention.norm_rotate(q, k, torch.tensor(want), torch.zeros(1, 16, dtype=torch.float64))
+    assert seen["position"] == want
+
+
+def test_c_entry_refuses_position_types_and_addresses():
+    lib = N.lib()
+    for bad, match in ((dict(position_float=3), "position type"), (dict(position_float=-1), "position type"),
+                       (dict(position_float=2, position=36), "aligned"), (dict(position=34), "aligned")):
+        args = dict(q=16, k=16, out_q=16, out_k=16, position=32, freqs=32, rows=3, heads=2, kv_heads=2, dim=32,
+                    pairs=8, axes=1)
+        r = N.RotateArgs(**{**args, **bad})
+        assert lib.mpo_norm_rotate(ctypes.byref(r), None) == 1 and match in N.last_error()

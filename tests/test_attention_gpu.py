@@ -580,3 +580,30 @@ def test_example_trains_and_serves(cuda_device):
     losses = example.train(20, cuda_device)
     assert losses[-1] < 0.8 * losses[0]
     assert example.cached_rows(cuda_device) <= 4 * 2 * 2 * 2.0 ** -8
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("angle", [torch.float32, torch.float64])
+@pytest.mark.parametrize("top", [1 << 30, 1 << 40])
+def test_norm_rotate_of_long_positions(cuda_device, dtype, angle, top):
+    """int64 positions past 32 bits.  The reference forms the angle as the kernel does, in
+    the frequencies' type; what is left is the reduction to one turn (2^-53 of it and
+    float32's rounding of a half turn, 2^-24 pi) and the arithmetic of the other tests."""
+    g = torch.Generator().manual_seed(31)
+    n, D, P = 70, 32, 16
+    q, k, gq, gk = (rand(g, n, h, D, dtype=dtype).to(cuda_device) for h in (3, 1, 3, 1))
+    pos = torch.randint(-top, top, (n, 2), generator=g, dtype=torch.int64)
+    pos[0, 0], pos[1, 1] = (1 << 32) + 3, -(1 << 31) - 1
+    pos = pos.to(cuda_device)
+    freqs = torch.rand(2, P, generator=g).to(cuda_device, angle)
+    xs = [x.requires_grad_() for x in (q, k)]
+    ys = attention.norm_rotate(*xs, pos, freqs)
+    grads = torch.autograd.grad(ys, xs, (gq, gk))
+    for x, gr, y, dx in zip(xs, (gq, gk), ys, grads):
+        ry, rdx, _ = rotate_reference(x, None, pos, freqs, 1e-6, False, gr)
+        assert ((y.detach().cpu().double() - ry).abs() <= 1.02 * C.UNIT[dtype] * ry.abs()
+                + 2.0 ** -20 * ry.abs().amax(-1, keepdim=True)).all()
+        bound = 2 * gr.cpu().double().abs().amax(-1, keepdim=True) * \
+            x.detach().cpu().double().square().mean(-1, keepdim=True).add(1e-6).rsqrt()
+        assert ((dx.cpu().double() - rdx).abs() <= 1.02 * C.UNIT[dtype] * rdx.abs()
+                + 2.0 ** -18 * (rdx.abs().amax(-1, keepdim=True) + bound)).all()
