@@ -38,6 +38,7 @@ from . import _native as N
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _MAX_ENTRIES = 256
 _MAX_REACH = 1024
+_MAX_POSITION = (1 << 30) - 1
 
 
 def _ends(value: Tensor, name: str) -> list[int]:
@@ -428,6 +429,13 @@ def _positions(value: Tensor | None, rows: int, axes: int, like: Tensor, name: s
     return value
 
 
+def _int32(position: Tensor) -> Tensor:
+    """Dense int32 positions; int64 ones end at the kernels' limits."""
+    if position.dtype == torch.int64:
+        position = position.clamp(-_MAX_POSITION, _MAX_POSITION).to(torch.int32)
+    return position.contiguous()
+
+
 def window_attention(q: Tensor, k: Tensor, v: Tensor, segments: Segments | Tensor, *,
                      window: tuple[int, int] = (-1, -1), sinks: int = 0, causal: bool = False,
                      scale: float | None = None, bias_table: Tensor | None = None,
@@ -446,7 +454,8 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, segments: Segments | Tenso
     sees no key gets zeros.  Scores are ``scale * q.k`` (default 1 / sqrt(D)) plus
     the bias ``sum_a bias_table[a, bucket_a, h]``: ``position`` (N, A) and
     ``key_position`` (M, A; default ``position``) are integers below 2^30 in
-    magnitude, ``bias_table`` (A, buckets, H) is learned, and the bucket of an axis
+    magnitude (int64 ones beyond are taken as 2^30 - 1 of their sign; longer codes
+    need an origin of their own), ``bias_table`` (A, buckets, H) is learned, and the bucket of an axis
     is the difference key - query clamped to [-R, R], plus R, where
     ``buckets = 2 R + 1``; or, with the map ``buckets`` (2 R + 1,), what the map
     names there (``log_buckets``; names are clamped to the table).  A * buckets
@@ -521,8 +530,8 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, segments: Segments | Tenso
     bias = (None,) * 4
     if bias_table is not None:
         same = kpos is qpos
-        qpos = qpos.to(torch.int32).contiguous()
-        kpos = qpos if same else kpos.to(torch.int32).contiguous()
+        qpos = _int32(qpos)
+        kpos = qpos if same else _int32(kpos)
         bias = (bias_table.contiguous(), qpos, kpos, None if buckets is None else buckets.contiguous())
     grad = torch.is_grad_enabled()
     o.train = grad and (q.requires_grad or k.requires_grad or v.requires_grad or

@@ -314,3 +314,14 @@ def test_c_entry_refuses_position_types_and_addresses():
                     pairs=8, axes=1)
         r = N.RotateArgs(**{**args, **bad})
         assert lib.mpo_norm_rotate(ctypes.byref(r), None) == 1 and match in N.last_error()
+
+
+def test_long_positions_of_the_bias_clamp(recorder):
+    """int64 positions beyond the kernels' range end at its limits, they do not wrap."""
+    far = torch.tensor([0, 5, (1 << 32) + 3, -(1 << 32) - 3, (1 << 31), 1 << 62, -(1 << 63), (1 << 30) - 1, -7, 1])
+    call(*qkv(), bias_table=torch.zeros(1, 5, 4), position=far, key_position=far.flip(0))
+    top = (1 << 30) - 1
+    want = [0, 5, top, -top, top, top, -top, top, -7, 1]
+    _, (_, _, _, _, (_, qpos, kpos, _), *_) = recorder[0]
+    assert qpos.dtype == kpos.dtype == torch.int32
+    assert qpos[:, 0].tolist() == want and kpos[:, 0].tolist() == want[::-1]
