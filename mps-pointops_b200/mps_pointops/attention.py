@@ -31,6 +31,7 @@ import math
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
@@ -168,6 +169,15 @@ def _dense(x: Tensor | None) -> Tensor | None:
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
+def _tracked(*tensors: Tensor | None) -> bool:
+    """Whether a result has to know its inputs: some require gradients, or carry a
+    forward-mode tangent (which the autograd functions refuse).  Calls without go past
+    the functions, 7 to 10 us of host time each."""
+    grad = torch.is_grad_enabled()
+    return any(x is not None and ((grad and x.requires_grad) or
+                                  forward_ad.unpack_dual(x).tangent is not None) for x in tensors)
+
+
 def _address(x: Tensor | None) -> int:
     return 0 if x is None else x.data_ptr()
 
@@ -299,8 +309,7 @@ def norm_rotate(q: Tensor, k: Tensor, position: Tensor | None, freqs: Tensor | N
         if freqs.shape[1] == 0:
             position = freqs = None
     args = (*weights, position, freqs, float(eps), bool(interleaved))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or any(
-            w is not None and w.requires_grad for w in weights)):
+    if _tracked(q, k, *weights):
         return _NormRotate.apply(q, k, *args)
     return _rotate_forward(_rows(q, 4), _rows(k, 4), *args)
 
@@ -327,8 +336,7 @@ def _status(device: torch.device) -> int:
 class _Options:
     """What a call of ``window_attention`` fixes besides its tensors."""
 
-    __slots__ = ("segments", "left", "right", "sinks", "causal", "scale", "reach", "train",
-                 "want_lse")
+    __slots__ = ("segments", "left", "right", "sinks", "causal", "scale", "reach", "want_lse")
 
 
 _pack_attention = N.packer(N.AttentionArgs)
@@ -369,11 +377,9 @@ def _attention_call(backward: bool, o: _Options, q, k, v, bias, out, lse, grad=N
 
 
 def _forward(q, k, v, bias, o: _Options):
-    device = q.device
-    out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    lse = None
-    if o.train or o.want_lse:
-        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=device)
+    out, lse = torch.empty(q.shape, dtype=q.dtype, device=q.device), None
+    if o.want_lse:
+        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
     _attention_call(False, o, q, k, v, bias, out, lse)
     return out, lse
 
@@ -533,11 +539,9 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, segments: Segments | Tenso
         qpos = _int32(qpos)
         kpos = qpos if same else _int32(kpos)
         bias = (bias_table.contiguous(), qpos, kpos, None if buckets is None else buckets.contiguous())
-    grad = torch.is_grad_enabled()
-    o.train = grad and (q.requires_grad or k.requires_grad or v.requires_grad or
-                        (bias_table is not None and bias_table.requires_grad))
-    o.want_lse = bool(return_lse)
-    if o.train:
+    tracked = _tracked(q, k, v, bias_table)
+    o.want_lse = bool(return_lse) or tracked
+    if tracked:
         out, lse = _WindowAttention.apply(q, k, v, o, *bias)
     else:
         vec = 16 // q.element_size()

@@ -8,6 +8,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from mps_pointops import _native as N
 from mps_pointops import attention
@@ -325,3 +326,42 @@ def test_long_positions_of_the_bias_clamp(recorder):
     _, (_, _, _, _, (_, qpos, kpos, _), *_) = recorder[0]
     assert qpos.dtype == kpos.dtype == torch.int32
     assert qpos[:, 0].tolist() == want and kpos[:, 0].tolist() == want[::-1]
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_are_refused(recorder, monkeypatch, grad):
+    """No forward-mode formula: a tangent is an error, not lost, where no input requires
+    a gradient and where gradients are off."""
+    def rotate_call(backward, q, k, wq, wk, position, freqs, eps, interleaved, out_q, out_k, *_):
+        out_q.zero_()
+        out_k.zero_()
+
+    monkeypatch.setattr(attention, "_rotate_call", rotate_call)
+    q, k, v = qkv()
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        dual = forward_ad.make_dual(k, torch.ones_like(k))
+        with pytest.raises(RuntimeError, match="forward mode AD"):
+            call(q, dual, v)
+        with pytest.raises(RuntimeError, match="forward mode AD"):
+            attention.norm_rotate(q, dual, None, None)
+        weight = forward_ad.make_dual(torch.ones(32), torch.ones(32))
+        with pytest.raises(RuntimeError, match="forward mode AD"):
+            attention.norm_rotate(q, k, None, None, k_weight=weight)
+        table = forward_ad.make_dual(torch.zeros(1, 5, 4), torch.ones(1, 5, 4))
+        with pytest.raises(RuntimeError, match="forward mode AD"):
+            call(q, k, v, bias_table=table, position=torch.zeros(10, dtype=torch.int32))
+
+
+def test_calls_without_gradients_keep_nothing(recorder):
+    q, k, v = qkv()
+    out = call(q, k, v)
+    assert out.grad_fn is None and not out.requires_grad
+    out, lse = call(q, k, v, return_lse=True)
+    assert lse.shape == (4, 10) and lse.grad_fn is None
+    q.requires_grad_()
+    with torch.no_grad():
+        out = call(q, k, v)
+    assert out.grad_fn is None
+    with torch.inference_mode():
+        assert call(q, k, v).is_inference()
+    assert [args[6] is None for _, args in recorder] == [True, False, True, True]  # lse only where it is used
