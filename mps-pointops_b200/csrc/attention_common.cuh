@@ -16,6 +16,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+#include <string>
 #include <type_traits>
 
 #include "../../include/mpo_b200.h"
@@ -28,6 +30,7 @@ constexpr int kAttnMaxDim = 128;
 constexpr int kAttnMaxAxes = 3;
 constexpr int kAttnMaxEntries = 256;  // axes x buckets of a bias table
 constexpr int kAttnMaxMap = 2049;     // 2 R + 1 of a bucket map
+constexpr size_t kAttnSmem = 232448;  // shared memory of a block at most
 
 // One planned tile: `rows` consecutive rows of one cloud on the owning side.
 struct AttnTile {
@@ -202,6 +205,19 @@ __device__ __forceinline__ float table_entry(const mpo_attention& a, int e, int 
 }
 
 // ---------------------------------------------------------------- launchers
+// Lets a kernel take all of an SM's shared memory, once per device: a limit of
+// each call's own size would be lowered by other host threads before the launch.
+template <auto Kernel>
+int attn_prepare(const char* what) {
+    static std::atomic<uint64_t> prepared{0};
+    const uint64_t bit = 1ull << (current_device() & 63);
+    if (prepared.load(std::memory_order_acquire) & bit) return kOk;
+    if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kAttnSmem) != cudaSuccess)
+        return fail(kCudaError, std::string(what) + ": cannot reserve shared memory");
+    prepared.fetch_or(bit, std::memory_order_release);
+    return kOk;
+}
+
 // attention_tc_fwd.cu, attention_tc_bwd.cu: 16-bit types on the tensor cores.
 int attn_tc_forward(const AttnArgs& A, cudaStream_t s);
 int attn_tc_backward(const AttnArgs& A, cudaStream_t s);

@@ -548,17 +548,10 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __gri
 }
 
 // ---------------------------------------------------------------- launches
-template <typename K>
-int prepare(K kernel, size_t bytes, const char* what) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) !=
-        cudaSuccess)
-        return fail(kCudaError, std::string(what) + ": cannot reserve shared memory");
-    return kOk;
-}
 template <typename T, int DP>
 int run_fwd(const AttnArgs& A, cudaStream_t s) {
     const size_t bytes = SimtSmem::bytes(DP, 3, 0);
-    const int st = prepare(attn_simt_fwd_kernel<T, DP>, bytes, "attn_simt_fwd_kernel");
+    const int st = attn_prepare<&attn_simt_fwd_kernel<T, DP>>("attn_simt_fwd_kernel");
     if (st != kOk) return st;
     const dim3 grid((unsigned)(2 * A.a.q_tile_count), (unsigned)A.a.heads);
     attn_simt_fwd_kernel<T, DP><<<grid, kThreads, bytes, s>>>(A);
@@ -573,8 +566,8 @@ int run_bwd(const AttnArgs& A, cudaStream_t s) {
                                     : nullptr;
     const size_t qb = SimtSmem::bytes(DP, 4, partial ? entries : 0);
     const size_t kb = SimtSmem::bytes(DP, 4, 0);
-    int st = prepare(attn_simt_grad_q_kernel<T, DP>, qb, "attn_simt_grad_q_kernel");
-    if (st == kOk) st = prepare(attn_simt_grad_kv_kernel<T, DP>, kb, "attn_simt_grad_kv_kernel");
+    int st = attn_prepare<&attn_simt_grad_q_kernel<T, DP>>("attn_simt_grad_q_kernel");
+    if (st == kOk) st = attn_prepare<&attn_simt_grad_kv_kernel<T, DP>>("attn_simt_grad_kv_kernel");
     if (st != kOk) return st;
     if (A.a.q_tile_count) {
         const dim3 grid((unsigned)(2 * A.a.q_tile_count), (unsigned)A.a.heads);

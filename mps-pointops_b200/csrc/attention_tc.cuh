@@ -14,7 +14,6 @@
 
 #include <cuda.h>
 
-#include <atomic>
 #include <string>
 
 #include "attention_common.cuh"
@@ -25,7 +24,6 @@ namespace {
 constexpr int kTcRows = 128;  // rows of a tile: TMEM lanes, one thread (per column group) each
 constexpr int kTcCols = 64;   // columns of a score tile
 constexpr unsigned long long kTcWaitNs = 2000000000ull;
-constexpr size_t kTcSmem = 232448;  // shared memory of a block at most
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return (uint32_t)__cvta_generic_to_shared(p);
@@ -472,17 +470,6 @@ int make_maps(TcMaps& M, const AttnArgs& A, bool backward) {
 template <int THREADS>
 __device__ __forceinline__ void compute_sync() {
     asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
-}
-// Lets a kernel take all of an SM's shared memory, once per device.
-template <auto Kernel>
-int tc_prepare(const char* what) {
-    static std::atomic<uint64_t> prepared{0};
-    const uint64_t bit = 1ull << (current_device() & 63);
-    if (prepared.load(std::memory_order_acquire) & bit) return kOk;
-    if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTcSmem) != cudaSuccess)
-        return fail(kCudaError, std::string(what) + ": cannot reserve shared memory");
-    prepared.fetch_or(bit, std::memory_order_release);
-    return kOk;
 }
 
 }  // namespace

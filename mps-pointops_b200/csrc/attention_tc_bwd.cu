@@ -92,7 +92,7 @@ struct QueryShape {
         return need > least ? need : least;
     }
     // One copy of the table where a copy per lane does not fit beside the cells.
-    static bool one_copy(int axes, int entries) { return kTight || bytes(axes, entries, false) > kTcSmem; }
+    static bool one_copy(int axes, int entries) { return kTight || bytes(axes, entries, false) > kAttnSmem; }
 };
 
 template <typename T, int DP, int BIAS, int MODE, bool ONE>
@@ -485,7 +485,7 @@ struct GradKvShape {
                               kBar = kPos + kRowStages * 3 * kTcCols * 4, kTable = kBar + 128;
     // Barriers: products (2); stages of queries and gradients (4), K and V; then TMEM's address, row flags.
     static constexpr uint32_t kFull = kBar + 16, kFullK = kBar + 48, kSlot = kBar + 56, kFlags = kBar + 64;
-    static bool one_copy(int entries) { return kTable + (size_t)entries * 128 + 1024 > kTcSmem; }
+    static bool one_copy(int entries) { return kTable + (size_t)entries * 128 + 1024 > kAttnSmem; }
     static size_t bytes(int entries, bool one) {
         const size_t need = kTable + (size_t)entries * (one ? 4 : 128) + 1024;
         const size_t least = 233472 / (kBlocks + 1);  // no more blocks than TMEM serves
@@ -773,7 +773,7 @@ int run_q(const AttnArgs& A, const TcMaps& M, float* partial, cudaStream_t s) {
         if (!ONE && Shape::one_copy(axes, entries)) return run_q<T, DP, BIAS, MODE, true>(A, M, partial, s);
     }
     const size_t bytes = Shape::bytes(axes, entries, ONE);
-    const int st = tc_prepare<&attn_tc_query_kernel<T, DP, BIAS, MODE, ONE>>("attn_tc_query_kernel");
+    const int st = attn_prepare<&attn_tc_query_kernel<T, DP, BIAS, MODE, ONE>>("attn_tc_query_kernel");
     if (st != kOk) return st;
     const dim3 grid((unsigned)A.a.q_tile_count, (unsigned)A.a.heads);
     attn_tc_query_kernel<T, DP, BIAS, MODE, ONE><<<grid, Shape::kThreads, bytes, s>>>(A, M, partial);
@@ -786,7 +786,7 @@ int run_kv(const AttnArgs& A, const TcMaps& M, float* partial, cudaStream_t s) {
         if (!ONE && GradKvShape<DP>::one_copy(entries)) return run_kv<T, DP, BIAS, true>(A, M, partial, s);
     }
     const size_t bytes = GradKvShape<DP>::bytes(entries, ONE);
-    int st = tc_prepare<&attn_tc_grad_kv_kernel<T, DP, BIAS, ONE>>("attn_tc_grad_kv_kernel");
+    int st = attn_prepare<&attn_tc_grad_kv_kernel<T, DP, BIAS, ONE>>("attn_tc_grad_kv_kernel");
     if (st != kOk) return st;
     const KeyShares K = key_shares(A);
     const dim3 grid((unsigned)key_blocks(A, K), (unsigned)A.a.kv_heads);

@@ -318,7 +318,7 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
 template <typename T, int DP, int BIAS>
 int run(const AttnArgs& A, cudaStream_t s) {
     const size_t bytes = FwdShape<DP>::bytes(BIAS ? A.a.axes * A.a.buckets : 0);
-    const int st = tc_prepare<&attn_tc_fwd_kernel<T, DP, BIAS>>("attn_tc_fwd_kernel");
+    const int st = attn_prepare<&attn_tc_fwd_kernel<T, DP, BIAS>>("attn_tc_fwd_kernel");
     if (st != kOk) return st;
     TcMaps maps = {};
     const int mapped = make_maps<DP>(maps, A, false);

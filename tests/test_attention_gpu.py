@@ -607,3 +607,64 @@ def test_norm_rotate_of_long_positions(cuda_device, dtype, angle, top):
             x.detach().cpu().double().square().mean(-1, keepdim=True).add(1e-6).rsqrt()
         assert ((dx.cpu().double() - rdx).abs() <= 1.02 * C.UNIT[dtype] * rdx.abs()
                 + 2.0 ** -18 * (rdx.abs().amax(-1, keepdim=True) + bound)).all()
+
+
+def test_two_host_threads(cuda_device, monkeypatch):
+    """Float32 backward calls that need different amounts of shared memory, from two host
+    threads: neither lowers the other's limit."""
+    import threading
+
+    g = torch.Generator().manual_seed(41)
+    n, H, D = 140, 2, 128
+    blocks, kept, errors = [], [], []
+    pack, workspace = attention._pack_attention, N.workspace
+
+    def note(*values):
+        blocks.append(pack(*values))
+        return blocks[-1]
+
+    def keep(nbytes, device):
+        kept.append(workspace(nbytes, device))
+        return kept[-1]
+
+    def prepare(biased):
+        """Results, and a call at the C entry that forms them again."""
+        q, k, v, grad = (rand(g, n, H, D).to(cuda_device) for _ in range(4))
+        leaves = [x.requires_grad_() for x in (q, k, v)]
+        kw = {}
+        if biased:
+            leaves.append(rand(g, 3, 85, H).to(cuda_device).requires_grad_())
+            kw = dict(bias_table=leaves[3], position=torch.randint(0, 99, (n, 3), generator=g).int().to(cuda_device))
+        seg = attention.Segments(ends([n], cuda_device))
+        out, lse = attention.window_attention(*leaves[:3], seg, return_lse=True, **kw)
+        want = torch.autograd.grad(out, leaves, grad, retain_graph=True)
+        o, saved = out.grad_fn.options, out.grad_fn.saved_tensors
+        results, delta = [torch.empty_like(x) for x in want], torch.empty_like(lse)
+        with monkeypatch.context() as m:
+            m.setattr(attention, "_pack_attention", note)
+            m.setattr(N, "workspace", keep)
+            attention._attention_call(True, o, *saved[:3], saved[5:], *saved[3:5], grad, delta,
+                                      *results, *(() if biased else (None,)))
+        kept.extend((out, saved, grad, delta, seg))
+        return want, results, blocks[-1]
+
+    def loop(stream, block):
+        call = N.lib().mpo_window_attention_backward
+        for _ in range(3000):
+            if call(block, stream):
+                errors.append(N.last_error())
+                return
+
+    cases = [prepare(True), prepare(False)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    threads = [threading.Thread(target=loop, args=(s.cuda_stream, block)) for s, (_, _, block) in zip(streams, cases)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for want, results, _ in cases:
+        for a, b in zip(results, want):
+            assert torch.equal(a, b)
