@@ -455,7 +455,7 @@ attn_rows_f32_kernel(const __grid_constant__ AttnArgs A, int units, int splits, 
 // ---------------------------------------------------------------- join
 // A warp per (query row, head): the splits' rows by their maxima and sums.
 template <typename T>
-__global__ void __launch_bounds__(kRowsThreads)
+__global__ void __launch_bounds__(kRowsThreads, 4)
 attn_rows_join_kernel(const __grid_constant__ AttnArgs A, int splits, const float* __restrict__ partial) {
     const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.q_tiles)[blockIdx.x];
     const int lane = threadIdx.x & 31, h = blockIdx.y * kRowsWarps + (threadIdx.x >> 5);

@@ -38,7 +38,7 @@ __device__ __forceinline__ float* share_sums(const AttnArgs& A, float* partial, 
 // grad_k and grad_v of the tiles that are divided: the shares' sums in order.  A
 // warp per key row.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 3)
 attn_join_shares_kernel(const __grid_constant__ AttnArgs A, const KeyShares K, const float* __restrict__ partial) {
     const AttnTile t = reinterpret_cast<const AttnTile*>(A.a.k_tiles)[blockIdx.x];
     if (t.first >= K.limit) return;

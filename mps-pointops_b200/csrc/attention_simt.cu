@@ -436,8 +436,11 @@ __global__ void __launch_bounds__(kThreads) attn_simt_grad_q_kernel(const __grid
 }
 
 // ---------------------------------------------------------------- backward: keys and values
+// Three blocks per SM up to 32 elements: at two (234 registers) the time was 270 us or,
+// in some runs, 457, against 287.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attn_simt_grad_kv_kernel(const __grid_constant__ AttnArgs A, const KeyShares K,
+__global__ void __launch_bounds__(kThreads, DP <= 32 ? 3 : 1)
+attn_simt_grad_kv_kernel(const __grid_constant__ AttnArgs A, const KeyShares K,
                          float* __restrict__ partial) {
     extern __shared__ __align__(16) unsigned char smem[];
     const SimtSmem S(smem, DP, 4);

@@ -451,12 +451,16 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
         const unsigned bad_here = __ballot_sync(FULL_MASK, nan), apart = __ballot_sync(FULL_MASK, far);
         if (lane == 0 && bad_here) atomicOr(flags + quarter, bad_here);
         compute_sync<Shape::kCompute>();
-        if (group == 0)
-            for (unsigned bad = flags[quarter]; bad; bad &= bad - 1) {
-                const int b = __ffs(bad) - 1, row = (r & ~31) + b;
-                exact_grad_q_row<T>(A, (int64_t)t.row + row, t.first + row, t.other, t.lk, h,
-                                    Shape::kCells && ((apart >> b) & 1u) ? cells : nullptr);
-            }
+        // The groups' warps take the quarter's rows in turn; those that add to its cells are the
+        // first group's.
+        int turn = 0;
+        for (unsigned bad = flags[quarter]; bad; bad &= bad - 1, ++turn) {
+            const int b = __ffs(bad) - 1, row = (r & ~31) + b;
+            const bool whole = (apart >> b) & 1u;
+            float* own_cells = Shape::kCells && whole ? cells : nullptr;
+            if ((own_cells ? 0 : turn % Shape::kGroups) != group) continue;
+            exact_grad_q_row<T>(A, (int64_t)t.row + row, t.first + row, t.other, t.lk, h, whole, own_cells);
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -756,8 +760,9 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
     const unsigned bad_here = __ballot_sync(FULL_MASK, nan);
     if (lane == 0 && bad_here) atomicOr(flags + quarter, bad_here);
     compute_sync<Shape::kCompute>();
-    if (!shared && group == 0)
-        for (unsigned bad = flags[quarter]; bad; bad &= bad - 1) {
+    int turn = 0;
+    for (unsigned bad = shared ? 0u : flags[quarter]; bad; bad &= bad - 1, ++turn)
+        if (turn % Shape::kGroups == group) {  // the groups' warps take the quarter's rows in turn
             const int row = (r & ~31) + __ffs(bad) - 1;
             exact_grad_kv_row<T>(A, t.base, t.first + row, t.other, t.lq, t.lk, hk);
         }

@@ -280,7 +280,8 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
     done.wait(tiles);
     if (kBuffers == 2) done.wait(tiles + 1);
     const bool live = tid < t.rows;
-    bool nan = BIAS && live && bias.far;
+    const bool far = BIAS && live && bias.far;
+    bool nan = far;
     const int64_t at = (((int64_t)t.row + tid) * A.a.heads + h) * A.a.dim;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
@@ -307,9 +308,10 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
         A.a.lse[(int64_t)h * A.a.q_rows + t.row + tid] =
             sum == 0.f ? -INFINITY : fmaf(top * mul, kLn2, logf(sum));
     __syncwarp();
+    const unsigned apart = __ballot_sync(FULL_MASK, far);
     for (unsigned bad = __ballot_sync(FULL_MASK, nan); bad; bad &= bad - 1) {
-        const int r = (tid & ~31) + __ffs(bad) - 1;
-        exact_forward_row<T>(A, (int64_t)t.row + r, t.first + r, t.other, t.lk, h);
+        const int b = __ffs(bad) - 1, r = (tid & ~31) + b;
+        exact_forward_row<T>(A, (int64_t)t.row + r, t.first + r, t.other, t.lk, h, (apart >> b) & 1u);
     }
     tc_fence_before();
     __syncthreads();

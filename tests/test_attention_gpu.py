@@ -668,3 +668,78 @@ def test_two_host_threads(cuda_device, monkeypatch):
     for want, results, _ in cases:
         for a, b in zip(results, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+@pytest.mark.parametrize("bias", [False, True])
+def test_gradients_that_are_not_finite(cuda_device, dtype, bias):
+    """What an overflow in the loss sends back reaches the results whose pairs hold it, element
+    by element, and no others; rows that are NaN throughout end early."""
+    g = torch.Generator().manual_seed(51)
+    lens, D, r, e = [1500, 260], 32, 700, 3
+    n = sum(lens)
+    q, k, v, grad = (rand(g, n, h, D, dtype=dtype).to(cuda_device) for h in (2, 1, 1, 2))
+    ref, kw = {}, {}
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    if bias:
+        pos = torch.randint(0, 40, (n, 1), generator=g, dtype=torch.int32)
+        pos[::50] = 1 << 20  # some rows far from the others of their tile
+        leaves.append(rand(g, 1, 15, 2).to(cuda_device).requires_grad_())
+        kw = dict(bias_table=leaves[3], position=pos.to(cuda_device))
+        ref = dict(table=leaves[3], qpos=pos, kpos=pos)
+    out = attention.window_attention(*leaves[:3], ends(lens, cuda_device), window=(100, 50), sinks=2, **kw)
+    want = C.attention(q, k, v, lens, lens, left=100, right=50, sinks=2, grad=grad, **ref)
+    seen = C.visible(lens[0], lens[0], 100, 50, 2, False)[r]  # keys of row r
+
+    def grads(value, rows, element):
+        bad = grad.clone()
+        bad[rows, :, element] = value
+        return [x.cpu().double() for x in torch.autograd.grad(out, leaves, bad, retain_graph=True)]
+
+    def close(got, name, keep):
+        value, bound = want[name]
+        assert ((got - value)[keep].abs() <= 1.02 * bound[keep] + 2.0 ** -24).all(), name
+
+    for got in grads(math.nan, slice(None), slice(None))[:3]:
+        assert torch.isnan(got).all()
+    # One NaN in the gradient of row r: all of dq there, dk of the keys it sees, one element of their dv.
+    dq, dk, dv, *dtable = grads(math.nan, r, e)
+    keep = torch.ones(n, dtype=torch.bool)
+    keep[r] = False
+    assert torch.isnan(dq[r]).all()
+    close(dq, "dq", keep)
+    keep = torch.ones(n, dtype=torch.bool)
+    keep[:lens[0]] = ~seen
+    assert torch.isnan(dk[~keep]).all() and torch.isnan(dv[~keep][..., e]).all()
+    close(dk, "dk", keep)
+    elements = keep[:, None, None].expand(n, 1, D).clone()
+    elements[..., :e] = elements[..., e + 1:] = True
+    close(dv, "dv", elements)
+    # An infinity in one element of all rows: that element of dv, of one sign; nothing else of dv.
+    *_, dv = grads(math.inf, slice(None), e)[:3]
+    assert (dv[..., e] == math.inf).all()
+    elements = torch.ones(n, 1, D, dtype=torch.bool)
+    elements[..., e] = False
+    close(dv, "dv", elements)
+
+
+@pytest.mark.parametrize("dtype,K,D", [(BF, 4, 64), (HF, 1, 128), (FP, 4, 32)])
+def test_gradients_that_are_all_nan_take_no_longer(cuda_device, dtype, K, D):
+    """A skipped step of loss scaling: 20 ms against 0.3 when every pair was gone through."""
+    g = torch.Generator().manual_seed(52)
+    n = 4096
+    leaves = [rand(g, n, h, D, dtype=dtype).to(cuda_device).requires_grad_() for h in (4, K, K)]
+    out = attention.window_attention(*leaves, ends([n], cuda_device), window=(256, 255))
+    grad = rand(g, n, 4, D, dtype=dtype).to(cuda_device)
+    times = []
+    for gr in (grad, torch.full_like(grad, math.nan)):
+        best = math.inf
+        for _ in range(4):
+            start, stop = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            torch.autograd.grad(out, leaves, gr, retain_graph=True)
+            stop.record()
+            stop.synchronize()
+            best = min(best, start.elapsed_time(stop))
+        times.append(best)
+    assert times[1] <= 10 * times[0], times
