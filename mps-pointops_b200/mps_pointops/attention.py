@@ -316,21 +316,46 @@ def norm_rotate(q: Tensor, k: Tensor, position: Tensor | None, freqs: Tensor | N
 
 # ----------------------------------------------------------------------------- attention
 
-_statuses: dict[int, tuple[Tensor, ctypes.c_int32]] = {}
+# (device index, stream) -> a word in pinned host memory, and the same as a ctypes integer.
+_statuses: dict[tuple[int, int], tuple[Tensor | None, ctypes.c_int32]] = {}
 
 
-def _status(device: torch.device) -> int:
-    """Address of the word that a kernel on ``device`` sets when a bounded wait runs
-    out; it lies in pinned host memory and is read here without waiting for the GPU."""
-    entry = _statuses.get(device.index)
+def _ran_out(word: ctypes.c_int32) -> bool:
+    """Whether a wait ran out since this was last asked."""
+    if not word.value:
+        return False
+    word.value = 0
+    return True
+
+
+def _raise_ran_out() -> None:
+    raise RuntimeError("mps_pointops: a wait inside an earlier window_attention kernel ran out; "
+                       "its results are not valid")
+
+
+def _status(device: torch.device, stream: int) -> int:
+    """Address of the word that a kernel on this stream sets when a bounded wait runs
+    out; it is read here without waiting for the GPU."""
+    entry = _statuses.get((device.index, stream))
     if entry is None:
-        word = torch.zeros(1, dtype=torch.int32).pin_memory()
-        entry = _statuses[device.index] = (word, ctypes.c_int32.from_address(word.data_ptr()))
-    elif entry[1].value:
-        entry[1].value = 0
-        raise RuntimeError("mps_pointops: a wait inside an earlier window_attention kernel ran out; "
-                           "its results are not valid")
-    return entry[0].data_ptr()
+        pinned = torch.zeros(1, dtype=torch.int32).pin_memory()
+        entry = _statuses.setdefault((device.index, stream),
+                                     (pinned, ctypes.c_int32.from_address(pinned.data_ptr())))
+    elif _ran_out(entry[1]):
+        _raise_ran_out()
+    return ctypes.addressof(entry[1])
+
+
+def check(device: torch.device | str | None = None) -> None:
+    """Raise if a wait inside a ``window_attention`` kernel on ``device`` (default: the
+    current one) ran out, which makes its results invalid (synchronises).  The waits
+    are for the kernel's own copies and products, two seconds each at most; the next ``window_attention`` call on the same stream raises as well, without waiting,
+    if the word has been set by then."""
+    device = torch.device("cuda" if device is None else device)
+    index = torch.cuda.current_device() if device.index is None else device.index
+    torch.cuda.synchronize(index)
+    if any([_ran_out(word) for (owner, _), (_, word) in list(_statuses.items()) if owner == index]):
+        _raise_ran_out()
 
 
 class _Options:
@@ -347,6 +372,7 @@ def _attention_call(backward: bool, o: _Options, q, k, v, bias, out, lse, grad=N
     """``bias``: the table, the positions of queries and keys and the bucket map (or None)."""
     seg, device = o.segments, q.device
     table, qpos, kpos, mapping = bias
+    stream = _stream(device)
     shape = (0,) * 4 if table is None else (_DTYPES[table.dtype], table.shape[0], table.shape[1],
                                             o.reach)
 
@@ -357,20 +383,20 @@ def _attention_call(backward: bool, o: _Options, q, k, v, bias, out, lse, grad=N
             _address(grad), _address(delta), _address(dq), _address(dk),
             _address(dv), _address(table), _address(dtable), _address(qpos), _address(kpos),
             _address(mapping), seg.query_tiles.data_ptr(), seg.key_tiles.data_ptr(),
-            _status(device), seg.query_tiles.shape[0], seg.key_tiles.shape[0], q.shape[0],
+            status, seg.query_tiles.shape[0], seg.key_tiles.shape[0], q.shape[0],
             k.shape[0], _address(ws), nbytes, q.shape[1], k.shape[1], q.shape[2],
             _DTYPES[q.dtype], *shape, o.left, o.right, o.sinks, o.causal, seg.max_rows,
             seg.max_keys, seg.clouds, o.scale, int(backward))
 
     with N.on_device(device):
         lib = N.lib()
+        status = _status(device, stream)
         args = pack(None, 0)
         nbytes = int(lib.mpo_window_attention_workspace_bytes(args))
         ws = None
         if nbytes:
             ws = N.workspace(nbytes, device)
             args = pack(ws, nbytes)
-        stream = _stream(device)
         seg._use(stream)
         call = lib.mpo_window_attention_backward if backward else lib.mpo_window_attention
         N.check(call(args, stream), "window_attention backward" if backward else "window_attention")
@@ -549,4 +575,4 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, segments: Segments | Tenso
     return (out, lse) if return_lse else out
 
 
-__all__ = ["Segments", "log_buckets", "norm_rotate", "window_attention"]
+__all__ = ["Segments", "check", "log_buckets", "norm_rotate", "window_attention"]

@@ -365,3 +365,27 @@ def test_calls_without_gradients_keep_nothing(recorder):
     with torch.inference_mode():
         assert call(q, k, v).is_inference()
     assert [args[6] is None for _, args in recorder] == [True, False, True, True]  # lse only where it is used
+
+
+def test_waits_that_ran_out_are_reported_to_their_stream(monkeypatch):
+    """The word that a kernel sets belongs to its stream: the next call there is told, once;
+    calls on other streams are not, and check() is told without a further call."""
+    first, second = torch.device("cuda", 0), torch.device("cuda", 1)
+    words = {key: ctypes.c_int32(0) for key in ((0, 16), (0, 32), (1, 16))}
+    monkeypatch.setattr(attention, "_statuses", {key: (None, word) for key, word in words.items()})
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: None)
+    words[0, 16].value = 1
+    for device, stream in ((first, 32), (second, 16)):
+        assert attention._status(device, stream) == ctypes.addressof(words[device.index, stream])
+    with pytest.raises(RuntimeError, match="ran out"):
+        attention._status(first, 16)
+    assert attention._status(first, 16) == ctypes.addressof(words[0, 16])
+    words[0, 32].value = 1
+    attention.check(second)
+    with pytest.raises(RuntimeError, match="ran out"):
+        attention.check(first)
+    attention.check(first)
+    words[0, 16].value = words[0, 32].value = 1
+    with pytest.raises(RuntimeError, match="ran out"):
+        attention.check("cuda:0")
+    assert attention._status(first, 16) and attention._status(first, 32)  # both words were read
