@@ -389,3 +389,23 @@ def test_waits_that_ran_out_are_reported_to_their_stream(monkeypatch):
     with pytest.raises(RuntimeError, match="ran out"):
         attention.check("cuda:0")
     assert attention._status(first, 16) and attention._status(first, 32)  # both words were read
+
+
+def test_entry_addresses_for_every_reach():
+    """As above for each reach that a table or a bucket map can have: rows at the ends of
+    their range and beside the tile's first, differences around the clamps and at random."""
+    import numpy as np
+
+    f = np.float32
+    rng = np.random.default_rng(1)
+    rows = np.array([0, 1, -1, 5, 32767, 32768, -32767, -32768, *rng.integers(-32768, 32769, 24)])[:, None]
+    for reach in range(attention._MAX_REACH + 1):
+        inv = f(1) / f(2 * reach) if reach else f(0)
+        d = np.unique(np.concatenate([np.arange(-3, 4), reach + np.arange(-3, 3), -reach + np.arange(-2, 4),
+                                      rng.integers(-reach - 1, reach + 2, 40), [-98304, 98304]]))[None]
+        part = (0.5 - rows * float(inv)).astype(f)
+        column = np.clip(d + rows, -65536, 65536)
+        t = np.clip((column * float(inv) + part.astype(np.float64)).astype(f), f(0), f(1))
+        want = 128 * (np.clip(column - rows, -reach, reach) + reach)
+        for first in (1028, 200004):
+            assert (np.rint(t.astype(np.float64) * (256 * reach) + first) == first + want).all(), reach

@@ -743,3 +743,14 @@ def test_gradients_that_are_all_nan_take_no_longer(cuda_device, dtype, K, D):
             best = min(best, start.elapsed_time(stop))
         times.append(best)
     assert times[1] <= 10 * times[0], times
+
+
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+@pytest.mark.parametrize("D", [16, 64, 128])
+@pytest.mark.parametrize("bias", ["grid", "log"])
+def test_whole_tiles_with_a_table(cuda_device, dtype, D, bias):
+    """Tiles of 128 rows each of which sees every key of a tile of 64 or 128, beside tiles
+    that are cut by the window, all with a table; float32 sums over up to 500 pairs."""
+    run(cuda_device, dtype, 2, 1, D, [700, 256], left=260, right=230, sinks=1, bias=bias,
+        reach=7 if bias == "grid" else 50)
+    run(cuda_device, dtype, 2, 2, D, [384, 130], bias=bias, reach=7 if bias == "grid" else 50, seed=1)
