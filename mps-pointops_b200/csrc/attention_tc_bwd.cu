@@ -202,7 +202,7 @@ attn_tc_query_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__
     if (tid < 4) flags[tid] = 0u;
     const bool live = r < t.rows;
     BiasRow bias;
-    if (BIAS) bias.init(A, A.a.qpos, t.row, r, live, sb + Shape::kTable, 1);
+    if (BIAS) bias.init(A, A.a.qpos, t.row, r, t.rows, sb + Shape::kTable, 1);
     Columns columns;
     auto fetch_columns = [&](int i) {
         if (!BIAS || i >= tiles) return;
@@ -597,7 +597,7 @@ attn_tc_grad_kv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant
     const f32x2 scale2 = pack2(A.scale_log2, A.scale_log2);
     const bool live = r < t.rows;
     BiasRow bias;
-    if (BIAS) bias.init(A, A.a.kpos, t.row, r, live, sb + Shape::kTable, -1);
+    if (BIAS) bias.init(A, A.a.kpos, t.row, r, t.rows, sb + Shape::kTable, -1);
     auto load_table = [&](int h) {
         if (!BIAS) return;
         if (!ONE) tc_load_table(A, table, h);

@@ -147,7 +147,7 @@ attn_tc_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ T
     }
 
     BiasRow bias;
-    if (BIAS) bias.init(A, A.a.qpos, t.row, tid, tid < t.rows, sb + Shape::kTable, 1);
+    if (BIAS) bias.init(A, A.a.qpos, t.row, tid, t.rows, sb + Shape::kTable, 1);
     auto first_key = [&](int i, int& k0, int& n) {
         k0 = span.tile(i) * kTcCols;
         n = min(kTcCols, t.lk - k0);

@@ -754,3 +754,44 @@ def test_whole_tiles_with_a_table(cuda_device, dtype, D, bias):
     run(cuda_device, dtype, 2, 1, D, [700, 256], left=260, right=230, sinks=1, bias=bias,
         reach=7 if bias == "grid" else 50)
     run(cuda_device, dtype, 2, 2, D, [384, 130], bias=bias, reach=7 if bias == "grid" else 50, seed=1)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_summary_rows_far_from_the_points(cuda_device, dtype):
+    """A row at the head of each cloud with coordinates of its own, millions of cells away:
+    results, and the rows beside it stay with the tile (they counted as far from it: 9.8 ms
+    forward, against 0.10 without such a row and 0.33 with it)."""
+    g = torch.Generator().manual_seed(61)
+    lens, H, D = [700, 130, 2], 2, 32
+    n = sum(lens)
+    q, k, v, grad = (rand(g, n, H, D, dtype=dtype).to(cuda_device) for _ in range(4))
+    pos = torch.randint(0, 40, (n, 3), generator=g, dtype=torch.int32)
+    pos[[0, 700, 830]] = -(1 << 29)
+    table = rand(g, 3, 15, H, scale=0.5).to(cuda_device)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v, table)]
+    out = attention.window_attention(*leaves[:3], ends(lens, cuda_device), window=(60, 60), sinks=1,
+                                     bias_table=leaves[3], position=pos.to(cuda_device))
+    grads = torch.autograd.grad(out, leaves, grad)
+    want = C.attention(q, k, v, lens, lens, left=60, right=60, sinks=1, table=table, qpos=pos, kpos=pos,
+                       grad=grad)
+    for name, got in zip(("out", "dq", "dk", "dv", "dtable"), (out, *grads)):
+        C.check(got, want[name], name)
+
+    def time(head):
+        n = 4096
+        x = torch.randn(n, 4, 64, device=cuda_device).to(dtype)
+        pos = torch.randint(0, 40, (n, 3), dtype=torch.int32, device=cuda_device)
+        pos[0] = head
+        seg, table = attention.Segments(torch.tensor([n], device=cuda_device)), torch.zeros(3, 15, 4, device=cuda_device)
+        best = math.inf
+        for _ in range(4):
+            start, stop = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            attention.window_attention(x, x, x, seg, window=(512, 511), sinks=1, bias_table=table, position=pos)
+            stop.record()
+            stop.synchronize()
+            best = min(best, start.elapsed_time(stop))
+        return best
+
+    near, far = time(0), time(-(1 << 29))
+    assert far <= 20 * near, (near, far)
