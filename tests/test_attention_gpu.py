@@ -795,3 +795,35 @@ def test_summary_rows_far_from_the_points(cuda_device, dtype):
 
     near, far = time(0), time(-(1 << 29))
     assert far <= 20 * near, (near, far)
+
+
+@pytest.mark.parametrize("new", [None, 1])
+def test_captured_calls(cuda_device, new):
+    """A captured graph of both operators, on a stream that has not run them, gives what the
+    calls give on the data of each replay."""
+    g = torch.Generator().manual_seed(71)
+    keys = [300, 90]
+    lens = keys if new is None else [new] * 2
+    q, k, v = (rand(g, sum(n), 2, 64, dtype=BF).to(cuda_device) for n in (lens, keys, keys))
+    seg = attention.Segments(ends(lens, cuda_device), ends(keys, cuda_device))
+    freqs = torch.rand(1, 16, generator=g).to(cuda_device)
+    table = rand(g, 1, 15, 2).to(cuda_device)
+    pos = torch.arange(sum(keys), dtype=torch.int32, device=cuda_device)
+    rows = torch.arange(sum(lens), dtype=torch.int32, device=cuda_device)
+
+    def both():
+        kn, _ = attention.norm_rotate(k, k, pos, freqs)
+        return attention.window_attention(q, kn, v, seg, window=(50, 20), bias_table=table, position=rows,
+                                          key_position=pos)
+
+    both()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = both()
+    for seed in (1, 2):
+        q.copy_(rand(torch.Generator().manual_seed(seed), *q.shape, dtype=BF))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, both())
+    attention.check(cuda_device)
