@@ -69,7 +69,6 @@ __device__ __forceinline__ bool rows_unit(const AttnArgs& A, int per, int units,
 struct Partial {
     float* base;
     int64_t stride;  // floats of one row
-    int dim;
     __device__ __forceinline__ float* at(const AttnArgs& A, int64_t q, int h, int z) const {
         return base + (((int64_t)z * A.a.q_rows + q) * A.a.heads + h) * stride;
     }
@@ -104,7 +103,7 @@ __device__ __forceinline__ void join_warps(const AttnArgs& A, const Unit& U, con
         float l = 0.f;
         for (int w = 0; w < slots; ++w)
             l = fmaf(sh[(w * 16 + r) * pitch + 1], exp2_sfu(sh[(w * 16 + r) * pitch] - ref), l);
-        float* dst = splits > 1 ? Partial{partial, partial_stride(A.a.dim), A.a.dim}.at(A, q, h, blockIdx.z)
+        float* dst = splits > 1 ? Partial{partial, partial_stride(A.a.dim)}.at(A, q, h, blockIdx.z)
                                 : nullptr;
         bool nan = false;
         for (int d = lane; d < A.a.dim; d += 32) {
@@ -550,7 +549,23 @@ int run(const AttnArgs& A, cudaStream_t s) {
 
 // At most 16 rows of queries and shared heads per key head and cloud: then a
 // key is read by one unit (by group / 16 where more heads share it), where a
-// tile kernel would fill 1/8 of its rows or less.
+// tile kernel would fill 1/8 of its rows or less.  Beyond, this kernel reads the
+// keys again for every 16 rows, and the tile kernels read them once but by one
+// block per 128 rows and head, so they gain with many rows and many clouds only.
+// Kernel times in us over 8192 keys per cloud, this kernel | tile kernel:
+//   bf16, 32 heads of 128 over 8   5 rows   16       32        128
+//     1 cloud                      21 | 94  34 | 94  59 | 94   164 | 94
+//     8 clouds                    118 | 152 194 | 154 299 | 155 975 | 157
+//     64 clouds                   581 | 1144 1041 | 1154 1978 | 1183
+//   bf16, 8 heads of 64           17 rows   32       64        128
+//     1 cloud                      20 | 110 21 | 110 26 | 110  39 | 111
+//     8 clouds                     79 | 109 86 | 109 139 | 109 227 | 109
+//     64 clouds                   423 | 254 450 | 254 805 | 255
+//   float32, 8 heads of 64
+//     1 cloud                      85 | 866 151 | 867 267 | 714 520 | 715
+//     8 clouds                    619 | 1074 1182 | 1074 2290 | 927
+// The limit is right for many clouds without shared heads; with few clouds, or a few
+// rows of shared heads, a limit by the count of blocks would gain up to 5 times.
 bool attn_rows_eligible(const AttnArgs& A) {
     return (int64_t)A.a.max_rows * min64(A.group, 16) <= 16;
 }

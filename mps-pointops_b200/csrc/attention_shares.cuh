@@ -80,11 +80,11 @@ int join_shares(const AttnArgs& A, const KeyShares& K, const float* partial, cud
 // sinks would outlast all others (5 times the kernel's time on clouds of 4096 points
 // and a window of 512).  All tiles: where there are fewer blocks than half of the SMs,
 // as many as fill them, of 64 queries or more (undivided against divided and joined, us:
-// float32, clouds of 304, 200 and 100 points, 4 heads of 128 over 1: 446, 71; 700 and 300
-// points, 8 heads of 64 over 2, window 400: 619, 169; bf16, 1024 and 900 points, 8 over 2:
-// 61, 26; 2048 points, 16 heads of 128 over 4, causal: 119, 80; one cloud of 1024 points, 4
-// heads of 32, window 256: 10.5, 10.6).  float32 divides the query heads of a key head too;
-// with 16-bit types that gave the first of these cases 23 against 20 us and took the
+// float32, clouds of 304, 200 and 100 points, 4 heads of 128 over 1: 455, 70; 700 and 300
+// points, 8 heads of 64 over 2, window 400, 4 sinks: 637, 171; bf16, 1024 and 900 points, 8
+// over 2, window 600: 61, 26; 2048 points, 16 heads of 128 over 4, causal: 118, 80; one cloud
+// of 1024 points, 4 heads of 32, window 256: 10.7, 10.6).  float32 divides the query heads of
+// a key head too; with 16-bit types that gave the first of these shapes 23 against 21 us and took the
 // registers of the table's kernel (987 against 897 us at 8 x 8192 points).
 inline KeyShares key_shares(const AttnArgs& A) {
     const int64_t rows = A.a.max_rows, window = (int64_t)A.left + A.right + kAttnTile;

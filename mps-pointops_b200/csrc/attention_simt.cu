@@ -7,7 +7,7 @@
 // four elements of a dot product a thread loads 8 + 4 vectors of 16 bytes for
 // 128 multiply-adds, about half of what shared memory can deliver in that
 // time.  3 ragged clouds of up to 4096 points, 4 heads of 32, window 512, a table:
-// forward 127, queries 326, keys and values 288 us, where the products alone would
+// forward 126, queries 325, keys and values 287 us, where the products alone would
 // take 30, 44 and 59 us of the FP32 pipes' 74 TFLOP/s: at 32 elements the bias of a
 // pair (and the table's cells) costs more than its products, and there are at most
 // 768 blocks of 64 rows, of unequal clouds.

@@ -14,11 +14,11 @@
 // the same columns, and these are the left operands of the accumulating products.
 //
 // 8 clouds of 8192 points, 8 heads of 64, window 1024, a table of 3 x 63 entries:
-// keys and values 900 us, D alone 738 us, dq and the table 1616 us (880 of them its
+// keys and values 904 us, D alone 733 us, dq and the table 1607 us (880 of them its
 // cells: shared memory at 59 % and the issue slots at 57 % of their peaks bind).
 // Without a table, 5 ragged clouds of up to 4099 points, 16 heads of 128 over 4:
-// keys and values 288 us, queries 285 us, tensor cores at 39 % of their rate in the
-// former; latency at one block per SM binds.
+// keys and values 287 us, queries 285 us, tensor memory busy for 59 and 44 % of the
+// cycles; latency at one block per SM binds.
 #include <string>
 
 #include "attention_shares.cuh"
@@ -32,7 +32,9 @@ namespace {
 // result.  For the table's gradient, which is kept in float32, D has to be the
 // sum over the pairs of the very weights and dP that it is subtracted from:
 // stored and tensor-core results are off by 2e-3 and (sums rounded towards zero)
-// 3e-6 of it, always the same way for all pairs of a row.  kDelta forms D = sum
+// 3e-6 of it, always the same way for all pairs of a row (in dq and dk, which round each
+// score gradient to 16 bits anyway, the stored result's share is 0.0003 to 0.001 of their norm
+// beside 0.0024 for bf16).  kDelta forms D = sum
 // P dP in float32 first; kGradQTable then forms dq and the table's gradient.
 enum QueryMode { kGradQ = 0, kDelta = 1, kGradQTable = 2 };
 

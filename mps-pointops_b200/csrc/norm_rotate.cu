@@ -17,8 +17,8 @@
 // them; float64 for positions whose float32 angle would be off by too much),
 // reduced to one turn in double with the rest of 1 / pi, then sincospif.
 //
-// At that size the forward moves 4.5 TB/s and the backward 4.6 TB/s, 69 % of a
-// plain copy.  Instructions hold it (67 % of the issue slots in the forward), not
+// At that size the forward moves 4.6 TB/s and the backward 4.7 TB/s, 70 % of a
+// plain copy.  Instructions hold it (68 % of the issue slots in the forward), not
 // loads in flight: fetching the next row's heads ahead took 281 and 411 us against
 // 246 and 362, and weights read once per row instead of once per round 348 against
 // 358 us in the backward.
@@ -33,7 +33,7 @@ namespace {
 constexpr int kRotThreads = 256;
 constexpr int kRotWarps = kRotThreads / 32;
 // Resident, by registers.  262144 rows of 8 + 8 heads of 64 (bf16, 48 elements turned on
-// three axes): forward at 2 / 3 / 4 blocks 268 / 240 / 247 us, backward at 2 / 3 348 / 575 us.
+// three axes): forward at 2 / 3 / 4 blocks 266 / 235 / 241 us, backward at 2 / 3 344 / 535 us.
 constexpr int kFwdBlocksPerSm = 3, kBwdBlocksPerSm = 2;
 
 template <typename T>

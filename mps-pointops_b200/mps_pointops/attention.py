@@ -20,7 +20,8 @@ its neighbours along the order of its own cloud.
 
 float32, float16 and bfloat16; scores, softmax, sums and norms are held in
 float32, weights and score gradients of 16-bit inputs are rounded to the input
-type as operands of the tensor cores.  All results are bit-reproducible.
+type as operands of the tensor cores (float16 score gradients below 2^-24 vanish:
+scale the loss).  All results are bit-reproducible.
 CUDA tensors only; other tensors raise ``RuntimeError`` after validation.
 """
 
@@ -491,7 +492,10 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, segments: Segments | Tenso
     is the difference key - query clamped to [-R, R], plus R, where
     ``buckets = 2 R + 1``; or, with the map ``buckets`` (2 R + 1,), what the map
     names there (``log_buckets``; names are clamped to the table).  A * buckets
-    is at most 256.
+    is at most 256.  Positions may change after the call, but not between a forward
+    and its backward, where autograd refuses the change.  16-bit types: a row more than
+    2^15 on some axis from the middle one of its 128 is formed pair by pair, about a
+    microsecond for each; keep such rows few.
 
     ``return_lse``: also the logarithm of each row's softmax denominator, (H, N)
     float32, -inf for a row that sees no key (no gradient through it).
